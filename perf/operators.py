@@ -65,7 +65,7 @@ def listed():
     ]
 
 
-_MOST_TOKENS = 8.0e5   # of a cache, times heads * head_dim / 1024; the largest listed case has 4.4e5 with 1024
+_MOST_TOKENS = 6.0e5   # of a cache, times kv_heads * head_dim / 1024; the largest listed case has 3.0e5, and as many bytes again to read
 _MOST_PAIRS = 1.0e9    # (query, key) pairs of the padded rectangle, times heads; the largest listed case has 2.1e9
 _MOST_SLOTS = 1.0e6    # new tokens of a "tables" case; the largest listed case has 1.2e6
 
@@ -166,7 +166,8 @@ def _up(x, m):
 def _power_of_two(amax):
     """The smallest power of two with amax / scale <= 448, at least 2^-100 (fp32, exact)."""
     mantissa, exponent = torch.frexp(amax)  # amax = mantissa * 2^exponent, mantissa in [0.5, 1); 448 = 0.875 * 2^9
-    return torch.ldexp(torch.ones_like(amax), (exponent - 9 + (mantissa > 0.875).int()).clamp_min(-100))
+    exponent = torch.where(amax > 0, exponent - 9 + (mantissa > 0.875).int(), -100).clamp_min(-100)
+    return torch.ldexp(torch.ones_like(amax), exponent)
 
 
 def _int32(x):

@@ -424,6 +424,209 @@ int run_mxfp8(const GdpaMxParams* p, int quantize, gdpa_stream_t stream) {
 int gdpa_quantize_mxfp8(const GdpaMxParams* p, gdpa_stream_t stream) { return run_mxfp8(p, 1, stream); }
 int gdpa_dequantize_mxfp8(const GdpaMxParams* p, gdpa_stream_t stream) { return run_mxfp8(p, 0, stream); }
 
+namespace {
+// log2 of a cache's block size; -1 for one that is not supported
+int block_shift_of(int block_size) {
+  return block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : block_size == 128 ? 7 : -1;
+}
+
+// A cache's strides {block, row, head} with the contiguous ones in the place of zeros, checked.
+int cache_strides(const int64_t (&given)[3], int block_size, int heads, int head_dim, long long (&out)[3]) {
+  out[2] = given[2] != 0 ? given[2] : head_dim;
+  out[1] = given[1] != 0 ? given[1] : static_cast<long long>(heads) * head_dim;
+  out[0] = given[0] != 0 ? given[0] : static_cast<long long>(block_size) * heads * head_dim;
+  for (long long s : out) {
+    if (s <= 0 || s >= (1ll << 40)) return GDPA_ERR_BAD_ARG;
+    if (s % 16 != 0) return GDPA_ERR_MISALIGNED;
+  }
+  return GDPA_OK;
+}
+
+// Token and head stride of a [tokens, heads, head_dim] tensor of `elem` bytes, checked.
+int row_strides(const int64_t (&given)[2], int heads, int head_dim, int elem, long long (&out)[2]) {
+  out[1] = given[1] != 0 ? given[1] : head_dim;
+  out[0] = given[0] != 0 ? given[0] : static_cast<long long>(heads) * head_dim;
+  if (out[0] < 0 || out[1] < 0) return GDPA_ERR_BAD_ARG;
+  return (out[0] * elem) % 16 != 0 || (out[1] * elem) % 16 != 0 ? GDPA_ERR_MISALIGNED : GDPA_OK;
+}
+
+// The map of a cache whose boxes are one block of one head.
+int make_cache_tmap(CUtensorMap* m, const void* base, const long long (&strides)[3], long long blocks, int block_size, int heads, int head_dim) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (enc == nullptr) return GDPA_ERR_DRIVER;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(block_size), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(blocks)};
+  const cuuint64_t bytes[3] = {static_cast<cuuint64_t>(strides[1]), static_cast<cuuint64_t>(strides[2]), static_cast<cuuint64_t>(strides[0])};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(head_dim), static_cast<cuuint32_t>(block_size), 1u, 1u}, step[4] = {1u, 1u, 1u, 1u};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, bytes, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? GDPA_OK : GDPA_ERR_DRIVER;
+}
+
+bool aligned16(const void* a, const void* b) { return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u) == 0; }
+
+// Rows of a row tile: the small one where a request's (query, head of the group) rows fit in it.
+int paged_rows(int group, int max_q) { return static_cast<long long>(group) * max_q <= kPagedRowsSmall ? kPagedRowsSmall : kPagedRowsLarge; }
+
+// Parts of the workspace: counters, then the pieces' O, then their row statistics; two pieces per CTA.
+size_t paged_counter_bytes(int ctas) { return (static_cast<size_t>(ctas) * sizeof(int) + 127) / 128 * 128; }
+size_t paged_part_bytes(int ctas, int rows, int head_dim) { return static_cast<size_t>(2) * ctas * rows * head_dim * sizeof(float); }
+size_t paged_stat_bytes(int ctas, int rows) { return static_cast<size_t>(2) * ctas * 2 * rows * sizeof(float); }
+}  // namespace
+
+int gdpa_build_block_tables(const GdpaBlockTableParams* p, gdpa_stream_t stream) {
+  if (p == nullptr || p->struct_size != sizeof(GdpaBlockTableParams)) return GDPA_ERR_BAD_ARG;
+  const int shift = block_shift_of(p->block_size);
+  if (shift < 0 || p->batch < 0 || p->table_width < 0 || p->total_new < 0 || p->total_new > 0x7fffffffll || p->free_capacity < 0) return GDPA_ERR_BAD_ARG;
+  if ((static_cast<long long>(p->table_width) << shift) > (1ll << 30) || p->table_stride < 0) return GDPA_ERR_BAD_ARG;
+  if (p->num_free == nullptr || p->query_offset == nullptr || p->num_free_after == nullptr || p->num_free == p->num_free_after) return GDPA_ERR_BAD_ARG;
+  if (p->total_new > 0 && p->slots == nullptr) return GDPA_ERR_BAD_ARG;
+  if (p->batch > 0 && (p->cached_lens == nullptr || p->new_lens == nullptr || p->seq_lens == nullptr)) return GDPA_ERR_BAD_ARG;
+  if (p->batch > 0 && p->table_width > 0 && p->block_tables == nullptr) return GDPA_ERR_BAD_ARG;
+  if (p->free_capacity > 0 && p->free_blocks == nullptr) return GDPA_ERR_BAD_ARG;
+  DeviceInfo di;
+  int rc = device_info(&di);
+  if (rc != GDPA_OK) return rc;
+  BlockTableArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.cached_lens = p->cached_lens;
+  a.new_lens = p->new_lens;
+  a.lens_are_int64 = p->lens_are_int64 != 0 ? kOffsets64 : 0;
+  a.batch = p->batch;
+  a.block_tables = p->block_tables;
+  a.table_stride = p->table_stride;
+  a.table_width = p->table_width;
+  a.block_shift = shift;
+  a.free_blocks = p->free_blocks;
+  a.free_capacity = p->free_capacity;
+  a.num_free = p->num_free;
+  a.total_new = p->total_new;
+  a.slots = reinterpret_cast<long long*>(p->slots);
+  a.query_offset = p->query_offset;
+  a.seq_lens = p->seq_lens;
+  a.num_free_after = p->num_free_after;
+  rc = launch_block_tables(a, di.sm_count, static_cast<cudaStream_t>(stream));
+  if (rc == 0) g_launches.fetch_add(1);
+  return rc;
+}
+
+int gdpa_append_kv_cache_fp8(const GdpaCacheAppendParams* p, gdpa_stream_t stream) {
+  if (p == nullptr || p->struct_size != sizeof(GdpaCacheAppendParams)) return GDPA_ERR_BAD_ARG;
+  const int shift = block_shift_of(p->block_size);
+  if (shift < 0 || p->tokens < 0 || p->num_blocks < 0 || p->kv_heads <= 0) return GDPA_ERR_BAD_ARG;
+  if (p->head_dim != 64 && p->head_dim != 128) return GDPA_ERR_UNSUPPORTED_DIM;
+  if (p->tokens > 32ll * 0x7fffffffll || p->kv_heads > (1 << 20)) return GDPA_ERR_BAD_ARG;
+  CacheAppendArgs a;
+  std::memset(&a, 0, sizeof(a));
+  const int elem = p->x_is_fp32 != 0 ? 4 : 2;
+  int rc;
+  if ((rc = row_strides(p->key_strides, p->kv_heads, p->head_dim, elem, a.key_strides)) != GDPA_OK) return rc;
+  if ((rc = row_strides(p->value_strides, p->kv_heads, p->head_dim, elem, a.value_strides)) != GDPA_OK) return rc;
+  if ((rc = cache_strides(p->k_cache_strides, p->block_size, p->kv_heads, p->head_dim, a.k_cache_strides)) != GDPA_OK) return rc;
+  if ((rc = cache_strides(p->v_cache_strides, p->block_size, p->kv_heads, p->head_dim, a.v_cache_strides)) != GDPA_OK) return rc;
+  if (p->tokens == 0 || p->num_blocks == 0) return GDPA_OK;
+  if (p->key == nullptr || p->value == nullptr || p->k_cache == nullptr || p->v_cache == nullptr || p->k_scales == nullptr ||
+      p->v_scales == nullptr || p->slot_mapping == nullptr)
+    return GDPA_ERR_BAD_ARG;
+  if (!aligned16(p->key, p->value) || !aligned16(p->k_cache, p->v_cache)) return GDPA_ERR_MISALIGNED;
+  DeviceInfo di;
+  if ((rc = device_info(&di)) != GDPA_OK) return rc;
+  a.key = p->key;
+  a.value = p->value;
+  a.k_cache = static_cast<uint8_t*>(p->k_cache);
+  a.v_cache = static_cast<uint8_t*>(p->v_cache);
+  a.k_scales = p->k_scales;
+  a.v_scales = p->v_scales;
+  a.slot_mapping = reinterpret_cast<const long long*>(p->slot_mapping);
+  a.tokens = p->tokens;
+  a.num_blocks = p->num_blocks;
+  a.block_shift = shift;
+  a.heads = p->kv_heads;
+  rc = launch_cache_append(a, p->head_dim, p->x_is_fp32 != 0, di.sm_count, static_cast<cudaStream_t>(stream));
+  if (rc == 0) g_launches.fetch_add(1);
+  return rc;
+}
+
+size_t gdpa_paged_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t max_seq_len_q) {
+  DeviceInfo di;
+  if (heads <= 0 || kv_heads <= 0 || head_dim <= 0 || max_seq_len_q < 0 || device_info(&di) != GDPA_OK) return 0;
+  const int rows = paged_rows(heads / kv_heads, max_seq_len_q);
+  return paged_counter_bytes(di.sm_count) + paged_part_bytes(di.sm_count, rows, head_dim) + paged_stat_bytes(di.sm_count, rows);
+}
+
+int gdpa_fwd_paged_fp8(const GdpaPagedParams* p, gdpa_stream_t stream) {
+  if (p == nullptr || p->struct_size != sizeof(GdpaPagedParams)) return GDPA_ERR_BAD_ARG;
+  const int act = act_class_from_id(p->activation);
+  if (act < 0) return GDPA_ERR_UNSUPPORTED_ACT;
+  if (p->head_dim != 64 && p->head_dim != 128) return GDPA_ERR_UNSUPPORTED_DIM;
+  const int shift = block_shift_of(p->block_size);
+  if (shift < 0 || p->batch < 0 || p->heads <= 0 || p->kv_heads <= 0 || p->heads % p->kv_heads != 0) return GDPA_ERR_BAD_ARG;
+  if (p->total_q < 0 || p->total_q > 0x7fffffffll || p->max_seq_len_q < 0 || p->table_width < 0 || p->table_stride < 0) return GDPA_ERR_BAD_ARG;
+  if (p->num_blocks < 0 || p->num_blocks > 0x7fffffffll || (static_cast<long long>(p->table_width) << shift) > (1ll << 30)) return GDPA_ERR_BAD_ARG;
+  if (p->window_plus_one < 0 || p->window_plus_one > (1 << 29)) return GDPA_ERR_BAD_ARG;
+  const int group = p->heads / p->kv_heads;
+  if (static_cast<long long>(p->max_seq_len_q) * group > (1ll << 30)) return GDPA_ERR_BAD_ARG;
+  PagedLaunch l;
+  std::memset(&l, 0, sizeof(l));
+  int rc;
+  long long ks[3], vs[3];
+  if ((rc = row_strides(p->q_strides, p->heads, p->head_dim, 2, l.args.q_strides)) != GDPA_OK) return rc;
+  if ((rc = cache_strides(p->k_cache_strides, p->block_size, p->kv_heads, p->head_dim, ks)) != GDPA_OK) return rc;
+  if ((rc = cache_strides(p->v_cache_strides, p->block_size, p->kv_heads, p->head_dim, vs)) != GDPA_OK) return rc;
+  if (p->total_q == 0 || p->batch == 0 || p->max_seq_len_q == 0) return GDPA_OK;
+  if (p->q == nullptr || p->o == nullptr || p->q_offsets == nullptr || p->seq_lens == nullptr || p->workspace == nullptr) return GDPA_ERR_BAD_ARG;
+  if (p->table_width > 0 && p->block_tables == nullptr) return GDPA_ERR_BAD_ARG;
+  if (p->num_blocks > 0 && (p->k_cache == nullptr || p->v_cache == nullptr || p->k_scales == nullptr || p->v_scales == nullptr)) return GDPA_ERR_BAD_ARG;
+  if (!aligned16(p->q, p->o) || !aligned16(p->k_cache, p->v_cache) || !aligned16(p->workspace, nullptr)) return GDPA_ERR_MISALIGNED;
+  DeviceInfo di;
+  if ((rc = device_info(&di)) != GDPA_OK) return rc;
+  l.rows = paged_rows(group, p->max_seq_len_q);
+  l.grid = di.sm_count;
+  const size_t counters = paged_counter_bytes(l.grid), parts = paged_part_bytes(l.grid, l.rows, p->head_dim);
+  if (p->workspace_bytes < static_cast<int64_t>(counters + parts + paged_stat_bytes(l.grid, l.rows))) return GDPA_ERR_CAPACITY;
+  // a cache without blocks still needs valid maps: of one block in the place of Q, which no coordinate reaches
+  const long long blocks = p->num_blocks > 0 ? p->num_blocks : 1;
+  if ((rc = make_cache_tmap(&l.tm_k, p->num_blocks > 0 ? p->k_cache : p->q, ks, blocks, p->block_size, p->kv_heads, p->head_dim)) != GDPA_OK) return rc;
+  if ((rc = make_cache_tmap(&l.tm_v, p->num_blocks > 0 ? p->v_cache : p->q, vs, blocks, p->block_size, p->kv_heads, p->head_dim)) != GDPA_OK) return rc;
+  uint8_t* const ws = static_cast<uint8_t*>(p->workspace);
+  PagedArgs& a = l.args;
+  a.q = static_cast<const __nv_bfloat16*>(p->q);
+  a.o = static_cast<__nv_bfloat16*>(p->o);
+  a.k_scales = p->k_scales;
+  a.v_scales = p->v_scales;
+  a.block_tables = p->block_tables;
+  a.table_stride = p->table_stride;
+  a.table_width = p->table_width;
+  a.num_blocks = static_cast<int>(p->num_blocks);
+  a.block_shift = shift;
+  a.q_off = p->q_offsets;
+  a.seq_lens = p->seq_lens;
+  a.off64 = p->offsets_are_int64 != 0 ? kOffsets64 : 0;
+  a.lens64 = p->lens_are_int64 != 0 ? kOffsets64 : 0;
+  a.batch = p->batch;
+  a.heads = p->heads;
+  a.kv_heads = p->kv_heads;
+  a.group = group;
+  a.max_q = p->max_seq_len_q;
+  a.total_q = p->total_q;
+  a.act = act;
+  a.scale = p->qk_scale;
+  a.causal = p->causal != 0;
+  a.window = p->window_plus_one - 1;
+  a.counters = reinterpret_cast<int*>(ws);
+  a.part_o = reinterpret_cast<float*>(ws + counters);
+  a.part_ml = reinterpret_cast<float*>(ws + counters + parts);
+  a.status = p->status;
+  l.stream = static_cast<cudaStream_t>(stream);
+  if (cudaMemsetAsync(ws, 0, counters, l.stream) != cudaSuccess) return GDPA_ERR_LAUNCH;
+  if (p->timing_start_event != nullptr) cudaEventRecord(static_cast<cudaEvent_t>(p->timing_start_event), l.stream);
+  rc = launch_paged(l, p->head_dim);
+  if (p->timing_stop_event != nullptr) cudaEventRecord(static_cast<cudaEvent_t>(p->timing_stop_event), l.stream);
+  if (rc == 0) g_launches.fetch_add(1);
+  return rc;
+}
+
 int gdpa_norm_rows_bwd(const GdpaNormBwdParams* p, gdpa_stream_t stream) {
   if (p == nullptr || p->struct_size != sizeof(GdpaNormBwdParams)) return GDPA_ERR_BAD_ARG;
   if (p->mode < 0 || p->mode > 2 || p->rows < 0 || p->n <= 0 || p->n % 8 != 0) return GDPA_ERR_BAD_ARG;

@@ -180,6 +180,81 @@ struct SchedArgs {
   int kv_batch;          // sequences the KV offsets describe (bounds kv_index entries)
 };
 
+struct BlockTableArgs {
+  const void* cached_lens;
+  const void* new_lens;
+  int lens_are_int64;
+  int batch;
+  int* block_tables;
+  long long table_stride;
+  int table_width;
+  int block_shift;  // block_size = 1 << block_shift
+  const int* free_blocks;
+  long long free_capacity;
+  const int* num_free;
+  long long total_new;
+  long long* slots;
+  int* query_offset;
+  int* seq_lens;
+  int* num_free_after;
+  int per;  // requests per thread in one round (set by the launcher)
+};
+
+struct CacheAppendArgs {
+  const void* key;
+  const void* value;
+  long long key_strides[2];      // token, head; in elements
+  long long value_strides[2];
+  uint8_t* k_cache;
+  uint8_t* v_cache;
+  long long k_cache_strides[3];  // block, row, head; in elements
+  long long v_cache_strides[3];
+  float* k_scales;               // [blocks, heads]
+  float* v_scales;
+  const long long* slot_mapping;
+  long long tokens;
+  long long num_blocks;
+  int block_shift;
+  int heads;
+};
+
+struct PagedArgs {
+  const __nv_bfloat16* q;
+  long long q_strides[2];  // token, head; in elements
+  __nv_bfloat16* o;        // [total_q, heads, head_dim]
+  const float* k_scales;   // [blocks, kv_heads]
+  const float* v_scales;
+  const int* block_tables;
+  long long table_stride;
+  int table_width;
+  int num_blocks;
+  int block_shift;
+  const void* q_off;
+  const void* seq_lens;
+  int off64, lens64;
+  int batch;
+  int heads, kv_heads, group;  // group = heads / kv_heads
+  int max_q;
+  long long total_q;
+  int act;                     // activation class
+  float scale;
+  int causal;
+  int window;                  // -1 = none
+  int* counters;               // one per CTA, zero at the launch
+  float* part_o;               // [2 per CTA][rows of a tile][head_dim]
+  float* part_ml;              // [2 per CTA][2][rows of a tile]
+  int* status;
+};
+
+struct PagedLaunch {
+  CUtensorMap tm_k, tm_v;  // over [blocks, kv_heads, block_size, head_dim]: a box is one block of one head
+  PagedArgs args;
+  int rows;                // rows of a tile: kPagedRowsSmall or kPagedRowsLarge
+  int grid;
+  cudaStream_t stream;
+};
+constexpr int kPagedRowsSmall = 32, kPagedRowsLarge = 128;
+
 }  // namespace gdpa
 struct GdpaFwdParams;
 namespace gdpa {
@@ -200,5 +275,8 @@ int launch_quant_fp8(const QuantArgs& a, int in_is_fp32, cudaStream_t stream);
 int launch_mxfp8(const MxArgs& a, int quantize, int x_is_fp32, cudaStream_t stream);
 int launch_norm_rows_bwd(const NormBwdArgs& a, int mode, cudaStream_t stream);
 int launch_build_schedule(const SchedArgs& a, cudaStream_t stream);
+int launch_block_tables(const BlockTableArgs& a, int sm_count, cudaStream_t stream);
+int launch_cache_append(const CacheAppendArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream);
+int launch_paged(const PagedLaunch& l, int head_dim);
 
 }  // namespace gdpa

@@ -1,0 +1,946 @@
+// GDPA forward over a paged cache of 8-bit keys and values, for sm_100a:  O = act(Q K^T) * scale V  (or the softmax form) for the last
+// queries of every request, K and V e4m3 with one fp32 scale per (block, head).
+//
+// What bounds it: with few queries (a step of generation) the bytes of the cache, with many the tensor cores.  Both are served by one
+// transposed form.  A tile is 128 cached tokens of one K / V head against N rows, the rows being the (query, head of the group) pairs
+// that share this K / V head:
+//     S^T [128 tokens x N] = K Q^T          tcgen05.mma kind::f8f6f4, A = the K tile as it lies in the cache
+//     P^T = act(S^T) per token and row      a thread has one token: its scales are two registers, a mask is a compare
+//     O^T [D x N] += V^T P^T                A = the V tile, MN-major, as it lies in the cache
+// The cache bytes go from HBM through TMA into the tensor cores without a conversion, the 128-row side of the MMA is always full, and
+// N is as small as the rows are few (16 to 128), where the untransposed form would compute 128 rows for one query.
+//
+// Both small operands have to be e4m3 as well, and one e4m3 value has four significant bits.  So Q and P are each the sum of two:
+// hi = e4m3(x), lo = e4m3(x - hi), both multiplied into the same accumulator.  For a bf16 Q (eight significant bits) scaled by a
+// power of two per row the sum is exact (down to 2^-19 of the row's largest element); for P it leaves 2^-8 of a value at most
+// (7e-4 rms), like the rounding to bf16 elsewhere.  The second product costs tensor time that a cache-bound call has to spare.
+//
+// P^T is scaled per row so that its largest element (times V's block scale) lies at kTarget.  The scale, for the softmax the
+// running maximum, is kept until a product would pass 448 (e4m3's largest): only then, and for the first tile, is the exact maximum
+// taken and O rescaled, a vote of the warpgroup per tile and group of columns otherwise.  The exact value of a row's reference does
+// not enter the result.
+//
+// Work: units are tiles; the units of all (request, K / V head, row tile) items in order are cut into equal stretches, one per CTA
+// (one persistent CTA per SM), whatever the requests' lengths.  An item that is cut leaves partial sums in a workspace, and the
+// CTA that finishes it last (an atomic count per item) joins them in the order of the pieces, so the result does not depend on who
+// was last.  No CTA waits for another.
+//
+// Roles: kGroups warpgroups (element-wise work, epilogue), one warp of TMA loads, one warp that issues MMAs, two that fetch Q.
+#include <cuda_bf16.h>
+
+#include "gdpa_common.cuh"
+#include "gdpa_launch.h"
+
+namespace gdpa {
+
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kItemSlots = 4;
+constexpr float kMax8 = 448.f;
+constexpr float kNoMax = -3.0e38f;     // running maximum of a row that has seen no key
+constexpr float kLeastScale = 7.888609e-31f;  // 2^-100
+
+template <int D, int NMAX>
+struct PagedShape {
+  static constexpr int kGroups = NMAX > 32 ? 2 : 1;    // warpgroups
+  static constexpr int kTileBytes = kTile * D;         // K or V tile
+  static constexpr int kStages = NMAX > 32 ? 3 : 6;
+  static constexpr int kQBytes = NMAX * D;             // hi, then lo
+  static constexpr int kPBytes = NMAX * kTile;
+  static constexpr int kWarps = 4 * kGroups + 4;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kLoadWarp = 4 * kGroups, kMmaWarp = kLoadWarp + 1, kQWarp = kLoadWarp + 2;
+  static constexpr int kTmemCols = NMAX > 32 ? 512 : 128;  // S0, S1, O of NMAX columns each
+  static constexpr float kTarget = NMAX > 32 ? 64.f : 256.f;
+
+  static constexpr int kKvOff = 0;                                  // [stage]{K, V}
+  static constexpr int kQOff = kKvOff + kStages * 2 * kTileBytes;   // [2]{hi, lo}
+  static constexpr int kPOff = kQOff + 2 * 2 * kQBytes;             // {hi, lo}
+  static constexpr int kScaleOff = kPOff + 2 * kPBytes;             // float[stage][16]: K scales of up to 8 blocks, V scales
+  static constexpr int kQaOff = kScaleOff + kStages * 64;           // float[2][NMAX]: factor of a row's scores
+  static constexpr int kRefOff = kQaOff + 2 * NMAX * 4;             // float[NMAX]: running maximum / multiplier of a row
+  static constexpr int kFacOff = kRefOff + NMAX * 4;                // float[NMAX]
+  static constexpr int kRedOff = kFacOff + NMAX * 4;                // float[4][NMAX]
+  static constexpr int kRangeOff = kRedOff + 4 * NMAX * 4;          // int2[NMAX]: keys a row takes part with
+  static constexpr int kRingOff = kRangeOff + NMAX * 8;             // int[kItemSlots][16]
+  static constexpr int kBarOff = kRingOff + kItemSlots * 64;
+  enum : int {
+    B_KV_FULL = 0,
+    B_KV_EMPTY = B_KV_FULL + kStages,
+    B_SC_FULL = B_KV_EMPTY + kStages,
+    B_S_FULL = B_SC_FULL + kStages,   // [2]
+    B_P_FULL = B_S_FULL + 2,
+    B_PV_DONE = B_P_FULL + 1,
+    B_Q_FULL = B_PV_DONE + 1,         // [2]
+    B_Q_EMPTY = B_Q_FULL + 2,         // [2]
+    B_ITEM_FULL = B_Q_EMPTY + 2,      // [kItemSlots]
+    B_ITEM_EMPTY = B_ITEM_FULL + kItemSlots,
+    B_COUNT = B_ITEM_EMPTY + kItemSlots
+  };
+  static constexpr int kMiscOff = kBarOff + B_COUNT * 8;  // tmem address, abort flag, last-arrival flag, pad; then the scan's scratch
+  static constexpr int kScanOff = kMiscOff + 16;          // long long[32] + start state
+  static constexpr int kBytes = kScanOff + 32 * 8 + 48;
+  static constexpr int kDynBytes = kBytes + 1024;
+  static_assert(kDynBytes <= 227 * 1024, "shared memory");
+};
+
+// One stretch of tiles of one item, as the loader publishes it.
+struct PagedItem {
+  int h;        // K / V head; -1 ends the walk, -2: a wait ran out
+  int q_start;  // first query row of the request
+  int q_len;
+  int row0;     // first (query, head of the group) row of the tile
+  int rows;
+  int len;      // tokens of the request
+  int lo, hi;   // keys that any of the rows takes part with
+  int tile0, tiles;
+  int pieces;   // stretches the item is cut into
+  int first;    // CTA of the first of them
+};
+
+struct KeyRange {
+  int lo, hi;
+};
+// keys that query i takes part with; the queries are the last q_len positions of the request
+__device__ __forceinline__ KeyRange keys_of(int i, int q_len, int len, int causal, int window) {
+  const int p = len - q_len + i;
+  KeyRange r{0, len};
+  if (causal) r.hi = min(r.hi, p + 1);
+  if (window >= 0) r.lo = max(0, p - window), r.hi = min(r.hi, p + window + 1);
+  if (r.hi <= r.lo) r.lo = r.hi = 0;
+  return r;
+}
+// ... and any of queries i0 .. i1
+__device__ __forceinline__ KeyRange keys_of_any(int i0, int i1, int q_len, int len, int causal, int window) {
+  const int p0 = len - q_len + i0, p1 = len - q_len + i1;
+  KeyRange r{0, len};
+  if (causal) r.hi = min(r.hi, p1 + 1);
+  if (window >= 0) r.lo = max(0, p0 - window), r.hi = min(r.hi, p1 + window + 1);
+  if (r.hi <= r.lo) r.lo = r.hi = 0;
+  return r;
+}
+__device__ __forceinline__ int tiles_of(const KeyRange& r) { return r.hi > r.lo ? (r.hi + kTile - 1) / kTile - r.lo / kTile : 0; }
+
+struct Request {
+  int q_start, q_len, len;
+};
+__device__ __forceinline__ Request load_request(const PagedArgs& a, int b) {
+  long long q0 = load_offset(a.q_off, b, a.off64), q1 = load_offset(a.q_off, b + 1, a.off64);
+  q0 = clamp_ll(q0, 0, a.total_q);
+  q1 = clamp_ll(q1, q0, a.total_q);
+  const long long most = static_cast<long long>(a.table_width) << a.block_shift;
+  Request r;
+  r.q_start = static_cast<int>(q0);
+  r.q_len = static_cast<int>(min(q1 - q0, static_cast<long long>(a.max_q)));
+  r.len = static_cast<int>(clamp_ll(load_offset(a.seq_lens, b, a.lens64), 0, most));
+  return r;
+}
+
+// Units of one K / V head of a request: its row tiles' KV tiles, one at least each (a row tile without keys has zeros to write).
+template <int NMAX>
+__device__ __forceinline__ long long units_of(const PagedArgs& a, const Request& r) {
+  const int rows = r.q_len * a.group, nt = (rows + NMAX - 1) / NMAX;
+  if (!a.causal && a.window < 0) return static_cast<long long>(nt) * max(1, tiles_of(KeyRange{0, r.len}));
+  long long n = 0;
+  for (int t = 0; t < nt; ++t)
+    n += max(1, tiles_of(keys_of_any(t * NMAX / a.group, (min(rows, (t + 1) * NMAX) - 1) / a.group, r.q_len, r.len, a.causal, a.window)));
+  return n;
+}
+
+template <int ACT>
+__device__ __forceinline__ void act16(const float (&x)[16], float m, float (&p)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    // x/2 erfc(-x / sqrt 2): 1 + erf would cancel where x is well below zero, and a row's scale brings such a P up when it has no larger
+    if constexpr (ACT == ACT_GELU_ERF) p[i] = 0.5f * m * x[i] * erfcf(x[i] * -0.70710678118654752f);
+    else p[i] = act_scaled<ACT>(x[i], m, 0.5f * m);
+  }
+}
+// act(x) * m for a run-time activation class
+__device__ __forceinline__ void act16_any(int act, const float (&x)[16], float m, float (&p)[16]) {
+  switch (act) {
+    case ACT_GELU_ERF: act16<ACT_GELU_ERF>(x, m, p); break;
+    case ACT_GELU_TANH: act16<ACT_GELU_TANH>(x, m, p); break;
+    case ACT_LEAKY_RELU: act16<ACT_LEAKY_RELU>(x, m, p); break;
+    case ACT_RELU: act16<ACT_RELU>(x, m, p); break;
+    case ACT_SILU: act16<ACT_SILU>(x, m, p); break;
+    case ACT_HARDSWISH: act16<ACT_HARDSWISH>(x, m, p); break;
+    case ACT_RELU_SQUARE: act16<ACT_RELU_SQUARE>(x, m, p); break;
+    default: act16<ACT_RAW>(x, m, p); break;
+  }
+}
+
+// Four consecutive floats from shared memory, the same for all lanes.
+__device__ __forceinline__ void lds16(const float* s, float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 f = reinterpret_cast<const float4*>(s)[i];
+    v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+  }
+}
+
+#define PAGED_WAIT(bar_idx, parity, role)                                                                             \
+  {                                                                                                                   \
+    const bool ok_ = mbar_wait(bar_base + 8u * (bar_idx), (parity), abort_flag, a.status, ((bar_idx) << 8) | (role)); \
+    if (!__all_sync(kFull, ok_)) goto role_done;                                                                      \
+  }
+
+// The element-wise warps meet at barriers of their own, so none of them may leave alone: a wait that runs out is recorded (the abort
+// flag ends every later wait at once) and they go on, on whatever is there, to the end of the item, where they leave together.
+#define PAGED_WAIT_ON(bar_idx, parity)                                                                                       \
+  {                                                                                                                         \
+    (void)mbar_wait(bar_base + 8u * (bar_idx), (parity), abort_flag, a.status, ((bar_idx) << 8) | ST_ROLE_ACT);              \
+    __syncwarp();                                                                                                           \
+  }
+
+template <int D, int NMAX, bool SOFTMAX>
+__global__ void __launch_bounds__(PagedShape<D, NMAX>::kThreads, 1)
+gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PagedArgs a) {
+  using L = PagedShape<D, NMAX>;
+  constexpr int kGroups = L::kGroups;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t smem_base = smem_u32(smem);
+  const uint32_t bar_base = smem_base + L::kBarOff;
+  volatile uint32_t* const tmem_ptr = reinterpret_cast<volatile uint32_t*>(smem + L::kMiscOff);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
+  volatile int* const last_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 8);
+  const int warp = warp_uniform(threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::B_COUNT; ++i) {
+      uint32_t n = 1;
+      if (i >= L::B_SC_FULL && i < L::B_SC_FULL + L::kStages) n = 32;
+      if (i == L::B_P_FULL) n = 128 * kGroups;
+      if (i >= L::B_Q_FULL && i < L::B_Q_FULL + 2) n = 64;
+      if (i >= L::B_Q_EMPTY && i < L::B_Q_EMPTY + 2) n = 1 + 4 * kGroups;
+      if (i >= L::B_ITEM_EMPTY && i < L::B_ITEM_EMPTY + kItemSlots) n = 3 + 4 * kGroups;
+      mbar_init(bar_base + 8u * i, n);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == L::kMmaWarp) {
+    tmem_alloc(smem_base + L::kMiscOff, L::kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == L::kLoadWarp && lane == 0) {
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  // Where this CTA begins: every CTA sums the units of all requests (a run of them per thread) and looks for its own first one.
+  long long* const scan = reinterpret_cast<long long*>(smem + L::kScanOff);
+  struct Start {
+    long long all, before;  // all units; units before request b
+    int b;
+  };
+  Start* const start = reinterpret_cast<Start*>(scan + 32);
+  {
+    const int per = (a.batch + L::kThreads - 1) / L::kThreads;
+    const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
+    long long sum = 0;
+    for (int b = b0; b < b1; ++b) sum += units_of<NMAX>(a, load_request(a, b)) * a.kv_heads;
+    long long incl = sum;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const long long o = __shfl_up_sync(kFull, incl, s);
+      if (lane >= s) incl += o;
+    }
+    if (lane == 31) scan[warp] = incl;
+    if (threadIdx.x == 0) *start = Start{0, 0, a.batch};
+    __syncthreads();
+    long long all = 0, before = 0;
+    for (int w = 0; w < L::kWarps; ++w) {
+      before += w < warp ? scan[w] : 0;
+      all += scan[w];
+    }
+    if (threadIdx.x == 0) start->all = all;
+    const long long ctas = min(static_cast<long long>(gridDim.x), all);
+    if (blockIdx.x < ctas) {
+      const long long u0 = all * blockIdx.x / ctas;
+      long long at = before + incl - sum;
+      if (u0 >= at && u0 < at + sum) {
+        for (int b = b0; b < b1; ++b) {
+          const long long n = units_of<NMAX>(a, load_request(a, b)) * a.kv_heads;
+          if (u0 < at + n) {
+            start->before = at, start->b = b;
+            break;
+          }
+          at += n;
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = warp_uniform(*tmem_ptr);
+  const long long all_units = start->all;
+  const long long ctas = min(static_cast<long long>(gridDim.x), all_units);
+
+  int* const ring = reinterpret_cast<int*>(smem + L::kRingOff);
+  uint32_t item_pos = 0;  // items this role has taken
+  [[maybe_unused]] uint32_t loaded = 0;  // the loader: tiles asked for
+  auto take_item = [&](int role) -> PagedItem {
+    const uint32_t slot = item_pos % kItemSlots, parity = (item_pos / kItemSlots) & 1u;
+    ++item_pos;
+    PagedItem it;
+    it.h = -2;
+    const bool ok = mbar_wait(bar_base + 8u * (L::B_ITEM_FULL + slot), parity, abort_flag, a.status, ((L::B_ITEM_FULL + slot) << 8) | role);
+    if (!__all_sync(kFull, ok)) return it;
+    const int4* const r = reinterpret_cast<const int4*>(ring + slot * 16);
+    const int4 x = r[0], y = r[1], z = r[2];
+    it = PagedItem{warp_uniform(x.x), warp_uniform(x.y), warp_uniform(x.z), warp_uniform(x.w), warp_uniform(y.x), warp_uniform(y.y),
+                   warp_uniform(y.z), warp_uniform(y.w), warp_uniform(z.x), warp_uniform(z.y), warp_uniform(z.z), warp_uniform(z.w)};
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar_base + 8u * (L::B_ITEM_EMPTY + slot));
+    return it;
+  };
+
+  if (warp == L::kLoadWarp) {
+    // ------------------------------------------------------------------ TMA loader, and the walk over the items
+    auto publish = [&](const PagedItem& it) -> bool {
+      const uint32_t slot = item_pos % kItemSlots, parity = (item_pos / kItemSlots) & 1u;
+      const bool ok = mbar_wait(bar_base + 8u * (L::B_ITEM_EMPTY + slot), parity ^ 1u, abort_flag, a.status,
+                                ((L::B_ITEM_EMPTY + slot) << 8) | ST_ROLE_LOAD);
+      if (!__all_sync(kFull, ok)) return false;
+      if (lane == 0) {
+        int4* const r = reinterpret_cast<int4*>(ring + slot * 16);
+        r[0] = make_int4(it.h, it.q_start, it.q_len, it.row0);
+        r[1] = make_int4(it.rows, it.len, it.lo, it.hi);
+        r[2] = make_int4(it.tile0, it.tiles, it.pieces, it.first);
+        mbar_arrive(bar_base + 8u * (L::B_ITEM_FULL + slot));
+      }
+      ++item_pos;
+      return true;
+    };
+    const int per_tile = kTile >> a.block_shift;  // blocks of a tile
+    const int block_size = 1 << a.block_shift;
+    uint32_t pos = 0;                             // tiles before this one
+    if (blockIdx.x < ctas) {
+      const long long u0 = all_units * blockIdx.x / ctas, u1 = all_units * (blockIdx.x + 1) / ctas;
+      long long at = start->before;  // units before the item
+      for (int b = start->b; b < a.batch && at < u1; ++b) {
+        const Request rq = load_request(a, b);
+        const int rows = rq.q_len * a.group, nt = (rows + NMAX - 1) / NMAX;
+        const int n_blocks = min((rq.len + block_size - 1) >> a.block_shift, a.table_width);
+        const int* const table = a.block_tables + static_cast<long long>(b) * a.table_stride;
+        for (int h = 0; h < a.kv_heads && at < u1; ++h) {
+          for (int t = 0; t < nt && at < u1; ++t) {
+            PagedItem it;
+            it.h = h, it.q_start = rq.q_start, it.q_len = rq.q_len, it.len = rq.len;
+            it.row0 = t * NMAX;
+            it.rows = min(NMAX, rows - it.row0);
+            const KeyRange r = keys_of_any(it.row0 / a.group, (it.row0 + it.rows - 1) / a.group, rq.q_len, rq.len, a.causal, a.window);
+            it.lo = r.lo, it.hi = r.hi;
+            const int n = tiles_of(r);
+            const long long units = max(1, n);
+            const long long s = at;
+            at += units;
+            if (at <= u0) continue;
+            const int skip = static_cast<int>(max(u0 - s, 0ll));
+            it.tile0 = r.lo / kTile + skip;
+            it.tiles = n == 0 ? 0 : static_cast<int>(min(u1 - s, units)) - skip;
+            // the CTA that has unit u is the largest c with all * c / ctas <= u
+            it.first = static_cast<int>(((s + 1) * ctas - 1) / all_units);
+            it.pieces = static_cast<int>(((s + units) * ctas - 1) / all_units) - it.first + 1;
+            if (!publish(it)) goto role_done;
+            int cached = 0, cached_at = -1;  // 32 entries of the table, from entry cached_at on
+            for (int j = 0; j < it.tiles; ++j, ++pos) {
+              const uint32_t stage = pos % L::kStages;
+              const int p0 = (it.tile0 + j) * per_tile;
+              if (cached_at < 0 || p0 + per_tile > cached_at + 32) {
+                cached_at = p0;
+                cached = cached_at + lane < n_blocks ? table[cached_at + lane] : -1;
+              }
+              const int blk = __shfl_sync(kFull, cached, (p0 - cached_at + lane) & 31);
+              const bool valid = lane < per_tile && p0 + lane < n_blocks && blk >= 0 && blk < a.num_blocks;
+              PAGED_WAIT(L::B_KV_EMPTY + stage, ((pos / L::kStages) & 1u) ^ 1u, ST_ROLE_LOAD);
+              const uint32_t bar = bar_base + 8u * (L::B_KV_FULL + stage);
+              const unsigned n_valid = __popc(__ballot_sync(kFull, valid));
+              if (lane == 0) mbar_arrive_expect_tx(bar, n_valid * block_size * D * 2);
+              __syncwarp();
+              const uint32_t dst = smem_base + L::kKvOff + stage * 2 * L::kTileBytes + lane * block_size * D;
+              if (valid) {
+                tma_load_4d(dst, &tm_k, bar, 0, 0, h, blk);
+                tma_load_4d(dst + L::kTileBytes, &tm_v, bar, 0, 0, h, blk);
+              }
+              // a block that is not there has scale 0, which tells the others
+              if (lane < per_tile) {
+                const uint32_t sc = smem_base + L::kScaleOff + stage * 64 + lane * 4;
+                const long long si = valid ? static_cast<long long>(blk) * a.kv_heads + h : 0;
+                cp_async4(sc, a.k_scales + si, valid);
+                cp_async4(sc + 32, a.v_scales + si, valid);
+              }
+              cp_async_mbar_arrive(bar_base + 8u * (L::B_SC_FULL + stage));
+              loaded = pos + 1;
+            }
+          }
+        }
+      }
+    }
+    PagedItem end{};
+    end.h = -1;
+    if (!publish(end)) goto role_done;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == L::kMmaWarp) {
+    // ------------------------------------------------------------------ MMA issuer
+    constexpr int kSwizzle = D == 128 ? 128 : 64;
+    // K: rows of D bytes, K-major, eight rows after eight rows; V: the same bytes, MN-major (with 64 columns the second half of the
+    // MMA's 128 rows repeats the first: its lanes of O are not read).
+    const uint64_t dk0 = umma_smem_desc(smem_base + L::kKvOff, 16, 8 * D, kSwizzle);
+    const uint64_t dv0 = umma_smem_desc(smem_base + L::kKvOff + L::kTileBytes, 0, 8 * D, kSwizzle);
+    const uint64_t dq0 = umma_smem_desc(smem_base + L::kQOff, 16, 8 * D, kSwizzle);
+    const uint64_t dp0 = umma_smem_desc(smem_base + L::kPOff, 128, 16 * kTile, 0);
+    uint32_t pos = 0, q_pos = 0, pv_pos = 0;
+    struct {
+      int n16;
+      uint32_t stage;
+      bool accumulate, any;
+    } owed{0, 0, false, false};  // the tile whose P V has not been issued
+    auto issue_pv = [&]() -> bool {
+      const bool ok = mbar_wait(bar_base + 8u * L::B_P_FULL, pv_pos & 1u, abort_flag, a.status, (L::B_P_FULL << 8) | ST_ROLE_MMA);
+      if (!__all_sync(kFull, ok)) return false;
+      ++pv_pos;
+      tc_fence_after();
+      const uint32_t idesc = umma_idesc(0, 0, 1, 1, kTile, 16 * owed.n16);
+      const uint64_t dv = umma_desc_advance(dv0, owed.stage * 2 * L::kTileBytes);
+#pragma unroll
+      for (int kk = 0; kk < kTile / 32; ++kk) {
+        const uint64_t dvk = umma_desc_advance(dv, kk * 32 * D);
+        umma_ss_f8(tmem_base + 2 * NMAX, dvk, umma_desc_advance(dp0, kk * 512), idesc, owed.accumulate || kk > 0 ? 1u : 0u);
+        umma_ss_f8(tmem_base + 2 * NMAX, dvk, umma_desc_advance(dp0, L::kPBytes + kk * 512), idesc, 1u);
+      }
+      tc_commit(bar_base + 8u * (L::B_KV_EMPTY + owed.stage));
+      tc_commit(bar_base + 8u * L::B_PV_DONE);
+      owed.any = false;
+      return true;
+    };
+    while (true) {
+      const PagedItem it = take_item(ST_ROLE_MMA);
+      if (it.h < 0) {
+        if (it.h == -2) goto role_done;
+        break;
+      }
+      if (it.tiles == 0) continue;
+      const int n16 = (it.rows + 15) / 16;
+      const uint32_t q_buf = q_pos & 1u;
+      PAGED_WAIT(L::B_Q_FULL + q_buf, (q_pos >> 1) & 1u, ST_ROLE_MMA);
+      ++q_pos;
+      const uint32_t idesc = umma_idesc(0, 0, 0, 0, kTile, 16 * n16);
+      const uint64_t dq = umma_desc_advance(dq0, q_buf * 2 * L::kQBytes);
+      for (int j = 0; j < it.tiles; ++j, ++pos) {
+        const uint32_t stage = pos % L::kStages;
+        PAGED_WAIT(L::B_KV_FULL + stage, (pos / L::kStages) & 1u, ST_ROLE_MMA);
+        tc_fence_after();
+        const uint64_t dk = umma_desc_advance(dk0, stage * 2 * L::kTileBytes);
+        const uint32_t s_tmem = tmem_base + (pos & 1u) * NMAX;
+#pragma unroll
+        for (int kk = 0; kk < D / 32; ++kk) {
+          umma_ss_f8(s_tmem, umma_desc_advance(dk, kk * 32), umma_desc_advance(dq, kk * 32), idesc, kk > 0 ? 1u : 0u);
+          umma_ss_f8(s_tmem, umma_desc_advance(dk, kk * 32), umma_desc_advance(dq, L::kQBytes + kk * 32), idesc, 1u);
+        }
+        tc_commit(bar_base + 8u * (L::B_S_FULL + (pos & 1u)));
+        if (j + 1 == it.tiles) tc_commit(bar_base + 8u * (L::B_Q_EMPTY + q_buf));
+        if (owed.any && !issue_pv()) goto role_done;
+        owed = {n16, stage, j > 0, true};
+      }
+    }
+    if (owed.any && !issue_pv()) goto role_done;
+  } else if (warp >= L::kQWarp) {
+    // ------------------------------------------------------------------ Q: fetched, scaled, split in two
+    constexpr int kLanes = D / 8;  // lanes of one row, 16 bytes each
+    constexpr int kRowsAt = 32 / kLanes;
+    const int wq = warp - L::kQWarp;
+    uint32_t q_pos = 0;
+    while (true) {
+      const PagedItem it = take_item(ST_ROLE_LOAD);
+      if (it.h < 0) {
+        if (it.h == -2) goto role_done;
+        break;
+      }
+      if (it.tiles == 0) continue;
+      const uint32_t q_buf = q_pos & 1u;
+      PAGED_WAIT(L::B_Q_EMPTY + q_buf, ((q_pos >> 1) & 1u) ^ 1u, ST_ROLE_LOAD);
+      ++q_pos;
+      uint8_t* const hi = smem + L::kQOff + q_buf * 2 * L::kQBytes;
+      float* const qa = reinterpret_cast<float*>(smem + L::kQaOff) + q_buf * NMAX;
+      const int n = (it.rows + 15) / 16 * 16;
+      const int c8 = lane % kLanes;
+      constexpr int kAhead = 4;
+      for (int r0 = wq * kRowsAt + lane / kLanes; r0 - lane / kLanes < n; r0 += 2 * kRowsAt * kAhead) {
+        uint4 u[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int r = r0 + i * 2 * kRowsAt, g = it.row0 + r;
+          u[i] = make_uint4(0, 0, 0, 0);
+          if (r < it.rows)
+            u[i] = *reinterpret_cast<const uint4*>(a.q + (it.q_start + static_cast<long long>(g / a.group)) * a.q_strides[0] +
+                                                   (it.h * a.group + g % a.group) * a.q_strides[1] + c8 * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int r = r0 + i * 2 * kRowsAt;
+          const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+          uint32_t top = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = max_u16x2(top, w[e] & 0x7fff7fffu);
+          top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+          for (int s = kLanes / 2; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(kFull, top, s));
+          // 2^k with amax / 2^k in (224, 448]; a row that is not finite gives NaN
+          const bool finite = top < 0x7f80u;
+          int k = static_cast<int>(top >> 7) - 127 - 8 + ((top & 0x7fu) > 0x60u ? 1 : 0);
+          k = max(k, -100);
+          const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+          uint32_t w_hi[2], w_lo[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x[4];
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+              x[2 * f] = finite ? __uint_as_float(w[2 * e + f] << 16) * inv : 0.f;
+              x[2 * f + 1] = finite ? __uint_as_float(w[2 * e + f] & 0xffff0000u) * inv : 0.f;
+            }
+            w_hi[e] = w_lo[e] = 0;
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+              const uint32_t h = pack_f16x2(x[2 * f], x[2 * f + 1]);  // exact but for what lies 2^-24 below
+              const uint16_t eh = e4m3x2_from_f16x2(h);
+              const uint16_t el = e4m3x2_from_f16x2(sub_f16x2(h, f16x2_from_e4m3x2(eh)));
+              w_hi[e] |= static_cast<uint32_t>(eh) << (16 * f);
+              w_lo[e] |= static_cast<uint32_t>(el) << (16 * f);
+            }
+          }
+          if (r < n) {
+            // 16-byte pieces of a row change places with its number, as the tensor cores read them (128- or 64-byte swizzle)
+            const int piece = D == 128 ? (c8 >> 1) ^ (r & 7) : (c8 >> 1) ^ ((r >> 1) & 3);
+            uint8_t* const p = hi + r * D + piece * 16 + (c8 & 1) * 8;
+            *reinterpret_cast<uint2*>(p) = make_uint2(w_hi[0], w_hi[1]);
+            *reinterpret_cast<uint2*>(p + L::kQBytes) = make_uint2(w_lo[0], w_lo[1]);
+            if (c8 == 0) {
+              const float s = __uint_as_float(static_cast<uint32_t>(k + 127) << 23) * (SOFTMAX ? a.scale * 1.4426950408889634f : 1.f);
+              qa[r] = finite ? s : __uint_as_float(0x7fffffffu);
+            }
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(bar_base + 8u * (L::B_Q_FULL + q_buf));
+    }
+  } else {
+    // ------------------------------------------------------------------ element-wise work and epilogue
+    constexpr int kSets = NMAX / 32 / kGroups;  // groups of 32 columns of this warpgroup
+    constexpr float kHeadroom = (L::kTarget == 256.f ? 0.8073549f : 2.8073549f) + 0.001f;  // log2(448 / kTarget)
+    static_assert(L::kTarget == 256.f || L::kTarget == 64.f, "kHeadroom");
+    const int wg = warp >> 2, tid = threadIdx.x & 127, quarter = warp & 3;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t o_tmem = tmem_base + 2 * NMAX + lane_base;
+    float* const ref = reinterpret_cast<float*>(smem + L::kRefOff);
+    float* const fac = reinterpret_cast<float*>(smem + L::kFacOff);
+    float* const red = reinterpret_cast<float*>(smem + L::kRedOff);
+    int2* const range = reinterpret_cast<int2*>(smem + L::kRangeOff);
+    const int bar_wg = 1 + wg;
+    uint32_t pos = 0, q_pos = 0;  // tiles, items with tiles
+    float l[kSets][32];
+    while (true) {
+      const PagedItem it = take_item(ST_ROLE_ACT);
+      if (named_bar_or(3, 128 * kGroups, it.h < 0)) break;
+      const int n16 = (it.rows + 15) / 16;
+      if (it.tiles == 0) {
+        // no row of the tile has a key
+        for (int i = threadIdx.x; i < it.rows * D / 2; i += 128 * kGroups) {
+          const int g = it.row0 + i / (D / 2);
+          reinterpret_cast<uint32_t*>(a.o + ((it.q_start + static_cast<long long>(g / a.group)) * a.heads + it.h * a.group + g % a.group) * D)[i % (D / 2)] = 0u;
+        }
+        continue;
+      }
+      const uint32_t q_buf = q_pos & 1u;
+      const float* const qa = reinterpret_cast<const float*>(smem + L::kQaOff) + q_buf * NMAX;
+      // the columns of this warpgroup: sets wg, wg + kGroups, ... of 32
+      if (tid < NMAX && (tid >> 5) % kGroups == wg) {
+        const int g = it.row0 + tid;
+        const KeyRange r = tid < it.rows ? keys_of(g / a.group, it.q_len, it.len, a.causal, a.window) : KeyRange{0, 0};
+        range[tid] = make_int2(r.lo, r.hi);
+        ref[tid] = SOFTMAX ? kNoMax : 1.f;
+      }
+#pragma unroll
+      for (int s = 0; s < kSets; ++s)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) l[s][i] = 0.f;
+      const int i0 = it.row0 / a.group, i1 = (it.row0 + it.rows - 1) / a.group;
+      const KeyRange r0 = keys_of(i0, it.q_len, it.len, a.causal, a.window), r1 = keys_of(i1, it.q_len, it.len, a.causal, a.window);
+      const int all_lo = max(r0.lo, r1.lo), all_hi = min(r0.hi, r1.hi);  // keys that every row takes part with (if any)
+      named_bar_sync(bar_wg, 128);
+      PAGED_WAIT_ON(L::B_Q_FULL + q_buf, (q_pos >> 1) & 1u);
+      ++q_pos;
+      for (int j = 0; j < it.tiles; ++j, ++pos) {
+        const uint32_t stage = pos % L::kStages, phase = (pos / L::kStages) & 1u;
+        const int key0 = (it.tile0 + j) * kTile, key = key0 + tid;
+        const bool first = j == 0;
+        PAGED_WAIT_ON(L::B_SC_FULL + stage, phase);
+        const float* const sc = reinterpret_cast<const float*>(smem + L::kScaleOff) + stage * 16 + (tid >> a.block_shift);
+        const float ks = sc[0];
+        float vs = sc[8];
+        const bool out = key < it.lo || key >= it.hi || vs == 0.f;  // no row takes part with this token
+        vs = fmaxf(vs, kLeastScale);
+        const bool every = key0 >= all_lo && key0 + kTile <= all_hi;  // the tile needs no mask but that of `out`
+        const bool masked = !every || __any_sync(kFull, out);
+        PAGED_WAIT_ON(L::B_S_FULL + (pos & 1u), (pos >> 1) & 1u);
+        tc_fence_after();
+        bool poisoned = false;
+        if (masked) {
+          // P of a token that takes no part is 0, and 0 times what its V row holds (an unused row, NaN) has to be 0
+          PAGED_WAIT_ON(L::B_KV_FULL + stage, phase);
+          uint4* const v_row = reinterpret_cast<uint4*>(smem + L::kKvOff + (2 * stage + 1) * L::kTileBytes + tid * D);
+          if (!every && !out) {
+            // some row may take part and some not: a NaN goes into P of those that do
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              const uint4 u = v_row[i];
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) poisoned |= __vcmpeq4(w[e] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0u;
+            }
+          }
+          if (kGroups > 1 && !every) named_bar_sync(3, 128 * kGroups);  // both warpgroups have looked
+          if (wg == 0 && (out || poisoned)) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) v_row[i] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        bool pv_waited = false;
+#pragma unroll
+        for (int s = 0; s < kSets; ++s) {
+          const int c0 = (s * kGroups + wg) * 32;  // first column
+          const int chunks = min(2, n16 - c0 / 16);
+          if (chunks <= 0) continue;
+          const uint32_t s_tmem = tmem_base + (pos & 1u) * NMAX + lane_base + c0;
+          float p[32];
+          // P of the chunks, for the reference the rows have now; whether it fits e4m3
+          auto compute = [&]() -> bool {
+            float most = 0.f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              if (c < chunks) {
+                uint32_t raw[16];
+                tmem_ld16(s_tmem + c * 16, raw);
+                float f[16], x[16], rf[16];
+                lds16(qa + c0 + c * 16, f);
+                lds16(ref + c0 + c * 16, rf);
+                tmem_wait_ld();
+                tmem_regs_ready(raw);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(raw[i]) * (f[i] * ks);
+                if constexpr (SOFTMAX) {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) p[c * 16 + i] = ex2_approx(x[i] - rf[i]);
+                } else {
+                  float q[16];
+                  act16_any(a.act, x, a.scale, q);
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) p[c * 16 + i] = q[i] * rf[i];
+                }
+                if (masked) {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) {
+                    const int2 rg = range[c0 + c * 16 + i];
+                    const bool in = !out && key >= rg.x && key < rg.y;
+                    p[c * 16 + i] = in ? (poisoned ? __uint_as_float(0x7fffffffu) : p[c * 16 + i]) : 0.f;
+                  }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(p[c * 16 + i]));
+              }
+            }
+            return most * (vs * (SOFTMAX ? L::kTarget : 1.f)) <= kMax8;
+          };
+          const bool fits = compute();
+          if (named_bar_or(bar_wg, 128, first || !fits)) {
+            // the exact reference of every column, and O and the row sums moved to it
+            if (!pv_waited && pos > 0) {
+              PAGED_WAIT_ON(L::B_PV_DONE, (pos - 1) & 1u);
+              tc_fence_after();
+            }
+            pv_waited = true;
+            const float lv = SOFTMAX ? log2f(vs) : 0.f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              if (c < chunks) {
+                uint32_t raw[16];
+                tmem_ld16(s_tmem + c * 16, raw);
+                float f[16], x[16];
+                lds16(qa + c0 + c * 16, f);
+                tmem_wait_ld();
+                tmem_regs_ready(raw);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(raw[i]) * (f[i] * ks);
+                float u[16];
+                if constexpr (SOFTMAX) {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) u[i] = x[i] + lv;
+                } else {
+                  act16_any(a.act, x, a.scale, u);
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) u[i] = fabsf(u[i]) * vs;
+                }
+                float keep = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const int2 rg = range[c0 + c * 16 + i];
+                  const bool in = !masked || (!out && key >= rg.x && key < rg.y);
+                  const float m = warp_max(in ? u[i] : (SOFTMAX ? kNoMax : 0.f));
+                  keep = lane == i ? m : keep;
+                }
+                if (lane < 16) red[quarter * NMAX + c0 + c * 16 + lane] = keep;
+              }
+            }
+            named_bar_sync(bar_wg, 128);
+            if (tid < 16 * chunks) {
+              const int n = c0 + tid;
+              const float m = fmaxf(fmaxf(red[n], red[NMAX + n]), fmaxf(red[2 * NMAX + n], red[3 * NMAX + n]));
+              const float old = ref[n];
+              // a column that fits keeps its reference: no row's bits depend on another row's values (the margin of 2^-10 keeps the
+              // two ways to say that one does not fit from differing)
+              if constexpr (SOFTMAX) {
+                const float now = first || m - old > kHeadroom ? fmaxf(old, fminf(m, 3.0e38f)) : old;
+                fac[n] = first ? 0.f : ex2_approx(old - now);
+                ref[n] = now;
+              } else {
+                // the largest power of two that keeps |P| V's scale at or below the target; 2^100 for a row of zeros
+                float now = 1.2676506e30f;
+                if (m > 0.f) now = exp2f(fminf(fmaxf(floorf(log2f(L::kTarget / m)), -100.f), 100.f));
+                if (!first) now = m * old > kMax8 * 1.001f ? fminf(now, old) : old;
+                fac[n] = first ? 0.f : now / old;
+                ref[n] = now;
+              }
+            }
+            named_bar_sync(bar_wg, 128);
+            if (!first) {
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                if (c < chunks) {
+                  float f[16];
+                  lds16(fac + c0 + c * 16, f);
+                  uint32_t raw[16];
+                  tmem_ld16(o_tmem + c0 + c * 16, raw);
+                  tmem_wait_ld();
+                  tmem_regs_ready(raw);
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) raw[i] = __float_as_uint(__uint_as_float(raw[i]) * f[i]);
+                  tmem_st16(o_tmem + c0 + c * 16, raw);
+                  tmem_wait_st();
+                  if constexpr (SOFTMAX) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) l[s][c * 16 + i] *= f[i];
+                  }
+                }
+              }
+            }
+            compute();
+          }
+          if (!pv_waited && pos > 0) {
+            PAGED_WAIT_ON(L::B_PV_DONE, (pos - 1) & 1u);  // P's buffer is free
+            pv_waited = true;
+          }
+          // P, times V's scale, as the sum of two e4m3 values
+          const float m = vs * (SOFTMAX ? L::kTarget : 1.f);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            if (c < chunks) {
+              uint32_t w_hi[4] = {0, 0, 0, 0}, w_lo[4] = {0, 0, 0, 0};
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float x0 = p[c * 16 + 2 * i], x1 = p[c * 16 + 2 * i + 1];
+                if constexpr (SOFTMAX) l[s][c * 16 + 2 * i] += x0, l[s][c * 16 + 2 * i + 1] += x1;
+                const uint32_t h = pack_f16x2(x0 * m, x1 * m);
+                const uint16_t eh = e4m3x2_from_f16x2(h);
+                const uint16_t el = e4m3x2_from_f16x2(sub_f16x2(h, f16x2_from_e4m3x2(eh)));
+                w_hi[i >> 1] |= static_cast<uint32_t>(eh) << (16 * (i & 1));
+                w_lo[i >> 1] |= static_cast<uint32_t>(el) << (16 * (i & 1));
+              }
+              uint8_t* const dst = smem + L::kPOff + (c0 / 16 + c) * 16 * kTile + tid * 16;
+              *reinterpret_cast<uint4*>(dst) = make_uint4(w_hi[0], w_hi[1], w_hi[2], w_hi[3]);
+              *reinterpret_cast<uint4*>(dst + L::kPBytes) = make_uint4(w_lo[0], w_lo[1], w_lo[2], w_lo[3]);
+            }
+          }
+        }
+        // (a warpgroup without columns waits too: its arrival for the next tile must not count for this one)
+        if (!pv_waited && pos > 0) PAGED_WAIT_ON(L::B_PV_DONE, (pos - 1) & 1u);
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(bar_base + 8u * L::B_P_FULL);
+      }
+      // ---- the end of the stretch: row sums over the 128 tokens' threads, then O
+      if (lane == 0) mbar_arrive(bar_base + 8u * (L::B_Q_EMPTY + q_buf));
+      if constexpr (SOFTMAX) {
+#pragma unroll
+        for (int s = 0; s < kSets; ++s) {
+          const int c0 = (s * kGroups + wg) * 32;
+          if (c0 < 16 * n16) {
+            // 32 columns over 32 lanes: halves change places until lane i has the sum of column i
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) {
+              const bool upper = lane & w;
+#pragma unroll
+              for (int i = 0; i < w; ++i) {
+                const float mine = upper ? l[s][i + w] : l[s][i], other = upper ? l[s][i] : l[s][i + w];
+                l[s][i] = mine + __shfl_xor_sync(kFull, other, w);
+              }
+            }
+            red[quarter * NMAX + c0 + lane] = l[s][0];
+          }
+        }
+      }
+      PAGED_WAIT_ON(L::B_PV_DONE, (pos - 1) & 1u);
+      tc_fence_after();
+      named_bar_sync(bar_wg, 128);
+      const bool cut = it.pieces > 1;
+      const int part = 2 * blockIdx.x + (static_cast<int>(blockIdx.x) == it.first ? 1 : 0);
+      if (tid < NMAX && (tid >> 5) % kGroups == wg && tid < it.rows) {
+        const float sum = SOFTMAX ? red[tid] + red[NMAX + tid] + red[2 * NMAX + tid] + red[3 * NMAX + tid] : 1.f;
+        if (cut) {
+          float* const ml = a.part_ml + static_cast<long long>(part) * 2 * NMAX;
+          ml[tid] = ref[tid];
+          ml[NMAX + tid] = sum;
+          fac[tid] = SOFTMAX ? 1.f / L::kTarget : 1.f / ref[tid];
+        } else {
+          fac[tid] = SOFTMAX ? (sum > 0.f || sum != sum ? 1.f / (sum * L::kTarget) : 0.f) : 1.f / ref[tid];
+        }
+      }
+      named_bar_sync(bar_wg, 128);
+#pragma unroll
+      for (int s = 0; s < kSets; ++s) {
+        const int c0 = (s * kGroups + wg) * 32;
+        const int chunks = min(2, n16 - c0 / 16);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (c < chunks) {
+            uint32_t raw[16];
+            tmem_ld16(o_tmem + c0 + c * 16, raw);
+            float f[16];
+            lds16(fac + c0 + c * 16, f);
+            tmem_wait_ld();
+            tmem_regs_ready(raw);
+            if (tid < D) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int r = c0 + c * 16 + i;
+                if (r < it.rows) {
+                  const float v = __uint_as_float(raw[i]) * f[i];
+                  if (cut) {
+                    a.part_o[(static_cast<long long>(part) * NMAX + r) * D + tid] = v;
+                  } else {
+                    const int g = it.row0 + r;
+                    a.o[((it.q_start + static_cast<long long>(g / a.group)) * a.heads + it.h * a.group + g % a.group) * D + tid] = __float2bfloat16_rn(v);
+                  }
+                }
+              }
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      if (cut) {
+        // the last of the item's CTAs joins the pieces
+        __threadfence();
+        named_bar_sync(3, 128 * kGroups);
+        if (threadIdx.x == 0) {
+          const bool last = atomicAdd(a.counters + it.first, 1) == it.pieces - 1;
+          __threadfence();
+          *last_flag = last;
+        }
+        named_bar_sync(3, 128 * kGroups);
+        if (*last_flag) {
+          // a warp has a row: the weights of its pieces over the lanes, then the pieces in order
+          for (int r = warp; r < it.rows; r += 4 * kGroups) {
+            const int g = it.row0 + r;
+            constexpr int V = D / 32;
+            float acc[V], m_all = kNoMax, l_all = 0.f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] = 0.f;
+            auto slot_of = [&](int k) { return static_cast<long long>(2 * (it.first + k) + (k == 0 ? 1 : 0)); };
+            if constexpr (SOFTMAX) {
+              for (int k0 = 0; k0 < it.pieces; k0 += 32) {
+                const int k = k0 + lane;
+                m_all = fmaxf(m_all, warp_max(k < it.pieces ? __ldcg(a.part_ml + slot_of(k) * 2 * NMAX + r) : kNoMax));
+              }
+            }
+            for (int k0 = 0; k0 < it.pieces; k0 += 32) {
+              const int k = k0 + lane;
+              float w = 0.f;
+              if (k < it.pieces) {
+                const float* const ml = a.part_ml + slot_of(k) * 2 * NMAX;
+                w = SOFTMAX ? ex2_approx(__ldcg(ml + r) - m_all) : 1.f;
+                if constexpr (SOFTMAX) l_all += w * __ldcg(ml + NMAX + r);
+              }
+              const int n = min(32, it.pieces - k0);
+#pragma unroll 8
+              for (int i = 0; i < n; ++i) {
+                const float wi = __shfl_sync(kFull, w, i);
+                const float* const po = a.part_o + (slot_of(k0 + i) * NMAX + r) * D + lane * V;
+                float v[V];
+                if constexpr (V == 4) {
+                  const float4 x = __ldcg(reinterpret_cast<const float4*>(po));
+                  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+                } else {
+                  const float2 x = __ldcg(reinterpret_cast<const float2*>(po));
+                  v[0] = x.x, v[1] = x.y;
+                }
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[e] = fmaf(wi, v[e], acc[e]);
+              }
+            }
+            float inv = 1.f;
+            if constexpr (SOFTMAX) {
+#pragma unroll
+              for (int s = 16; s > 0; s >>= 1) l_all += __shfl_xor_sync(kFull, l_all, s);
+              inv = l_all > 0.f || l_all != l_all ? 1.f / l_all : 0.f;
+            }
+            uint32_t* const dst = reinterpret_cast<uint32_t*>(
+                a.o + ((it.q_start + static_cast<long long>(g / a.group)) * a.heads + it.h * a.group + g % a.group) * D + lane * V);
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) dst[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+          }
+        }
+      }
+    }
+  }
+role_done:
+  __syncwarp();
+  if (warp == L::kLoadWarp && *abort_flag != 0) {
+    // after a wait that ran out: not before this CTA's own copies have landed (again with a limit)
+    const uint64_t t0 = global_timer_ns();
+    for (uint32_t k = loaded > L::kStages ? loaded - L::kStages : 0; k < loaded; ++k)
+      while (!mbar_try_wait(bar_base + 8u * (L::B_KV_FULL + k % L::kStages), (k / L::kStages) & 1u) && global_timer_ns() - t0 < kWaitLimitNs) {
+      }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == L::kMmaWarp) tmem_dealloc(tmem_base, L::kTmemCols);
+}
+
+template <int D, int NMAX>
+int launch(const PagedLaunch& l) {
+  using L = PagedShape<D, NMAX>;
+  auto go = [&](auto kernel) -> int {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynBytes) != cudaSuccess) return GDPA_ERR_LAUNCH_;
+    kernel<<<l.grid, L::kThreads, L::kDynBytes, l.stream>>>(l.tm_k, l.tm_v, l.args);
+    return cudaGetLastError() == cudaSuccess ? 0 : GDPA_ERR_LAUNCH_;
+  };
+  return l.args.act == ACT_SOFTMAX ? go(gdpa_paged_kernel<D, NMAX, true>) : go(gdpa_paged_kernel<D, NMAX, false>);
+}
+
+}  // namespace
+
+int launch_paged(const PagedLaunch& l, int head_dim) {
+  if (l.rows == kPagedRowsSmall) return head_dim == 128 ? launch<128, kPagedRowsSmall>(l) : launch<64, kPagedRowsSmall>(l);
+  return head_dim == 128 ? launch<128, kPagedRowsLarge>(l) : launch<64, kPagedRowsLarge>(l);
+}
+
+}  // namespace gdpa

@@ -12,5 +12,11 @@ from .ops import (  # noqa: F401
     quantize_fp8_blockwise,
     set_offset_validation,
 )
+from .paged import (  # noqa: F401
+    PagedKVCache,
+    append_kv_cache_fp8,
+    build_block_tables,
+    generalized_dot_product_attention_paged_fp8,
+)
 from .sharding import gather_rows, max_over_ranks, plan_token_balanced_shards, shard_inputs, shard_jagged  # noqa: F401
 from .workloads import WORKLOADS, make_workload, useful_flops  # noqa: F401

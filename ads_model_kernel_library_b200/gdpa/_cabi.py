@@ -35,6 +35,10 @@ EXPORTS = (
     "gdpa_quantize_fp8_blockwise",
     "gdpa_quantize_mxfp8",
     "gdpa_dequantize_mxfp8",
+    "gdpa_build_block_tables",
+    "gdpa_append_kv_cache_fp8",
+    "gdpa_paged_workspace_bytes",
+    "gdpa_fwd_paged_fp8",
     "gdpa_bwd_workspace_bytes",
     "gdpa_bwd",
     "gdpa_strerror",
@@ -221,6 +225,92 @@ class GdpaBwdParams(C.Structure):
     ]
 
 
+class GdpaBlockTableParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("lens_are_int64", C.c_int32),
+        ("cached_lens", C.c_void_p),
+        ("new_lens", C.c_void_p),
+        ("batch", C.c_int32),
+        ("block_size", C.c_int32),
+        ("block_tables", C.c_void_p),
+        ("table_stride", C.c_int64),
+        ("table_width", C.c_int32),
+        ("reserved", C.c_int32),
+        ("free_blocks", C.c_void_p),
+        ("free_capacity", C.c_int64),
+        ("num_free", C.c_void_p),
+        ("total_new", C.c_int64),
+        ("slots", C.c_void_p),
+        ("query_offset", C.c_void_p),
+        ("seq_lens", C.c_void_p),
+        ("num_free_after", C.c_void_p),
+    ]
+
+
+class GdpaCacheAppendParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("x_is_fp32", C.c_int32),
+        ("key", C.c_void_p),
+        ("value", C.c_void_p),
+        ("key_strides", C.c_int64 * 2),
+        ("value_strides", C.c_int64 * 2),
+        ("k_cache", C.c_void_p),
+        ("v_cache", C.c_void_p),
+        ("k_cache_strides", C.c_int64 * 3),
+        ("v_cache_strides", C.c_int64 * 3),
+        ("k_scales", C.c_void_p),
+        ("v_scales", C.c_void_p),
+        ("slot_mapping", C.c_void_p),
+        ("tokens", C.c_int64),
+        ("num_blocks", C.c_int64),
+        ("block_size", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class GdpaPagedParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("activation", C.c_int32),
+        ("q", C.c_void_p),
+        ("o", C.c_void_p),
+        ("q_strides", C.c_int64 * 2),
+        ("k_cache", C.c_void_p),
+        ("v_cache", C.c_void_p),
+        ("k_cache_strides", C.c_int64 * 3),
+        ("v_cache_strides", C.c_int64 * 3),
+        ("k_scales", C.c_void_p),
+        ("v_scales", C.c_void_p),
+        ("block_tables", C.c_void_p),
+        ("table_stride", C.c_int64),
+        ("table_width", C.c_int32),
+        ("block_size", C.c_int32),
+        ("num_blocks", C.c_int64),
+        ("q_offsets", C.c_void_p),
+        ("seq_lens", C.c_void_p),
+        ("offsets_are_int64", C.c_int32),
+        ("lens_are_int64", C.c_int32),
+        ("batch", C.c_int32),
+        ("heads", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("total_q", C.c_int64),
+        ("max_seq_len_q", C.c_int32),
+        ("qk_scale", C.c_float),
+        ("causal", C.c_int32),
+        ("window_plus_one", C.c_int32),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+        ("status", C.c_void_p),
+        ("timing_start_event", C.c_void_p),
+        ("timing_stop_event", C.c_void_p),
+    ]
+
+
 def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -252,6 +342,12 @@ def _load() -> C.CDLL:
     lib.gdpa_bwd_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32]
     lib.gdpa_bwd.restype = C.c_int
     lib.gdpa_bwd.argtypes = [C.POINTER(GdpaBwdParams), C.c_void_p]
+    for fn, params in ((lib.gdpa_build_block_tables, GdpaBlockTableParams), (lib.gdpa_append_kv_cache_fp8, GdpaCacheAppendParams),
+                       (lib.gdpa_fwd_paged_fp8, GdpaPagedParams)):
+        fn.restype = C.c_int
+        fn.argtypes = [C.POINTER(params), C.c_void_p]
+    lib.gdpa_paged_workspace_bytes.restype = C.c_size_t
+    lib.gdpa_paged_workspace_bytes.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32]
     lib.gdpa_strerror.restype = C.c_char_p
     lib.gdpa_strerror.argtypes = [C.c_int]
     lib.gdpa_launch_count.restype = C.c_int64

@@ -356,6 +356,122 @@ int gdpa_dequantize_mxfp8(const GdpaMxParams* params, gdpa_stream_t stream);
 int gdpa_fwd_fp8(const GdpaFwdParams* params, gdpa_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Serving from a paged key / value cache in 8 bits (no counterpart in the reference).  A cache is
+ * [num_blocks, block_size, kv_heads, head_dim] e4m3 for K and one for V, each with fp32 scales
+ * [num_blocks, kv_heads] (value = e4m3 * scale); block_size is 16, 32, 64 or 128, head_dim 64 or 128.
+ * Strides are in elements; the last dimension is contiguous, the others are free, multiples of 16.
+ * A slot is block * block_size + row.  Row b of block_tables ([batch, table_width] int32, rows
+ * table_stride apart) holds the blocks of request b's tokens in order.
+ * Slots of one call's tokens must lie in blocks that no other request writes to in that call.
+ * ------------------------------------------------------------------------------------------- */
+
+/* Blocks for the new tokens of a batch, and their slots.  Request b holds cached_lens[b] tokens in
+ * ceil(cached / block_size) blocks and gets new_lens[b] more: further blocks are taken from the top of the
+ * stack free_blocks[0 .. *num_free), in the order of the requests, and written into its table row.
+ * A request's new token i gets the slot of position cached + i, -1 where the stack has run out (the
+ * table then holds -1) or the table row is full.  The stack itself is only read: the caller takes
+ * *num_free_after, which is negative by the number of blocks that were missing, for the next call. */
+typedef struct GdpaBlockTableParams {
+  uint32_t struct_size;        /* sizeof(GdpaBlockTableParams) */
+  int32_t lens_are_int64;      /* type of cached_lens and new_lens */
+  const void* cached_lens;     /* [batch] */
+  const void* new_lens;        /* [batch] */
+  int32_t batch;
+  int32_t block_size;
+  int32_t* block_tables;       /* in / out */
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t reserved;
+  const int32_t* free_blocks;
+  int64_t free_capacity;       /* entries of free_blocks; *num_free is clamped to it */
+  const int32_t* num_free;     /* device */
+  int64_t total_new;           /* entries of slots; entries past the batch's new tokens become -1 */
+  int64_t* slots;              /* out [total_new] */
+  int32_t* query_offset;       /* out [batch + 1]: exclusive prefix sum of new_lens */
+  int32_t* seq_lens;           /* out [batch]: cached_lens + new_lens */
+  int32_t* num_free_after;     /* out [1], not the word num_free points to */
+} GdpaBlockTableParams;
+
+int gdpa_build_block_tables(const GdpaBlockTableParams* params, gdpa_stream_t stream);
+
+/* Quantises new keys and values into their slots.  A run is a stretch of tokens with consecutive slots of one
+ * block, o the row of its first.  For every run and head, K and V each: fresh = the smallest power of
+ * two with amax / fresh <= 448 over the run's finite values, at least 2^-100; scale = fresh if o is 0, else
+ * max(the block's scale, fresh).  Rows below o are rescaled when the scale grows, the run's rows become
+ * e4m3(x / scale) (to nearest even, infinities to 448 * scale, NaN to NaN); rows past the run are left as they are and
+ * count as unused.  Slots outside the cache (-1) are skipped.  A block's tokens must follow one another in
+ * the call: two runs of one block race. */
+typedef struct GdpaCacheAppendParams {
+  uint32_t struct_size;        /* sizeof(GdpaCacheAppendParams) */
+  int32_t x_is_fp32;           /* type of key and value: 0 bf16, 1 fp32 */
+  const void* key;             /* [tokens, kv_heads, head_dim] */
+  const void* value;
+  int64_t key_strides[2];      /* token, head; 0 = contiguous.  Multiples of 16 bytes */
+  int64_t value_strides[2];
+  void* k_cache;
+  void* v_cache;
+  int64_t k_cache_strides[3];  /* block, row, head; 0 = contiguous */
+  int64_t v_cache_strides[3];
+  float* k_scales;
+  float* v_scales;
+  const int64_t* slot_mapping; /* [tokens] */
+  int64_t tokens;
+  int64_t num_blocks;
+  int32_t block_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t reserved;
+} GdpaCacheAppendParams;
+
+int gdpa_append_kv_cache_fp8(const GdpaCacheAppendParams* params, gdpa_stream_t stream);
+
+/* GDPA forward over the cache.  Query i of request b (rows q_offsets[b] + i) has position
+ * seq_lens[b] - q_len + i; it takes part with keys j < seq_lens[b], with `causal` j <= position, with a
+ * window |j - position| <= window; a row without keys gives zeros.  Tokens of a block that the table has not (an entry outside
+ * [0, num_blocks)) take no part.  Scales must be positive.  O is [total_q, heads, head_dim] bf16. */
+typedef struct GdpaPagedParams {
+  uint32_t struct_size;        /* sizeof(GdpaPagedParams) */
+  int32_t activation;
+  const void* q;               /* [total_q, heads, head_dim] bf16 */
+  void* o;
+  int64_t q_strides[2];        /* token, head; 0 = contiguous */
+  const void* k_cache;
+  const void* v_cache;
+  int64_t k_cache_strides[3];  /* block, row, head; 0 = contiguous */
+  int64_t v_cache_strides[3];
+  const float* k_scales;
+  const float* v_scales;
+  const int32_t* block_tables;
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t block_size;
+  int64_t num_blocks;
+  const void* q_offsets;       /* [batch + 1] */
+  const void* seq_lens;        /* [batch], clamped to table_width * block_size */
+  int32_t offsets_are_int64;
+  int32_t lens_are_int64;
+  int32_t batch;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int64_t total_q;
+  int32_t max_seq_len_q;       /* requests' query counts are clamped to it */
+  float qk_scale;
+  int32_t causal;
+  int32_t window_plus_one;     /* window + 1, 0 = none */
+  void* workspace;             /* gdpa_paged_workspace_bytes() bytes, 16-byte aligned; one per call in flight */
+  int64_t workspace_bytes;
+  int32_t* status;
+  void* timing_start_event;    /* optional cudaEvent_t pair around the kernel */
+  void* timing_stop_event;
+} GdpaPagedParams;
+
+/* Bytes of the workspace of a call on the current device; 0 if there is none. */
+size_t gdpa_paged_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t max_seq_len_q);
+
+int gdpa_fwd_paged_fp8(const GdpaPagedParams* params, gdpa_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Backward.  Replaces torch.ops.gdpa.generalized_dot_product_attention_backward
  * (gdpa/triton/triton_generalized_dot_product_attention.py:3461-3788) and _flash_attn_bwd
  * (gdpa/src/interface.py:1257-1685): S and P are recomputed, dQ, dK, dV come out of one

@@ -466,8 +466,13 @@ int make_cache_tmap(CUtensorMap* m, const void* base, const long long (&strides)
 
 bool aligned16(const void* a, const void* b) { return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u) == 0; }
 
-// Rows of a row tile: the small one where a request's (query, head of the group) rows fit in it.
-int paged_rows(int group, int max_q) { return static_cast<long long>(group) * max_q <= kPagedRowsSmall ? kPagedRowsSmall : kPagedRowsLarge; }
+// Rows of a row tile: the smallest that holds a request's (query, head of the group) rows, 128 at most.
+int paged_rows(int group, int max_q) {
+  const long long rows = static_cast<long long>(group) * max_q;
+  return rows <= 16 ? 16 : rows <= 64 ? 64 : 128;
+}
+// CTAs of a launch: two on an SM where the row tile is small.
+int paged_ctas(int sm_count, int rows) { return rows == 16 ? 2 * sm_count : sm_count; }
 
 // Parts of the workspace: counters, then the pieces' O, then their row statistics; two pieces per CTA.
 size_t paged_counter_bytes(int ctas) { return (static_cast<size_t>(ctas) * sizeof(int) + 127) / 128 * 128; }
@@ -552,7 +557,8 @@ size_t gdpa_paged_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t head_
   DeviceInfo di;
   if (heads <= 0 || kv_heads <= 0 || head_dim <= 0 || max_seq_len_q < 0 || device_info(&di) != GDPA_OK) return 0;
   const int rows = paged_rows(heads / kv_heads, max_seq_len_q);
-  return paged_counter_bytes(di.sm_count) + paged_part_bytes(di.sm_count, rows, head_dim) + paged_stat_bytes(di.sm_count, rows);
+  const int ctas = paged_ctas(di.sm_count, rows);
+  return paged_counter_bytes(ctas) + paged_part_bytes(ctas, rows, head_dim) + paged_stat_bytes(ctas, rows);
 }
 
 int gdpa_fwd_paged_fp8(const GdpaPagedParams* p, gdpa_stream_t stream) {
@@ -582,7 +588,7 @@ int gdpa_fwd_paged_fp8(const GdpaPagedParams* p, gdpa_stream_t stream) {
   DeviceInfo di;
   if ((rc = device_info(&di)) != GDPA_OK) return rc;
   l.rows = paged_rows(group, p->max_seq_len_q);
-  l.grid = di.sm_count;
+  l.grid = paged_ctas(di.sm_count, l.rows);
   const size_t counters = paged_counter_bytes(l.grid), parts = paged_part_bytes(l.grid, l.rows, p->head_dim);
   if (p->workspace_bytes < static_cast<int64_t>(counters + parts + paged_stat_bytes(l.grid, l.rows))) return GDPA_ERR_CAPACITY;
   // a cache without blocks still needs valid maps: of one block in the place of Q, which no coordinate reaches

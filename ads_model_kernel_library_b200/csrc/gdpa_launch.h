@@ -249,11 +249,10 @@ struct PagedArgs {
 struct PagedLaunch {
   CUtensorMap tm_k, tm_v;  // over [blocks, kv_heads, block_size, head_dim]: a box is one block of one head
   PagedArgs args;
-  int rows;                // rows of a tile: kPagedRowsSmall or kPagedRowsLarge
+  int rows;                // rows of a tile: 16, 64 or 128
   int grid;
   cudaStream_t stream;
 };
-constexpr int kPagedRowsSmall = 32, kPagedRowsLarge = 128;
 
 }  // namespace gdpa
 struct GdpaFwdParams;

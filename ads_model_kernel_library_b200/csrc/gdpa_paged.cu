@@ -28,6 +28,8 @@
 // Roles: kGroups warpgroups (element-wise work, epilogue), one warp of TMA loads, one warp that issues MMAs, two that fetch Q.
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "gdpa_common.cuh"
 #include "gdpa_launch.h"
 
@@ -37,33 +39,37 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kItemSlots = 4;
+constexpr int kItemUnits = 2;           // what an item costs besides its tiles, in tiles
 constexpr float kMax8 = 448.f;
 constexpr float kNoMax = -3.0e38f;     // running maximum of a row that has seen no key
 constexpr float kLeastScale = 7.888609e-31f;  // 2^-100
 
 template <int D, int NMAX>
 struct PagedShape {
-  static constexpr int kGroups = NMAX > 32 ? 2 : 1;    // warpgroups
+  static constexpr int kCols = NMAX < 32 ? NMAX : 32;  // columns of a warpgroup
+  static constexpr int kGroups = NMAX / kCols;         // warpgroups
+  static constexpr int kCtasPerSm = NMAX <= 16 ? 2 : 1;
   static constexpr int kTileBytes = kTile * D;         // K or V tile
-  static constexpr int kStages = NMAX > 32 ? 3 : 6;
+  static constexpr int kStages = (NMAX <= 16 || NMAX > 64 ? 3 : 5) * (D == 128 ? 1 : 2);
   static constexpr int kQBytes = NMAX * D;             // hi, then lo
   static constexpr int kPBytes = NMAX * kTile;
   static constexpr int kWarps = 4 * kGroups + 4;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kLoadWarp = 4 * kGroups, kMmaWarp = kLoadWarp + 1, kQWarp = kLoadWarp + 2;
-  static constexpr int kTmemCols = NMAX > 32 ? 512 : 128;  // S0, S1, O of NMAX columns each
-  static constexpr float kTarget = NMAX > 32 ? 64.f : 256.f;
+  static constexpr int kTmemCols = NMAX <= 16 ? 64 : NMAX <= 64 ? 256 : 512;  // S0, S1, O of NMAX columns each
+  static constexpr float kTarget = 64.f;
 
   static constexpr int kKvOff = 0;                                  // [stage]{K, V}
   static constexpr int kQOff = kKvOff + kStages * 2 * kTileBytes;   // [2]{hi, lo}
   static constexpr int kPOff = kQOff + 2 * 2 * kQBytes;             // {hi, lo}
   static constexpr int kScaleOff = kPOff + 2 * kPBytes;             // float[stage][16]: K scales of up to 8 blocks, V scales
   static constexpr int kQaOff = kScaleOff + kStages * 64;           // float[2][NMAX]: factor of a row's scores
-  static constexpr int kRefOff = kQaOff + 2 * NMAX * 4;             // float[NMAX]: running maximum / multiplier of a row
+  static constexpr int kRefOff = kQaOff + 2 * NMAX * 4;             // float[NMAX]: minus the running maximum / multiplier of a row
   static constexpr int kFacOff = kRefOff + NMAX * 4;                // float[NMAX]
   static constexpr int kRedOff = kFacOff + NMAX * 4;                // float[4][NMAX]
   static constexpr int kRangeOff = kRedOff + 4 * NMAX * 4;          // int2[NMAX]: keys a row takes part with
-  static constexpr int kRingOff = kRangeOff + NMAX * 8;             // int[kItemSlots][16]
+  static constexpr int kRowOff = kRangeOff + NMAX * 8;              // long long[NMAX]: where a row of O begins
+  static constexpr int kRingOff = kRowOff + NMAX * 8;               // int[kItemSlots][16]
   static constexpr int kBarOff = kRingOff + kItemSlots * 64;
   enum : int {
     B_KV_FULL = 0,
@@ -82,7 +88,7 @@ struct PagedShape {
   static constexpr int kScanOff = kMiscOff + 16;          // long long[32] + start state
   static constexpr int kBytes = kScanOff + 32 * 8 + 48;
   static constexpr int kDynBytes = kBytes + 1024;
-  static_assert(kDynBytes <= 227 * 1024, "shared memory");
+  static_assert(kCtasPerSm * (kDynBytes + 1024) <= 228 * 1024, "shared memory");
 };
 
 // One stretch of tiles of one item, as the loader publishes it.
@@ -137,47 +143,71 @@ __device__ __forceinline__ Request load_request(const PagedArgs& a, int b) {
   return r;
 }
 
-// Units of one K / V head of a request: its row tiles' KV tiles, one at least each (a row tile without keys has zeros to write).
+// Units of one K / V head of a request: its row tiles' KV tiles, one at least each (a row tile without keys has zeros to write), and
+// kItemUnits for the beginning and the end of each.
 template <int NMAX>
 __device__ __forceinline__ long long units_of(const PagedArgs& a, const Request& r) {
   const int rows = r.q_len * a.group, nt = (rows + NMAX - 1) / NMAX;
-  if (!a.causal && a.window < 0) return static_cast<long long>(nt) * max(1, tiles_of(KeyRange{0, r.len}));
-  long long n = 0;
+  if (!a.causal && a.window < 0) return static_cast<long long>(nt) * (kItemUnits + max(1, tiles_of(KeyRange{0, r.len})));
+  long long n = static_cast<long long>(nt) * kItemUnits;
   for (int t = 0; t < nt; ++t)
     n += max(1, tiles_of(keys_of_any(t * NMAX / a.group, (min(rows, (t + 1) * NMAX) - 1) / a.group, r.q_len, r.len, a.causal, a.window)));
   return n;
 }
 
 template <int ACT>
-__device__ __forceinline__ void act16(const float (&x)[16], float m, float (&p)[16]) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    // x/2 erfc(-x / sqrt 2): 1 + erf would cancel where x is well below zero, and a row's scale brings such a P up when it has no larger
-    if constexpr (ACT == ACT_GELU_ERF) p[i] = 0.5f * m * x[i] * erfcf(x[i] * -0.70710678118654752f);
-    else p[i] = act_scaled<ACT>(x[i], m, 0.5f * m);
-  }
+__device__ __forceinline__ float act_one(float x, float m) {
+  // x/2 erfc(-x / sqrt 2): 1 + erf would cancel where x is well below zero, and a row's scale brings such a P up when it has no larger
+  if constexpr (ACT == ACT_GELU_ERF) return 0.5f * m * x * erfcf(x * -0.70710678118654752f);
+  else return act_scaled<ACT>(x, m, 0.5f * m);
 }
-// act(x) * m for a run-time activation class
-__device__ __forceinline__ void act16_any(int act, const float (&x)[16], float m, float (&p)[16]) {
+template <int ACT, int N>
+__device__ __forceinline__ void act_all(float (&x)[N], float m) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = act_one<ACT>(x[i], m);
+}
+// x = act(x) * m for a run-time activation class
+template <int N>
+__device__ __forceinline__ void act_any(int act, float (&x)[N], float m) {
   switch (act) {
-    case ACT_GELU_ERF: act16<ACT_GELU_ERF>(x, m, p); break;
-    case ACT_GELU_TANH: act16<ACT_GELU_TANH>(x, m, p); break;
-    case ACT_LEAKY_RELU: act16<ACT_LEAKY_RELU>(x, m, p); break;
-    case ACT_RELU: act16<ACT_RELU>(x, m, p); break;
-    case ACT_SILU: act16<ACT_SILU>(x, m, p); break;
-    case ACT_HARDSWISH: act16<ACT_HARDSWISH>(x, m, p); break;
-    case ACT_RELU_SQUARE: act16<ACT_RELU_SQUARE>(x, m, p); break;
-    default: act16<ACT_RAW>(x, m, p); break;
+    case ACT_GELU_ERF: act_all<ACT_GELU_ERF>(x, m); break;
+    case ACT_GELU_TANH: act_all<ACT_GELU_TANH>(x, m); break;
+    case ACT_LEAKY_RELU: act_all<ACT_LEAKY_RELU>(x, m); break;
+    case ACT_RELU: act_all<ACT_RELU>(x, m); break;
+    case ACT_SILU: act_all<ACT_SILU>(x, m); break;
+    case ACT_HARDSWISH: act_all<ACT_HARDSWISH>(x, m); break;
+    case ACT_RELU_SQUARE: act_all<ACT_RELU_SQUARE>(x, m); break;
+    default: act_all<ACT_RAW>(x, m); break;
   }
 }
 
-// Four consecutive floats from shared memory, the same for all lanes.
-__device__ __forceinline__ void lds16(const float* s, float (&v)[16]) {
+// The N columns' values over the warp's 32 lanes, reduced: lane i gets column i % N's result.  Halves change places (N - 1 shuffles).
+template <int N, class F>
+__device__ __forceinline__ float reduce_columns(float (&v)[N], int lane, F op) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float4 f = reinterpret_cast<const float4*>(s)[i];
-    v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+  for (int w = N / 2; w > 0; w >>= 1) {
+    const bool upper = lane & w;
+#pragma unroll
+    for (int i = 0; i < w; ++i) {
+      const float mine = upper ? v[i + w] : v[i], other = upper ? v[i] : v[i + w];
+      v[i] = op(mine, __shfl_xor_sync(kFull, other, w));
+    }
   }
+  float r = v[0];
+#pragma unroll
+  for (int w = N; w < 32; w <<= 1) r = op(r, __shfl_xor_sync(kFull, r, w));
+  return r;
+}
+
+template <int N>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[N]) {
+  if constexpr (N == 32) tmem_ld32(taddr, r);
+  else tmem_ld16(taddr, r);
+}
+template <int N>
+__device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)[N]) {
+  if constexpr (N == 32) tmem_st32(taddr, r);
+  else tmem_st16(taddr, r);
 }
 
 #define PAGED_WAIT(bar_idx, parity, role)                                                                             \
@@ -195,7 +225,7 @@ __device__ __forceinline__ void lds16(const float* s, float (&v)[16]) {
   }
 
 template <int D, int NMAX, bool SOFTMAX>
-__global__ void __launch_bounds__(PagedShape<D, NMAX>::kThreads, 1)
+__global__ void __launch_bounds__(PagedShape<D, NMAX>::kThreads, PagedShape<D, NMAX>::kCtasPerSm)
 gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PagedArgs a) {
   using L = PagedShape<D, NMAX>;
   constexpr int kGroups = L::kGroups;
@@ -319,71 +349,84 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     const int per_tile = kTile >> a.block_shift;  // blocks of a tile
     const int block_size = 1 << a.block_shift;
     uint32_t pos = 0;                             // tiles before this one
-    if (blockIdx.x < ctas) {
-      const long long u0 = all_units * blockIdx.x / ctas, u1 = all_units * (blockIdx.x + 1) / ctas;
-      long long at = start->before;  // units before the item
-      for (int b = start->b; b < a.batch && at < u1; ++b) {
-        const Request rq = load_request(a, b);
-        const int rows = rq.q_len * a.group, nt = (rows + NMAX - 1) / NMAX;
-        const int n_blocks = min((rq.len + block_size - 1) >> a.block_shift, a.table_width);
-        const int* const table = a.block_tables + static_cast<long long>(b) * a.table_stride;
-        for (int h = 0; h < a.kv_heads && at < u1; ++h) {
-          for (int t = 0; t < nt && at < u1; ++t) {
-            PagedItem it;
-            it.h = h, it.q_start = rq.q_start, it.q_len = rq.q_len, it.len = rq.len;
-            it.row0 = t * NMAX;
-            it.rows = min(NMAX, rows - it.row0);
-            const KeyRange r = keys_of_any(it.row0 / a.group, (it.row0 + it.rows - 1) / a.group, rq.q_len, rq.len, a.causal, a.window);
-            it.lo = r.lo, it.hi = r.hi;
-            const int n = tiles_of(r);
-            const long long units = max(1, n);
-            const long long s = at;
-            at += units;
-            if (at <= u0) continue;
-            const int skip = static_cast<int>(max(u0 - s, 0ll));
-            it.tile0 = r.lo / kTile + skip;
-            it.tiles = n == 0 ? 0 : static_cast<int>(min(u1 - s, units)) - skip;
-            // the CTA that has unit u is the largest c with all * c / ctas <= u
-            it.first = static_cast<int>(((s + 1) * ctas - 1) / all_units);
-            it.pieces = static_cast<int>(((s + units) * ctas - 1) / all_units) - it.first + 1;
-            if (!publish(it)) goto role_done;
-            int cached = 0, cached_at = -1;  // 32 entries of the table, from entry cached_at on
-            for (int j = 0; j < it.tiles; ++j, ++pos) {
-              const uint32_t stage = pos % L::kStages;
-              const int p0 = (it.tile0 + j) * per_tile;
-              if (cached_at < 0 || p0 + per_tile > cached_at + 32) {
-                cached_at = p0;
-                cached = cached_at + lane < n_blocks ? table[cached_at + lane] : -1;
-              }
-              const int blk = __shfl_sync(kFull, cached, (p0 - cached_at + lane) & 31);
-              const bool valid = lane < per_tile && p0 + lane < n_blocks && blk >= 0 && blk < a.num_blocks;
-              PAGED_WAIT(L::B_KV_EMPTY + stage, ((pos / L::kStages) & 1u) ^ 1u, ST_ROLE_LOAD);
-              const uint32_t bar = bar_base + 8u * (L::B_KV_FULL + stage);
-              const unsigned n_valid = __popc(__ballot_sync(kFull, valid));
-              if (lane == 0) mbar_arrive_expect_tx(bar, n_valid * block_size * D * 2);
-              __syncwarp();
-              const uint32_t dst = smem_base + L::kKvOff + stage * 2 * L::kTileBytes + lane * block_size * D;
-              if (valid) {
-                tma_load_4d(dst, &tm_k, bar, 0, 0, h, blk);
-                tma_load_4d(dst + L::kTileBytes, &tm_v, bar, 0, 0, h, blk);
-              }
-              // a block that is not there has scale 0, which tells the others
-              if (lane < per_tile) {
-                const uint32_t sc = smem_base + L::kScaleOff + stage * 64 + lane * 4;
-                const long long si = valid ? static_cast<long long>(blk) * a.kv_heads + h : 0;
-                cp_async4(sc, a.k_scales + si, valid);
-                cp_async4(sc + 32, a.v_scales + si, valid);
-              }
-              cp_async_mbar_arrive(bar_base + 8u * (L::B_SC_FULL + stage));
-              loaded = pos + 1;
-            }
+    const long long u0 = blockIdx.x < ctas ? all_units * blockIdx.x / ctas : 0, u1 = blockIdx.x < ctas ? all_units * (blockIdx.x + 1) / ctas : 0;
+    // the walk: request, head and row tile that come next, units before them
+    int wb = start->b - 1, wh = a.kv_heads, wt = 0, w_nt = 0, w_rows = 0;
+    long long at = start->before;
+    Request rq{0, 0, 0};
+    // the next item of which this CTA has tiles, published; h = -1 at the end.  Its request is `b_of`.
+    auto next_item = [&](PagedItem& it, int& b_of) -> bool {
+      it = PagedItem{};
+      it.h = -1;
+      while (at < u1) {
+        if (wt >= w_nt) wt = 0, ++wh;
+        if (wh >= a.kv_heads) {
+          if (++wb >= a.batch) break;
+          rq = load_request(a, wb);
+          wh = 0;
+          w_rows = rq.q_len * a.group;
+          w_nt = (w_rows + NMAX - 1) / NMAX;
+          if (w_nt == 0) {
+            wh = a.kv_heads;
+            continue;
           }
         }
+        const int row0 = wt * NMAX, rows = min(NMAX, w_rows - row0);
+        ++wt;
+        const KeyRange r = keys_of_any(row0 / a.group, (row0 + rows - 1) / a.group, rq.q_len, rq.len, a.causal, a.window);
+        const int n = tiles_of(r), n1 = max(1, n);
+        const long long s = at + kItemUnits;  // where the tiles' units begin
+        at = s + n1;
+        const int from = static_cast<int>(min(max(u0 - s, 0ll), static_cast<long long>(n1))), to = static_cast<int>(min(max(u1 - s, 0ll), static_cast<long long>(n1)));
+        if (from >= to) continue;
+        // the CTA that has unit u is the largest c with all * c / ctas <= u
+        const int first = static_cast<int>(((s + 1) * ctas - 1) / all_units);
+        const int pieces = static_cast<int>(((s + n1) * ctas - 1) / all_units) - first + 1;
+        it = PagedItem{wh, rq.q_start, rq.q_len, row0, rows, rq.len, r.lo, r.hi, r.lo / kTile + from, n == 0 ? 0 : to - from, pieces, first};
+        b_of = wb;
+        break;
+      }
+      return publish(it);
+    };
+    PagedItem it, ahead;
+    int b = 0, b_ahead = 0;
+    if (!next_item(it, b)) goto role_done;
+    for (; it.h >= 0; it = ahead, b = b_ahead) {
+      // the others learn of the next item before this one's tiles are asked for: its Q is fetched meanwhile
+      if (!next_item(ahead, b_ahead)) goto role_done;
+      const int n_blocks = min((it.len + block_size - 1) >> a.block_shift, a.table_width);
+      const int* const table = a.block_tables + static_cast<long long>(b) * a.table_stride;
+      int cached = 0, cached_at = -1;  // 32 entries of the table, from entry cached_at on
+      for (int j = 0; j < it.tiles; ++j, ++pos) {
+        const uint32_t stage = pos % L::kStages;
+        const int p0 = (it.tile0 + j) * per_tile;
+        if (cached_at < 0 || p0 + per_tile > cached_at + 32) {
+          cached_at = p0;
+          cached = cached_at + lane < n_blocks ? table[cached_at + lane] : -1;
+        }
+        const int blk = __shfl_sync(kFull, cached, (p0 - cached_at + lane) & 31);
+        const bool valid = lane < per_tile && p0 + lane < n_blocks && blk >= 0 && blk < a.num_blocks;
+        PAGED_WAIT(L::B_KV_EMPTY + stage, ((pos / L::kStages) & 1u) ^ 1u, ST_ROLE_LOAD);
+        const uint32_t bar = bar_base + 8u * (L::B_KV_FULL + stage);
+        const unsigned n_valid = __popc(__ballot_sync(kFull, valid));
+        if (lane == 0) mbar_arrive_expect_tx(bar, n_valid * block_size * D * 2);
+        __syncwarp();
+        const uint32_t dst = smem_base + L::kKvOff + stage * 2 * L::kTileBytes + lane * block_size * D;
+        if (valid) {
+          tma_load_4d(dst, &tm_k, bar, 0, 0, it.h, blk);
+          tma_load_4d(dst + L::kTileBytes, &tm_v, bar, 0, 0, it.h, blk);
+        }
+        // a block that is not there has scale 0, which tells the others
+        if (lane < per_tile) {
+          const uint32_t sc = smem_base + L::kScaleOff + stage * 64 + lane * 4;
+          const long long si = valid ? static_cast<long long>(blk) * a.kv_heads + it.h : 0;
+          cp_async4(sc, a.k_scales + si, valid);
+          cp_async4(sc + 32, a.v_scales + si, valid);
+        }
+        cp_async_mbar_arrive(bar_base + 8u * (L::B_SC_FULL + stage));
+        loaded = pos + 1;
       }
     }
-    PagedItem end{};
-    end.h = -1;
-    if (!publish(end)) goto role_done;
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == L::kMmaWarp) {
     // ------------------------------------------------------------------ MMA issuer
@@ -425,7 +468,7 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         break;
       }
       if (it.tiles == 0) continue;
-      const int n16 = (it.rows + 15) / 16;
+      const int n16 = (it.rows + L::kCols - 1) / L::kCols * (L::kCols / 16);  // whole warpgroups' columns
       const uint32_t q_buf = q_pos & 1u;
       PAGED_WAIT(L::B_Q_FULL + q_buf, (q_pos >> 1) & 1u, ST_ROLE_MMA);
       ++q_pos;
@@ -467,9 +510,9 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       ++q_pos;
       uint8_t* const hi = smem + L::kQOff + q_buf * 2 * L::kQBytes;
       float* const qa = reinterpret_cast<float*>(smem + L::kQaOff) + q_buf * NMAX;
-      const int n = (it.rows + 15) / 16 * 16;
+      const int n = (it.rows + L::kCols - 1) / L::kCols * L::kCols;  // rows to the end of a warpgroup's columns: zeros
       const int c8 = lane % kLanes;
-      constexpr int kAhead = 4;
+      constexpr int kAhead = NMAX >= 64 ? 8 : 4;
       for (int r0 = wq * kRowsAt + lane / kLanes; r0 - lane / kLanes < n; r0 += 2 * kRowsAt * kAhead) {
         uint4 u[kAhead];
 #pragma unroll
@@ -532,48 +575,46 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     }
   } else {
     // ------------------------------------------------------------------ element-wise work and epilogue
-    constexpr int kSets = NMAX / 32 / kGroups;  // groups of 32 columns of this warpgroup
-    constexpr float kHeadroom = (L::kTarget == 256.f ? 0.8073549f : 2.8073549f) + 0.001f;  // log2(448 / kTarget)
-    static_assert(L::kTarget == 256.f || L::kTarget == 64.f, "kHeadroom");
-    const int wg = warp >> 2, tid = threadIdx.x & 127, quarter = warp & 3;
+    // Warpgroup wg has columns [wg * kCols, (wg + 1) * kCols) of the 128 tokens, a thread one token.
+    constexpr int C = L::kCols;
+    constexpr float kHeadroom = 2.8073549f + 0.001f;  // log2(448 / kTarget)
+    static_assert(L::kTarget == 64.f, "kHeadroom");
+    const int wg = warp >> 2, tid = threadIdx.x & 127, quarter = warp & 3, c0 = wg * C;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t o_tmem = tmem_base + 2 * NMAX + lane_base;
-    float* const ref = reinterpret_cast<float*>(smem + L::kRefOff);
-    float* const fac = reinterpret_cast<float*>(smem + L::kFacOff);
-    float* const red = reinterpret_cast<float*>(smem + L::kRedOff);
-    int2* const range = reinterpret_cast<int2*>(smem + L::kRangeOff);
-    const int bar_wg = 1 + wg;
+    const uint32_t o_tmem = tmem_base + 2 * NMAX + lane_base + c0;
+    float* const ref = reinterpret_cast<float*>(smem + L::kRefOff) + c0;
+    float* const fac = reinterpret_cast<float*>(smem + L::kFacOff) + c0;
+    float* const red = reinterpret_cast<float*>(smem + L::kRedOff) + c0;  // [quarter * NMAX + column]
+    int2* const range = reinterpret_cast<int2*>(smem + L::kRangeOff) + c0;
+    long long* const row_at = reinterpret_cast<long long*>(smem + L::kRowOff) + c0;
+    const int bar_wg = 4 + wg;
     uint32_t pos = 0, q_pos = 0;  // tiles, items with tiles
-    float l[kSets][32];
     while (true) {
       const PagedItem it = take_item(ST_ROLE_ACT);
       if (named_bar_or(3, 128 * kGroups, it.h < 0)) break;
-      const int n16 = (it.rows + 15) / 16;
+      const int rows = min(C, it.rows - c0);  // of this warpgroup; none or fewer: it only keeps step
+      if (tid < C) {
+        const int g = it.row0 + c0 + tid, i = g / a.group;
+        row_at[tid] = ((it.q_start + static_cast<long long>(i)) * a.heads + it.h * a.group + (g - i * a.group)) * D;
+        const KeyRange r = tid < rows ? keys_of(i, it.q_len, it.len, a.causal, a.window) : KeyRange{0, 0};
+        range[tid] = make_int2(r.lo, r.hi);
+        ref[tid] = SOFTMAX ? -kNoMax : 1.f;
+      }
+      named_bar_sync(bar_wg, 128);
       if (it.tiles == 0) {
         // no row of the tile has a key
-        for (int i = threadIdx.x; i < it.rows * D / 2; i += 128 * kGroups) {
-          const int g = it.row0 + i / (D / 2);
-          reinterpret_cast<uint32_t*>(a.o + ((it.q_start + static_cast<long long>(g / a.group)) * a.heads + it.h * a.group + g % a.group) * D)[i % (D / 2)] = 0u;
-        }
+        for (int i = tid; i < rows * (D / 2); i += 128) reinterpret_cast<uint32_t*>(a.o + row_at[i / (D / 2)])[i % (D / 2)] = 0u;
+        named_bar_sync(bar_wg, 128);
         continue;
       }
       const uint32_t q_buf = q_pos & 1u;
-      const float* const qa = reinterpret_cast<const float*>(smem + L::kQaOff) + q_buf * NMAX;
-      // the columns of this warpgroup: sets wg, wg + kGroups, ... of 32
-      if (tid < NMAX && (tid >> 5) % kGroups == wg) {
-        const int g = it.row0 + tid;
-        const KeyRange r = tid < it.rows ? keys_of(g / a.group, it.q_len, it.len, a.causal, a.window) : KeyRange{0, 0};
-        range[tid] = make_int2(r.lo, r.hi);
-        ref[tid] = SOFTMAX ? kNoMax : 1.f;
-      }
+      const float* const qa = reinterpret_cast<const float*>(smem + L::kQaOff) + q_buf * NMAX + c0;
+      uint64_t l[C / 2];  // row sums of this token's P, in pairs of columns
 #pragma unroll
-      for (int s = 0; s < kSets; ++s)
-#pragma unroll
-        for (int i = 0; i < 32; ++i) l[s][i] = 0.f;
+      for (int i = 0; i < C / 2; ++i) l[i] = 0ull;
       const int i0 = it.row0 / a.group, i1 = (it.row0 + it.rows - 1) / a.group;
       const KeyRange r0 = keys_of(i0, it.q_len, it.len, a.causal, a.window), r1 = keys_of(i1, it.q_len, it.len, a.causal, a.window);
       const int all_lo = max(r0.lo, r1.lo), all_hi = min(r0.hi, r1.hi);  // keys that every row takes part with (if any)
-      named_bar_sync(bar_wg, 128);
       PAGED_WAIT_ON(L::B_Q_FULL + q_buf, (q_pos >> 1) & 1u);
       ++q_pos;
       for (int j = 0; j < it.tiles; ++j, ++pos) {
@@ -605,170 +646,158 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
               for (int e = 0; e < 4; ++e) poisoned |= __vcmpeq4(w[e] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0u;
             }
           }
-          if (kGroups > 1 && !every) named_bar_sync(3, 128 * kGroups);  // both warpgroups have looked
+          if (kGroups > 1 && !every) named_bar_sync(3, 128 * kGroups);  // all warpgroups have looked
           if (wg == 0 && (out || poisoned)) {
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) v_row[i] = make_uint4(0, 0, 0, 0);
           }
         }
-        bool pv_waited = false;
-#pragma unroll
-        for (int s = 0; s < kSets; ++s) {
-          const int c0 = (s * kGroups + wg) * 32;  // first column
-          const int chunks = min(2, n16 - c0 / 16);
-          if (chunks <= 0) continue;
+        if (rows > 0) {
           const uint32_t s_tmem = tmem_base + (pos & 1u) * NMAX + lane_base + c0;
-          float p[32];
-          // P of the chunks, for the reference the rows have now; whether it fits e4m3
+          const float m = SOFTMAX ? vs * L::kTarget : vs;
+          float p[C];
+          // the scores, times the row's and the block's factors (for the softmax less the row's reference)
+          auto scores = [&](bool relative) {
+            uint32_t raw[C];
+            tmem_ld_cols(s_tmem, raw);
+            tmem_wait_ld();
+            tmem_regs_ready(raw);
+            const uint64_t k2 = pack_f32x2(ks, ks);
+#pragma unroll
+            for (int i = 0; i < C; i += 4) {
+              const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(qa + i);
+              ulonglong2 r = make_ulonglong2(0, 0);
+              if (relative) r = *reinterpret_cast<const ulonglong2*>(ref + i);
+              uint64_t x0 = mul_f32x2(pack_f32x2(__uint_as_float(raw[i]), __uint_as_float(raw[i + 1])), k2);
+              uint64_t x1 = mul_f32x2(pack_f32x2(__uint_as_float(raw[i + 2]), __uint_as_float(raw[i + 3])), k2);
+              x0 = relative ? fma_f32x2(x0, f.x, r.x) : mul_f32x2(x0, f.x);
+              x1 = relative ? fma_f32x2(x1, f.y, r.y) : mul_f32x2(x1, f.y);
+              unpack_f32x2(x0, p[i], p[i + 1]);
+              unpack_f32x2(x1, p[i + 2], p[i + 3]);
+            }
+          };
+          // P for the reference the rows have now; whether it fits e4m3
           auto compute = [&]() -> bool {
+            scores(SOFTMAX);
+            if constexpr (SOFTMAX) {
+#pragma unroll
+              for (int i = 0; i < C; ++i) p[i] = ex2_approx(p[i]);
+            } else {
+              act_any(a.act, p, a.scale);
+#pragma unroll
+              for (int i = 0; i < C; i += 4) {
+                const float4 r = *reinterpret_cast<const float4*>(ref + i);
+                p[i] *= r.x, p[i + 1] *= r.y, p[i + 2] *= r.z, p[i + 3] *= r.w;
+              }
+            }
+            if (masked) {
+#pragma unroll
+              for (int i = 0; i < C; ++i) {
+                const int2 rg = range[i];
+                const bool in = !out && key >= rg.x && key < rg.y;
+                p[i] = in ? (poisoned ? __uint_as_float(0x7fffffffu) : p[i]) : 0.f;
+              }
+            }
             float most = 0.f;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              if (c < chunks) {
-                uint32_t raw[16];
-                tmem_ld16(s_tmem + c * 16, raw);
-                float f[16], x[16], rf[16];
-                lds16(qa + c0 + c * 16, f);
-                lds16(ref + c0 + c * 16, rf);
-                tmem_wait_ld();
-                tmem_regs_ready(raw);
+            for (int i = 0; i < C; i += 2) most = SOFTMAX ? max3(most, p[i], p[i + 1]) : max3(most, fabsf(p[i]), fabsf(p[i + 1]));
+            return most * m <= kMax8;
+          };
+          bool fits = true;
+          if (!first) fits = compute();
+          if (first || named_bar_or(bar_wg, 128, !fits)) {
+            // the exact reference of every column, and O and the row sums moved to it
+            scores(false);
+            if constexpr (SOFTMAX) {
+              const float lv = log2f(vs);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(raw[i]) * (f[i] * ks);
-                if constexpr (SOFTMAX) {
+              for (int i = 0; i < C; ++i) p[i] += lv;
+            } else {
+              act_any(a.act, p, a.scale);
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) p[c * 16 + i] = ex2_approx(x[i] - rf[i]);
-                } else {
-                  float q[16];
-                  act16_any(a.act, x, a.scale, q);
+              for (int i = 0; i < C; ++i) p[i] = fabsf(p[i]) * vs;
+            }
+            if (masked) {
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) p[c * 16 + i] = q[i] * rf[i];
-                }
-                if (masked) {
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) {
-                    const int2 rg = range[c0 + c * 16 + i];
-                    const bool in = !out && key >= rg.x && key < rg.y;
-                    p[c * 16 + i] = in ? (poisoned ? __uint_as_float(0x7fffffffu) : p[c * 16 + i]) : 0.f;
-                  }
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(p[c * 16 + i]));
+              for (int i = 0; i < C; ++i) {
+                const int2 rg = range[i];
+                p[i] = !out && key >= rg.x && key < rg.y ? p[i] : (SOFTMAX ? kNoMax : 0.f);
               }
             }
-            return most * (vs * (SOFTMAX ? L::kTarget : 1.f)) <= kMax8;
-          };
-          const bool fits = compute();
-          if (named_bar_or(bar_wg, 128, first || !fits)) {
-            // the exact reference of every column, and O and the row sums moved to it
-            if (!pv_waited && pos > 0) {
-              PAGED_WAIT_ON(L::B_PV_DONE, (pos - 1) & 1u);
+            const float most = reduce_columns<C>(p, lane, [](float x, float y) { return fmaxf(x, y); });
+            if (lane < C) red[quarter * NMAX + lane] = most;
+            if (!first) {
+              PAGED_WAIT_ON(L::B_PV_DONE, (pos - 1) & 1u);  // O holds every tile before this one
               tc_fence_after();
             }
-            pv_waited = true;
-            const float lv = SOFTMAX ? log2f(vs) : 0.f;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              if (c < chunks) {
-                uint32_t raw[16];
-                tmem_ld16(s_tmem + c * 16, raw);
-                float f[16], x[16];
-                lds16(qa + c0 + c * 16, f);
-                tmem_wait_ld();
-                tmem_regs_ready(raw);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(raw[i]) * (f[i] * ks);
-                float u[16];
-                if constexpr (SOFTMAX) {
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) u[i] = x[i] + lv;
-                } else {
-                  act16_any(a.act, x, a.scale, u);
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) u[i] = fabsf(u[i]) * vs;
-                }
-                float keep = 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const int2 rg = range[c0 + c * 16 + i];
-                  const bool in = !masked || (!out && key >= rg.x && key < rg.y);
-                  const float m = warp_max(in ? u[i] : (SOFTMAX ? kNoMax : 0.f));
-                  keep = lane == i ? m : keep;
-                }
-                if (lane < 16) red[quarter * NMAX + c0 + c * 16 + lane] = keep;
-              }
-            }
             named_bar_sync(bar_wg, 128);
-            if (tid < 16 * chunks) {
-              const int n = c0 + tid;
-              const float m = fmaxf(fmaxf(red[n], red[NMAX + n]), fmaxf(red[2 * NMAX + n], red[3 * NMAX + n]));
-              const float old = ref[n];
-              // a column that fits keeps its reference: no row's bits depend on another row's values (the margin of 2^-10 keeps the
-              // two ways to say that one does not fit from differing)
+            if (tid < C) {
+              const float now = fmaxf(fmaxf(red[tid], red[NMAX + tid]), fmaxf(red[2 * NMAX + tid], red[3 * NMAX + tid]));
+              // a column that fits keeps its reference: no row's bits depend on another row's values (the margin keeps the two ways
+              // to say that one does not fit from differing)
               if constexpr (SOFTMAX) {
-                const float now = first || m - old > kHeadroom ? fmaxf(old, fminf(m, 3.0e38f)) : old;
-                fac[n] = first ? 0.f : ex2_approx(old - now);
-                ref[n] = now;
+                const float old = -ref[tid];
+                const float next = first || now - old > kHeadroom ? fmaxf(old, fminf(now, 3.0e38f)) : old;
+                fac[tid] = first ? 0.f : ex2_approx(old - next);
+                ref[tid] = -next;
               } else {
-                // the largest power of two that keeps |P| V's scale at or below the target; 2^100 for a row of zeros
-                float now = 1.2676506e30f;
-                if (m > 0.f) now = exp2f(fminf(fmaxf(floorf(log2f(L::kTarget / m)), -100.f), 100.f));
-                if (!first) now = m * old > kMax8 * 1.001f ? fminf(now, old) : old;
-                fac[n] = first ? 0.f : now / old;
-                ref[n] = now;
+                // the largest power of two that keeps |P| times V's scale at or below the target; 2^100 for a row of zeros
+                const float old = ref[tid];
+                float next = 1.2676506e30f;
+                if (now > 0.f) next = exp2f(fminf(fmaxf(floorf(log2f(L::kTarget / now)), -100.f), 100.f));
+                if (!first) next = now * old > kMax8 * 1.001f ? fminf(next, old) : old;
+                fac[tid] = first ? 0.f : next / old;
+                ref[tid] = next;
               }
             }
             named_bar_sync(bar_wg, 128);
             if (!first) {
+              uint32_t raw[C];
+              tmem_ld_cols(o_tmem, raw);
+              tmem_wait_ld();
+              tmem_regs_ready(raw);
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                if (c < chunks) {
-                  float f[16];
-                  lds16(fac + c0 + c * 16, f);
-                  uint32_t raw[16];
-                  tmem_ld16(o_tmem + c0 + c * 16, raw);
-                  tmem_wait_ld();
-                  tmem_regs_ready(raw);
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) raw[i] = __float_as_uint(__uint_as_float(raw[i]) * f[i]);
-                  tmem_st16(o_tmem + c0 + c * 16, raw);
-                  tmem_wait_st();
-                  if constexpr (SOFTMAX) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) l[s][c * 16 + i] *= f[i];
-                  }
-                }
+              for (int i = 0; i < C; i += 2) {
+                const float2 f = *reinterpret_cast<const float2*>(fac + i);
+                raw[i] = __float_as_uint(__uint_as_float(raw[i]) * f.x);
+                raw[i + 1] = __float_as_uint(__uint_as_float(raw[i + 1]) * f.y);
+                if constexpr (SOFTMAX) l[i / 2] = mul_f32x2(l[i / 2], pack_f32x2(f.x, f.y));
               }
+              tmem_st_cols(o_tmem, raw);
+              tmem_wait_st();
             }
             compute();
           }
-          if (!pv_waited && pos > 0) {
-            PAGED_WAIT_ON(L::B_PV_DONE, (pos - 1) & 1u);  // P's buffer is free
-            pv_waited = true;
-          }
           // P, times V's scale, as the sum of two e4m3 values
-          const float m = vs * (SOFTMAX ? L::kTarget : 1.f);
+          uint32_t w_hi[C / 4], w_lo[C / 4];
+          const uint64_t m2 = pack_f32x2(m, m);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            if (c < chunks) {
-              uint32_t w_hi[4] = {0, 0, 0, 0}, w_lo[4] = {0, 0, 0, 0};
+          for (int i = 0; i < C / 4; ++i) {
+            uint16_t eh[2], el[2];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float x0 = p[c * 16 + 2 * i], x1 = p[c * 16 + 2 * i + 1];
-                if constexpr (SOFTMAX) l[s][c * 16 + 2 * i] += x0, l[s][c * 16 + 2 * i + 1] += x1;
-                const uint32_t h = pack_f16x2(x0 * m, x1 * m);
-                const uint16_t eh = e4m3x2_from_f16x2(h);
-                const uint16_t el = e4m3x2_from_f16x2(sub_f16x2(h, f16x2_from_e4m3x2(eh)));
-                w_hi[i >> 1] |= static_cast<uint32_t>(eh) << (16 * (i & 1));
-                w_lo[i >> 1] |= static_cast<uint32_t>(el) << (16 * (i & 1));
-              }
-              uint8_t* const dst = smem + L::kPOff + (c0 / 16 + c) * 16 * kTile + tid * 16;
-              *reinterpret_cast<uint4*>(dst) = make_uint4(w_hi[0], w_hi[1], w_hi[2], w_hi[3]);
-              *reinterpret_cast<uint4*>(dst + L::kPBytes) = make_uint4(w_lo[0], w_lo[1], w_lo[2], w_lo[3]);
+            for (int e = 0; e < 2; ++e) {
+              const uint64_t x = pack_f32x2(p[4 * i + 2 * e], p[4 * i + 2 * e + 1]);
+              if constexpr (SOFTMAX) l[2 * i + e] = add_f32x2(l[2 * i + e], x);
+              float y0, y1;
+              unpack_f32x2(mul_f32x2(x, m2), y0, y1);
+              const uint32_t h = pack_f16x2(y0, y1);
+              eh[e] = e4m3x2_from_f16x2(h);
+              el[e] = e4m3x2_from_f16x2(sub_f16x2(h, f16x2_from_e4m3x2(eh[e])));
             }
+            w_hi[i] = static_cast<uint32_t>(eh[0]) | (static_cast<uint32_t>(eh[1]) << 16);
+            w_lo[i] = static_cast<uint32_t>(el[0]) | (static_cast<uint32_t>(el[1]) << 16);
           }
+          if (pos > 0) PAGED_WAIT_ON(L::B_PV_DONE, (pos - 1) & 1u);  // P's buffer is free
+          uint8_t* const dst = smem + L::kPOff + c0 * kTile + tid * 16;
+#pragma unroll
+          for (int c = 0; c < C / 16; ++c) {
+            *reinterpret_cast<uint4*>(dst + c * 16 * kTile) = make_uint4(w_hi[4 * c], w_hi[4 * c + 1], w_hi[4 * c + 2], w_hi[4 * c + 3]);
+            *reinterpret_cast<uint4*>(dst + L::kPBytes + c * 16 * kTile) = make_uint4(w_lo[4 * c], w_lo[4 * c + 1], w_lo[4 * c + 2], w_lo[4 * c + 3]);
+          }
+        } else if (pos > 0) {
+          // a warpgroup without columns waits too: its arrival for the next tile must not count for this one
+          PAGED_WAIT_ON(L::B_PV_DONE, (pos - 1) & 1u);
         }
-        // (a warpgroup without columns waits too: its arrival for the next tile must not count for this one)
-        if (!pv_waited && pos > 0) PAGED_WAIT_ON(L::B_PV_DONE, (pos - 1) & 1u);
         fence_proxy_async_smem();
         tc_fence_before();
         mbar_arrive(bar_base + 8u * L::B_P_FULL);
@@ -776,34 +805,22 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       // ---- the end of the stretch: row sums over the 128 tokens' threads, then O
       if (lane == 0) mbar_arrive(bar_base + 8u * (L::B_Q_EMPTY + q_buf));
       if constexpr (SOFTMAX) {
+        float sums[C];
 #pragma unroll
-        for (int s = 0; s < kSets; ++s) {
-          const int c0 = (s * kGroups + wg) * 32;
-          if (c0 < 16 * n16) {
-            // 32 columns over 32 lanes: halves change places until lane i has the sum of column i
-#pragma unroll
-            for (int w = 16; w > 0; w >>= 1) {
-              const bool upper = lane & w;
-#pragma unroll
-              for (int i = 0; i < w; ++i) {
-                const float mine = upper ? l[s][i + w] : l[s][i], other = upper ? l[s][i] : l[s][i + w];
-                l[s][i] = mine + __shfl_xor_sync(kFull, other, w);
-              }
-            }
-            red[quarter * NMAX + c0 + lane] = l[s][0];
-          }
-        }
+        for (int i = 0; i < C / 2; ++i) unpack_f32x2(l[i], sums[2 * i], sums[2 * i + 1]);
+        const float sum = reduce_columns<C>(sums, lane, [](float x, float y) { return x + y; });
+        if (lane < C) red[quarter * NMAX + lane] = sum;
       }
       PAGED_WAIT_ON(L::B_PV_DONE, (pos - 1) & 1u);
       tc_fence_after();
       named_bar_sync(bar_wg, 128);
       const bool cut = it.pieces > 1;
       const int part = 2 * blockIdx.x + (static_cast<int>(blockIdx.x) == it.first ? 1 : 0);
-      if (tid < NMAX && (tid >> 5) % kGroups == wg && tid < it.rows) {
+      if (tid < rows) {
         const float sum = SOFTMAX ? red[tid] + red[NMAX + tid] + red[2 * NMAX + tid] + red[3 * NMAX + tid] : 1.f;
         if (cut) {
-          float* const ml = a.part_ml + static_cast<long long>(part) * 2 * NMAX;
-          ml[tid] = ref[tid];
+          float* const ml = a.part_ml + static_cast<long long>(part) * 2 * NMAX + c0;
+          ml[tid] = -ref[tid];
           ml[NMAX + tid] = sum;
           fac[tid] = SOFTMAX ? 1.f / L::kTarget : 1.f / ref[tid];
         } else {
@@ -811,39 +828,27 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         }
       }
       named_bar_sync(bar_wg, 128);
+      if (rows > 0) {
+        uint32_t raw[C];
+        tmem_ld_cols(o_tmem, raw);
+        tmem_wait_ld();
+        tmem_regs_ready(raw);
+        if (tid < D) {
+          float* const po = a.part_o + (static_cast<long long>(part) * NMAX + c0) * D + tid;
 #pragma unroll
-      for (int s = 0; s < kSets; ++s) {
-        const int c0 = (s * kGroups + wg) * 32;
-        const int chunks = min(2, n16 - c0 / 16);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          if (c < chunks) {
-            uint32_t raw[16];
-            tmem_ld16(o_tmem + c0 + c * 16, raw);
-            float f[16];
-            lds16(fac + c0 + c * 16, f);
-            tmem_wait_ld();
-            tmem_regs_ready(raw);
-            if (tid < D) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int r = c0 + c * 16 + i;
-                if (r < it.rows) {
-                  const float v = __uint_as_float(raw[i]) * f[i];
-                  if (cut) {
-                    a.part_o[(static_cast<long long>(part) * NMAX + r) * D + tid] = v;
-                  } else {
-                    const int g = it.row0 + r;
-                    a.o[((it.q_start + static_cast<long long>(g / a.group)) * a.heads + it.h * a.group + g % a.group) * D + tid] = __float2bfloat16_rn(v);
-                  }
-                }
-              }
+          for (int i = 0; i < C; ++i) {
+            if (i < rows) {
+              const float v = __uint_as_float(raw[i]) * fac[i];
+              if (cut) po[i * D] = v;
+              else a.o[row_at[i] + tid] = __float2bfloat16_rn(v);
             }
           }
         }
       }
       tc_fence_before();
-      if (cut) {
+      if (!cut) {
+        named_bar_sync(bar_wg, 128);  // the next item writes over fac and row_at
+      } else {
         // the last of the item's CTAs joins the pieces
         __threadfence();
         named_bar_sync(3, 128 * kGroups);
@@ -856,7 +861,6 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         if (*last_flag) {
           // a warp has a row: the weights of its pieces over the lanes, then the pieces in order
           for (int r = warp; r < it.rows; r += 4 * kGroups) {
-            const int g = it.row0 + r;
             constexpr int V = D / 32;
             float acc[V], m_all = kNoMax, l_all = 0.f;
 #pragma unroll
@@ -899,12 +903,12 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
               for (int s = 16; s > 0; s >>= 1) l_all += __shfl_xor_sync(kFull, l_all, s);
               inv = l_all > 0.f || l_all != l_all ? 1.f / l_all : 0.f;
             }
-            uint32_t* const dst = reinterpret_cast<uint32_t*>(
-                a.o + ((it.q_start + static_cast<long long>(g / a.group)) * a.heads + it.h * a.group + g % a.group) * D + lane * V);
+            uint32_t* const dst = reinterpret_cast<uint32_t*>(a.o + reinterpret_cast<const long long*>(smem + L::kRowOff)[r] + lane * V);
 #pragma unroll
             for (int e = 0; e < V / 2; ++e) dst[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
           }
         }
+        named_bar_sync(3, 128 * kGroups);
       }
     }
   }
@@ -939,8 +943,11 @@ int launch(const PagedLaunch& l) {
 }  // namespace
 
 int launch_paged(const PagedLaunch& l, int head_dim) {
-  if (l.rows == kPagedRowsSmall) return head_dim == 128 ? launch<128, kPagedRowsSmall>(l) : launch<64, kPagedRowsSmall>(l);
-  return head_dim == 128 ? launch<128, kPagedRowsLarge>(l) : launch<64, kPagedRowsLarge>(l);
+  auto go = [&](auto dim) -> int {
+    constexpr int D = decltype(dim)::value;
+    return l.rows == 16 ? launch<D, 16>(l) : l.rows == 64 ? launch<D, 64>(l) : launch<D, 128>(l);
+  };
+  return head_dim == 128 ? go(std::integral_constant<int, 128>{}) : go(std::integral_constant<int, 64>{});
 }
 
 }  // namespace gdpa

@@ -1,4 +1,5 @@
-"""Build libgdpa_b200.so (the C-ABI kernel library) in-tree with nvcc for sm_100a.
+"""Build libgdpa_b200.so (the C-ABI kernel library) in-tree with nvcc for sm_100a, and libgdpa_b200_torch.so (torch operators that
+call it from C++) with the host compiler.
 
     python -m ads_model_kernel_library_b200.build [--force] [--verbose]
 
@@ -10,6 +11,7 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -18,6 +20,8 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 OUT = os.path.join(PKG, "libgdpa_b200.so")
+TORCH_SRC = os.path.join(CSRC, "gdpa_torch.cpp")
+TORCH_OUT = os.path.join(PKG, "libgdpa_b200_torch.so")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17", "--expt-relaxed-constexpr",
@@ -42,8 +46,24 @@ def _newest_header() -> float:
     return max(os.path.getmtime(h) for h in hdrs)
 
 
+def _build_torch_ops(force: bool, verbose: bool) -> None:
+    header = os.path.join(os.path.dirname(PKG), "include", "gdpa_b200.h")
+    if not force and os.path.exists(TORCH_OUT) and os.path.getmtime(TORCH_OUT) >= max(os.path.getmtime(TORCH_SRC), os.path.getmtime(header)):
+        return
+    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-I{torch}/include", f"-I{cuda}/include", TORCH_SRC,
+           "-o", TORCH_OUT, f"-L{torch}/lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or r.returncode != 0:
+        sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed; see output above")
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     nvcc = _nvcc()
+    _build_torch_ops(force, verbose)
     objdir = os.path.join(CSRC, "build")
     os.makedirs(objdir, exist_ok=True)
     hdr_time = _newest_header()

@@ -471,8 +471,7 @@ int paged_rows(int group, int max_q) {
   const long long rows = static_cast<long long>(group) * max_q;
   return rows <= 16 ? 16 : rows <= 64 ? 64 : 128;
 }
-// CTAs of a launch: two on an SM where the row tile is small.
-int paged_ctas(int sm_count, int rows) { return rows == 16 ? 2 * sm_count : sm_count; }
+int paged_ctas(int sm_count, int rows) { return paged_ctas_per_sm(rows) * sm_count; }
 
 // Parts of the workspace: counters, then the pieces' O, then their row statistics; two pieces per CTA.
 size_t paged_counter_bytes(int ctas) { return (static_cast<size_t>(ctas) * sizeof(int) + 127) / 128 * 128; }

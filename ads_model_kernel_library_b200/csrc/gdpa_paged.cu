@@ -942,6 +942,8 @@ int launch(const PagedLaunch& l) {
 
 }  // namespace
 
+int paged_ctas_per_sm(int rows) { return rows == 16 ? PagedShape<128, 16>::kCtasPerSm : 1; }
+
 int launch_paged(const PagedLaunch& l, int head_dim) {
   auto go = [&](auto dim) -> int {
     constexpr int D = decltype(dim)::value;

@@ -39,7 +39,7 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kItemSlots = 4;
-constexpr int kItemUnits = 2;           // what an item costs besides its tiles, in tiles
+constexpr int kItemUnits = 4;           // what an item costs besides its tiles, in tiles
 constexpr float kMax8 = 448.f;
 constexpr float kNoMax = -3.0e38f;     // running maximum of a row that has seen no key
 constexpr float kLeastScale = 7.888609e-31f;  // 2^-100
@@ -104,6 +104,14 @@ struct PagedItem {
   int pieces;   // stretches the item is cut into
   int first;    // CTA of the first of them
 };
+
+// One more of the CTAs of an item: how many came before.  Release and acquire: what the caller's CTA wrote before its barrier is seen by
+// whoever counts after it.
+__device__ __forceinline__ int count_arrival(int* counter) {
+  int old;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+  return old;
+}
 
 struct KeyRange {
   int lo, hi;
@@ -850,62 +858,83 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         named_bar_sync(bar_wg, 128);  // the next item writes over fac and row_at
       } else {
         // the last of the item's CTAs joins the pieces
-        __threadfence();
         named_bar_sync(3, 128 * kGroups);
-        if (threadIdx.x == 0) {
-          const bool last = atomicAdd(a.counters + it.first, 1) == it.pieces - 1;
-          __threadfence();
-          *last_flag = last;
-        }
+        if (threadIdx.x == 0) *last_flag = count_arrival(a.counters + it.first) == it.pieces - 1;
         named_bar_sync(3, 128 * kGroups);
         if (*last_flag) {
-          // a warp has a row: the weights of its pieces over the lanes, then the pieces in order
-          for (int r = warp; r < it.rows; r += 4 * kGroups) {
-            constexpr int V = D / 32;
-            float acc[V], m_all = kNoMax, l_all = 0.f;
+          // A warp has two rows: the weights of 32 pieces over its lanes, then the pieces in order.  What this takes is trips to L2: eight
+          // pieces' values of both rows are asked for before the first is used, and with the pieces' statistics.
+          constexpr int V = D / 32, kAhead = 8, kWarpsHere = 4 * kGroups;
+          const auto slot_of = [&](int k) { return static_cast<long long>(2 * (it.first + k) + (k == 0 ? 1 : 0)); };
+          for (int ra = warp; ra < it.rows; ra += 2 * kWarpsHere) {
+            const int row[2] = {ra, min(ra + kWarpsHere, it.rows - 1)};
+            float acc[2][V], m_all[2] = {kNoMax, kNoMax}, l_all[2] = {0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < V; ++e) acc[e] = 0.f;
-            auto slot_of = [&](int k) { return static_cast<long long>(2 * (it.first + k) + (k == 0 ? 1 : 0)); };
+            for (int e = 0; e < V; ++e) acc[0][e] = acc[1][e] = 0.f;
             if constexpr (SOFTMAX) {
-              for (int k0 = 0; k0 < it.pieces; k0 += 32) {
-                const int k = k0 + lane;
-                m_all = fmaxf(m_all, warp_max(k < it.pieces ? __ldcg(a.part_ml + slot_of(k) * 2 * NMAX + r) : kNoMax));
+              for (int k = lane; k < it.pieces; k += 32) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) m_all[x] = fmaxf(m_all[x], __ldcg(a.part_ml + slot_of(k) * 2 * NMAX + row[x]));
               }
+#pragma unroll
+              for (int x = 0; x < 2; ++x) m_all[x] = warp_max(m_all[x]);
             }
             for (int k0 = 0; k0 < it.pieces; k0 += 32) {
-              const int k = k0 + lane;
-              float w = 0.f;
-              if (k < it.pieces) {
-                const float* const ml = a.part_ml + slot_of(k) * 2 * NMAX;
-                w = SOFTMAX ? ex2_approx(__ldcg(ml + r) - m_all) : 1.f;
-                if constexpr (SOFTMAX) l_all += w * __ldcg(ml + NMAX + r);
-              }
               const int n = min(32, it.pieces - k0);
-#pragma unroll 8
-              for (int i = 0; i < n; ++i) {
-                const float wi = __shfl_sync(kFull, w, i);
-                const float* const po = a.part_o + (slot_of(k0 + i) * NMAX + r) * D + lane * V;
-                float v[V];
-                if constexpr (V == 4) {
-                  const float4 x = __ldcg(reinterpret_cast<const float4*>(po));
-                  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-                } else {
-                  const float2 x = __ldcg(reinterpret_cast<const float2*>(po));
-                  v[0] = x.x, v[1] = x.y;
+              float w[2];
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                w[x] = lane < n ? 1.f : 0.f;
+                if constexpr (SOFTMAX) {
+                  const float* const ml = a.part_ml + slot_of(k0 + min(lane, n - 1)) * 2 * NMAX + row[x];
+                  const float m = __ldcg(ml), l = __ldcg(ml + NMAX);
+                  w[x] *= ex2_approx(m - m_all[x]);
+                  if (lane < n) l_all[x] += w[x] * l;
+                }
+              }
+              for (int i0 = 0; i0 < n; i0 += kAhead) {
+                float v[2][kAhead][V];
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                  const float* const po = a.part_o + slot_of(k0 + min(i0 + i, n - 1)) * NMAX * D + lane * V;
+#pragma unroll
+                  for (int x = 0; x < 2; ++x) {
+                    if constexpr (V == 4) {
+                      const float4 u = __ldcg(reinterpret_cast<const float4*>(po + row[x] * D));
+                      v[x][i][0] = u.x, v[x][i][1] = u.y, v[x][i][2] = u.z, v[x][i][3] = u.w;
+                    } else {
+                      const float2 u = __ldcg(reinterpret_cast<const float2*>(po + row[x] * D));
+                      v[x][i][0] = u.x, v[x][i][1] = u.y;
+                    }
+                  }
                 }
 #pragma unroll
-                for (int e = 0; e < V; ++e) acc[e] = fmaf(wi, v[e], acc[e]);
+                for (int i = 0; i < kAhead; ++i) {
+                  if (i0 + i < n) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                      const float wi = __shfl_sync(kFull, w[x], i0 + i);
+#pragma unroll
+                      for (int e = 0; e < V; ++e) acc[x][e] = fmaf(wi, v[x][i][e], acc[x][e]);
+                    }
+                  }
+                }
               }
             }
-            float inv = 1.f;
-            if constexpr (SOFTMAX) {
 #pragma unroll
-              for (int s = 16; s > 0; s >>= 1) l_all += __shfl_xor_sync(kFull, l_all, s);
-              inv = l_all > 0.f || l_all != l_all ? 1.f / l_all : 0.f;
+            for (int x = 0; x < 2; ++x) {
+              float inv = 1.f;
+              if constexpr (SOFTMAX) {
+#pragma unroll
+                for (int s = 16; s > 0; s >>= 1) l_all[x] += __shfl_xor_sync(kFull, l_all[x], s);
+                inv = l_all[x] > 0.f || l_all[x] != l_all[x] ? 1.f / l_all[x] : 0.f;
+              }
+              if (x == 0 || ra + kWarpsHere < it.rows) {
+                uint32_t* const dst = reinterpret_cast<uint32_t*>(a.o + reinterpret_cast<const long long*>(smem + L::kRowOff)[row[x]] + lane * V);
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) dst[e] = pack_bf16x2(acc[x][2 * e] * inv, acc[x][2 * e + 1] * inv);
+              }
             }
-            uint32_t* const dst = reinterpret_cast<uint32_t*>(a.o + reinterpret_cast<const long long*>(smem + L::kRowOff)[r] + lane * V);
-#pragma unroll
-            for (int e = 0; e < V / 2; ++e) dst[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
           }
         }
         named_bar_sync(3, 128 * kGroups);

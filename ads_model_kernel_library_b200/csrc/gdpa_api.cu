@@ -464,6 +464,19 @@ int make_cache_tmap(CUtensorMap* m, const void* base, const long long (&strides)
   return r == CUDA_SUCCESS ? GDPA_OK : GDPA_ERR_DRIVER;
 }
 
+// The map of the split Q: boxes of `box_rows` rows of one plane.
+int make_q8_tmap(CUtensorMap* m, const void* base, int planes, long long rows, int head_dim, int box_rows) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (enc == nullptr) return GDPA_ERR_DRIVER;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(planes)};
+  const cuuint64_t bytes[2] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(rows) * head_dim};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(head_dim), static_cast<cuuint32_t>(box_rows), 1u}, step[3] = {1u, 1u, 1u};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, bytes, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? GDPA_OK : GDPA_ERR_DRIVER;
+}
+
 bool aligned16(const void* a, const void* b) { return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u) == 0; }
 
 // Rows of a row tile: the smallest that holds a request's (query, head of the group) rows, 128 at most.
@@ -473,10 +486,21 @@ int paged_rows(int group, int max_q) {
 }
 int paged_ctas(int sm_count, int rows) { return paged_ctas_per_sm(rows) * sm_count; }
 
-// Parts of the workspace: counters, then the pieces' O, then their row statistics; two pieces per CTA.
-size_t paged_counter_bytes(int ctas) { return (static_cast<size_t>(ctas) * sizeof(int) + 127) / 128 * 128; }
-size_t paged_part_bytes(int ctas, int rows, int head_dim) { return static_cast<size_t>(2) * ctas * rows * head_dim * sizeof(float); }
-size_t paged_stat_bytes(int ctas, int rows) { return static_cast<size_t>(2) * ctas * 2 * rows * sizeof(float); }
+// The workspace: counters, the pieces' O and row statistics (two pieces per CTA), Q in two halves, the rows' factors.
+struct PagedWorkspace {
+  size_t part_o, part_ml, q8, qa, bytes;
+};
+PagedWorkspace paged_workspace(int ctas, int rows, long long total_q, int heads, int head_dim) {
+  auto up = [](size_t x) { return (x + 127) / 128 * 128; };
+  const size_t n = static_cast<size_t>(total_q) * heads;
+  PagedWorkspace w;
+  w.part_o = up(static_cast<size_t>(ctas) * sizeof(int));
+  w.part_ml = w.part_o + up(static_cast<size_t>(2) * ctas * rows * head_dim * sizeof(float));
+  w.q8 = w.part_ml + up(static_cast<size_t>(2) * ctas * 2 * rows * sizeof(float));
+  w.qa = w.q8 + up(2 * n * head_dim);
+  w.bytes = w.qa + up(n * sizeof(float));
+  return w;
+}
 }  // namespace
 
 int gdpa_build_block_tables(const GdpaBlockTableParams* p, gdpa_stream_t stream) {
@@ -552,12 +576,11 @@ int gdpa_append_kv_cache_fp8(const GdpaCacheAppendParams* p, gdpa_stream_t strea
   return rc;
 }
 
-size_t gdpa_paged_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t max_seq_len_q) {
+size_t gdpa_paged_workspace_bytes(int64_t total_q, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t max_seq_len_q) {
   DeviceInfo di;
-  if (heads <= 0 || kv_heads <= 0 || head_dim <= 0 || max_seq_len_q < 0 || device_info(&di) != GDPA_OK) return 0;
+  if (total_q < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || max_seq_len_q < 0 || device_info(&di) != GDPA_OK) return 0;
   const int rows = paged_rows(heads / kv_heads, max_seq_len_q);
-  const int ctas = paged_ctas(di.sm_count, rows);
-  return paged_counter_bytes(ctas) + paged_part_bytes(ctas, rows, head_dim) + paged_stat_bytes(ctas, rows);
+  return paged_workspace(paged_ctas(di.sm_count, rows), rows, total_q, heads, head_dim).bytes;
 }
 
 int gdpa_fwd_paged_fp8(const GdpaPagedParams* p, gdpa_stream_t stream) {
@@ -571,7 +594,7 @@ int gdpa_fwd_paged_fp8(const GdpaPagedParams* p, gdpa_stream_t stream) {
   if (p->num_blocks < 0 || p->num_blocks > 0x7fffffffll || (static_cast<long long>(p->table_width) << shift) > (1ll << 30)) return GDPA_ERR_BAD_ARG;
   if (p->window_plus_one < 0 || p->window_plus_one > (1 << 29)) return GDPA_ERR_BAD_ARG;
   const int group = p->heads / p->kv_heads;
-  if (static_cast<long long>(p->max_seq_len_q) * group > (1ll << 30)) return GDPA_ERR_BAD_ARG;
+  if (static_cast<long long>(p->max_seq_len_q) * group > (1ll << 30) || p->total_q * group > 0x7fffff00ll) return GDPA_ERR_BAD_ARG;
   PagedLaunch l;
   std::memset(&l, 0, sizeof(l));
   int rc;
@@ -588,13 +611,14 @@ int gdpa_fwd_paged_fp8(const GdpaPagedParams* p, gdpa_stream_t stream) {
   if ((rc = device_info(&di)) != GDPA_OK) return rc;
   l.rows = paged_rows(group, p->max_seq_len_q);
   l.grid = paged_ctas(di.sm_count, l.rows);
-  const size_t counters = paged_counter_bytes(l.grid), parts = paged_part_bytes(l.grid, l.rows, p->head_dim);
-  if (p->workspace_bytes < static_cast<int64_t>(counters + parts + paged_stat_bytes(l.grid, l.rows))) return GDPA_ERR_CAPACITY;
+  const PagedWorkspace w = paged_workspace(l.grid, l.rows, p->total_q, p->heads, p->head_dim);
+  if (p->workspace_bytes < static_cast<int64_t>(w.bytes)) return GDPA_ERR_CAPACITY;
+  uint8_t* const ws = static_cast<uint8_t*>(p->workspace);
+  if ((rc = make_q8_tmap(&l.tm_q, ws + w.q8, 2 * p->kv_heads, p->total_q * group, p->head_dim, l.rows)) != GDPA_OK) return rc;
   // a cache without blocks still needs valid maps: of one block in the place of Q, which no coordinate reaches
   const long long blocks = p->num_blocks > 0 ? p->num_blocks : 1;
   if ((rc = make_cache_tmap(&l.tm_k, p->num_blocks > 0 ? p->k_cache : p->q, ks, blocks, p->block_size, p->kv_heads, p->head_dim)) != GDPA_OK) return rc;
   if ((rc = make_cache_tmap(&l.tm_v, p->num_blocks > 0 ? p->v_cache : p->q, vs, blocks, p->block_size, p->kv_heads, p->head_dim)) != GDPA_OK) return rc;
-  uint8_t* const ws = static_cast<uint8_t*>(p->workspace);
   PagedArgs& a = l.args;
   a.q = static_cast<const __nv_bfloat16*>(p->q);
   a.o = static_cast<__nv_bfloat16*>(p->o);
@@ -620,15 +644,16 @@ int gdpa_fwd_paged_fp8(const GdpaPagedParams* p, gdpa_stream_t stream) {
   a.causal = p->causal != 0;
   a.window = p->window_plus_one - 1;
   a.counters = reinterpret_cast<int*>(ws);
-  a.part_o = reinterpret_cast<float*>(ws + counters);
-  a.part_ml = reinterpret_cast<float*>(ws + counters + parts);
+  a.part_o = reinterpret_cast<float*>(ws + w.part_o);
+  a.part_ml = reinterpret_cast<float*>(ws + w.part_ml);
+  a.qa = reinterpret_cast<float*>(ws + w.qa);
+  l.q8 = ws + w.q8;
   a.status = p->status;
   l.stream = static_cast<cudaStream_t>(stream);
-  if (cudaMemsetAsync(ws, 0, counters, l.stream) != cudaSuccess) return GDPA_ERR_LAUNCH;
   if (p->timing_start_event != nullptr) cudaEventRecord(static_cast<cudaEvent_t>(p->timing_start_event), l.stream);
   rc = launch_paged(l, p->head_dim);
   if (p->timing_stop_event != nullptr) cudaEventRecord(static_cast<cudaEvent_t>(p->timing_stop_event), l.stream);
-  if (rc == 0) g_launches.fetch_add(1);
+  if (rc == 0) g_launches.fetch_add(2);
   return rc;
 }
 

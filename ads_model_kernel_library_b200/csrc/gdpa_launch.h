@@ -239,14 +239,17 @@ struct PagedArgs {
   float scale;
   int causal;
   int window;                  // -1 = none
-  int* counters;               // one per CTA, zero at the launch
+  float* qa;                   // [kv_heads, total_q * group]: factor of a row's scores
+  int* counters;               // one per CTA
   float* part_o;               // [2 per CTA][rows of a tile][head_dim]
   float* part_ml;              // [2 per CTA][2][rows of a tile]
   int* status;
 };
 
 struct PagedLaunch {
+  CUtensorMap tm_q;        // over q8, [2 * kv_heads, total_q * group, head_dim]: a box is a row tile of one head, hi or lo
   CUtensorMap tm_k, tm_v;  // over [blocks, kv_heads, block_size, head_dim]: a box is one block of one head
+  uint8_t* q8;
   PagedArgs args;
   int rows;                // rows of a tile: 16, 64 or 128
   int grid;

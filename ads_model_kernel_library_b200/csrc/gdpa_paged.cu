@@ -25,7 +25,8 @@
 // CTA that finishes it last (an atomic count per item) joins them in the order of the pieces, so the result does not depend on who
 // was last.  No CTA waits for another.
 //
-// Roles: kGroups warpgroups (element-wise work, epilogue), one warp of TMA loads, one warp that issues MMAs, two that fetch Q.
+// Roles: kGroups warpgroups (element-wise work, epilogue), one warp of TMA loads, one warp that issues MMAs.  A small kernel before this one
+// splits Q and zeroes the items' counters; this one's beginning (barriers, tensor memory, the scan of the lengths) overlaps it.
 #include <cuda_bf16.h>
 
 #include <type_traits>
@@ -53,9 +54,9 @@ struct PagedShape {
   static constexpr int kStages = (NMAX <= 16 || NMAX > 64 ? 3 : 5) * (D == 128 ? 1 : 2);
   static constexpr int kQBytes = NMAX * D;             // hi, then lo
   static constexpr int kPBytes = NMAX * kTile;
-  static constexpr int kWarps = 4 * kGroups + 4;
+  static constexpr int kWarps = 4 * kGroups + 2;
   static constexpr int kThreads = 32 * kWarps;
-  static constexpr int kLoadWarp = 4 * kGroups, kMmaWarp = kLoadWarp + 1, kQWarp = kLoadWarp + 2;
+  static constexpr int kLoadWarp = 4 * kGroups, kMmaWarp = kLoadWarp + 1;
   static constexpr int kTmemCols = NMAX <= 16 ? 64 : NMAX <= 64 ? 256 : 512;  // S0, S1, O of NMAX columns each
   static constexpr float kTarget = 64.f;
 
@@ -234,7 +235,8 @@ __device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)
 
 template <int D, int NMAX, bool SOFTMAX>
 __global__ void __launch_bounds__(PagedShape<D, NMAX>::kThreads, PagedShape<D, NMAX>::kCtasPerSm)
-gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PagedArgs a) {
+gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                  const PagedArgs a) {
   using L = PagedShape<D, NMAX>;
   constexpr int kGroups = L::kGroups;
   extern __shared__ uint8_t smem_raw[];
@@ -252,9 +254,9 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       uint32_t n = 1;
       if (i >= L::B_SC_FULL && i < L::B_SC_FULL + L::kStages) n = 32;
       if (i == L::B_P_FULL) n = 128 * kGroups;
-      if (i >= L::B_Q_FULL && i < L::B_Q_FULL + 2) n = 64;
+      if (i >= L::B_Q_FULL && i < L::B_Q_FULL + 2) n = 33;
       if (i >= L::B_Q_EMPTY && i < L::B_Q_EMPTY + 2) n = 1 + 4 * kGroups;
-      if (i >= L::B_ITEM_EMPTY && i < L::B_ITEM_EMPTY + kItemSlots) n = 3 + 4 * kGroups;
+      if (i >= L::B_ITEM_EMPTY && i < L::B_ITEM_EMPTY + kItemSlots) n = 1 + 4 * kGroups;
       mbar_init(bar_base + 8u * i, n);
     }
     *abort_flag = 0;
@@ -265,6 +267,7 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     tmem_relinquish();
   }
   if (warp == L::kLoadWarp && lane == 0) {
+    tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
@@ -396,11 +399,33 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       }
       return publish(it);
     };
+    // Q of an item (both halves of its values, all NMAX rows: those past the item's are another request's, or zeros) and its rows'
+    // factors.  The kernel before this one makes them and may still run: nothing of it is read before this wait.
+    uint32_t q_pos = 0;
+    auto load_q = [&](const PagedItem& i) -> bool {
+      const uint32_t buf = q_pos & 1u;
+      const bool ok = mbar_wait(bar_base + 8u * (L::B_Q_EMPTY + buf), ((q_pos >> 1) & 1u) ^ 1u, abort_flag, a.status,
+                                 ((L::B_Q_EMPTY + buf) << 8) | ST_ROLE_LOAD);
+      if (!__all_sync(kFull, ok)) return false;
+      ++q_pos;
+      const long long row = static_cast<long long>(i.q_start) * a.group + i.row0;
+      const uint32_t bar = bar_base + 8u * (L::B_Q_FULL + buf), dst = smem_base + L::kQOff + buf * 2 * L::kQBytes;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, 2 * L::kQBytes);
+        tma_load_3d(dst, &tm_q, bar, 0, static_cast<int>(row), i.h);
+        tma_load_3d(dst + L::kQBytes, &tm_q, bar, 0, static_cast<int>(row), a.kv_heads + i.h);
+      }
+      for (int r = lane; r < NMAX; r += 32)
+        cp_async4(smem_base + L::kQaOff + (buf * NMAX + r) * 4, a.qa + i.h * a.total_q * a.group + row + min(r, i.rows - 1), true);
+      cp_async_mbar_arrive(bar);
+      return true;
+    };
     PagedItem it, ahead;
     int b = 0, b_ahead = 0;
     if (!next_item(it, b)) goto role_done;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (it.h >= 0 && it.tiles > 0 && !load_q(it)) goto role_done;
     for (; it.h >= 0; it = ahead, b = b_ahead) {
-      // the others learn of the next item before this one's tiles are asked for: its Q is fetched meanwhile
       if (!next_item(ahead, b_ahead)) goto role_done;
       const int n_blocks = min((it.len + block_size - 1) >> a.block_shift, a.table_width);
       const int* const table = a.block_tables + static_cast<long long>(b) * a.table_stride;
@@ -433,7 +458,10 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         }
         cp_async_mbar_arrive(bar_base + 8u * (L::B_SC_FULL + stage));
         loaded = pos + 1;
+        // the next item's Q: its buffer is the last item's, which is done when this item's first stages have been used
+        if (j == min(L::kStages, it.tiles - 1) && ahead.h >= 0 && ahead.tiles > 0 && !load_q(ahead)) goto role_done;
       }
+      if (it.tiles == 0 && ahead.h >= 0 && ahead.tiles > 0 && !load_q(ahead)) goto role_done;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == L::kMmaWarp) {
@@ -500,87 +528,6 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       }
     }
     if (owed.any && !issue_pv()) goto role_done;
-  } else if (warp >= L::kQWarp) {
-    // ------------------------------------------------------------------ Q: fetched, scaled, split in two
-    constexpr int kLanes = D / 8;  // lanes of one row, 16 bytes each
-    constexpr int kRowsAt = 32 / kLanes;
-    const int wq = warp - L::kQWarp;
-    uint32_t q_pos = 0;
-    while (true) {
-      const PagedItem it = take_item(ST_ROLE_LOAD);
-      if (it.h < 0) {
-        if (it.h == -2) goto role_done;
-        break;
-      }
-      if (it.tiles == 0) continue;
-      const uint32_t q_buf = q_pos & 1u;
-      PAGED_WAIT(L::B_Q_EMPTY + q_buf, ((q_pos >> 1) & 1u) ^ 1u, ST_ROLE_LOAD);
-      ++q_pos;
-      uint8_t* const hi = smem + L::kQOff + q_buf * 2 * L::kQBytes;
-      float* const qa = reinterpret_cast<float*>(smem + L::kQaOff) + q_buf * NMAX;
-      const int n = (it.rows + L::kCols - 1) / L::kCols * L::kCols;  // rows to the end of a warpgroup's columns: zeros
-      const int c8 = lane % kLanes;
-      constexpr int kAhead = NMAX >= 64 ? 8 : 4;
-      for (int r0 = wq * kRowsAt + lane / kLanes; r0 - lane / kLanes < n; r0 += 2 * kRowsAt * kAhead) {
-        uint4 u[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const int r = r0 + i * 2 * kRowsAt, g = it.row0 + r;
-          u[i] = make_uint4(0, 0, 0, 0);
-          if (r < it.rows)
-            u[i] = *reinterpret_cast<const uint4*>(a.q + (it.q_start + static_cast<long long>(g / a.group)) * a.q_strides[0] +
-                                                   (it.h * a.group + g % a.group) * a.q_strides[1] + c8 * 8);
-        }
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const int r = r0 + i * 2 * kRowsAt;
-          const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-          uint32_t top = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = max_u16x2(top, w[e] & 0x7fff7fffu);
-          top = max(top & 0xffffu, top >> 16);
-#pragma unroll
-          for (int s = kLanes / 2; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(kFull, top, s));
-          // 2^k with amax / 2^k in (224, 448]; a row that is not finite gives NaN
-          const bool finite = top < 0x7f80u;
-          int k = static_cast<int>(top >> 7) - 127 - 8 + ((top & 0x7fu) > 0x60u ? 1 : 0);
-          k = max(k, -100);
-          const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
-          uint32_t w_hi[2], w_lo[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float x[4];
-#pragma unroll
-            for (int f = 0; f < 2; ++f) {
-              x[2 * f] = finite ? __uint_as_float(w[2 * e + f] << 16) * inv : 0.f;
-              x[2 * f + 1] = finite ? __uint_as_float(w[2 * e + f] & 0xffff0000u) * inv : 0.f;
-            }
-            w_hi[e] = w_lo[e] = 0;
-#pragma unroll
-            for (int f = 0; f < 2; ++f) {
-              const uint32_t h = pack_f16x2(x[2 * f], x[2 * f + 1]);  // exact but for what lies 2^-24 below
-              const uint16_t eh = e4m3x2_from_f16x2(h);
-              const uint16_t el = e4m3x2_from_f16x2(sub_f16x2(h, f16x2_from_e4m3x2(eh)));
-              w_hi[e] |= static_cast<uint32_t>(eh) << (16 * f);
-              w_lo[e] |= static_cast<uint32_t>(el) << (16 * f);
-            }
-          }
-          if (r < n) {
-            // 16-byte pieces of a row change places with its number, as the tensor cores read them (128- or 64-byte swizzle)
-            const int piece = D == 128 ? (c8 >> 1) ^ (r & 7) : (c8 >> 1) ^ ((r >> 1) & 3);
-            uint8_t* const p = hi + r * D + piece * 16 + (c8 & 1) * 8;
-            *reinterpret_cast<uint2*>(p) = make_uint2(w_hi[0], w_hi[1]);
-            *reinterpret_cast<uint2*>(p + L::kQBytes) = make_uint2(w_lo[0], w_lo[1]);
-            if (c8 == 0) {
-              const float s = __uint_as_float(static_cast<uint32_t>(k + 127) << 23) * (SOFTMAX ? a.scale * 1.4426950408889634f : 1.f);
-              qa[r] = finite ? s : __uint_as_float(0x7fffffffu);
-            }
-          }
-        }
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(bar_base + 8u * (L::B_Q_FULL + q_buf));
-    }
   } else {
     // ------------------------------------------------------------------ element-wise work and epilogue
     // Warpgroup wg has columns [wg * kCols, (wg + 1) * kCols) of the 128 tokens, a thread one token.
@@ -958,13 +905,78 @@ role_done:
   if (warp == L::kMmaWarp) tmem_dealloc(tmem_base, L::kTmemCols);
 }
 
+// Q in the form the tensor cores take it, for the kernel after this one: rows of one K / V head one after the other (query, head of the
+// group), each scaled by a power of two to a largest element in (224, 448] and split in two e4m3 values, hi first, all rows' lo behind; their
+// factors; and the item counters, zeroed.  A row that is not finite becomes zeros with a factor of NaN.
+template <int D>
+__global__ void __launch_bounds__(256) gdpa_paged_prepare_kernel(const PagedArgs a, uint8_t* q8, int ctas) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // that kernel waits before it reads any of this
+  constexpr int kLanes = D / 8;  // lanes of one row, 16 bytes each
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < ctas; i += 256) a.counters[i] = 0;
+  const long long n = a.total_q * a.heads, rows = a.total_q * a.group;  // of one K / V head
+  const int c8 = threadIdx.x % kLanes;
+  const long long row0 = static_cast<long long>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  for (long long i = row0; i - threadIdx.x / kLanes < n; i += static_cast<long long>(gridDim.x) * (256 / kLanes)) {
+    const long long t = min(i, n - 1) / a.heads;
+    const int hd = static_cast<int>(min(i, n - 1) - t * a.heads), h = hd / a.group;
+    const uint4 u = *reinterpret_cast<const uint4*>(a.q + t * a.q_strides[0] + hd * a.q_strides[1] + c8 * 8);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = max_u16x2(top, w[e] & 0x7fff7fffu);
+    top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+    for (int s = kLanes / 2; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(kFull, top, s));
+    const bool finite = top < 0x7f80u;
+    const int k = max(static_cast<int>(top >> 7) - 127 - 8 + ((top & 0x7fu) > 0x60u ? 1 : 0), -100);
+    const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+    uint32_t hi[2], lo[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      uint16_t eh[2], el[2];
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        const uint32_t v = finite ? w[2 * e + f] : 0u;
+        const uint32_t x = pack_f16x2(__uint_as_float(v << 16) * inv, __uint_as_float(v & 0xffff0000u) * inv);  // exact but for what lies 2^-24 below
+        eh[f] = e4m3x2_from_f16x2(x);
+        el[f] = e4m3x2_from_f16x2(sub_f16x2(x, f16x2_from_e4m3x2(eh[f])));
+      }
+      hi[e] = __byte_perm(eh[0], eh[1], 0x5410);
+      lo[e] = __byte_perm(el[0], el[1], 0x5410);
+    }
+    if (i < n) {
+      const long long r = h * rows + t * a.group + (hd - h * a.group);
+      *reinterpret_cast<uint2*>(q8 + r * D + c8 * 8) = make_uint2(hi[0], hi[1]);
+      *reinterpret_cast<uint2*>(q8 + (a.kv_heads * rows + r) * D + c8 * 8) = make_uint2(lo[0], lo[1]);
+      const float s = __uint_as_float(static_cast<uint32_t>(k + 127) << 23) * (a.act == ACT_SOFTMAX ? a.scale * 1.4426950408889634f : 1.f);
+      if (c8 == 0) a.qa[r] = finite ? s : __uint_as_float(0x7fffffffu);
+    }
+  }
+}
+
+// Launch of `kernel` that may begin while the kernel before it in the stream still runs (it waits for that one itself).
+template <class... P, class... A>
+int launch_after(void (*kernel)(P...), int grid, int threads, int smem, cudaStream_t stream, const A&... args) {
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(grid);
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  c.attrs = &early;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, args...) == cudaSuccess ? 0 : GDPA_ERR_LAUNCH_;
+}
+
 template <int D, int NMAX>
 int launch(const PagedLaunch& l) {
   using L = PagedShape<D, NMAX>;
   auto go = [&](auto kernel) -> int {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynBytes) != cudaSuccess) return GDPA_ERR_LAUNCH_;
-    kernel<<<l.grid, L::kThreads, L::kDynBytes, l.stream>>>(l.tm_k, l.tm_v, l.args);
-    return cudaGetLastError() == cudaSuccess ? 0 : GDPA_ERR_LAUNCH_;
+    return launch_after(kernel, l.grid, L::kThreads, L::kDynBytes, l.stream, l.tm_q, l.tm_k, l.tm_v, l.args);
   };
   return l.args.act == ACT_SOFTMAX ? go(gdpa_paged_kernel<D, NMAX, true>) : go(gdpa_paged_kernel<D, NMAX, false>);
 }
@@ -974,6 +986,11 @@ int launch(const PagedLaunch& l) {
 int paged_ctas_per_sm(int rows) { return rows == 16 ? PagedShape<128, 16>::kCtasPerSm : 1; }
 
 int launch_paged(const PagedLaunch& l, int head_dim) {
+  const long long blocks = (l.args.total_q * l.args.heads * (head_dim / 8) + 255) / 256;
+  const int grid = static_cast<int>(blocks < 4096 ? blocks : 4096);
+  if (head_dim == 128) gdpa_paged_prepare_kernel<128><<<grid, 256, 0, l.stream>>>(l.args, l.q8, l.grid);
+  else gdpa_paged_prepare_kernel<64><<<grid, 256, 0, l.stream>>>(l.args, l.q8, l.grid);
+  if (cudaGetLastError() != cudaSuccess) return GDPA_ERR_LAUNCH_;
   auto go = [&](auto dim) -> int {
     constexpr int D = decltype(dim)::value;
     return l.rows == 16 ? launch<D, 16>(l) : l.rows == 64 ? launch<D, 64>(l) : launch<D, 128>(l);

@@ -21,7 +21,7 @@ namespace {
 struct EntryPoints {
   int (*build_block_tables)(const GdpaBlockTableParams*, gdpa_stream_t);
   int (*append)(const GdpaCacheAppendParams*, gdpa_stream_t);
-  size_t (*workspace_bytes)(int32_t, int32_t, int32_t, int32_t);
+  size_t (*workspace_bytes)(int64_t, int32_t, int32_t, int32_t, int32_t);
   int (*attend)(const GdpaPagedParams*, gdpa_stream_t);
   const char* (*strerror)(int);
 } g_call{};
@@ -206,7 +206,7 @@ at::Tensor attend_paged_fp8(const at::Tensor& query, const at::Tensor& k_cache, 
   const c10::cuda::CUDAGuard guard(query.device());
   at::Tensor o = empty({total_q, heads, dim}, at::kBFloat16, query);
   if (total_q == 0 || batch == 0) return o;
-  const size_t bytes = g_call.workspace_bytes(static_cast<int32_t>(heads), static_cast<int32_t>(kv_heads), static_cast<int32_t>(dim),
+  const size_t bytes = g_call.workspace_bytes(total_q, static_cast<int32_t>(heads), static_cast<int32_t>(kv_heads), static_cast<int32_t>(dim),
                                               static_cast<int32_t>(max_seq_len_q));
   const at::Tensor workspace = empty({static_cast<int64_t>(bytes)}, at::kByte, query);
   GdpaPagedParams p{};

@@ -347,7 +347,7 @@ def _load() -> C.CDLL:
         fn.restype = C.c_int
         fn.argtypes = [C.POINTER(params), C.c_void_p]
     lib.gdpa_paged_workspace_bytes.restype = C.c_size_t
-    lib.gdpa_paged_workspace_bytes.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32]
+    lib.gdpa_paged_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32]
     lib.gdpa_strerror.restype = C.c_char_p
     lib.gdpa_strerror.argtypes = [C.c_int]
     lib.gdpa_launch_count.restype = C.c_int64

@@ -462,12 +462,12 @@ typedef struct GdpaPagedParams {
   void* workspace;             /* gdpa_paged_workspace_bytes() bytes, 16-byte aligned; one per call in flight */
   int64_t workspace_bytes;
   int32_t* status;
-  void* timing_start_event;    /* optional cudaEvent_t pair around the kernel */
+  void* timing_start_event;    /* optional cudaEvent_t pair around the kernels */
   void* timing_stop_event;
 } GdpaPagedParams;
 
 /* Bytes of the workspace of a call on the current device; 0 if there is none. */
-size_t gdpa_paged_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t max_seq_len_q);
+size_t gdpa_paged_workspace_bytes(int64_t total_q, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t max_seq_len_q);
 
 int gdpa_fwd_paged_fp8(const GdpaPagedParams* params, gdpa_stream_t stream);
 

@@ -484,7 +484,7 @@ int paged_rows(int group, int max_q) {
   const long long rows = static_cast<long long>(group) * max_q;
   return rows <= 16 ? 16 : rows <= 64 ? 64 : 128;
 }
-int paged_ctas(int sm_count, int rows) { return paged_ctas_per_sm(rows) * sm_count; }
+int paged_ctas(int sm_count, int rows, int head_dim) { return paged_ctas_per_sm(rows, head_dim) * sm_count; }
 
 // The workspace: counters, the pieces' O and row statistics (two pieces per CTA), Q in two halves, the rows' factors.
 struct PagedWorkspace {
@@ -580,7 +580,7 @@ size_t gdpa_paged_workspace_bytes(int64_t total_q, int32_t heads, int32_t kv_hea
   DeviceInfo di;
   if (total_q < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || max_seq_len_q < 0 || device_info(&di) != GDPA_OK) return 0;
   const int rows = paged_rows(heads / kv_heads, max_seq_len_q);
-  return paged_workspace(paged_ctas(di.sm_count, rows), rows, total_q, heads, head_dim).bytes;
+  return paged_workspace(paged_ctas(di.sm_count, rows, head_dim), rows, total_q, heads, head_dim).bytes;
 }
 
 int gdpa_fwd_paged_fp8(const GdpaPagedParams* p, gdpa_stream_t stream) {
@@ -610,7 +610,7 @@ int gdpa_fwd_paged_fp8(const GdpaPagedParams* p, gdpa_stream_t stream) {
   DeviceInfo di;
   if ((rc = device_info(&di)) != GDPA_OK) return rc;
   l.rows = paged_rows(group, p->max_seq_len_q);
-  l.grid = paged_ctas(di.sm_count, l.rows);
+  l.grid = paged_ctas(di.sm_count, l.rows, p->head_dim);
   const PagedWorkspace w = paged_workspace(l.grid, l.rows, p->total_q, p->heads, p->head_dim);
   if (p->workspace_bytes < static_cast<int64_t>(w.bytes)) return GDPA_ERR_CAPACITY;
   uint8_t* const ws = static_cast<uint8_t*>(p->workspace);

@@ -279,6 +279,6 @@ int launch_build_schedule(const SchedArgs& a, cudaStream_t stream);
 int launch_block_tables(const BlockTableArgs& a, int sm_count, cudaStream_t stream);
 int launch_cache_append(const CacheAppendArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream);
 int launch_paged(const PagedLaunch& l, int head_dim);
-int paged_ctas_per_sm(int rows);  // resident CTAs of the kernel for row tiles of `rows`: a launch has that many
+int paged_ctas_per_sm(int rows, int head_dim);  // resident CTAs of the kernel for row tiles of `rows`: a launch has that many
 
 }  // namespace gdpa

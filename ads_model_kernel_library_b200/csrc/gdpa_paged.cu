@@ -49,9 +49,9 @@ template <int D, int NMAX>
 struct PagedShape {
   static constexpr int kCols = NMAX < 32 ? NMAX : 32;  // columns of a warpgroup
   static constexpr int kGroups = NMAX / kCols;         // warpgroups
-  static constexpr int kCtasPerSm = NMAX <= 16 ? 2 : 1;
+  static constexpr int kCtasPerSm = NMAX > 16 ? 1 : D == 128 ? 2 : 3;
   static constexpr int kTileBytes = kTile * D;         // K or V tile
-  static constexpr int kStages = (NMAX <= 16 || NMAX > 64 ? 3 : 5) * (D == 128 ? 1 : 2);
+  static constexpr int kStages = NMAX <= 16 ? 3 : (NMAX > 64 ? 3 : 5) * (D == 128 ? 1 : 2);
   static constexpr int kQBytes = NMAX * D;             // hi, then lo
   static constexpr int kPBytes = NMAX * kTile;
   static constexpr int kWarps = 4 * kGroups + 2;
@@ -983,7 +983,9 @@ int launch(const PagedLaunch& l) {
 
 }  // namespace
 
-int paged_ctas_per_sm(int rows) { return rows == 16 ? PagedShape<128, 16>::kCtasPerSm : 1; }
+int paged_ctas_per_sm(int rows, int head_dim) {
+  return rows > 16 ? 1 : head_dim == 128 ? PagedShape<128, 16>::kCtasPerSm : PagedShape<64, 16>::kCtasPerSm;
+}
 
 int launch_paged(const PagedLaunch& l, int head_dim) {
   const long long blocks = (l.args.total_q * l.args.heads * (head_dim / 8) + 255) / 256;

@@ -479,10 +479,10 @@ int make_q8_tmap(CUtensorMap* m, const void* base, int planes, long long rows, i
 
 bool aligned16(const void* a, const void* b) { return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u) == 0; }
 
-// Rows of a row tile: the smallest that holds a request's (query, head of the group) rows, 128 at most.
+// Rows of an item: the smallest of the kernels' that holds a request's (query, head of the group) rows, 256 at most.
 int paged_rows(int group, int max_q) {
   const long long rows = static_cast<long long>(group) * max_q;
-  return rows <= 16 ? 16 : rows <= 64 ? 64 : 128;
+  return rows <= 16 ? 16 : rows <= 64 ? 64 : 256;
 }
 int paged_ctas(int sm_count, int rows, int head_dim) { return paged_ctas_per_sm(rows, head_dim) * sm_count; }
 
@@ -614,7 +614,7 @@ int gdpa_fwd_paged_fp8(const GdpaPagedParams* p, gdpa_stream_t stream) {
   const PagedWorkspace w = paged_workspace(l.grid, l.rows, p->total_q, p->heads, p->head_dim);
   if (p->workspace_bytes < static_cast<int64_t>(w.bytes)) return GDPA_ERR_CAPACITY;
   uint8_t* const ws = static_cast<uint8_t*>(p->workspace);
-  if ((rc = make_q8_tmap(&l.tm_q, ws + w.q8, 2 * p->kv_heads, p->total_q * group, p->head_dim, l.rows)) != GDPA_OK) return rc;
+  if ((rc = make_q8_tmap(&l.tm_q, ws + w.q8, 2 * p->kv_heads, p->total_q * group, p->head_dim, l.rows < kTile ? l.rows : kTile)) != GDPA_OK) return rc;
   // a cache without blocks still needs valid maps: of one block in the place of Q, which no coordinate reaches
   const long long blocks = p->num_blocks > 0 ? p->num_blocks : 1;
   if ((rc = make_cache_tmap(&l.tm_k, p->num_blocks > 0 ? p->k_cache : p->q, ks, blocks, p->block_size, p->kv_heads, p->head_dim)) != GDPA_OK) return rc;

@@ -251,7 +251,7 @@ struct PagedLaunch {
   CUtensorMap tm_k, tm_v;  // over [blocks, kv_heads, block_size, head_dim]: a box is one block of one head
   uint8_t* q8;
   PagedArgs args;
-  int rows;                // rows of a tile: 16, 64 or 128
+  int rows;                // rows of an item: 16, 64 or 256
   int grid;
   cudaStream_t stream;
 };
@@ -279,6 +279,7 @@ int launch_build_schedule(const SchedArgs& a, cudaStream_t stream);
 int launch_block_tables(const BlockTableArgs& a, int sm_count, cudaStream_t stream);
 int launch_cache_append(const CacheAppendArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream);
 int launch_paged(const PagedLaunch& l, int head_dim);
+int launch_paged_rows(const PagedLaunch& l, int head_dim);  // of launch_paged, for row tiles of 256
 int paged_ctas_per_sm(int rows, int head_dim);  // resident CTAs of the kernel for row tiles of `rows`: a launch has that many
 
 }  // namespace gdpa

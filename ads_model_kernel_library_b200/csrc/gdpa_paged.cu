@@ -31,19 +31,11 @@
 
 #include <type_traits>
 
-#include "gdpa_common.cuh"
-#include "gdpa_launch.h"
+#include "gdpa_paged.cuh"
 
 namespace gdpa {
 
 namespace {
-
-constexpr unsigned kFull = 0xffffffffu;
-constexpr int kItemSlots = 4;
-constexpr int kItemUnits = 4;           // what an item costs besides its tiles, in tiles
-constexpr float kMax8 = 448.f;
-constexpr float kNoMax = -3.0e38f;     // running maximum of a row that has seen no key
-constexpr float kLeastScale = 7.888609e-31f;  // 2^-100
 
 template <int D, int NMAX>
 struct PagedShape {
@@ -58,6 +50,7 @@ struct PagedShape {
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kLoadWarp = 4 * kGroups, kMmaWarp = kLoadWarp + 1;
   static constexpr int kTmemCols = NMAX <= 16 ? 64 : NMAX <= 64 ? 256 : 512;  // S0, S1, O of NMAX columns each
+  static constexpr int kQBuffers = 2;
   static constexpr float kTarget = 64.f;
 
   static constexpr int kKvOff = 0;                                  // [stage]{K, V}
@@ -92,104 +85,6 @@ struct PagedShape {
   static_assert(kCtasPerSm * (kDynBytes + 1024) <= 228 * 1024, "shared memory");
 };
 
-// One stretch of tiles of one item, as the loader publishes it.
-struct PagedItem {
-  int h;        // K / V head; -1 ends the walk, -2: a wait ran out
-  int q_start;  // first query row of the request
-  int q_len;
-  int row0;     // first (query, head of the group) row of the tile
-  int rows;
-  int len;      // tokens of the request
-  int lo, hi;   // keys that any of the rows takes part with
-  int tile0, tiles;
-  int pieces;   // stretches the item is cut into
-  int first;    // CTA of the first of them
-};
-
-// One more of the CTAs of an item: how many came before.  Release and acquire: what the caller's CTA wrote before its barrier is seen by
-// whoever counts after it.
-__device__ __forceinline__ int count_arrival(int* counter) {
-  int old;
-  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
-  return old;
-}
-
-struct KeyRange {
-  int lo, hi;
-};
-// keys that query i takes part with; the queries are the last q_len positions of the request
-__device__ __forceinline__ KeyRange keys_of(int i, int q_len, int len, int causal, int window) {
-  const int p = len - q_len + i;
-  KeyRange r{0, len};
-  if (causal) r.hi = min(r.hi, p + 1);
-  if (window >= 0) r.lo = max(0, p - window), r.hi = min(r.hi, p + window + 1);
-  if (r.hi <= r.lo) r.lo = r.hi = 0;
-  return r;
-}
-// ... and any of queries i0 .. i1
-__device__ __forceinline__ KeyRange keys_of_any(int i0, int i1, int q_len, int len, int causal, int window) {
-  const int p0 = len - q_len + i0, p1 = len - q_len + i1;
-  KeyRange r{0, len};
-  if (causal) r.hi = min(r.hi, p1 + 1);
-  if (window >= 0) r.lo = max(0, p0 - window), r.hi = min(r.hi, p1 + window + 1);
-  if (r.hi <= r.lo) r.lo = r.hi = 0;
-  return r;
-}
-__device__ __forceinline__ int tiles_of(const KeyRange& r) { return r.hi > r.lo ? (r.hi + kTile - 1) / kTile - r.lo / kTile : 0; }
-
-struct Request {
-  int q_start, q_len, len;
-};
-__device__ __forceinline__ Request load_request(const PagedArgs& a, int b) {
-  long long q0 = load_offset(a.q_off, b, a.off64), q1 = load_offset(a.q_off, b + 1, a.off64);
-  q0 = clamp_ll(q0, 0, a.total_q);
-  q1 = clamp_ll(q1, q0, a.total_q);
-  const long long most = static_cast<long long>(a.table_width) << a.block_shift;
-  Request r;
-  r.q_start = static_cast<int>(q0);
-  r.q_len = static_cast<int>(min(q1 - q0, static_cast<long long>(a.max_q)));
-  r.len = static_cast<int>(clamp_ll(load_offset(a.seq_lens, b, a.lens64), 0, most));
-  return r;
-}
-
-// Units of one K / V head of a request: its row tiles' KV tiles, one at least each (a row tile without keys has zeros to write), and
-// kItemUnits for the beginning and the end of each.
-template <int NMAX>
-__device__ __forceinline__ long long units_of(const PagedArgs& a, const Request& r) {
-  const int rows = r.q_len * a.group, nt = (rows + NMAX - 1) / NMAX;
-  if (!a.causal && a.window < 0) return static_cast<long long>(nt) * (kItemUnits + max(1, tiles_of(KeyRange{0, r.len})));
-  long long n = static_cast<long long>(nt) * kItemUnits;
-  for (int t = 0; t < nt; ++t)
-    n += max(1, tiles_of(keys_of_any(t * NMAX / a.group, (min(rows, (t + 1) * NMAX) - 1) / a.group, r.q_len, r.len, a.causal, a.window)));
-  return n;
-}
-
-template <int ACT>
-__device__ __forceinline__ float act_one(float x, float m) {
-  // x/2 erfc(-x / sqrt 2): 1 + erf would cancel where x is well below zero, and a row's scale brings such a P up when it has no larger
-  if constexpr (ACT == ACT_GELU_ERF) return 0.5f * m * x * erfcf(x * -0.70710678118654752f);
-  else return act_scaled<ACT>(x, m, 0.5f * m);
-}
-template <int ACT, int N>
-__device__ __forceinline__ void act_all(float (&x)[N], float m) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = act_one<ACT>(x[i], m);
-}
-// x = act(x) * m for a run-time activation class
-template <int N>
-__device__ __forceinline__ void act_any(int act, float (&x)[N], float m) {
-  switch (act) {
-    case ACT_GELU_ERF: act_all<ACT_GELU_ERF>(x, m); break;
-    case ACT_GELU_TANH: act_all<ACT_GELU_TANH>(x, m); break;
-    case ACT_LEAKY_RELU: act_all<ACT_LEAKY_RELU>(x, m); break;
-    case ACT_RELU: act_all<ACT_RELU>(x, m); break;
-    case ACT_SILU: act_all<ACT_SILU>(x, m); break;
-    case ACT_HARDSWISH: act_all<ACT_HARDSWISH>(x, m); break;
-    case ACT_RELU_SQUARE: act_all<ACT_RELU_SQUARE>(x, m); break;
-    default: act_all<ACT_RAW>(x, m); break;
-  }
-}
-
 // The N columns' values over the warp's 32 lanes, reduced: lane i gets column i % N's result.  Halves change places (N - 1 shuffles).
 template <int N, class F>
 __device__ __forceinline__ float reduce_columns(float (&v)[N], int lane, F op) {
@@ -218,20 +113,6 @@ __device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)
   if constexpr (N == 32) tmem_st32(taddr, r);
   else tmem_st16(taddr, r);
 }
-
-#define PAGED_WAIT(bar_idx, parity, role)                                                                             \
-  {                                                                                                                   \
-    const bool ok_ = mbar_wait(bar_base + 8u * (bar_idx), (parity), abort_flag, a.status, ((bar_idx) << 8) | (role)); \
-    if (!__all_sync(kFull, ok_)) goto role_done;                                                                      \
-  }
-
-// The element-wise warps meet at barriers of their own, so none of them may leave alone: a wait that runs out is recorded (the abort
-// flag ends every later wait at once) and they go on, on whatever is there, to the end of the item, where they leave together.
-#define PAGED_WAIT_ON(bar_idx, parity)                                                                                       \
-  {                                                                                                                         \
-    (void)mbar_wait(bar_base + 8u * (bar_idx), (parity), abort_flag, a.status, ((bar_idx) << 8) | ST_ROLE_ACT);              \
-    __syncwarp();                                                                                                           \
-  }
 
 template <int D, int NMAX, bool SOFTMAX>
 __global__ void __launch_bounds__(PagedShape<D, NMAX>::kThreads, PagedShape<D, NMAX>::kCtasPerSm)
@@ -271,142 +152,22 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  // Where this CTA begins: every CTA sums the units of all requests (a run of them per thread) and looks for its own first one.
-  long long* const scan = reinterpret_cast<long long*>(smem + L::kScanOff);
-  struct Start {
-    long long all, before;  // all units; units before request b
-    int b;
-  };
-  Start* const start = reinterpret_cast<Start*>(scan + 32);
-  {
-    const int per = (a.batch + L::kThreads - 1) / L::kThreads;
-    const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
-    long long sum = 0;
-    for (int b = b0; b < b1; ++b) sum += units_of<NMAX>(a, load_request(a, b)) * a.kv_heads;
-    long long incl = sum;
-#pragma unroll
-    for (int s = 1; s < 32; s <<= 1) {
-      const long long o = __shfl_up_sync(kFull, incl, s);
-      if (lane >= s) incl += o;
-    }
-    if (lane == 31) scan[warp] = incl;
-    if (threadIdx.x == 0) *start = Start{0, 0, a.batch};
-    __syncthreads();
-    long long all = 0, before = 0;
-    for (int w = 0; w < L::kWarps; ++w) {
-      before += w < warp ? scan[w] : 0;
-      all += scan[w];
-    }
-    if (threadIdx.x == 0) start->all = all;
-    const long long ctas = min(static_cast<long long>(gridDim.x), all);
-    if (blockIdx.x < ctas) {
-      const long long u0 = all * blockIdx.x / ctas;
-      long long at = before + incl - sum;
-      if (u0 >= at && u0 < at + sum) {
-        for (int b = b0; b < b1; ++b) {
-          const long long n = units_of<NMAX>(a, load_request(a, b)) * a.kv_heads;
-          if (u0 < at + n) {
-            start->before = at, start->b = b;
-            break;
-          }
-          at += n;
-        }
-      }
-    }
-  }
+  PagedStart* const start = reinterpret_cast<PagedStart*>(smem + L::kScanOff + 32 * 8);
+  find_start<L, NMAX>(a, reinterpret_cast<long long*>(smem + L::kScanOff), start, warp, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = warp_uniform(*tmem_ptr);
-  const long long all_units = start->all;
-  const long long ctas = min(static_cast<long long>(gridDim.x), all_units);
-
-  int* const ring = reinterpret_cast<int*>(smem + L::kRingOff);
-  uint32_t item_pos = 0;  // items this role has taken
-  [[maybe_unused]] uint32_t loaded = 0;  // the loader: tiles asked for
-  auto take_item = [&](int role) -> PagedItem {
-    const uint32_t slot = item_pos % kItemSlots, parity = (item_pos / kItemSlots) & 1u;
-    ++item_pos;
-    PagedItem it;
-    it.h = -2;
-    const bool ok = mbar_wait(bar_base + 8u * (L::B_ITEM_FULL + slot), parity, abort_flag, a.status, ((L::B_ITEM_FULL + slot) << 8) | role);
-    if (!__all_sync(kFull, ok)) return it;
-    const int4* const r = reinterpret_cast<const int4*>(ring + slot * 16);
-    const int4 x = r[0], y = r[1], z = r[2];
-    it = PagedItem{warp_uniform(x.x), warp_uniform(x.y), warp_uniform(x.z), warp_uniform(x.w), warp_uniform(y.x), warp_uniform(y.y),
-                   warp_uniform(y.z), warp_uniform(y.w), warp_uniform(z.x), warp_uniform(z.y), warp_uniform(z.z), warp_uniform(z.w)};
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar_base + 8u * (L::B_ITEM_EMPTY + slot));
-    return it;
-  };
+  PagedCta<L> cta{a, smem, smem_base, bar_base, abort_flag, lane};
 
   if (warp == L::kLoadWarp) {
     // ------------------------------------------------------------------ TMA loader, and the walk over the items
-    auto publish = [&](const PagedItem& it) -> bool {
-      const uint32_t slot = item_pos % kItemSlots, parity = (item_pos / kItemSlots) & 1u;
-      const bool ok = mbar_wait(bar_base + 8u * (L::B_ITEM_EMPTY + slot), parity ^ 1u, abort_flag, a.status,
-                                ((L::B_ITEM_EMPTY + slot) << 8) | ST_ROLE_LOAD);
-      if (!__all_sync(kFull, ok)) return false;
-      if (lane == 0) {
-        int4* const r = reinterpret_cast<int4*>(ring + slot * 16);
-        r[0] = make_int4(it.h, it.q_start, it.q_len, it.row0);
-        r[1] = make_int4(it.rows, it.len, it.lo, it.hi);
-        r[2] = make_int4(it.tile0, it.tiles, it.pieces, it.first);
-        mbar_arrive(bar_base + 8u * (L::B_ITEM_FULL + slot));
-      }
-      ++item_pos;
-      return true;
-    };
-    const int per_tile = kTile >> a.block_shift;  // blocks of a tile
-    const int block_size = 1 << a.block_shift;
-    uint32_t pos = 0;                             // tiles before this one
-    const long long u0 = blockIdx.x < ctas ? all_units * blockIdx.x / ctas : 0, u1 = blockIdx.x < ctas ? all_units * (blockIdx.x + 1) / ctas : 0;
-    // the walk: request, head and row tile that come next, units before them
-    int wb = start->b - 1, wh = a.kv_heads, wt = 0, w_nt = 0, w_rows = 0;
-    long long at = start->before;
-    Request rq{0, 0, 0};
-    // the next item of which this CTA has tiles, published; h = -1 at the end.  Its request is `b_of`.
-    auto next_item = [&](PagedItem& it, int& b_of) -> bool {
-      it = PagedItem{};
-      it.h = -1;
-      while (at < u1) {
-        if (wt >= w_nt) wt = 0, ++wh;
-        if (wh >= a.kv_heads) {
-          if (++wb >= a.batch) break;
-          rq = load_request(a, wb);
-          wh = 0;
-          w_rows = rq.q_len * a.group;
-          w_nt = (w_rows + NMAX - 1) / NMAX;
-          if (w_nt == 0) {
-            wh = a.kv_heads;
-            continue;
-          }
-        }
-        const int row0 = wt * NMAX, rows = min(NMAX, w_rows - row0);
-        ++wt;
-        const KeyRange r = keys_of_any(row0 / a.group, (row0 + rows - 1) / a.group, rq.q_len, rq.len, a.causal, a.window);
-        const int n = tiles_of(r), n1 = max(1, n);
-        const long long s = at + kItemUnits;  // where the tiles' units begin
-        at = s + n1;
-        const int from = static_cast<int>(min(max(u0 - s, 0ll), static_cast<long long>(n1))), to = static_cast<int>(min(max(u1 - s, 0ll), static_cast<long long>(n1)));
-        if (from >= to) continue;
-        // the CTA that has unit u is the largest c with all * c / ctas <= u
-        const int first = static_cast<int>(((s + 1) * ctas - 1) / all_units);
-        const int pieces = static_cast<int>(((s + n1) * ctas - 1) / all_units) - first + 1;
-        it = PagedItem{wh, rq.q_start, rq.q_len, row0, rows, rq.len, r.lo, r.hi, r.lo / kTile + from, n == 0 ? 0 : to - from, pieces, first};
-        b_of = wb;
-        break;
-      }
-      return publish(it);
-    };
     // Q of an item (both halves of its values, all NMAX rows: those past the item's are another request's, or zeros) and its rows'
-    // factors.  The kernel before this one makes them and may still run: nothing of it is read before this wait.
+    // factors.
     uint32_t q_pos = 0;
     auto load_q = [&](const PagedItem& i) -> bool {
       const uint32_t buf = q_pos & 1u;
-      const bool ok = mbar_wait(bar_base + 8u * (L::B_Q_EMPTY + buf), ((q_pos >> 1) & 1u) ^ 1u, abort_flag, a.status,
-                                 ((L::B_Q_EMPTY + buf) << 8) | ST_ROLE_LOAD);
-      if (!__all_sync(kFull, ok)) return false;
+      if (!cta.wait(L::B_Q_EMPTY + buf, ((q_pos >> 1) & 1u) ^ 1u, ST_ROLE_LOAD)) return false;
       ++q_pos;
       const long long row = static_cast<long long>(i.q_start) * a.group + i.row0;
       const uint32_t bar = bar_base + 8u * (L::B_Q_FULL + buf), dst = smem_base + L::kQOff + buf * 2 * L::kQBytes;
@@ -420,50 +181,7 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       cp_async_mbar_arrive(bar);
       return true;
     };
-    PagedItem it, ahead;
-    int b = 0, b_ahead = 0;
-    if (!next_item(it, b)) goto role_done;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (it.h >= 0 && it.tiles > 0 && !load_q(it)) goto role_done;
-    for (; it.h >= 0; it = ahead, b = b_ahead) {
-      if (!next_item(ahead, b_ahead)) goto role_done;
-      const int n_blocks = min((it.len + block_size - 1) >> a.block_shift, a.table_width);
-      const int* const table = a.block_tables + static_cast<long long>(b) * a.table_stride;
-      int cached = 0, cached_at = -1;  // 32 entries of the table, from entry cached_at on
-      for (int j = 0; j < it.tiles; ++j, ++pos) {
-        const uint32_t stage = pos % L::kStages;
-        const int p0 = (it.tile0 + j) * per_tile;
-        if (cached_at < 0 || p0 + per_tile > cached_at + 32) {
-          cached_at = p0;
-          cached = cached_at + lane < n_blocks ? table[cached_at + lane] : -1;
-        }
-        const int blk = __shfl_sync(kFull, cached, (p0 - cached_at + lane) & 31);
-        const bool valid = lane < per_tile && p0 + lane < n_blocks && blk >= 0 && blk < a.num_blocks;
-        PAGED_WAIT(L::B_KV_EMPTY + stage, ((pos / L::kStages) & 1u) ^ 1u, ST_ROLE_LOAD);
-        const uint32_t bar = bar_base + 8u * (L::B_KV_FULL + stage);
-        const unsigned n_valid = __popc(__ballot_sync(kFull, valid));
-        if (lane == 0) mbar_arrive_expect_tx(bar, n_valid * block_size * D * 2);
-        __syncwarp();
-        const uint32_t dst = smem_base + L::kKvOff + stage * 2 * L::kTileBytes + lane * block_size * D;
-        if (valid) {
-          tma_load_4d(dst, &tm_k, bar, 0, 0, it.h, blk);
-          tma_load_4d(dst + L::kTileBytes, &tm_v, bar, 0, 0, it.h, blk);
-        }
-        // a block that is not there has scale 0, which tells the others
-        if (lane < per_tile) {
-          const uint32_t sc = smem_base + L::kScaleOff + stage * 64 + lane * 4;
-          const long long si = valid ? static_cast<long long>(blk) * a.kv_heads + it.h : 0;
-          cp_async4(sc, a.k_scales + si, valid);
-          cp_async4(sc + 32, a.v_scales + si, valid);
-        }
-        cp_async_mbar_arrive(bar_base + 8u * (L::B_SC_FULL + stage));
-        loaded = pos + 1;
-        // the next item's Q: its buffer is the last item's, which is done when this item's first stages have been used
-        if (j == min(L::kStages, it.tiles - 1) && ahead.h >= 0 && ahead.tiles > 0 && !load_q(ahead)) goto role_done;
-      }
-      if (it.tiles == 0 && ahead.h >= 0 && ahead.tiles > 0 && !load_q(ahead)) goto role_done;
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    paged_load<L, D, NMAX>(cta, start, tm_k, tm_v, load_q);
   } else if (warp == L::kMmaWarp) {
     // ------------------------------------------------------------------ MMA issuer
     constexpr int kSwizzle = D == 128 ? 128 : 64;
@@ -498,7 +216,7 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       return true;
     };
     while (true) {
-      const PagedItem it = take_item(ST_ROLE_MMA);
+      const PagedItem it = cta.take_item(ST_ROLE_MMA);
       if (it.h < 0) {
         if (it.h == -2) goto role_done;
         break;
@@ -545,7 +263,7 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int bar_wg = 4 + wg;
     uint32_t pos = 0, q_pos = 0;  // tiles, items with tiles
     while (true) {
-      const PagedItem it = take_item(ST_ROLE_ACT);
+      const PagedItem it = cta.take_item(ST_ROLE_ACT);
       if (named_bar_or(3, 128 * kGroups, it.h < 0)) break;
       const int rows = min(C, it.rows - c0);  // of this warpgroup; none or fewer: it only keeps step
       if (tid < C) {
@@ -809,80 +527,7 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (threadIdx.x == 0) *last_flag = count_arrival(a.counters + it.first) == it.pieces - 1;
         named_bar_sync(3, 128 * kGroups);
         if (*last_flag) {
-          // A warp has two rows: the weights of 32 pieces over its lanes, then the pieces in order.  What this takes is trips to L2: eight
-          // pieces' values of both rows are asked for before the first is used, and with the pieces' statistics.
-          constexpr int V = D / 32, kAhead = 8, kWarpsHere = 4 * kGroups;
-          const auto slot_of = [&](int k) { return static_cast<long long>(2 * (it.first + k) + (k == 0 ? 1 : 0)); };
-          for (int ra = warp; ra < it.rows; ra += 2 * kWarpsHere) {
-            const int row[2] = {ra, min(ra + kWarpsHere, it.rows - 1)};
-            float acc[2][V], m_all[2] = {kNoMax, kNoMax}, l_all[2] = {0.f, 0.f};
-#pragma unroll
-            for (int e = 0; e < V; ++e) acc[0][e] = acc[1][e] = 0.f;
-            if constexpr (SOFTMAX) {
-              for (int k = lane; k < it.pieces; k += 32) {
-#pragma unroll
-                for (int x = 0; x < 2; ++x) m_all[x] = fmaxf(m_all[x], __ldcg(a.part_ml + slot_of(k) * 2 * NMAX + row[x]));
-              }
-#pragma unroll
-              for (int x = 0; x < 2; ++x) m_all[x] = warp_max(m_all[x]);
-            }
-            for (int k0 = 0; k0 < it.pieces; k0 += 32) {
-              const int n = min(32, it.pieces - k0);
-              float w[2];
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                w[x] = lane < n ? 1.f : 0.f;
-                if constexpr (SOFTMAX) {
-                  const float* const ml = a.part_ml + slot_of(k0 + min(lane, n - 1)) * 2 * NMAX + row[x];
-                  const float m = __ldcg(ml), l = __ldcg(ml + NMAX);
-                  w[x] *= ex2_approx(m - m_all[x]);
-                  if (lane < n) l_all[x] += w[x] * l;
-                }
-              }
-              for (int i0 = 0; i0 < n; i0 += kAhead) {
-                float v[2][kAhead][V];
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                  const float* const po = a.part_o + slot_of(k0 + min(i0 + i, n - 1)) * NMAX * D + lane * V;
-#pragma unroll
-                  for (int x = 0; x < 2; ++x) {
-                    if constexpr (V == 4) {
-                      const float4 u = __ldcg(reinterpret_cast<const float4*>(po + row[x] * D));
-                      v[x][i][0] = u.x, v[x][i][1] = u.y, v[x][i][2] = u.z, v[x][i][3] = u.w;
-                    } else {
-                      const float2 u = __ldcg(reinterpret_cast<const float2*>(po + row[x] * D));
-                      v[x][i][0] = u.x, v[x][i][1] = u.y;
-                    }
-                  }
-                }
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                  if (i0 + i < n) {
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                      const float wi = __shfl_sync(kFull, w[x], i0 + i);
-#pragma unroll
-                      for (int e = 0; e < V; ++e) acc[x][e] = fmaf(wi, v[x][i][e], acc[x][e]);
-                    }
-                  }
-                }
-              }
-            }
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              float inv = 1.f;
-              if constexpr (SOFTMAX) {
-#pragma unroll
-                for (int s = 16; s > 0; s >>= 1) l_all[x] += __shfl_xor_sync(kFull, l_all[x], s);
-                inv = l_all[x] > 0.f || l_all[x] != l_all[x] ? 1.f / l_all[x] : 0.f;
-              }
-              if (x == 0 || ra + kWarpsHere < it.rows) {
-                uint32_t* const dst = reinterpret_cast<uint32_t*>(a.o + reinterpret_cast<const long long*>(smem + L::kRowOff)[row[x]] + lane * V);
-#pragma unroll
-                for (int e = 0; e < V / 2; ++e) dst[e] = pack_bf16x2(acc[x][2 * e] * inv, acc[x][2 * e + 1] * inv);
-              }
-            }
-          }
+          paged_join<D, NMAX, SOFTMAX, 4 * kGroups>(a, it, warp, lane, [&](int r) { return reinterpret_cast<const long long*>(smem + L::kRowOff)[r]; });
         }
         named_bar_sync(3, 128 * kGroups);
       }
@@ -890,15 +535,6 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   }
 role_done:
   __syncwarp();
-  if (warp == L::kLoadWarp && *abort_flag != 0) {
-    // after a wait that ran out: not before this CTA's own copies have landed (again with a limit)
-    const uint64_t t0 = global_timer_ns();
-    for (uint32_t k = loaded > L::kStages ? loaded - L::kStages : 0; k < loaded; ++k)
-      while (!mbar_try_wait(bar_base + 8u * (L::B_KV_FULL + k % L::kStages), (k / L::kStages) & 1u) && global_timer_ns() - t0 < kWaitLimitNs) {
-      }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncwarp();
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -955,22 +591,6 @@ __global__ void __launch_bounds__(256) gdpa_paged_prepare_kernel(const PagedArgs
   }
 }
 
-// Launch of `kernel` that may begin while the kernel before it in the stream still runs (it waits for that one itself).
-template <class... P, class... A>
-int launch_after(void (*kernel)(P...), int grid, int threads, int smem, cudaStream_t stream, const A&... args) {
-  cudaLaunchAttribute early;
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3(grid);
-  c.blockDim = dim3(threads);
-  c.dynamicSmemBytes = smem;
-  c.stream = stream;
-  c.attrs = &early;
-  c.numAttrs = 1;
-  return cudaLaunchKernelEx(&c, kernel, args...) == cudaSuccess ? 0 : GDPA_ERR_LAUNCH_;
-}
-
 template <int D, int NMAX>
 int launch(const PagedLaunch& l) {
   using L = PagedShape<D, NMAX>;
@@ -995,8 +615,9 @@ int launch_paged(const PagedLaunch& l, int head_dim) {
   if (cudaGetLastError() != cudaSuccess) return GDPA_ERR_LAUNCH_;
   auto go = [&](auto dim) -> int {
     constexpr int D = decltype(dim)::value;
-    return l.rows == 16 ? launch<D, 16>(l) : l.rows == 64 ? launch<D, 64>(l) : launch<D, 128>(l);
+    return l.rows == 16 ? launch<D, 16>(l) : launch<D, 64>(l);
   };
+  if (l.rows > 64) return launch_paged_rows(l, head_dim);
   return head_dim == 128 ? go(std::integral_constant<int, 128>{}) : go(std::integral_constant<int, 64>{});
 }
 

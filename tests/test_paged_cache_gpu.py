@@ -324,6 +324,13 @@ def test_attend_many_queries(q_lens, activation):
     Case([500, 129, 31], q_lens, 4, 2, 64, 32, seed=1).check(scale, activation)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attend_many_queries_over_long_histories(dim):
+    # items of more tiles than the kernels have stages, one after another in a CTA
+    Case([3000, 2500, 1700], [130, 257, 100], 4, 2, dim, 64).check(0.1, "softmax", causal=True)
+    Case([2000] * 3, [40, 64, 33], 32, 32, dim, 128).check(1 / 2000, "relu")
+
+
 @pytest.mark.parametrize("window", [None, 0, 1, 100, 128, 5000])
 @pytest.mark.parametrize("causal", [False, True])
 def test_attend_masks(causal, window):

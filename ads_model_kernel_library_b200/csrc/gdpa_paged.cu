@@ -50,7 +50,8 @@ struct PagedShape {
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kLoadWarp = 4 * kGroups, kMmaWarp = kLoadWarp + 1;
   static constexpr int kTmemCols = NMAX <= 16 ? 64 : NMAX <= 64 ? 256 : 512;  // S0, S1, O of NMAX columns each
-  static constexpr int kQBuffers = 2;
+  static constexpr int kItemUnits = 4, kMostTileUnits = 1;
+  static constexpr __host__ __device__ int tile_units(int) { return 1; }
   static constexpr float kTarget = 64.f;
 
   static constexpr int kKvOff = 0;                                  // [stage]{K, V}

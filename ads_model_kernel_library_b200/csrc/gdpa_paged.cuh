@@ -12,7 +12,6 @@ namespace gdpa {
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kItemSlots = 4;
-constexpr int kItemUnits = 4;           // what an item costs besides its tiles, in tiles
 constexpr float kMax8 = 448.f;
 constexpr float kNoMax = -3.0e38f;     // running maximum of a row that has seen no key
 constexpr float kLeastScale = 7.888609e-31f;  // 2^-100
@@ -77,16 +76,32 @@ __device__ __forceinline__ Request load_request(const PagedArgs& a, int b) {
   return r;
 }
 
-// Units of one K / V head of a request: its row tiles' KV tiles, one at least each (a row tile without keys has zeros to write), and
-// kItemUnits for the beginning and the end of each.
-template <int NMAX>
+// What an item costs, in units: L::kItemUnits for its beginning and end, and for each of its KV tiles (one at least: a row tile without keys
+// has zeros to write) L::tile_units(rows).
+template <class L>
+__device__ __forceinline__ long long units_of_item(int rows, int tiles) {
+  return L::kItemUnits + static_cast<long long>(max(1, tiles)) * L::tile_units(rows);
+}
+// ... and one K / V head of a request.
+template <class L, int NMAX>
 __device__ __forceinline__ long long units_of(const PagedArgs& a, const Request& r) {
   const int rows = r.q_len * a.group, nt = (rows + NMAX - 1) / NMAX;
-  if (!a.causal && a.window < 0) return static_cast<long long>(nt) * (kItemUnits + max(1, tiles_of(KeyRange{0, r.len})));
-  long long n = static_cast<long long>(nt) * kItemUnits;
-  for (int t = 0; t < nt; ++t)
-    n += max(1, tiles_of(keys_of_any(t * NMAX / a.group, (min(rows, (t + 1) * NMAX) - 1) / a.group, r.q_len, r.len, a.causal, a.window)));
+  if (nt == 0) return 0;
+  if (!a.causal && a.window < 0) {
+    const int tiles = tiles_of(KeyRange{0, r.len});
+    return (nt - 1) * units_of_item<L>(NMAX, tiles) + units_of_item<L>(rows - (nt - 1) * NMAX, tiles);
+  }
+  long long n = 0;
+  for (int t = 0; t < nt; ++t) {
+    const int last = min(rows, (t + 1) * NMAX);
+    n += units_of_item<L>(last - t * NMAX, tiles_of(keys_of_any(t * NMAX / a.group, (last - 1) / a.group, r.q_len, r.len, a.causal, a.window)));
+  }
   return n;
+}
+// CTAs that have a share of `all` units: no share is smaller than a tile.
+template <class L>
+__device__ __forceinline__ long long sharing_ctas(long long all) {
+  return min(static_cast<long long>(gridDim.x), max(1LL, all / L::kMostTileUnits));
 }
 
 template <int ACT>
@@ -137,11 +152,39 @@ __device__ __forceinline__ void split_e4m3(const float (&x)[16], uint32_t (&hi)[
     lo[i] = __byte_perm(l[2 * i], l[2 * i + 1], 0x5410);
   }
 }
-// 2^x of all of them, kept together as well.
-template <int N>
-__device__ __forceinline__ void ex2_all(float (&x)[N]) {
+// What an activation asks of the special-function pipe, per element.
+enum PagedMufu { MUFU_NONE, MUFU_EX2, MUFU_TANH };
+template <PagedMufu M>
+__device__ __forceinline__ void mufu(float& u) {
+  if constexpr (M == MUFU_EX2) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(u));
+  if constexpr (M == MUFU_TANH) asm volatile("tanh.approx.f32 %0, %0;" : "+f"(u));
+}
+template <PagedMufu M, int N>
+__device__ __forceinline__ void mufu_all(float (&u)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(x[i]));
+  for (int i = 0; i < N; ++i) mufu<M>(u[i]);
+}
+// split_e4m3 of x with the special functions of the next sixteen values between its steps, two to five of them: the two take
+// about the same time on different pipes, and a warp issues in order.
+template <PagedMufu M>
+__device__ __forceinline__ void split_e4m3_and(const float (&x)[16], uint32_t (&hi)[4], uint32_t (&lo)[4], float (&next)[16]) {
+  uint32_t u[8], v[8];
+  uint16_t h[8], l[8];
+#pragma unroll
+  for (int k = 0; k < 40; ++k) {
+    const int i = k % 8;
+    if ((2 * k) % 5 < 2) mufu<M>(next[(2 * k) / 5]);
+    if (k < 8) asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
+    else if (k < 16) asm volatile("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h[i]) : "r"(u[i]));
+    else if (k < 24) asm volatile("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(v[i]) : "h"(h[i]));
+    else if (k < 32) asm volatile("sub.f16x2 %0, %0, %1;" : "+r"(u[i]) : "r"(v[i]));
+    else asm volatile("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l[i]) : "r"(u[i]));
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    hi[i] = __byte_perm(h[2 * i], h[2 * i + 1], 0x5410);
+    lo[i] = __byte_perm(l[2 * i], l[2 * i + 1], 0x5410);
+  }
 }
 __device__ __forceinline__ float2 e4m3x2_values(uint32_t v) {
   const uint32_t h = f16x2_from_e4m3x2(static_cast<uint16_t>(v));
@@ -217,7 +260,7 @@ __device__ __forceinline__ void find_start(const PagedArgs& a, long long* scan, 
   const int per = (a.batch + L::kThreads - 1) / L::kThreads;
   const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
   long long sum = 0;
-  for (int b = b0; b < b1; ++b) sum += units_of<NMAX>(a, load_request(a, b)) * a.kv_heads;
+  for (int b = b0; b < b1; ++b) sum += units_of<L, NMAX>(a, load_request(a, b)) * a.kv_heads;
   long long incl = sum;
 #pragma unroll
   for (int s = 1; s < 32; s <<= 1) {
@@ -233,13 +276,13 @@ __device__ __forceinline__ void find_start(const PagedArgs& a, long long* scan, 
     all += scan[w];
   }
   if (threadIdx.x == 0) start->all = all;
-  const long long ctas = min(static_cast<long long>(gridDim.x), all);
+  const long long ctas = sharing_ctas<L>(all);
   if (blockIdx.x < ctas) {
     const long long u0 = all * blockIdx.x / ctas;
     long long at = before + incl - sum;
     if (u0 >= at && u0 < at + sum) {
       for (int b = b0; b < b1; ++b) {
-        const long long n = units_of<NMAX>(a, load_request(a, b)) * a.kv_heads;
+        const long long n = units_of<L, NMAX>(a, load_request(a, b)) * a.kv_heads;
         if (u0 < at + n) {
           start->before = at, start->b = b;
           break;
@@ -258,7 +301,7 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
   const PagedArgs& a = cta.a;
   const int lane = cta.lane;
   const uint32_t smem_base = cta.smem_base, bar_base = cta.bar_base;
-  const long long all_units = start->all, ctas = min(static_cast<long long>(gridDim.x), all_units);
+  const long long all_units = start->all, ctas = sharing_ctas<L>(all_units);
   uint32_t loaded = 0;  // tiles asked for
   auto walk = [&]() -> bool {
     const int per_tile = kTile >> a.block_shift;  // blocks of a tile
@@ -290,13 +333,16 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
         ++wt;
         const KeyRange r = keys_of_any(row0 / a.group, (row0 + rows - 1) / a.group, rq.q_len, rq.len, a.causal, a.window);
         const int n = tiles_of(r), n1 = max(1, n);
-        const long long s = at + kItemUnits;  // where the tiles' units begin
-        at = s + n1;
-        const int from = static_cast<int>(min(max(u0 - s, 0ll), static_cast<long long>(n1))), to = static_cast<int>(min(max(u1 - s, 0ll), static_cast<long long>(n1)));
+        const int w = L::tile_units(rows);
+        const long long s = at + L::kItemUnits;  // where the tiles' units begin
+        at = s + static_cast<long long>(n1) * w;
+        // a tile belongs to the CTA that has its first unit
+        auto tile_from = [&](long long u) { return static_cast<int>(min(max((u - s + w - 1) / w, 0ll), static_cast<long long>(n1))); };
+        const int from = u0 <= s ? 0 : tile_from(u0), to = u1 <= s ? 0 : tile_from(u1);
         if (from >= to) continue;
         // the CTA that has unit u is the largest c with all * c / ctas <= u
         const int first = static_cast<int>(((s + 1) * ctas - 1) / all_units);
-        const int pieces = static_cast<int>(((s + n1) * ctas - 1) / all_units) - first + 1;
+        const int pieces = static_cast<int>(((s + static_cast<long long>(n1 - 1) * w + 1) * ctas - 1) / all_units) - first + 1;
         it = PagedItem{wh, rq.q_start, rq.q_len, row0, rows, rq.len, r.lo, r.hi, r.lo / kTile + from, n == 0 ? 0 : to - from, pieces, first};
         b_of = wb;
         break;
@@ -307,7 +353,7 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
     int b = 0, b_ahead = 0;
     if (!next_item(it, b)) return false;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (L::kQBuffers == 2 && it.h >= 0 && it.tiles > 0 && !load_q(it)) return false;
+    if (it.h >= 0 && it.tiles > 0 && !load_q(it)) return false;
     for (; it.h >= 0; it = ahead, b = b_ahead) {
       if (!next_item(ahead, b_ahead)) return false;
       const int n_blocks = min((it.len + block_size - 1) >> a.block_shift, a.table_width);
@@ -341,15 +387,10 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
         }
         cp_async_mbar_arrive(bar_base + 8u * (L::B_SC_FULL + stage));
         loaded = pos + 1;
-        if constexpr (L::kQBuffers == 2) {
-          // the next item's Q: its buffer is the last item's, which is done when this item's first stages have been used
-          if (j == min(L::kStages, it.tiles - 1) && ahead.h >= 0 && ahead.tiles > 0 && !load_q(ahead)) return false;
-        } else {
-          // this item's Q: the buffer is the last item's, whose tiles have all been asked for; this item's first ones go out before the wait
-          if (j == min(L::kStages, it.tiles) - 1 && !load_q(it)) return false;
-        }
+        // the next item's Q: its buffer is the last item's, which is done when this item's first stages have been used
+        if (j == min(L::kStages, it.tiles - 1) && ahead.h >= 0 && ahead.tiles > 0 && !load_q(ahead)) return false;
       }
-      if (L::kQBuffers == 2 && it.tiles == 0 && ahead.h >= 0 && ahead.tiles > 0 && !load_q(ahead)) return false;
+      if (it.tiles == 0 && ahead.h >= 0 && ahead.tiles > 0 && !load_q(ahead)) return false;
     }
     return true;
   };

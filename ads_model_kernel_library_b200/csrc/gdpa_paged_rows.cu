@@ -6,9 +6,8 @@
 // A work item is 256 rows (two row tiles) of one (request, K / V head); the tiles' element-wise warps and MMAs take turns, one tile's
 // MMAs under the other's exponentials.  A token's scales are the same for a whole row of threads: for each block of 16 tokens and more
 // the score's factor and the reference less log2 of V's scale are two registers, so that P times V's scale is one FMA and one
-// exponential.  The reference of a row (its running maximum, in whole powers of two) moves only when a product would pass 448: a warp
-// looks at 32 columns at a time before P takes the place of their scores, and where one does not fit, the row's O, sum and
-// earlier columns of the tile are scaled down, exactly, and the 32 are computed again.
+// exponential.  A first look at a tile's scores (one maximum in two of them, of the numbers as they are) says whether a product would pass
+// 448 for the reference that a row has; only then it moves (by whole powers of two) and the row's O and sum with it.
 //
 // Against the transposed form on 128 rows (one B200): candidates (SiLU) 917 us, causal chunks 757 us there.
 //
@@ -27,17 +26,18 @@ constexpr int kRows = 256;  // of an item
 template <int D>
 struct RowsShape {
   static constexpr int kTileBytes = kTile * D;               // K or V tile, or a plane of a row tile of Q
-  static constexpr int kStages = D == 128 ? 4 : 8;
+  static constexpr int kStages = D == 128 ? 2 : 4;
   static constexpr int kWarps = 11, kThreads = 32 * kWarps;
   static constexpr int kLoadWarp = 8, kMmaWarp = 9, kFixWarp = 10;
-  static constexpr int kQBuffers = 1;
+  static constexpr int kItemUnits = 2, kMostTileUnits = 1;
+  static constexpr __host__ __device__ int tile_units(int) { return 1; }
   static constexpr float kTarget = 64.f;
   static constexpr int kKvOff = 0;                                 // [stage]{K, V}
-  static constexpr int kQOff = kStages * 2 * kTileBytes;           // [row tile]{hi, lo}
-  static constexpr int kScaleOff = kQOff + 4 * kTileBytes;         // float[stage][16]: K scales of up to 8 blocks, V scales
+  static constexpr int kQOff = kStages * 2 * kTileBytes;           // [2][row tile]{hi, lo}
+  static constexpr int kScaleOff = kQOff + 8 * kTileBytes;         // float[stage][16]: K scales of up to 8 blocks, V scales
   static constexpr int kPoisonOff = kScaleOff + kStages * 64;      // uint[stage][4]: tokens whose V row held a NaN
-  static constexpr int kQaOff = kPoisonOff + kStages * 16;         // float[kRows]
-  static constexpr int kRingOff = kQaOff + kRows * 4;              // int[kItemSlots][16]
+  static constexpr int kQaOff = kPoisonOff + kStages * 16;         // float[2][kRows]
+  static constexpr int kRingOff = kQaOff + 2 * kRows * 4;              // int[kItemSlots][16]
   static constexpr int kBarOff = kRingOff + kItemSlots * 64;
   enum : int {
     B_KV_FULL = 0,
@@ -47,9 +47,9 @@ struct RowsShape {
     B_S_FULL = B_V_READY + kStages,  // [2]
     B_P_FULL = B_S_FULL + 2,         // [2]
     B_PV_DONE = B_P_FULL + 2,        // [2]
-    B_Q_FULL = B_PV_DONE + 2,
-    B_Q_EMPTY,
-    B_ITEM_FULL,                     // [kItemSlots]
+    B_Q_FULL = B_PV_DONE + 2,        // [2]
+    B_Q_EMPTY = B_Q_FULL + 2,        // [2]
+    B_ITEM_FULL = B_Q_EMPTY + 2,     // [kItemSlots]
     B_ITEM_EMPTY = B_ITEM_FULL + kItemSlots,
     B_COUNT = B_ITEM_EMPTY + kItemSlots
   };
@@ -60,11 +60,13 @@ struct RowsShape {
   static_assert(kDynBytes <= 227 * 1024, "shared memory");
 };
 
-template <int D, bool SOFTMAX>
+template <int D, int ACT>
 __global__ void __launch_bounds__(RowsShape<D>::kThreads, 1)
 gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                        const PagedArgs a) {
   using L = RowsShape<D>;
+  constexpr bool SOFTMAX = ACT == ACT_SOFTMAX;
+  constexpr PagedMufu kMufu = SOFTMAX ? MUFU_EX2 : ACT == ACT_SILU || ACT == ACT_GELU_TANH ? MUFU_TANH : MUFU_NONE;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem_base = smem_u32(smem);
@@ -80,8 +82,8 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       uint32_t n = 1;
       if (i >= L::B_SC_FULL && i < L::B_SC_FULL + L::kStages) n = 32;
       if (i >= L::B_P_FULL && i < L::B_P_FULL + 2) n = 4;
-      if (i == L::B_Q_FULL) n = 33;
-      if (i == L::B_Q_EMPTY) n = 1 + 8;
+      if (i >= L::B_Q_FULL && i < L::B_Q_FULL + 2) n = 33;
+      if (i >= L::B_Q_EMPTY && i < L::B_Q_EMPTY + 2) n = 1 + 8;
       if (i >= L::B_ITEM_EMPTY && i < L::B_ITEM_EMPTY + kItemSlots) n = 10;
       mbar_init(bar_base + 8u * i, n);
     }
@@ -109,19 +111,20 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     // ------------------------------------------------------------------ TMA loader, and the walk over the items
     uint32_t q_pos = 0;
     auto load_q = [&](const PagedItem& i) -> bool {
-      if (!cta.wait(L::B_Q_EMPTY, (q_pos & 1u) ^ 1u, ST_ROLE_LOAD)) return false;
+      const uint32_t buf = q_pos & 1u;
+      if (!cta.wait(L::B_Q_EMPTY + buf, ((q_pos >> 1) & 1u) ^ 1u, ST_ROLE_LOAD)) return false;
       ++q_pos;
       const long long row = static_cast<long long>(i.q_start) * a.group + i.row0;
-      const uint32_t bar = bar_base + 8u * L::B_Q_FULL;
+      const uint32_t bar = bar_base + 8u * (L::B_Q_FULL + buf);
       const int tiles = i.rows > kTile ? 2 : 1;
       if (lane == 0) {
         mbar_arrive_expect_tx(bar, tiles * 2 * L::kTileBytes);
         for (int t = 0; t < tiles; ++t)
           for (int plane = 0; plane < 2; ++plane)
-            tma_load_3d(smem_base + L::kQOff + (2 * t + plane) * L::kTileBytes, &tm_q, bar, 0, static_cast<int>(row) + t * kTile, plane * a.kv_heads + i.h);
+            tma_load_3d(smem_base + L::kQOff + (4 * buf + 2 * t + plane) * L::kTileBytes, &tm_q, bar, 0, static_cast<int>(row) + t * kTile, plane * a.kv_heads + i.h);
       }
       for (int r = lane; r < kRows; r += 32)
-        cp_async4(smem_base + L::kQaOff + r * 4, a.qa + i.h * a.total_q * a.group + row + min(r, i.rows - 1), true);
+        cp_async4(smem_base + L::kQaOff + (buf * kRows + r) * 4, a.qa + i.h * a.total_q * a.group + row + min(r, i.rows - 1), true);
       cp_async_mbar_arrive(bar);
       return true;
     };
@@ -134,8 +137,8 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const uint64_t dv0 = umma_smem_desc(smem_base + L::kKvOff + L::kTileBytes, 0, 8 * D, kSwizzle);
     const uint64_t dq0 = umma_smem_desc(smem_base + L::kQOff, 16, 8 * D, kSwizzle);
     uint32_t pos = 0, q_pos = 0, p_phase = 0;
-    auto issue_qk = [&](int s, uint32_t stage) {
-      const uint64_t dk = umma_desc_advance(dk0, stage * 2 * L::kTileBytes), dq = umma_desc_advance(dq0, s * 2 * L::kTileBytes);
+    auto issue_qk = [&](int s, uint32_t stage, uint32_t buf) {
+      const uint64_t dk = umma_desc_advance(dk0, stage * 2 * L::kTileBytes), dq = umma_desc_advance(dq0, (2 * buf + s) * 2 * L::kTileBytes);
 #pragma unroll
       for (int kk = 0; kk < D / 32; ++kk) {
         umma_ss_f8(tmem_base + s * kTile, umma_desc_advance(dq, kk * 32), umma_desc_advance(dk, kk * 32), kIdescQK, kk > 0 ? 1u : 0u);
@@ -151,12 +154,13 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
       if (it.tiles == 0) continue;
       const int nst = it.rows > kTile ? 2 : 1;
-      PAGED_WAIT(L::B_Q_FULL, q_pos & 1u, ST_ROLE_MMA);
+      const uint32_t buf = q_pos & 1u;
+      PAGED_WAIT(L::B_Q_FULL + buf, (q_pos >> 1) & 1u, ST_ROLE_MMA);
       ++q_pos;
       PAGED_WAIT(L::B_KV_FULL + pos % L::kStages, (pos / L::kStages) & 1u, ST_ROLE_MMA);
       tc_fence_after();
-      for (int s = 0; s < nst; ++s) issue_qk(s, pos % L::kStages);
-      if (it.tiles == 1) tc_commit(bar_base + 8u * L::B_Q_EMPTY);
+      for (int s = 0; s < nst; ++s) issue_qk(s, pos % L::kStages, buf);
+      if (it.tiles == 1) tc_commit(bar_base + 8u * (L::B_Q_EMPTY + buf));
       for (int j = 0; j < it.tiles; ++j, ++pos) {
         const uint32_t stage = pos % L::kStages, next = (pos + 1) % L::kStages;
         const bool more = j + 1 < it.tiles;
@@ -177,11 +181,11 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           if (more) {
             if (s == 0) PAGED_WAIT(L::B_KV_FULL + next, ((pos + 1) / L::kStages) & 1u, ST_ROLE_MMA);
             tc_fence_after();
-            issue_qk(s, next);
+            issue_qk(s, next, buf);
           }
         }
         tc_commit(bar_base + 8u * (L::B_KV_EMPTY + stage));
-        if (j + 2 == it.tiles) tc_commit(bar_base + 8u * L::B_Q_EMPTY);
+        if (j + 2 == it.tiles) tc_commit(bar_base + 8u * (L::B_Q_EMPTY + buf));
       }
     }
   } else if (warp == L::kFixWarp) {
@@ -255,9 +259,10 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       const KeyRange rf = keys_of(it.row0 / a.group, it.q_len, it.len, a.causal, a.window),
                      rl = keys_of((it.row0 + it.rows - 1) / a.group, it.q_len, it.len, a.causal, a.window);
       const int all_lo = max(rf.lo, rl.lo), all_hi = min(rf.hi, rl.hi);
-      PAGED_WAIT_ON(L::B_Q_FULL, q_pos & 1u);
+      const uint32_t buf = q_pos & 1u;
+      PAGED_WAIT_ON(L::B_Q_FULL + buf, (q_pos >> 1) & 1u);
       ++q_pos;
-      const float qa = reinterpret_cast<const float*>(smem + L::kQaOff)[r];
+      const float qa = reinterpret_cast<const float*>(smem + L::kQaOff)[buf * kRows + r];
       float ref = SOFTMAX ? kNoMax : 1.f, l = 0.f;  // running maximum / multiplier; sum of P
       for (int j = 0; j < it.tiles; ++j, ++pos) {
         const uint32_t stage = pos % L::kStages, phase = (pos / L::kStages) & 1u;
@@ -289,89 +294,82 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             if (sc[8 + ((c * 32 + 16) >> a.block_shift)] == 0.f) m &= 0x0000ffffu;
             return m;
           };
-          // the scores of 32 columns, times the row's and the blocks' factors (for the softmax in powers of two, V's scale and the
-          // target with them, less the reference), in x
-          uint32_t raw[32];
-          float x[32];
-          auto scores = [&](int c) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float kf, vs;
-              factors(c, h, kf, vs);
-              const float off = SOFTMAX ? __log2f(vs) + kLogTarget - ref : 0.f;
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                x[16 * h + e] = SOFTMAX ? fmaf(__uint_as_float(raw[16 * h + e]), kf, off) : __uint_as_float(raw[16 * h + e]) * kf;
+          // ---- first look: how large this tile's P, times V's scale, gets (softmax: its logarithm).  Monotone in the score on its positive side,
+          // |activation| is bounded by a constant on the other (exactly so, or 0.38 at most).
+          float top = SOFTMAX ? kNoMax : 0.f;
+          const bool flip = SOFTMAX && a.scale < 0.f;  // then the smallest product is the largest score
+          auto look = [&](float most, float least, float kf, float vs) {
+            if constexpr (SOFTMAX) {
+              const float m = (flip ? least : most) * kf;
+              top = fmaxf(top, (flip ? -least : most) > kNoMax ? m + __log2f(vs) : kNoMax);
+            } else {
+              float p = fabsf(act_one<ACT>(fmaxf(most * kf, 0.f), a.scale)), n = fmaxf(-least * kf, 0.f);
+              if constexpr (ACT == ACT_RAW || ACT == ACT_LEAKY_RELU) p = fmaxf(p, fabsf(act_one<ACT>(-n, a.scale)));
+              else if constexpr (ACT != ACT_RELU && ACT != ACT_RELU_SQUARE) p = fmaxf(p, fminf(n, 0.375f) * fabsf(a.scale));
+              top = fmaxf(top, p * vs);
             }
           };
-          auto read = [&](int c) {
-            tmem_ld32(s_tmem + c * 32, raw);
-            tmem_wait_ld();
-            tmem_regs_ready(raw);
-          };
-          // P of 32 columns does not fit for some row of the warp: the rows concerned move to a reference that it fits
-          auto move = [&](int c, uint32_t in) {
-            read(c);
-            float f = 1.f;
-            if constexpr (SOFTMAX) {
-              const bool none = ref == kNoMax;  // no key so far
-              if (none) ref = 0.f;
-              scores(c);
-              float most = kNoMax;
+          if (!masked) {
+            uint32_t s[2][16];
+            tmem_ld16(s_tmem, s[0]);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) most = fmaxf(most, (in >> e) & 1u ? x[e] : kNoMax);
-              if (none ? most > kNoMax : most > kLogTarget + kHeadroom) {
-                const float by = ceilf(fminf(most, 1.0e30f) - kLogTarget);  // to a largest element in (target / 2, target]
-                f = none ? 0.f : ex2_approx(-by);
-                ref += by;
-              } else if (none) {
-                ref = kNoMax;
+            for (int i = 0; i < 8; ++i) {
+              tmem_wait_ld();
+              tmem_regs_ready(s[i & 1]);
+              if (i < 7) tmem_ld16(s_tmem + (i + 1) * 16, s[(i + 1) & 1]);
+              float m[2], n[2] = {0.f, 0.f};
+              const float* const x = reinterpret_cast<const float*>(s[i & 1]);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                m[e] = n[e] = x[8 * e];
+                if (!flip) m[e] = max3(max3(max3(m[e], x[8 * e + 1], x[8 * e + 2]), x[8 * e + 3], x[8 * e + 4]), x[8 * e + 5], fmaxf(x[8 * e + 6], x[8 * e + 7]));
+                if (flip || !SOFTMAX)
+                  n[e] = -max3(max3(max3(-n[e], -x[8 * e + 1], -x[8 * e + 2]), -x[8 * e + 3], -x[8 * e + 4]), -x[8 * e + 5], fmaxf(-x[8 * e + 6], -x[8 * e + 7]));
               }
-            } else {
-              scores(c);
-              act_any(a.act, x, a.scale);
-              float most = 0.f;
+              float kf, vs;
+              factors(i / 2, i & 1, kf, vs);
+              look(fmaxf(m[0], m[1]), fminf(n[0], n[1]), kf, vs);
+            }
+          } else {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t in = part_of(c);
+              uint32_t s[32];
+              tmem_ld32(s_tmem + c * 32, s);
+              tmem_wait_ld();
+              tmem_regs_ready(s);
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                float kf, vs;
+                float kf, vs, most = kNoMax, least = -kNoMax;
                 factors(c, h, kf, vs);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) most = fmaxf(most, (in >> (16 * h + e)) & 1u ? fabsf(x[16 * h + e]) * vs : 0.f);
+                for (int e = 0; e < 16; ++e) {
+                  const float x = __uint_as_float(s[16 * h + e]);
+                  const bool part = (in >> (16 * h + e)) & 1u;
+                  most = fmaxf(most, part ? x : kNoMax), least = fminf(least, part ? x : -kNoMax);
+                }
+                if (SOFTMAX || most > kNoMax) look(most, least, kf, vs);
               }
-              if ((j == 0 && c == 0) || most * ref > kMax8) {
-                // the largest power of two that keeps them at or below the target; 2^100 for zeros
-                const float next = most > 0.f ? exp2f(fminf(fmaxf(floorf(log2f(L::kTarget / most)), -100.f), 100.f)) : 1.2676506e30f;
+            }
+          }
+          // ---- the reference moves to a largest P in (target / 2, target], where there is none yet or where P would not fit
+          bool moves;
+          if constexpr (SOFTMAX) moves = top > kNoMax && (ref == kNoMax || top - ref > kHeadroom);
+          else moves = j == 0 || top * ref > kMax8;
+          if (__any_sync(kFull, moves)) {
+            float f = 1.f;
+            if (moves) {
+              float next;
+              if constexpr (SOFTMAX) {
+                next = ceilf(fminf(top, 1.0e30f));
+                f = ref == kNoMax ? 0.f : ex2_approx(ref - next);
+              } else {
+                next = top > 0.f ? exp2f(fminf(fmaxf(floorf(log2f(L::kTarget / top)), -100.f), 100.f)) : 1.2676506e30f;
                 f = next / ref;
-                ref = next;
               }
+              ref = next;
             }
             l *= f;
-#pragma unroll 1
-            for (int b = 0; b < c; ++b) {  // the columns before, of this tile
-              uint32_t w[16], w_hi[4], w_lo[4];
-              tmem_ld16(s_tmem + b * 32, w);
-              tmem_wait_ld();
-              tmem_regs_ready(w);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float y[16];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                  for (int d = 0; d < 2; ++d) {
-                    const float2 u = e4m3x2_values(w[4 * h + e] >> (16 * d)), v = e4m3x2_values(w[8 + 4 * h + e] >> (16 * d));
-                    y[4 * e + 2 * d] = (u.x + v.x) * f, y[4 * e + 2 * d + 1] = (u.y + v.y) * f;
-                  }
-                }
-                split_e4m3(y, w_hi, w_lo);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  w[4 * h + e] = f == 1.f ? w[4 * h + e] : w_hi[e];
-                  w[8 + 4 * h + e] = f == 1.f ? w[8 + 4 * h + e] : w_lo[e];
-                }
-              }
-              tmem_st16(s_tmem + b * 32, w);
-            }
             if (j > 0) {
               PAGED_WAIT_ON(L::B_PV_DONE + qt, (done - 1) & 1u);  // O holds every tile before this one
               tc_fence_after();
@@ -385,76 +383,96 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                 for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
                 tmem_st32(o_tmem + b * 32, o);
               }
+              tmem_wait_st();
             }
-            tmem_wait_st();
-            read(c);
-          };
-          read(0);
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t in = ~0u, bad = 0u;
-            if (masked) in = part_of(c), bad = every ? 0u : poison[c] & in;
-            float part[2];
-            bool again = !SOFTMAX && j == 0 && c == 0;  // an activation's reference comes from the first columns, a maximum's from the first keys
-            if (again) move(c, in);
-            while (true) {
-              scores(c);
-              if constexpr (SOFTMAX) {
-                ex2_all(x);
-              } else {
-                act_any(a.act, x, a.scale);
+          }
+          // ---- P, over its own scores: of 32 tokens the hi plane, then the lo plane
+          if (!masked) {
+            // sixteen columns after sixteen, the special functions of one under the conversions of the one before, without a branch
+            uint32_t w[16], s[2][16];
+            float y[16], sum = 0.f;
+            tmem_ld16(s_tmem, s[0]);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  float kf, vs;
-                  factors(c, h, kf, vs);
+            for (int i = 0; i < 9; ++i) {
+              float u[16], z[16], kf = 0.f, vs = 0.f;
+              if (i < 8) {
+                tmem_wait_ld();
+                tmem_regs_ready(s[i & 1]);
+                if (i < 7) tmem_ld16(s_tmem + (i + 1) * 16, s[(i + 1) & 1]);
+                factors(i / 2, i & 1, kf, vs);
+                const float off = SOFTMAX ? __log2f(vs) + kLogTarget - ref : 0.f;
 #pragma unroll
-                  for (int e = 0; e < 16; ++e) x[16 * h + e] *= vs * ref;
+                for (int e = 0; e < 16; ++e) {
+                  z[e] = SOFTMAX ? 0.f : __uint_as_float(s[i & 1][e]) * kf;
+                  if constexpr (SOFTMAX) u[e] = fmaf(__uint_as_float(s[i & 1][e]), kf, off);
+                  else if constexpr (ACT == ACT_SILU) u[e] = 0.5f * z[e];
+                  else if constexpr (ACT == ACT_GELU_TANH) u[e] = z[e] * fmaf(z[e] * z[e], 0.7978845608028654f * 0.044715f, 0.7978845608028654f);
+                  else u[e] = 0.f;
                 }
               }
-              if (masked) {
+              if (i == 0) {
+                mufu_all<kMufu>(u);
+              } else {
+                uint32_t w_hi[4], w_lo[4];
+                if (i < 8) split_e4m3_and<kMufu>(y, w_hi, w_lo, u);
+                else split_e4m3(y, w_hi, w_lo);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) x[e] = (in >> e) & 1u ? x[e] : 0.f;
+                for (int e = 0; e < 4; ++e) w[4 * ((i - 1) & 1) + e] = w_hi[e], w[8 + 4 * ((i - 1) & 1) + e] = w_lo[e];
+                if ((i & 1) == 0) tmem_st16(s_tmem + (i / 2 - 1) * 32, w);
               }
-              float most[2] = {0.f, 0.f};
+              if (i < 8) {
+                const float m = a.scale * vs * ref;
 #pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                if constexpr (SOFTMAX) most[0] = max3(most[0], x[e], x[e + 1]), most[1] = max3(most[1], x[e + 2], x[e + 3]);
-                else most[0] = max3(most[0], fabsf(x[e]), fabsf(x[e + 1])), most[1] = max3(most[1], fabsf(x[e + 2]), fabsf(x[e + 3]));
+                for (int e = 0; e < 16; ++e) {
+                  if constexpr (SOFTMAX) y[e] = u[e];
+                  else if constexpr (kMufu == MUFU_TANH) y[e] = fmaf(z[e] * (0.5f * m), u[e], z[e] * (0.5f * m));
+                  else y[e] = act_one<ACT>(z[e], m);
+                }
+                if constexpr (SOFTMAX) {
+                  float p[4];
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) p[e] = (y[e] + y[e + 4]) + (y[e + 8] + y[e + 12]);
+                  sum = fmaf((p[0] + p[1]) + (p[2] + p[3]), __fdividef(1.f, vs * L::kTarget), sum);
+                }
               }
-              if (again || !__any_sync(kFull, fmaxf(most[0], most[1]) > kMax8)) break;
-              move(c, in);
-              again = true;
             }
-            if (c < 3) tmem_ld32(s_tmem + (c + 1) * 32, raw);  // under the conversions
-            if (bad != 0u) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] = (bad >> e) & 1u ? __uint_as_float(0x7fffffffu) : x[e];
-            }
-            uint32_t w[16];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float y[16];
-              uint32_t w_hi[4], w_lo[4];
-#pragma unroll
-              for (int e = 0; e < 16; ++e) y[e] = x[16 * h + e];
-              if constexpr (SOFTMAX) {
-                float s[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[e] = (y[e] + y[e + 4]) + (y[e + 8] + y[e + 12]);
-                float kf, vs;
-                factors(c, h, kf, vs);
-                part[h] = ((s[0] + s[1]) + (s[2] + s[3])) * __fdividef(1.f, vs * L::kTarget);
-              }
-              split_e4m3(y, w_hi, w_lo);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) w[4 * h + e] = w_hi[e], w[8 + 4 * h + e] = w_lo[e];
-            }
-            if constexpr (SOFTMAX) l += part[0] + part[1];
-            if (c < 3) {
+            if constexpr (SOFTMAX) l += sum;
+          } else {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t in = part_of(c), bad = every ? 0u : poison[c] & in;
+              uint32_t s[32], w[16];
+              tmem_ld32(s_tmem + c * 32, s);
               tmem_wait_ld();
-              tmem_regs_ready(raw);
+              tmem_regs_ready(s);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                float kf, vs, y[16];
+                uint32_t w_hi[4], w_lo[4];
+                factors(c, h, kf, vs);
+                const float off = SOFTMAX ? __log2f(vs) + kLogTarget - ref : 0.f, m = a.scale * vs * ref;
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  y[e] = SOFTMAX ? fmaf(__uint_as_float(s[16 * h + e]), kf, off) : act_one<ACT>(__uint_as_float(s[16 * h + e]) * kf, m);
+                if constexpr (SOFTMAX) mufu_all<MUFU_EX2>(y);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) y[e] = (in >> (16 * h + e)) & 1u ? y[e] : 0.f;
+                if (bad != 0u) {
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) y[e] = (bad >> (16 * h + e)) & 1u ? __uint_as_float(0x7fffffffu) : y[e];
+                }
+                if constexpr (SOFTMAX) {
+                  float p[4];
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) p[e] = (y[e] + y[e + 4]) + (y[e + 8] + y[e + 12]);
+                  l = fmaf((p[0] + p[1]) + (p[2] + p[3]), __fdividef(1.f, vs * L::kTarget), l);
+                }
+                split_e4m3(y, w_hi, w_lo);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[4 * h + e] = w_hi[e], w[8 + 4 * h + e] = w_lo[e];
+              }
+              tmem_st16(s_tmem + c * 32, w);
             }
-            tmem_st16(s_tmem + c * 32, w);  // over their scores: the hi plane, then the lo plane of these tokens
           }
           tmem_wait_st();
         }
@@ -464,7 +482,7 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         ++done;
       }
       // ---- the end of the stretch
-      if (lane == 0) mbar_arrive(bar_base + 8u * L::B_Q_EMPTY);
+      if (lane == 0) mbar_arrive(bar_base + 8u * (L::B_Q_EMPTY + buf));
       const bool cut = it.pieces > 1;
       const int part = 2 * blockIdx.x + (static_cast<int>(blockIdx.x) == it.first ? 1 : 0);
       if (warp_live) {
@@ -532,7 +550,17 @@ int launch(const PagedLaunch& l) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynBytes) != cudaSuccess) return GDPA_ERR_LAUNCH_;
     return launch_after(kernel, l.grid, L::kThreads, L::kDynBytes, l.stream, l.tm_q, l.tm_k, l.tm_v, l.args);
   };
-  return l.args.act == ACT_SOFTMAX ? go(gdpa_paged_rows_kernel<D, true>) : go(gdpa_paged_rows_kernel<D, false>);
+  switch (l.args.act) {
+    case ACT_SOFTMAX: return go(gdpa_paged_rows_kernel<D, ACT_SOFTMAX>);
+    case ACT_GELU_ERF: return go(gdpa_paged_rows_kernel<D, ACT_GELU_ERF>);
+    case ACT_GELU_TANH: return go(gdpa_paged_rows_kernel<D, ACT_GELU_TANH>);
+    case ACT_LEAKY_RELU: return go(gdpa_paged_rows_kernel<D, ACT_LEAKY_RELU>);
+    case ACT_RELU: return go(gdpa_paged_rows_kernel<D, ACT_RELU>);
+    case ACT_SILU: return go(gdpa_paged_rows_kernel<D, ACT_SILU>);
+    case ACT_HARDSWISH: return go(gdpa_paged_rows_kernel<D, ACT_HARDSWISH>);
+    case ACT_RELU_SQUARE: return go(gdpa_paged_rows_kernel<D, ACT_RELU_SQUARE>);
+    default: return go(gdpa_paged_rows_kernel<D, ACT_RAW>);
+  }
 }
 
 }  // namespace

@@ -479,7 +479,9 @@ int make_q8_tmap(CUtensorMap* m, const void* base, int planes, long long rows, i
 
 bool aligned16(const void* a, const void* b) { return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u) == 0; }
 
-// Rows of an item: the smallest of the kernels' that holds a request's (query, head of the group) rows, 256 at most.
+// Rows of an item: the smallest of the kernels' that holds a request's (query, head of the group) rows, 256 at most.  The narrower kernel
+// against the wider, one B200, 64 requests of 4096 tokens, 8 heads on 2 of 128 values: 16 rows 46 us against 60, 64 rows 77 against 101; at
+// 64 values and SiLU 40 against 62, 76 against 81.
 int paged_rows(int group, int max_q) {
   const long long rows = static_cast<long long>(group) * max_q;
   return rows <= 16 ? 16 : rows <= 64 ? 64 : 256;

@@ -1,14 +1,14 @@
 // GDPA forward over a paged cache of 8-bit keys and values, for sm_100a:  O = act(Q K^T) * scale V  (or the softmax form) for the last
 // queries of every request, K and V e4m3 with one fp32 scale per (block, head).
 //
-// What bounds it: with few queries (a step of generation) the bytes of the cache, with many the tensor cores.  Both are served by one
-// transposed form.  A tile is 128 cached tokens of one K / V head against N rows, the rows being the (query, head of the group) pairs
-// that share this K / V head:
+// This is the form for few queries (a step of generation: up to 64 rows), where the bytes of the cache bound it; many queries have the kernel
+// of gdpa_paged_rows.cu.  It is transposed.  A tile is 128 cached tokens of one K / V head against N rows, the rows being the (query, head of
+// the group) pairs that share this K / V head:
 //     S^T [128 tokens x N] = K Q^T          tcgen05.mma kind::f8f6f4, A = the K tile as it lies in the cache
 //     P^T = act(S^T) per token and row      a thread has one token: its scales are two registers, a mask is a compare
 //     O^T [D x N] += V^T P^T                A = the V tile, MN-major, as it lies in the cache
 // The cache bytes go from HBM through TMA into the tensor cores without a conversion, the 128-row side of the MMA is always full, and
-// N is as small as the rows are few (16 to 128), where the untransposed form would compute 128 rows for one query.
+// N is as small as the rows are few (16 or 64), where the untransposed form would compute 128 rows for one query.
 //
 // Both small operands have to be e4m3 as well, and one e4m3 value has four significant bits.  So Q and P are each the sum of two:
 // hi = e4m3(x), lo = e4m3(x - hi), both multiplied into the same accumulator.  For a bf16 Q (eight significant bits) scaled by a
@@ -43,15 +43,15 @@ struct PagedShape {
   static constexpr int kGroups = NMAX / kCols;         // warpgroups
   static constexpr int kCtasPerSm = NMAX > 16 ? 1 : D == 128 ? 2 : 3;
   static constexpr int kTileBytes = kTile * D;         // K or V tile
-  static constexpr int kStages = NMAX <= 16 ? 3 : (NMAX > 64 ? 3 : 5) * (D == 128 ? 1 : 2);
+  static constexpr int kStages = NMAX <= 16 ? 3 : D == 128 ? 5 : 10;
   static constexpr int kQBytes = NMAX * D;             // hi, then lo
   static constexpr int kPBytes = NMAX * kTile;
   static constexpr int kWarps = 4 * kGroups + 2;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kLoadWarp = 4 * kGroups, kMmaWarp = kLoadWarp + 1;
-  static constexpr int kTmemCols = NMAX <= 16 ? 64 : NMAX <= 64 ? 256 : 512;  // S0, S1, O of NMAX columns each
-  static constexpr int kItemUnits = 4, kMostTileUnits = 1;
-  static constexpr __host__ __device__ int tile_units(int) { return 1; }
+  static constexpr int kTmemCols = NMAX <= 16 ? 64 : 256;  // S0, S1, O of NMAX columns each
+  static constexpr bool kOwnV = false;  // a stage has K and V
+  static constexpr int kItemUnits = 4;
   static constexpr float kTarget = 64.f;
 
   static constexpr int kKvOff = 0;                                  // [stage]{K, V}

@@ -77,32 +77,27 @@ __device__ __forceinline__ Request load_request(const PagedArgs& a, int b) {
 }
 
 // What an item costs, in units: L::kItemUnits for its beginning and end, and for each of its KV tiles (one at least: a row tile without keys
-// has zeros to write) L::tile_units(rows).
+// has zeros to write) one.
 template <class L>
-__device__ __forceinline__ long long units_of_item(int rows, int tiles) {
-  return L::kItemUnits + static_cast<long long>(max(1, tiles)) * L::tile_units(rows);
+__device__ __forceinline__ long long units_of_item(int tiles) {
+  return L::kItemUnits + max(1, tiles);
 }
 // ... and one K / V head of a request.
 template <class L, int NMAX>
 __device__ __forceinline__ long long units_of(const PagedArgs& a, const Request& r) {
   const int rows = r.q_len * a.group, nt = (rows + NMAX - 1) / NMAX;
   if (nt == 0) return 0;
-  if (!a.causal && a.window < 0) {
-    const int tiles = tiles_of(KeyRange{0, r.len});
-    return (nt - 1) * units_of_item<L>(NMAX, tiles) + units_of_item<L>(rows - (nt - 1) * NMAX, tiles);
-  }
+  if (!a.causal && a.window < 0) return nt * units_of_item<L>(tiles_of(KeyRange{0, r.len}));
   long long n = 0;
   for (int t = 0; t < nt; ++t) {
     const int last = min(rows, (t + 1) * NMAX);
-    n += units_of_item<L>(last - t * NMAX, tiles_of(keys_of_any(t * NMAX / a.group, (last - 1) / a.group, r.q_len, r.len, a.causal, a.window)));
+    n += units_of_item<L>(tiles_of(keys_of_any(t * NMAX / a.group, (last - 1) / a.group, r.q_len, r.len, a.causal, a.window)));
   }
   return n;
 }
-// CTAs that have a share of `all` units: no share is smaller than a tile.
-template <class L>
-__device__ __forceinline__ long long sharing_ctas(long long all) {
-  return min(static_cast<long long>(gridDim.x), max(1LL, all / L::kMostTileUnits));
-}
+// CTAs that have a share of `all` units: no share is smaller than a unit, or a CTA between an item's first and last would have none of its
+// tiles, and the join would wait for a piece that nobody makes.
+__device__ __forceinline__ long long sharing_ctas(long long all) { return min(static_cast<long long>(gridDim.x), max(1ll, all)); }
 
 template <int ACT>
 __device__ __forceinline__ float act_one(float x, float m) {
@@ -131,8 +126,7 @@ __device__ __forceinline__ void act_any(int act, float (&x)[N], float m) {
 }
 
 // Sixteen values -> the sum of two e4m3 values each, hi = e4m3(x) and lo = e4m3(x - hi), packed four to a register.  Stage after stage over
-// all of them, in an order that the volatile statements keep: a value's chain of six conversions takes some 100 cycles, and left to
-// itself the compiler, short of registers, goes through the chains one after the other (128 values of a thread: 10000 cycles).
+// all of them, in an order that the volatile statements keep, so that the chains of conversions run beside one another.
 __device__ __forceinline__ void split_e4m3(const float (&x)[16], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
   uint32_t u[8], v[8];
   uint16_t h[8], l[8];
@@ -151,44 +145,6 @@ __device__ __forceinline__ void split_e4m3(const float (&x)[16], uint32_t (&hi)[
     hi[i] = __byte_perm(h[2 * i], h[2 * i + 1], 0x5410);
     lo[i] = __byte_perm(l[2 * i], l[2 * i + 1], 0x5410);
   }
-}
-// What an activation asks of the special-function pipe, per element.
-enum PagedMufu { MUFU_NONE, MUFU_EX2, MUFU_TANH };
-template <PagedMufu M>
-__device__ __forceinline__ void mufu(float& u) {
-  if constexpr (M == MUFU_EX2) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(u));
-  if constexpr (M == MUFU_TANH) asm volatile("tanh.approx.f32 %0, %0;" : "+f"(u));
-}
-template <PagedMufu M, int N>
-__device__ __forceinline__ void mufu_all(float (&u)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) mufu<M>(u[i]);
-}
-// split_e4m3 of x with the special functions of the next sixteen values between its steps, two to five of them: the two take
-// about the same time on different pipes, and a warp issues in order.
-template <PagedMufu M>
-__device__ __forceinline__ void split_e4m3_and(const float (&x)[16], uint32_t (&hi)[4], uint32_t (&lo)[4], float (&next)[16]) {
-  uint32_t u[8], v[8];
-  uint16_t h[8], l[8];
-#pragma unroll
-  for (int k = 0; k < 40; ++k) {
-    const int i = k % 8;
-    if ((2 * k) % 5 < 2) mufu<M>(next[(2 * k) / 5]);
-    if (k < 8) asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
-    else if (k < 16) asm volatile("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h[i]) : "r"(u[i]));
-    else if (k < 24) asm volatile("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(v[i]) : "h"(h[i]));
-    else if (k < 32) asm volatile("sub.f16x2 %0, %0, %1;" : "+r"(u[i]) : "r"(v[i]));
-    else asm volatile("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l[i]) : "r"(u[i]));
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    hi[i] = __byte_perm(h[2 * i], h[2 * i + 1], 0x5410);
-    lo[i] = __byte_perm(l[2 * i], l[2 * i + 1], 0x5410);
-  }
-}
-__device__ __forceinline__ float2 e4m3x2_values(uint32_t v) {
-  const uint32_t h = f16x2_from_e4m3x2(static_cast<uint16_t>(v));
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
 // Where a CTA's walk over the items begins.
@@ -276,7 +232,7 @@ __device__ __forceinline__ void find_start(const PagedArgs& a, long long* scan, 
     all += scan[w];
   }
   if (threadIdx.x == 0) start->all = all;
-  const long long ctas = sharing_ctas<L>(all);
+  const long long ctas = sharing_ctas(all);
   if (blockIdx.x < ctas) {
     const long long u0 = all * blockIdx.x / ctas;
     long long at = before + incl - sum;
@@ -301,8 +257,8 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
   const PagedArgs& a = cta.a;
   const int lane = cta.lane;
   const uint32_t smem_base = cta.smem_base, bar_base = cta.bar_base;
-  const long long all_units = start->all, ctas = sharing_ctas<L>(all_units);
-  uint32_t loaded = 0;  // tiles asked for
+  const long long all_units = start->all, ctas = sharing_ctas(all_units);
+  uint32_t loaded = 0, loaded_v = 0;  // tiles asked for
   auto walk = [&]() -> bool {
     const int per_tile = kTile >> a.block_shift;  // blocks of a tile
     const int block_size = 1 << a.block_shift;
@@ -333,16 +289,15 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
         ++wt;
         const KeyRange r = keys_of_any(row0 / a.group, (row0 + rows - 1) / a.group, rq.q_len, rq.len, a.causal, a.window);
         const int n = tiles_of(r), n1 = max(1, n);
-        const int w = L::tile_units(rows);
         const long long s = at + L::kItemUnits;  // where the tiles' units begin
-        at = s + static_cast<long long>(n1) * w;
+        at = s + n1;
         // a tile belongs to the CTA that has its first unit
-        auto tile_from = [&](long long u) { return static_cast<int>(min(max((u - s + w - 1) / w, 0ll), static_cast<long long>(n1))); };
+        auto tile_from = [&](long long u) { return static_cast<int>(min(max(u - s, 0ll), static_cast<long long>(n1))); };
         const int from = u0 <= s ? 0 : tile_from(u0), to = u1 <= s ? 0 : tile_from(u1);
         if (from >= to) continue;
         // the CTA that has unit u is the largest c with all * c / ctas <= u
         const int first = static_cast<int>(((s + 1) * ctas - 1) / all_units);
-        const int pieces = static_cast<int>(((s + static_cast<long long>(n1 - 1) * w + 1) * ctas - 1) / all_units) - first + 1;
+        const int pieces = static_cast<int>(((s + n1) * ctas - 1) / all_units) - first + 1;
         it = PagedItem{wh, rq.q_start, rq.q_len, row0, rows, rq.len, r.lo, r.hi, r.lo / kTile + from, n == 0 ? 0 : to - from, pieces, first};
         b_of = wb;
         break;
@@ -371,12 +326,12 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
         if (!cta.wait(L::B_KV_EMPTY + stage, ((pos / L::kStages) & 1u) ^ 1u, ST_ROLE_LOAD)) return false;
         const uint32_t bar = bar_base + 8u * (L::B_KV_FULL + stage);
         const unsigned n_valid = __popc(__ballot_sync(kFull, valid));
-        if (lane == 0) mbar_arrive_expect_tx(bar, n_valid * block_size * D * 2);
+        if (lane == 0) mbar_arrive_expect_tx(bar, n_valid * block_size * D * (L::kOwnV ? 1 : 2));
         __syncwarp();
-        const uint32_t dst = smem_base + L::kKvOff + stage * 2 * L::kTileBytes + lane * block_size * D;
+        const uint32_t dst = smem_base + L::kKvOff + stage * (L::kOwnV ? 1 : 2) * L::kTileBytes + lane * block_size * D;
         if (valid) {
           tma_load_4d(dst, &tm_k, bar, 0, 0, it.h, blk);
-          tma_load_4d(dst + L::kTileBytes, &tm_v, bar, 0, 0, it.h, blk);
+          if constexpr (!L::kOwnV) tma_load_4d(dst + L::kTileBytes, &tm_v, bar, 0, 0, it.h, blk);
         }
         // a block that is not there has scale 0, which tells the others
         if (lane < per_tile) {
@@ -387,6 +342,14 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
         }
         cp_async_mbar_arrive(bar_base + 8u * (L::B_SC_FULL + stage));
         loaded = pos + 1;
+        if constexpr (L::kOwnV) {  // V has one place of its own
+          if (!cta.wait(L::B_V_EMPTY, (pos & 1u) ^ 1u, ST_ROLE_LOAD)) return false;
+          const uint32_t v_bar = bar_base + 8u * L::B_V_FULL;
+          if (lane == 0) mbar_arrive_expect_tx(v_bar, n_valid * block_size * D);
+          __syncwarp();
+          if (valid) tma_load_4d(smem_base + L::kVOff + lane * block_size * D, &tm_v, v_bar, 0, 0, it.h, blk);
+          loaded_v = pos + 1;
+        }
         // the next item's Q: its buffer is the last item's, which is done when this item's first stages have been used
         if (j == min(L::kStages, it.tiles - 1) && ahead.h >= 0 && ahead.tiles > 0 && !load_q(ahead)) return false;
       }
@@ -399,6 +362,9 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
     const uint64_t t0 = global_timer_ns();
     for (uint32_t k = loaded > L::kStages ? loaded - L::kStages : 0; k < loaded; ++k)
       while (!mbar_try_wait(bar_base + 8u * (L::B_KV_FULL + k % L::kStages), (k / L::kStages) & 1u) && global_timer_ns() - t0 < kWaitLimitNs) {
+      }
+    if constexpr (L::kOwnV)
+      while (loaded_v > 0 && !mbar_try_wait(bar_base + 8u * L::B_V_FULL, (loaded_v - 1) & 1u) && global_timer_ns() - t0 < kWaitLimitNs) {
       }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");

@@ -1,18 +1,29 @@
-// The attention over a paged 8-bit cache (gdpa_paged.cu) for many queries: candidates of a request, chunks of a prompt.  There the tensor
-// cores and the element-wise work bound it, and the form is the ordinary one, a row of scores to a thread:
-//     S [128 rows x 128 tokens] = Q K^T      A = Q (two e4m3 planes in shared memory), B = the K tile
-//     P = act(S) in registers                a thread has a row: its maximum, sum and reference are its own, nothing is exchanged
-//     O [128 rows x D] += P V                A = P (two e4m3 planes) in tensor memory over its own S, B = the V tile, MN-major
-// A work item is 256 rows (two row tiles) of one (request, K / V head); the tiles' element-wise warps and MMAs take turns, one tile's
-// MMAs under the other's exponentials.  A token's scales are the same for a whole row of threads: for each block of 16 tokens and more
-// the score's factor and the reference less log2 of V's scale are two registers, so that P times V's scale is one FMA and one
-// exponential.  A first look at a tile's scores (one maximum in two of them, of the numbers as they are) says whether a product would pass
-// 448 for the reference that a row has; only then it moves (by whole powers of two) and the row's O and sum with it.
+// The attention over a paged 8-bit cache (gdpa_paged.cu) for many queries: candidates of a request, chunks of a prompt.  The form is the
+// ordinary one, a row of scores to a thread:
+//     S [128 rows x 64 tokens] = Q K^T       kind::f8f6f4, A = Q (two e4m3 planes in shared memory), B = the K tile as it lies in the cache
+//     P = act(S) in registers, float16       a thread has a row: its maximum, sum and reference are its own, nothing is exchanged
+//     O [128 rows x D] += P V                kind::f16, A = P in tensor memory over its own S, B = V in float16, MN-major
+// A work item is 256 rows (two row tiles) of one (request, K / V head), a KV tile 128 tokens, taken in two halves: while a row tile's warps have
+// one half of its scores the tensor cores have the other, the products with V of the tile and the scores of the next.
 //
-// Against the transposed form on 128 rows (one B200): candidates (SiLU) 917 us, causal chunks 757 us there.
+// P in one float16 instead of two e4m3 values: the products take as long (half the rate, once instead of twice) and leave 2^-11 of a value,
+// and P takes one conversion for two elements, not four; V, which then has to be float16, is one conversion of 128 x D elements for all rows
+// of a tile, by warps of their own.  A token's scales are the same for a whole row of threads: the score's factor and the logarithm of V's
+// scale are two registers for 16 tokens, so that P times V's scale is one FMA and one exponential.
 //
-// Roles: warps 0-3 and 4-7 the element-wise work and epilogue of row tiles 0 and 1, warp 8 TMA loads and the walk, warp 9 MMAs, warp 10
-// overwrites V rows that no query may see with zeros (0 times NaN is NaN) before the products with V.
+// The reference of a row (the running maximum; for the other activations a power of two that P is multiplied by) is set so that the largest P
+// lies in (32, 64], and moves when 64 tokens' |P| sum up to 65504, float16's largest, or more: the sum that the softmax takes anyhow is the
+// whole test.  Then, for the first tokens of a stretch and where a mask leaves tokens out, the scores, which are still there, are gone through
+// again: once for the sum and maximum under the masks, once for P.  Both forms do the same arithmetic, so no row's bits depend on its neighbours.
+//
+// Measured (one B200, caches cold): causal chunks of 256 to 1024 queries 425 us, candidates (64 to 1024, SiLU) 729 us; the transposed form with
+// 128 rows 757 and 917, this form with P in two e4m3 values 478 and 815.  256 rows against 128 tokens take 2.5 us whatever the activation, 128
+// rows 2.2: neither the tensor cores (1.1 us of it) nor one pipe bounds it, but the chain from the scores of 64 tokens to the next ones' with two
+// warps on a scheduler.  Slower here: an MMA warp for each row tile (433, 775); scores of 128 tokens at once (437, 730); the row tiles' warps
+// taking strict turns (507, 967); 16 element-wise warps, half a row each, with two converting V, who are then late (600, 1110).
+//
+// Roles: warps 0-3 and 4-7 the element-wise work and epilogue of row tiles 0 and 1, warp 8 TMA loads and the walk, warp 9 MMAs, warps 10-13
+// V to float16, with zeros for tokens that no query may see (0 times NaN is NaN).
 #include <cuda_bf16.h>
 
 #include "gdpa_paged.cuh"
@@ -26,28 +37,33 @@ constexpr int kRows = 256;  // of an item
 template <int D>
 struct RowsShape {
   static constexpr int kTileBytes = kTile * D;               // K or V tile, or a plane of a row tile of Q
-  static constexpr int kStages = D == 128 ? 2 : 4;
-  static constexpr int kWarps = 11, kThreads = 32 * kWarps;
-  static constexpr int kLoadWarp = 8, kMmaWarp = 9, kFixWarp = 10;
-  static constexpr int kItemUnits = 2, kMostTileUnits = 1;
-  static constexpr __host__ __device__ int tile_units(int) { return 1; }
+  static constexpr int kStages = D == 128 ? 2 : 4;           // of K and the scales
+  static constexpr bool kOwnV = true;
+  static constexpr int kActWarps = 8, kConvertWarps = 4, kWarps = kActWarps + 2 + kConvertWarps, kThreads = 32 * kWarps;
+  static constexpr int kLoadWarp = kActWarps, kMmaWarp = kActWarps + 1, kConvertWarp = kActWarps + 2;
+  static constexpr int kItemUnits = 2;                       // against tiles, which take the same time for 128 rows and for 256, nearly
   static constexpr float kTarget = 64.f;
-  static constexpr int kKvOff = 0;                                 // [stage]{K, V}
-  static constexpr int kQOff = kStages * 2 * kTileBytes;           // [2][row tile]{hi, lo}
+  static constexpr int kKvOff = 0;                                 // [stage] K
+  static constexpr int kVOff = kStages * kTileBytes;               // V as it is in the cache
+  static constexpr int kV16Off = kVOff + kTileBytes;               // V in float16: [D / 64][128 tokens][64]
+  static constexpr int kQOff = kV16Off + 2 * kTileBytes;           // [2][row tile]{hi, lo}
   static constexpr int kScaleOff = kQOff + 8 * kTileBytes;         // float[stage][16]: K scales of up to 8 blocks, V scales
-  static constexpr int kPoisonOff = kScaleOff + kStages * 64;      // uint[stage][4]: tokens whose V row held a NaN
-  static constexpr int kQaOff = kPoisonOff + kStages * 16;         // float[2][kRows]
-  static constexpr int kRingOff = kQaOff + 2 * kRows * 4;              // int[kItemSlots][16]
+  static constexpr int kPoisonOff = kScaleOff + kStages * 64;      // uint16[8]: tokens whose V row held a NaN
+  static constexpr int kQaOff = kPoisonOff + 16;         // float[2][kRows]
+  static constexpr int kRingOff = kQaOff + 2 * kRows * 4;         // int[kItemSlots][16]
   static constexpr int kBarOff = kRingOff + kItemSlots * 64;
   enum : int {
     B_KV_FULL = 0,
     B_KV_EMPTY = B_KV_FULL + kStages,
     B_SC_FULL = B_KV_EMPTY + kStages,
-    B_V_READY = B_SC_FULL + kStages,
-    B_S_FULL = B_V_READY + kStages,  // [2]
-    B_P_FULL = B_S_FULL + 2,         // [2]
-    B_PV_DONE = B_P_FULL + 2,        // [2]
-    B_Q_FULL = B_PV_DONE + 2,        // [2]
+    B_V_FULL = B_SC_FULL + kStages,
+    B_V_EMPTY = B_V_FULL + 1,
+    B_V_READY = B_V_EMPTY + 1,  // [half]: V in float16
+    B_V_DONE = B_V_READY + 2,   // [half]
+    B_S_FULL = B_V_DONE + 2,  // [row tile][half]
+    B_P_FULL = B_S_FULL + 4,         // [row tile][half]
+    B_PV_DONE = B_P_FULL + 4,        // [row tile][half]
+    B_Q_FULL = B_PV_DONE + 4,        // [2]
     B_Q_EMPTY = B_Q_FULL + 2,        // [2]
     B_ITEM_FULL = B_Q_EMPTY + 2,     // [kItemSlots]
     B_ITEM_EMPTY = B_ITEM_FULL + kItemSlots,
@@ -66,7 +82,6 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                        const PagedArgs a) {
   using L = RowsShape<D>;
   constexpr bool SOFTMAX = ACT == ACT_SOFTMAX;
-  constexpr PagedMufu kMufu = SOFTMAX ? MUFU_EX2 : ACT == ACT_SILU || ACT == ACT_GELU_TANH ? MUFU_TANH : MUFU_NONE;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem_base = smem_u32(smem);
@@ -81,10 +96,11 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     for (int i = 0; i < L::B_COUNT; ++i) {
       uint32_t n = 1;
       if (i >= L::B_SC_FULL && i < L::B_SC_FULL + L::kStages) n = 32;
-      if (i >= L::B_P_FULL && i < L::B_P_FULL + 2) n = 4;
+      if (i >= L::B_V_EMPTY && i < L::B_V_READY + 2) n = L::kConvertWarps;  // V_EMPTY, V_READY
+      if (i >= L::B_P_FULL && i < L::B_P_FULL + 4) n = L::kActWarps / 2;
       if (i >= L::B_Q_FULL && i < L::B_Q_FULL + 2) n = 33;
-      if (i >= L::B_Q_EMPTY && i < L::B_Q_EMPTY + 2) n = 1 + 8;
-      if (i >= L::B_ITEM_EMPTY && i < L::B_ITEM_EMPTY + kItemSlots) n = 10;
+      if (i >= L::B_Q_EMPTY && i < L::B_Q_EMPTY + 2) n = 1 + L::kActWarps;
+      if (i >= L::B_ITEM_EMPTY && i < L::B_ITEM_EMPTY + kItemSlots) n = L::kActWarps + 1 + L::kConvertWarps;
       mbar_init(bar_base + 8u * i, n);
     }
     *abort_flag = 0;
@@ -104,7 +120,7 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = warp_uniform(*tmem_ptr);  // S0, S1 of 128 columns each, O0, O1
+  const uint32_t tmem_base = warp_uniform(*tmem_ptr);  // S0, S1 of 128 columns each (two halves), O0, O1
   PagedCta<L> cta{a, smem, smem_base, bar_base, abort_flag, lane};
 
   if (warp == L::kLoadWarp) {
@@ -132,19 +148,21 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   } else if (warp == L::kMmaWarp) {
     // ------------------------------------------------------------------ MMA issuer
     constexpr int kSwizzle = D == 128 ? 128 : 64;
-    constexpr uint32_t kIdescQK = umma_idesc(0, 0, 0, 0, kTile, kTile), kIdescPV = umma_idesc(0, 0, 0, 1, kTile, D);
+    constexpr uint32_t kIdescQK = umma_idesc(0, 0, 0, 0, kTile, kTile / 2), kIdescPV = umma_idesc(0, 0, 0, 1, kTile, D);  // e4m3 there, float16 here
     const uint64_t dk0 = umma_smem_desc(smem_base + L::kKvOff, 16, 8 * D, kSwizzle);
-    const uint64_t dv0 = umma_smem_desc(smem_base + L::kKvOff + L::kTileBytes, 0, 8 * D, kSwizzle);
+    const uint64_t dv0 = umma_smem_desc_sw128(smem_base + L::kV16Off, kTile * 128, 1024);
     const uint64_t dq0 = umma_smem_desc(smem_base + L::kQOff, 16, 8 * D, kSwizzle);
     uint32_t pos = 0, q_pos = 0, p_phase = 0;
-    auto issue_qk = [&](int s, uint32_t stage, uint32_t buf) {
-      const uint64_t dk = umma_desc_advance(dk0, stage * 2 * L::kTileBytes), dq = umma_desc_advance(dq0, (2 * buf + s) * 2 * L::kTileBytes);
+    auto issue_qk = [&](int s, int h, uint32_t stage, uint32_t buf) {  // scores of row tile s with tokens 64 h .. of the tile
+      const uint64_t dk = umma_desc_advance(dk0, stage * L::kTileBytes + h * L::kTileBytes / 2),
+                     dq = umma_desc_advance(dq0, (2 * buf + s) * 2 * L::kTileBytes);
+      const uint32_t d = tmem_base + s * kTile + h * (kTile / 2);
 #pragma unroll
       for (int kk = 0; kk < D / 32; ++kk) {
-        umma_ss_f8(tmem_base + s * kTile, umma_desc_advance(dq, kk * 32), umma_desc_advance(dk, kk * 32), kIdescQK, kk > 0 ? 1u : 0u);
-        umma_ss_f8(tmem_base + s * kTile, umma_desc_advance(dq, L::kTileBytes + kk * 32), umma_desc_advance(dk, kk * 32), kIdescQK, 1u);
+        umma_ss_f8(d, umma_desc_advance(dq, kk * 32), umma_desc_advance(dk, kk * 32), kIdescQK, kk > 0 ? 1u : 0u);
+        umma_ss_f8(d, umma_desc_advance(dq, L::kTileBytes + kk * 32), umma_desc_advance(dk, kk * 32), kIdescQK, 1u);
       }
-      tc_commit(bar_base + 8u * (L::B_S_FULL + s));
+      tc_commit(bar_base + 8u * (L::B_S_FULL + 2 * s + h));
     };
     while (true) {
       const PagedItem it = cta.take_item(ST_ROLE_MMA);
@@ -159,37 +177,55 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       ++q_pos;
       PAGED_WAIT(L::B_KV_FULL + pos % L::kStages, (pos / L::kStages) & 1u, ST_ROLE_MMA);
       tc_fence_after();
-      for (int s = 0; s < nst; ++s) issue_qk(s, pos % L::kStages, buf);
+      for (int h = 0; h < 2; ++h)
+        for (int s = 0; s < nst; ++s) issue_qk(s, h, pos % L::kStages, buf);
       if (it.tiles == 1) tc_commit(bar_base + 8u * (L::B_Q_EMPTY + buf));
       for (int j = 0; j < it.tiles; ++j, ++pos) {
         const uint32_t stage = pos % L::kStages, next = (pos + 1) % L::kStages;
         const bool more = j + 1 < it.tiles;
-        for (int s = 0; s < nst; ++s) {
-          PAGED_WAIT(L::B_P_FULL + s, (p_phase >> s) & 1u, ST_ROLE_MMA);
-          p_phase ^= 1u << s;
-          if (s == 0) PAGED_WAIT(L::B_V_READY + stage, (pos / L::kStages) & 1u, ST_ROLE_MMA);
-          tc_fence_after();
-          const uint64_t dv = umma_desc_advance(dv0, stage * 2 * L::kTileBytes);
-          const uint32_t o = tmem_base + 256 + s * kTile, p = tmem_base + s * kTile;
-#pragma unroll
-          for (int kk = 0; kk < kTile / 32; ++kk) {
-            const uint64_t dvk = umma_desc_advance(dv, kk * 32 * D);
-            umma_ts_f8(o, p + kk * 32, dvk, kIdescPV, j > 0 || kk > 0 ? 1u : 0u);
-            umma_ts_f8(o, p + kk * 32 + 8, dvk, kIdescPV, 1u);
-          }
-          tc_commit(bar_base + 8u * (L::B_PV_DONE + s));
-          if (more) {
-            if (s == 0) PAGED_WAIT(L::B_KV_FULL + next, ((pos + 1) / L::kStages) & 1u, ST_ROLE_MMA);
+        for (int h = 0; h < 2; ++h) {
+          for (int s = 0; s < nst; ++s) {
+            PAGED_WAIT(L::B_P_FULL + 2 * s + h, (p_phase >> s) & 1u, ST_ROLE_MMA);
+            if (h == 1) p_phase ^= 1u << s;
+            if (s == 0) PAGED_WAIT(L::B_V_READY + h, pos & 1u, ST_ROLE_MMA);
             tc_fence_after();
-            issue_qk(s, next, buf);
+            const uint32_t o = tmem_base + 256 + s * kTile, p = tmem_base + s * kTile + h * (kTile / 2);
+#pragma unroll
+            for (int kk = 0; kk < kTile / 32; ++kk)
+              umma_ts_f16(o, p + kk * 8, umma_desc_advance(dv0, (h * 4 + kk) * 16 * 128), kIdescPV, j > 0 || h > 0 || kk > 0 ? 1u : 0u);
+            if (s == nst - 1) tc_commit(bar_base + 8u * (L::B_V_DONE + h));
+            tc_commit(bar_base + 8u * (L::B_PV_DONE + 2 * s + h));
+            if (more) {
+              if (h == 0 && s == 0) PAGED_WAIT(L::B_KV_FULL + next, ((pos + 1) / L::kStages) & 1u, ST_ROLE_MMA);
+              tc_fence_after();
+              issue_qk(s, h, next, buf);
+            }
           }
         }
         tc_commit(bar_base + 8u * (L::B_KV_EMPTY + stage));
         if (j + 2 == it.tiles) tc_commit(bar_base + 8u * (L::B_Q_EMPTY + buf));
       }
     }
-  } else if (warp == L::kFixWarp) {
-    // ------------------------------------------------------------------ V rows that must not be seen
+  } else if (warp >= L::kConvertWarp) {
+    // ------------------------------------------------------------------ V to float16; rows that must not be seen, to zeros
+    constexpr int kChunks = D / 16, kTokens = 32 / kChunks, kSteps = 16 / kTokens;  // 16 bytes of a row to a lane, tokens of a warp at once
+    const int w = warp - L::kConvertWarp, chunk = lane % kChunks, t_lane = lane / kChunks, other = chunk >> 2;
+    // where a lane's 16 bytes are, as the copy's swizzle has them, and where their 16 values go: eight lanes at once to as many groups of banks,
+    // for which the second panel's halves are written in the other order
+    auto from_of = [&](int t) { return L::kVOff + t * D + (D == 128 ? chunk ^ (t & 7) : chunk ^ ((t >> 1) & 3)) * 16; };
+    auto to_of = [&](int t, int k) { return L::kV16Off + other * (kTile * 128) + t * 128 + ((2 * (chunk & 3) + (other ^ k)) ^ (t & 7)) * 16; };
+    auto put = [&](int t, const uint4& u) {
+      const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+      uint32_t f[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[2 * e] = f16x2_from_e4m3x2(static_cast<uint16_t>(v[e] & 0xffffu));
+        f[2 * e + 1] = f16x2_from_e4m3x2(static_cast<uint16_t>(v[e] >> 16));
+      }
+      const uint4 lo = make_uint4(f[0], f[1], f[2], f[3]), hi = make_uint4(f[4], f[5], f[6], f[7]);
+      *reinterpret_cast<uint4*>(smem + to_of(t, 0)) = other ? hi : lo;
+      *reinterpret_cast<uint4*>(smem + to_of(t, 1)) = other ? lo : hi;
+    };
     uint32_t pos = 0;
     while (true) {
       const PagedItem it = cta.take_item(ST_ROLE_FIX);
@@ -201,51 +237,63 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                      r1 = keys_of((it.row0 + it.rows - 1) / a.group, it.q_len, it.len, a.causal, a.window);
       const int all_lo = max(r0.lo, r1.lo), all_hi = min(r0.hi, r1.hi);  // keys that every row takes part with (if any)
       for (int j = 0; j < it.tiles; ++j, ++pos) {
-        const uint32_t stage = pos % L::kStages, phase = (pos / L::kStages) & 1u;
+        const uint32_t stage = pos % L::kStages;
         const int key0 = (it.tile0 + j) * kTile;
-        PAGED_WAIT(L::B_SC_FULL + stage, phase, ST_ROLE_FIX);
-        PAGED_WAIT(L::B_KV_FULL + stage, phase, ST_ROLE_FIX);
+        PAGED_WAIT(L::B_SC_FULL + stage, (pos / L::kStages) & 1u, ST_ROLE_FIX);
+        PAGED_WAIT(L::B_V_FULL, pos & 1u, ST_ROLE_FIX);
         const float* const sv = reinterpret_cast<const float*>(smem + L::kScaleOff) + stage * 16 + 8;
         const bool every = key0 >= all_lo && key0 + kTile <= all_hi;
-        bool touched = false;
+        const bool checks = !every || __any_sync(kFull, lane < kTile >> a.block_shift && sv[lane & 7] == 0.f);
 #pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          const int t = 32 * i + lane, key = key0 + t;
-          const bool out = key < it.lo || key >= it.hi || sv[t >> a.block_shift] == 0.f;
-          uint4* const v_row = reinterpret_cast<uint4*>(smem + L::kKvOff + (2 * stage + 1) * L::kTileBytes + t * D);
-          bool bad = false;
-          if (!every && !out) {
-            // some row may take part with this token and some not: a NaN goes into P of those that do
-            for (int e = 0; e < D / 16; ++e) {
-              const uint4 u = v_row[e];
-              bad |= (__vcmpeq4(u.x & 0x7f7f7f7fu, 0x7f7f7f7fu) | __vcmpeq4(u.y & 0x7f7f7f7fu, 0x7f7f7f7fu) |
-                      __vcmpeq4(u.z & 0x7f7f7f7fu, 0x7f7f7f7fu) | __vcmpeq4(u.w & 0x7f7f7f7fu, 0x7f7f7f7fu)) != 0u;
+        for (int half = 0; half < 2; ++half) {
+          const int t0 = half * 64 + w * 16 + t_lane;
+          PAGED_WAIT(L::B_V_DONE + half, (pos & 1u) ^ 1u, ST_ROLE_FIX);  // the products with the tile before
+          if (!checks) {
+            uint4 u[kSteps];
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) u[i] = *reinterpret_cast<const uint4*>(smem + from_of(t0 + i * kTokens));
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) put(t0 + i * kTokens, u[i]);
+          } else {
+            unsigned poison = 0;
+#pragma unroll 1
+            for (int i = 0; i < kSteps; ++i) {
+              const int t = t0 + i * kTokens, key = key0 + t;
+              uint4 u = *reinterpret_cast<const uint4*>(smem + from_of(t));
+              const bool out = key < it.lo || key >= it.hi || sv[t >> a.block_shift] == 0.f;
+              // some row may take part with this token and some not: a NaN goes into P of those that do
+              const bool nan = !every && !out && (__vcmpeq4(u.x & 0x7f7f7f7fu, 0x7f7f7f7fu) | __vcmpeq4(u.y & 0x7f7f7f7fu, 0x7f7f7f7fu) |
+                                                  __vcmpeq4(u.z & 0x7f7f7f7fu, 0x7f7f7f7fu) | __vcmpeq4(u.w & 0x7f7f7f7fu, 0x7f7f7f7fu)) != 0u;
+              const bool bad = ((__ballot_sync(kFull, nan) >> (t_lane * kChunks)) & ((1u << kChunks) - 1u)) != 0u;
+              if (bad) poison |= 1u << (i * kTokens + t_lane);
+              if (out || bad) u = make_uint4(0, 0, 0, 0);
+              put(t, u);
             }
+            poison = __reduce_or_sync(kFull, poison);
+            if (lane == 0) reinterpret_cast<uint16_t*>(smem + L::kPoisonOff)[half * 4 + w] = static_cast<uint16_t>(poison);
           }
-          if (out || bad)
-            for (int e = 0; e < D / 16; ++e) v_row[e] = make_uint4(0, 0, 0, 0);
-          touched |= out || bad;
-          const unsigned poison = __ballot_sync(kFull, bad);
-          if (lane == 0) reinterpret_cast<unsigned*>(smem + L::kPoisonOff)[stage * 4 + i] = poison;
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(bar_base + 8u * (L::B_V_READY + half));
+            if (half == 1) mbar_arrive(bar_base + 8u * L::B_V_EMPTY);
+          }
         }
-        if (touched) fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_base + 8u * (L::B_V_READY + stage));
       }
     }
   } else {
     // ------------------------------------------------------------------ element-wise work and epilogue: a row to a thread
-    constexpr float kHeadroom = 2.8073549f + 0.001f;  // log2(448 / kTarget)
     constexpr float kLogTarget = 6.f;
-    static_assert(L::kTarget == 64.f, "kHeadroom, kLogTarget");
+    static_assert(L::kTarget == 64.f, "kLogTarget");
+    constexpr float kMostSum = 65504.f;  // of 64 |P|: then each has its place in a float16
     const int qt = warp >> 2, quarter = warp & 3;
     const int r = qt * kTile + quarter * 32 + lane;  // row of the item
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_tmem = tmem_base + qt * kTile + lane_base, o_tmem = tmem_base + 256 + qt * kTile + lane_base;
+    const uint32_t s_rows = tmem_base + qt * kTile + lane_base, o_tmem = tmem_base + 256 + qt * kTile + lane_base;
     uint32_t pos = 0, q_pos = 0, done = 0;  // tiles, items with tiles, tiles of this row tile
     while (true) {
       const PagedItem it = cta.take_item(ST_ROLE_ACT);
-      if (named_bar_or(3, 256, it.h < 0)) break;
+      if (named_bar_or(3, 32 * L::kActWarps, it.h < 0)) break;
       const int g = it.row0 + r, i = g / a.group;
       const bool live = r < it.rows;
       __nv_bfloat16* const o_row = a.o + ((it.q_start + static_cast<long long>(i)) * a.heads + it.h * a.group + (g - i * a.group)) * D;
@@ -263,115 +311,128 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       PAGED_WAIT_ON(L::B_Q_FULL + buf, (q_pos >> 1) & 1u);
       ++q_pos;
       const float qa = reinterpret_cast<const float*>(smem + L::kQaOff)[buf * kRows + r];
-      float ref = SOFTMAX ? kNoMax : 1.f, l = 0.f;  // running maximum / multiplier; sum of P
+      float ref = SOFTMAX ? kNoMax : 1.2676506e30f, l = 0.f;  // running maximum / multiplier; sum of P
       for (int j = 0; j < it.tiles; ++j, ++pos) {
         const uint32_t stage = pos % L::kStages, phase = (pos / L::kStages) & 1u;
         if (!tile_live) continue;  // neither S nor P of this row tile in the item
         const int key0 = (it.tile0 + j) * kTile;
         PAGED_WAIT_ON(L::B_SC_FULL + stage, phase);
-        PAGED_WAIT_ON(L::B_S_FULL + qt, done & 1u);
-        tc_fence_after();
-        if (warp_live) {
-          const float* const sc = reinterpret_cast<const float*>(smem + L::kScaleOff) + stage * 16;
-          const bool every = key0 >= all_lo && key0 + kTile <= all_hi;
-          if (!every) PAGED_WAIT_ON(L::B_V_READY + stage, phase);  // with the tokens whose V held a NaN
-          const unsigned* const poison = reinterpret_cast<const unsigned*>(smem + L::kPoisonOff) + stage * 4;
-          bool missing = false;  // a block that the table has not
+        const float* const sc = reinterpret_cast<const float*>(smem + L::kScaleOff) + stage * 16;
+        const bool every = key0 >= all_lo && key0 + kTile <= all_hi;
+        // ... or a block that the table has not
+        const bool masked = !every || __any_sync(kFull, lane < kTile >> a.block_shift && sc[8 + (lane & 7)] == 0.f);
 #pragma unroll 1
-          for (int b = 0; b < kTile >> a.block_shift; ++b) missing |= sc[8 + b] == 0.f;
-          const bool masked = !every || missing;
-          const int from = rg.lo - key0, to = rg.hi - key0;  // columns of this row that count
-          // columns 32 c .. of the scores; `h`: which 16 of them
-          auto factors = [&](int c, int h, float& kf, float& vs) {
-            const int b = (c * 32 + h * 16) >> a.block_shift;
-            kf = sc[b] * qa;
-            vs = fmaxf(sc[8 + b], kLeastScale);
-          };
-          auto first_bits = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
-          auto part_of = [&](int c) -> uint32_t {  // a bit for each of the 32
-            uint32_t m = first_bits(to - c * 32) & ~first_bits(from - c * 32);
-            if (sc[8 + ((c * 32) >> a.block_shift)] == 0.f) m &= 0xffff0000u;
-            if (sc[8 + ((c * 32 + 16) >> a.block_shift)] == 0.f) m &= 0x0000ffffu;
-            return m;
-          };
-          // ---- first look: how large this tile's P, times V's scale, gets (softmax: its logarithm).  Monotone in the score on its positive side,
-          // |activation| is bounded by a constant on the other (exactly so, or 0.38 at most).
-          float top = SOFTMAX ? kNoMax : 0.f;
-          const bool flip = SOFTMAX && a.scale < 0.f;  // then the smallest product is the largest score
-          auto look = [&](float most, float least, float kf, float vs) {
-            if constexpr (SOFTMAX) {
-              const float m = (flip ? least : most) * kf;
-              top = fmaxf(top, (flip ? -least : most) > kNoMax ? m + __log2f(vs) : kNoMax);
-            } else {
-              float p = fabsf(act_one<ACT>(fmaxf(most * kf, 0.f), a.scale)), n = fmaxf(-least * kf, 0.f);
-              if constexpr (ACT == ACT_RAW || ACT == ACT_LEAKY_RELU) p = fmaxf(p, fabsf(act_one<ACT>(-n, a.scale)));
-              else if constexpr (ACT != ACT_RELU && ACT != ACT_RELU_SQUARE) p = fmaxf(p, fminf(n, 0.375f) * fabsf(a.scale));
-              top = fmaxf(top, p * vs);
-            }
-          };
-          if (!masked) {
-            uint32_t s[2][16];
-            tmem_ld16(s_tmem, s[0]);
+        for (int half = 0; half < 2; ++half) {
+          PAGED_WAIT_ON(L::B_S_FULL + 2 * qt + half, done & 1u);
+          tc_fence_after();
+          if (warp_live) {
+            const uint32_t s_tmem = s_rows + half * (kTile / 2);
+            if (!every) PAGED_WAIT_ON(L::B_V_READY + half, pos & 1u);  // with the tokens whose V held a NaN
+            const uint16_t* const poison = reinterpret_cast<const uint16_t*>(smem + L::kPoisonOff) + half * 4;
+            const int my_key0 = key0 + half * (kTile / 2);
+            const int from = rg.lo - my_key0, to = rg.hi - my_key0;  // columns of this half of the row that count
+            // columns 16 i .. of this half's scores
+            auto factors = [&](int i, float& kf, float& vs) {
+              const int b = (half * (kTile / 2) + i * 16) >> a.block_shift;
+              kf = sc[b] * qa;
+              vs = fmaxf(sc[8 + b], kLeastScale);
+            };
+            auto first_bits = [](int n) { return n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u; };
+            auto part_of = [&](int i) -> uint32_t {  // a bit for each of the 16
+              return sc[8 + ((half * (kTile / 2) + i * 16) >> a.block_shift)] == 0.f ? 0u : first_bits(to - i * 16) & ~first_bits(from - i * 16);
+            };
+            // P of 16 scores, and its sum (of |P|), the same in both forms below: no row's bits depend on what another row asks for
+            auto products = [&](const uint32_t (&s)[16], float kf, float vs, float (&y)[16]) {
+              const float off = SOFTMAX ? __log2f(vs) + kLogTarget - ref : 0.f, m = a.scale * vs * ref;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              tmem_wait_ld();
-              tmem_regs_ready(s[i & 1]);
-              if (i < 7) tmem_ld16(s_tmem + (i + 1) * 16, s[(i + 1) & 1]);
-              float m[2], n[2] = {0.f, 0.f};
-              const float* const x = reinterpret_cast<const float*>(s[i & 1]);
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                m[e] = n[e] = x[8 * e];
-                if (!flip) m[e] = max3(max3(max3(m[e], x[8 * e + 1], x[8 * e + 2]), x[8 * e + 3], x[8 * e + 4]), x[8 * e + 5], fmaxf(x[8 * e + 6], x[8 * e + 7]));
-                if (flip || !SOFTMAX)
-                  n[e] = -max3(max3(max3(-n[e], -x[8 * e + 1], -x[8 * e + 2]), -x[8 * e + 3], -x[8 * e + 4]), -x[8 * e + 5], fmaxf(-x[8 * e + 6], -x[8 * e + 7]));
+              for (int e = 0; e < 16; ++e) {
+                const float x = __uint_as_float(s[e]);
+                y[e] = SOFTMAX ? ex2_approx(fmaf(x, kf, off)) : act_one<ACT>(x * kf, m);
               }
-              float kf, vs;
-              factors(i / 2, i & 1, kf, vs);
-              look(fmaxf(m[0], m[1]), fminf(n[0], n[1]), kf, vs);
+            };
+            auto sum_of = [&](const float (&y)[16]) {
+              float p[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) p[e] = (fabsf(y[e]) + fabsf(y[e + 4])) + (fabsf(y[e + 8]) + fabsf(y[e + 12]));
+              return (p[0] + p[1]) + (p[2] + p[3]);
+            };
+            uint32_t w[32];                 // P in float16
+            float sum = 0.f, weights = 0.f;  // of |P|; of P before V's scale
+            const bool first = j == 0 && half == 0;
+            const float before = ref;
+            bool again = masked || first;
+            if (!again) {
+              uint32_t s[2][16];
+              tmem_ld16(s_tmem, s[0]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float kf, vs, y[16];
+                tmem_wait_ld();
+                tmem_regs_ready(s[i & 1]);
+                if (i < 3) tmem_ld16(s_tmem + (i + 1) * 16, s[(i + 1) & 1]);
+                factors(i, kf, vs);
+                products(s[i & 1], kf, vs, y);
+                const float part = sum_of(y);
+                sum += part;
+                if constexpr (SOFTMAX) weights = fmaf(part, __fdividef(1.f, vs * L::kTarget), weights);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[8 * i + e] = pack_f16x2(y[2 * e], y[2 * e + 1]);
+              }
             }
-          } else {
+            again = again || __any_sync(kFull, !(sum < kMostSum));
+            if (again) {
+              // with masks, or a reference that is new or has to move
+              auto pass = [&](bool keep) {
+                sum = weights = 0.f;
+                float top = SOFTMAX ? kNoMax : 0.f;  // the largest |P| without the reference (softmax: its logarithm)
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              const uint32_t in = part_of(c);
-              uint32_t s[32];
-              tmem_ld32(s_tmem + c * 32, s);
-              tmem_wait_ld();
-              tmem_regs_ready(s);
+                for (int i = 0; i < 4; ++i) {
+                  const uint32_t in = masked ? part_of(i) : 0xffffu, bad = every ? 0u : poison[i] & in;
+                  uint32_t s[16];
+                  float kf, vs, y[16];
+                  tmem_ld16(s_tmem + i * 16, s);
+                  tmem_wait_ld();
+                  tmem_regs_ready(s);
+                  factors(i, kf, vs);
+                  products(s, kf, vs, y);
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float kf, vs, most = kNoMax, least = -kNoMax;
-                factors(c, h, kf, vs);
+                  for (int e = 0; e < 16; ++e) {
+                    y[e] = (in >> e) & 1u ? y[e] : 0.f;
+                    y[e] = (bad >> e) & 1u ? __uint_as_float(0x7fffffffu) : y[e];
+                  }
+                  const float part = sum_of(y);
+                  sum += part;
+                  if constexpr (SOFTMAX) weights = fmaf(part, __fdividef(1.f, vs * L::kTarget), weights);
+                  if (keep) {
+                    uint32_t p[8];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  const float x = __uint_as_float(s[16 * h + e]);
-                  const bool part = (in >> (16 * h + e)) & 1u;
-                  most = fmaxf(most, part ? x : kNoMax), least = fminf(least, part ? x : -kNoMax);
+                    for (int e = 0; e < 8; ++e) p[e] = pack_f16x2(y[2 * e], y[2 * e + 1]);
+                    tmem_st8(s_tmem + i * 8, p);
+                  } else {
+                    const float log_vs = __log2f(vs);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                      const float x = __uint_as_float(s[e]) * kf, t = SOFTMAX ? x + log_vs : fabsf(act_one<ACT>(x, a.scale)) * vs;
+                      top = fmaxf(top, (in >> e) & 1u ? t : kNoMax);
+                    }
+                  }
                 }
-                if (SOFTMAX || most > kNoMax) look(most, least, kf, vs);
+                return top;
+              };
+              const float top = pass(false);
+              // ... to a largest P in (target / 2, target]
+              if (!(sum < kMostSum)) {
+                if constexpr (SOFTMAX) ref = ceilf(fminf(top, 1.0e30f));
+                else ref = top > 0.f ? exp2f(fminf(fmaxf(floorf(log2f(L::kTarget / top)), -100.f), 100.f)) : 1.2676506e30f;
               }
+              pass(true);
+            } else {
+              tmem_st32(s_tmem, w);
             }
-          }
-          // ---- the reference moves to a largest P in (target / 2, target], where there is none yet or where P would not fit
-          bool moves;
-          if constexpr (SOFTMAX) moves = top > kNoMax && (ref == kNoMax || top - ref > kHeadroom);
-          else moves = j == 0 || top * ref > kMax8;
-          if (__any_sync(kFull, moves)) {
-            float f = 1.f;
-            if (moves) {
-              float next;
-              if constexpr (SOFTMAX) {
-                next = ceilf(fminf(top, 1.0e30f));
-                f = ref == kNoMax ? 0.f : ex2_approx(ref - next);
-              } else {
-                next = top > 0.f ? exp2f(fminf(fmaxf(floorf(log2f(L::kTarget / top)), -100.f), 100.f)) : 1.2676506e30f;
-                f = next / ref;
-              }
-              ref = next;
-            }
-            l *= f;
-            if (j > 0) {
-              PAGED_WAIT_ON(L::B_PV_DONE + qt, (done - 1) & 1u);  // O holds every tile before this one
+            if constexpr (SOFTMAX) l = fmaf(l, ex2_approx(before - ref), weights);
+            if (!first && __any_sync(kFull, ref != before)) {
+              const float f = SOFTMAX ? ex2_approx(before - ref) : ref / before;
+              PAGED_WAIT_ON(L::B_PV_DONE + 2 * qt + (half ^ 1), (half ? done : done - 1) & 1u);  // O holds every token before these
               tc_fence_after();
 #pragma unroll 1
               for (int b = 0; b < D / 32; ++b) {
@@ -383,102 +444,13 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                 for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
                 tmem_st32(o_tmem + b * 32, o);
               }
-              tmem_wait_st();
             }
+            tmem_wait_st();
           }
-          // ---- P, over its own scores: of 32 tokens the hi plane, then the lo plane
-          if (!masked) {
-            // sixteen columns after sixteen, the special functions of one under the conversions of the one before, without a branch
-            uint32_t w[16], s[2][16];
-            float y[16], sum = 0.f;
-            tmem_ld16(s_tmem, s[0]);
-#pragma unroll
-            for (int i = 0; i < 9; ++i) {
-              float u[16], z[16], kf = 0.f, vs = 0.f;
-              if (i < 8) {
-                tmem_wait_ld();
-                tmem_regs_ready(s[i & 1]);
-                if (i < 7) tmem_ld16(s_tmem + (i + 1) * 16, s[(i + 1) & 1]);
-                factors(i / 2, i & 1, kf, vs);
-                const float off = SOFTMAX ? __log2f(vs) + kLogTarget - ref : 0.f;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  z[e] = SOFTMAX ? 0.f : __uint_as_float(s[i & 1][e]) * kf;
-                  if constexpr (SOFTMAX) u[e] = fmaf(__uint_as_float(s[i & 1][e]), kf, off);
-                  else if constexpr (ACT == ACT_SILU) u[e] = 0.5f * z[e];
-                  else if constexpr (ACT == ACT_GELU_TANH) u[e] = z[e] * fmaf(z[e] * z[e], 0.7978845608028654f * 0.044715f, 0.7978845608028654f);
-                  else u[e] = 0.f;
-                }
-              }
-              if (i == 0) {
-                mufu_all<kMufu>(u);
-              } else {
-                uint32_t w_hi[4], w_lo[4];
-                if (i < 8) split_e4m3_and<kMufu>(y, w_hi, w_lo, u);
-                else split_e4m3(y, w_hi, w_lo);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[4 * ((i - 1) & 1) + e] = w_hi[e], w[8 + 4 * ((i - 1) & 1) + e] = w_lo[e];
-                if ((i & 1) == 0) tmem_st16(s_tmem + (i / 2 - 1) * 32, w);
-              }
-              if (i < 8) {
-                const float m = a.scale * vs * ref;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  if constexpr (SOFTMAX) y[e] = u[e];
-                  else if constexpr (kMufu == MUFU_TANH) y[e] = fmaf(z[e] * (0.5f * m), u[e], z[e] * (0.5f * m));
-                  else y[e] = act_one<ACT>(z[e], m);
-                }
-                if constexpr (SOFTMAX) {
-                  float p[4];
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) p[e] = (y[e] + y[e + 4]) + (y[e + 8] + y[e + 12]);
-                  sum = fmaf((p[0] + p[1]) + (p[2] + p[3]), __fdividef(1.f, vs * L::kTarget), sum);
-                }
-              }
-            }
-            if constexpr (SOFTMAX) l += sum;
-          } else {
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              const uint32_t in = part_of(c), bad = every ? 0u : poison[c] & in;
-              uint32_t s[32], w[16];
-              tmem_ld32(s_tmem + c * 32, s);
-              tmem_wait_ld();
-              tmem_regs_ready(s);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float kf, vs, y[16];
-                uint32_t w_hi[4], w_lo[4];
-                factors(c, h, kf, vs);
-                const float off = SOFTMAX ? __log2f(vs) + kLogTarget - ref : 0.f, m = a.scale * vs * ref;
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                  y[e] = SOFTMAX ? fmaf(__uint_as_float(s[16 * h + e]), kf, off) : act_one<ACT>(__uint_as_float(s[16 * h + e]) * kf, m);
-                if constexpr (SOFTMAX) mufu_all<MUFU_EX2>(y);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) y[e] = (in >> (16 * h + e)) & 1u ? y[e] : 0.f;
-                if (bad != 0u) {
-#pragma unroll
-                  for (int e = 0; e < 16; ++e) y[e] = (bad >> (16 * h + e)) & 1u ? __uint_as_float(0x7fffffffu) : y[e];
-                }
-                if constexpr (SOFTMAX) {
-                  float p[4];
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) p[e] = (y[e] + y[e + 4]) + (y[e + 8] + y[e + 12]);
-                  l = fmaf((p[0] + p[1]) + (p[2] + p[3]), __fdividef(1.f, vs * L::kTarget), l);
-                }
-                split_e4m3(y, w_hi, w_lo);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[4 * h + e] = w_hi[e], w[8 + 4 * h + e] = w_lo[e];
-              }
-              tmem_st16(s_tmem + c * 32, w);
-            }
-          }
-          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_base + 8u * (L::B_P_FULL + 2 * qt + half));
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_base + 8u * (L::B_P_FULL + qt));
         ++done;
       }
       // ---- the end of the stretch
@@ -486,7 +458,7 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       const bool cut = it.pieces > 1;
       const int part = 2 * blockIdx.x + (static_cast<int>(blockIdx.x) == it.first ? 1 : 0);
       if (warp_live) {
-        PAGED_WAIT_ON(L::B_PV_DONE + qt, (done - 1) & 1u);
+        PAGED_WAIT_ON(L::B_PV_DONE + 2 * qt + 1, (done - 1) & 1u);
         tc_fence_after();
         float f;
         if (cut) f = SOFTMAX ? 1.f / L::kTarget : 1.f / ref;
@@ -523,15 +495,15 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
       if (cut) {
         // the last of the item's CTAs joins the pieces
-        named_bar_sync(3, 256);
+        named_bar_sync(3, 32 * L::kActWarps);
         if (threadIdx.x == 0) *last_flag = count_arrival(a.counters + it.first) == it.pieces - 1;
-        named_bar_sync(3, 256);
+        named_bar_sync(3, 32 * L::kActWarps);
         if (*last_flag)
-          paged_join<D, kRows, SOFTMAX, 8>(a, it, warp, lane, [&](int row) {
+          paged_join<D, kRows, SOFTMAX, L::kActWarps>(a, it, warp, lane, [&](int row) {
             const int at = it.row0 + row, q = at / a.group;
             return ((it.q_start + static_cast<long long>(q)) * a.heads + it.h * a.group + (at - q * a.group)) * D;
           });
-        named_bar_sync(3, 256);
+        named_bar_sync(3, 32 * L::kActWarps);
       }
     }
   }

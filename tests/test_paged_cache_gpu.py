@@ -331,6 +331,29 @@ def test_attend_many_queries_over_long_histories(dim):
     Case([2000] * 3, [40, 64, 33], 32, 32, dim, 128).check(1 / 2000, "relu")
 
 
+@pytest.mark.parametrize("tokens", [1, 64, 129, 300, 640, 1000])
+def test_attend_less_work_than_ctas(tokens):
+    # items whose tiles go to as many CTAs, with CTAs over that have none
+    for q, dim in ((70, 128), (300, 64)):
+        Case([tokens], [q], 1, 1, dim, 16).check(0.1, "softmax")
+        Case([tokens, 1], [q, 90], 2, 1, dim, 128).check(0.01, "silu", causal=True)
+    Case([tokens], [1], 1, 1, 128, 16).check(0.1, "softmax")
+    Case([tokens], [20], 1, 1, 64, 16).check(0.1, "softmax")
+
+
+def test_attend_growing_scores():
+    # references that have to move again and again, by a little and past any of the formats' ranges; V scales far apart
+    for q_len, dim in ((1, 128), (3, 64), (90, 128), (150, 64)):
+        case = Case([1500], [q_len], 2, 1, dim, 16, seed=q_len)
+        blocks = case.table[0, : -(-1500 // 16)].long()
+        case.ks[blocks, 0] *= torch.exp2(torch.arange(len(blocks)) // 24).to(case.ks.dtype)
+        case.vs[blocks, 0] *= torch.exp2(torch.arange(len(blocks)) % 5 * 4 - 8).to(case.vs.dtype)
+        case.check(0.05, "softmax")
+        case.check(0.05, "softmax", causal=True)
+        case.check(1e-4, "relu_square")
+        case.check(1e-4, "silu")
+
+
 @pytest.mark.parametrize("window", [None, 0, 1, 100, 128, 5000])
 @pytest.mark.parametrize("causal", [False, True])
 def test_attend_masks(causal, window):

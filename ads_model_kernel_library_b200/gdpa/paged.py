@@ -238,7 +238,7 @@ class PagedKVCache:
 
     def release(self, requests: Sequence[int]) -> None:
         """Give back the blocks of these requests (rows of the tables), which are empty afterwards."""
-        rows = torch.as_tensor(requests, dtype=torch.int64, device=self.block_tables.device)
+        rows = torch.tensor(sorted(set(requests)), dtype=torch.int64, device=self.block_tables.device)
         table = self.block_tables[rows]
         held = torch.arange(table.shape[1], device=table.device) < ((self.seq_lens[rows] + self.block_size - 1) // self.block_size)[:, None]
         held &= table >= 0

@@ -1,6 +1,9 @@
 """The paged 8-bit cache on the GPU: block tables, the quantiser and the attention against their plain 64-bit forms."""
 import itertools
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -607,3 +610,12 @@ def test_operators_trace():
     torch.library.opcheck(torch.ops.gdpa.generalized_dot_product_attention_paged_fp8.default, args, test_utils=("test_faketensor",))
     tables = (torch.full((2, 3), -1, dtype=torch.int32, device=DEV), i32([1, 2]), i32([1, 30]), i32([0, 1, 2, 3]), i32([4]), 16, 31)
     torch.library.opcheck(torch.ops.gdpa.build_block_tables.default, tables, test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.parametrize("options", [[], ["--activation", "silu", "--head-dim", "64", "--block", "16", "--requests", "5", "--most-tokens", "300"]])
+def test_example_serves(options):
+    # one bound on the error for both: uniform rounding of four significant bits leaves 2^-4 / sqrt(12) of a key's or value's size, 0.03 together
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, os.path.join(root, "examples", "serve_paged.py"), *options], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert "kernel status 0" in r.stdout

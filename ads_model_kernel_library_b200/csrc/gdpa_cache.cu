@@ -28,7 +28,7 @@ constexpr unsigned kFull = 0xffffffffu;
 //
 // Latency is all of it: three trips to memory one after the other (lengths, free blocks, slots) between a launch and its end.  PER is the
 // number of requests a thread has in one round, in registers; the small form (64 requests: 4.9 -> 4.0 us) has neither the
-// unrolled code nor the threads of the large one.
+// unrolled code nor the threads of the large one.  Alone: 64 requests with a token each 4.0 us, 512 new ones (1.2 M tokens) 11.6, 8192 9.5.
 __device__ __forceinline__ int clamp_len(const void* p, int b, int flags) {
   return static_cast<int>(clamp_ll(load_offset(p, b, flags), 0, 0x3fffff00));  // two of them and a block fit in an int
 }
@@ -171,7 +171,8 @@ __global__ void __launch_bounds__(kTableThreads) gdpa_block_tables_kernel(const 
 // What bounds it: HBM with long runs (2 or 4 bytes in, one out per value), latency with single tokens.  So with long runs four warps share a
 // (run, head, key or value) and hold it in registers between the maximum and the conversion: one pass over the values, 16 KB and more
 // in flight per CTA.  With short ones a warp has one to itself, and nothing waits for another.  The 32 tokens of a window find
-// their runs with a vote; a window's triples are dealt out to gridDim.y CTAs.
+// their runs with a vote; a window's triples are dealt out to gridDim.y CTAs.  Measured: 128 histories of 512 to 4096 tokens, 8 heads of 128
+// values, 318 us (5.8 TB/s; a warp to a run 577), one token for 256 requests 4.1, 300 ragged runs of fp32 7.0.
 constexpr int kAppendWarps = 4;
 
 template <class T>

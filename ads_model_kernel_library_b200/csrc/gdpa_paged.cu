@@ -25,6 +25,10 @@
 // CTA that finishes it last (an atomic count per item) joins them in the order of the pieces, so the result does not depend on who
 // was last.  No CTA waits for another.
 //
+// Measured (one B200, us a pass of both kernels, calls back to back): 256 requests of up to 4096 tokens, a query each, 32 heads on 4: 112 (5.0 TB/s
+// of cache); six of 32768 to 262144 tokens 80 (5.1 TB/s); one of 1500 tokens 14.3, most of it the host; up to four draft queries of 96 requests,
+// head_dim 64, window 1024: 47, a chain of latencies per item.
+//
 // Roles: kGroups warpgroups (element-wise work, epilogue), one warp of TMA loads, one warp that issues MMAs.  A small kernel before this one
 // splits Q and zeroes the items' counters; this one's beginning (barriers, tensor memory, the scan of the lengths) overlaps it.
 #include <cuda_bf16.h>

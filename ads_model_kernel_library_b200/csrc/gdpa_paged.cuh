@@ -342,12 +342,13 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
         }
         cp_async_mbar_arrive(bar_base + 8u * (L::B_SC_FULL + stage));
         loaded = pos + 1;
-        if constexpr (L::kOwnV) {  // V has one place of its own
-          if (!cta.wait(L::B_V_EMPTY, (pos & 1u) ^ 1u, ST_ROLE_LOAD)) return false;
-          const uint32_t v_bar = bar_base + 8u * L::B_V_FULL;
+        if constexpr (L::kOwnV) {  // V has places of its own
+          const uint32_t v_stage = pos % L::kVStages;
+          if (!cta.wait(L::B_V_EMPTY + v_stage, ((pos / L::kVStages) & 1u) ^ 1u, ST_ROLE_LOAD)) return false;
+          const uint32_t v_bar = bar_base + 8u * (L::B_V_FULL + v_stage);
           if (lane == 0) mbar_arrive_expect_tx(v_bar, n_valid * block_size * D);
           __syncwarp();
-          if (valid) tma_load_4d(smem_base + L::kVOff + lane * block_size * D, &tm_v, v_bar, 0, 0, it.h, blk);
+          if (valid) tma_load_4d(smem_base + L::kVOff + v_stage * L::kTileBytes + lane * block_size * D, &tm_v, v_bar, 0, 0, it.h, blk);
           loaded_v = pos + 1;
         }
         // the next item's Q: its buffer is the last item's, which is done when this item's first stages have been used
@@ -364,8 +365,9 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
       while (!mbar_try_wait(bar_base + 8u * (L::B_KV_FULL + k % L::kStages), (k / L::kStages) & 1u) && global_timer_ns() - t0 < kWaitLimitNs) {
       }
     if constexpr (L::kOwnV)
-      while (loaded_v > 0 && !mbar_try_wait(bar_base + 8u * L::B_V_FULL, (loaded_v - 1) & 1u) && global_timer_ns() - t0 < kWaitLimitNs) {
-      }
+      for (uint32_t k = loaded_v > L::kVStages ? loaded_v - L::kVStages : 0; k < loaded_v; ++k)
+        while (!mbar_try_wait(bar_base + 8u * (L::B_V_FULL + k % L::kVStages), (k / L::kVStages) & 1u) && global_timer_ns() - t0 < kWaitLimitNs) {
+        }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncwarp();

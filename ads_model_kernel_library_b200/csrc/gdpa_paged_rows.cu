@@ -16,11 +16,13 @@
 // whole test.  Then, for the first tokens of a stretch and where a mask leaves tokens out, the scores, which are still there, are gone through
 // again: once for the sum and maximum under the masks, once for P.  Both forms do the same arithmetic, so no row's bits depend on its neighbours.
 //
-// Measured (one B200, caches cold): causal chunks of 256 to 1024 queries 425 us, candidates (64 to 1024, SiLU) 729 us; the transposed form with
-// 128 rows 757 and 917, this form with P in two e4m3 values 478 and 815.  256 rows against 128 tokens take 2.5 us whatever the activation, 128
-// rows 2.2: neither the tensor cores (1.1 us of it) nor one pipe bounds it, but the chain from the scores of 64 tokens to the next ones' with two
-// warps on a scheduler.  Slower here: an MMA warp for each row tile (433, 775); scores of 128 tokens at once (437, 730); the row tiles' warps
-// taking strict turns (507, 967); 16 element-wise warps, half a row each, with two converting V, who are then late (600, 1110).
+// Measured (one B200, caches cold): causal chunks of 256 to 1024 queries 427 us, candidates (64 to 1024, SiLU) 724 us; the transposed form with
+// 128 rows 757 and 917, this form with P in two e4m3 values 478 and 815.  128 tokens against 256 rows take 2.4 to 2.5 us whatever the
+// activation, against 128 rows 1.85 (2.2 with one place for V as it comes from the cache: its next tile then waited for the conversion).
+// No pipe is near its end (tensor 23 %, ALU 28 %, issue 39 % on chunks); what bounds it is the way of 64 tokens from the products with Q to
+// those with V and back, with two warps on a scheduler.  No faster: an MMA warp for each row tile (429, 743); a row tile's two halves one
+// after the other (433, 735); scores of 128 tokens at once (438, 730); the row tiles' warps taking strict turns (507, 967); 16 element-wise
+// warps, half a row each, with two converting V, who are then late (600, 1110).
 //
 // Roles: warps 0-3 and 4-7 the element-wise work and epilogue of row tiles 0 and 1, warp 8 TMA loads and the walk, warp 9 MMAs, warps 10-13
 // V to float16, with zeros for tokens that no query may see (0 times NaN is NaN).
@@ -39,26 +41,26 @@ struct RowsShape {
   static constexpr int kTileBytes = kTile * D;               // K or V tile, or a plane of a row tile of Q
   static constexpr int kStages = D == 128 ? 2 : 4;           // of K and the scales
   static constexpr bool kOwnV = true;
+  static constexpr int kVStages = 2;
   static constexpr int kActWarps = 8, kConvertWarps = 4, kWarps = kActWarps + 2 + kConvertWarps, kThreads = 32 * kWarps;
   static constexpr int kLoadWarp = kActWarps, kMmaWarp = kActWarps + 1, kConvertWarp = kActWarps + 2;
-  static constexpr int kItemUnits = 2;                       // against tiles, which take the same time for 128 rows and for 256, nearly
+  static constexpr int kItemUnits = 2;  // beginning and end, in tiles; 2 : 3 for tiles of one and of two row tiles: candidates 916 us, not 815
   static constexpr float kTarget = 64.f;
   static constexpr int kKvOff = 0;                                 // [stage] K
-  static constexpr int kVOff = kStages * kTileBytes;               // V as it is in the cache
-  static constexpr int kV16Off = kVOff + kTileBytes;               // V in float16: [D / 64][128 tokens][64]
+  static constexpr int kVOff = kStages * kTileBytes;               // [V stage] V as it is in the cache
+  static constexpr int kV16Off = kVOff + kVStages * kTileBytes;            // V in float16: [D / 64][128 tokens][64]
   static constexpr int kQOff = kV16Off + 2 * kTileBytes;           // [2][row tile]{hi, lo}
   static constexpr int kScaleOff = kQOff + 8 * kTileBytes;         // float[stage][16]: K scales of up to 8 blocks, V scales
   static constexpr int kPoisonOff = kScaleOff + kStages * 64;      // uint16[8]: tokens whose V row held a NaN
-  static constexpr int kQaOff = kPoisonOff + 16;         // float[2][kRows]
-  static constexpr int kRingOff = kQaOff + 2 * kRows * 4;         // int[kItemSlots][16]
+  static constexpr int kRingOff = kPoisonOff + 16;         // int[kItemSlots][16]
   static constexpr int kBarOff = kRingOff + kItemSlots * 64;
   enum : int {
     B_KV_FULL = 0,
     B_KV_EMPTY = B_KV_FULL + kStages,
     B_SC_FULL = B_KV_EMPTY + kStages,
     B_V_FULL = B_SC_FULL + kStages,
-    B_V_EMPTY = B_V_FULL + 1,
-    B_V_READY = B_V_EMPTY + 1,  // [half]: V in float16
+    B_V_EMPTY = B_V_FULL + kVStages,
+    B_V_READY = B_V_EMPTY + kVStages,  // [half]: V in float16
     B_V_DONE = B_V_READY + 2,   // [half]
     B_S_FULL = B_V_DONE + 2,  // [row tile][half]
     B_P_FULL = B_S_FULL + 4,         // [row tile][half]
@@ -98,8 +100,6 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       if (i >= L::B_SC_FULL && i < L::B_SC_FULL + L::kStages) n = 32;
       if (i >= L::B_V_EMPTY && i < L::B_V_READY + 2) n = L::kConvertWarps;  // V_EMPTY, V_READY
       if (i >= L::B_P_FULL && i < L::B_P_FULL + 4) n = L::kActWarps / 2;
-      if (i >= L::B_Q_FULL && i < L::B_Q_FULL + 2) n = 33;
-      if (i >= L::B_Q_EMPTY && i < L::B_Q_EMPTY + 2) n = 1 + L::kActWarps;
       if (i >= L::B_ITEM_EMPTY && i < L::B_ITEM_EMPTY + kItemSlots) n = L::kActWarps + 1 + L::kConvertWarps;
       mbar_init(bar_base + 8u * i, n);
     }
@@ -139,9 +139,6 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           for (int plane = 0; plane < 2; ++plane)
             tma_load_3d(smem_base + L::kQOff + (4 * buf + 2 * t + plane) * L::kTileBytes, &tm_q, bar, 0, static_cast<int>(row) + t * kTile, plane * a.kv_heads + i.h);
       }
-      for (int r = lane; r < kRows; r += 32)
-        cp_async4(smem_base + L::kQaOff + (buf * kRows + r) * 4, a.qa + i.h * a.total_q * a.group + row + min(r, i.rows - 1), true);
-      cp_async_mbar_arrive(bar);
       return true;
     };
     paged_load<L, D, kRows>(cta, start, tm_k, tm_v, load_q);
@@ -212,7 +209,7 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const int w = warp - L::kConvertWarp, chunk = lane % kChunks, t_lane = lane / kChunks, other = chunk >> 2;
     // where a lane's 16 bytes are, as the copy's swizzle has them, and where their 16 values go: eight lanes at once to as many groups of banks,
     // for which the second panel's halves are written in the other order
-    auto from_of = [&](int t) { return L::kVOff + t * D + (D == 128 ? chunk ^ (t & 7) : chunk ^ ((t >> 1) & 3)) * 16; };
+    auto from_of = [&](uint32_t pos, int t) { return L::kVOff + pos % L::kVStages * L::kTileBytes + t * D + (D == 128 ? chunk ^ (t & 7) : chunk ^ ((t >> 1) & 3)) * 16; };
     auto to_of = [&](int t, int k) { return L::kV16Off + other * (kTile * 128) + t * 128 + ((2 * (chunk & 3) + (other ^ k)) ^ (t & 7)) * 16; };
     auto put = [&](int t, const uint4& u) {
       const uint32_t v[4] = {u.x, u.y, u.z, u.w};
@@ -240,7 +237,7 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         const uint32_t stage = pos % L::kStages;
         const int key0 = (it.tile0 + j) * kTile;
         PAGED_WAIT(L::B_SC_FULL + stage, (pos / L::kStages) & 1u, ST_ROLE_FIX);
-        PAGED_WAIT(L::B_V_FULL, pos & 1u, ST_ROLE_FIX);
+        PAGED_WAIT(L::B_V_FULL + pos % L::kVStages, (pos / L::kVStages) & 1u, ST_ROLE_FIX);
         const float* const sv = reinterpret_cast<const float*>(smem + L::kScaleOff) + stage * 16 + 8;
         const bool every = key0 >= all_lo && key0 + kTile <= all_hi;
         const bool checks = !every || __any_sync(kFull, lane < kTile >> a.block_shift && sv[lane & 7] == 0.f);
@@ -251,7 +248,7 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           if (!checks) {
             uint4 u[kSteps];
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) u[i] = *reinterpret_cast<const uint4*>(smem + from_of(t0 + i * kTokens));
+            for (int i = 0; i < kSteps; ++i) u[i] = *reinterpret_cast<const uint4*>(smem + from_of(pos, t0 + i * kTokens));
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) put(t0 + i * kTokens, u[i]);
           } else {
@@ -259,7 +256,7 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 #pragma unroll 1
             for (int i = 0; i < kSteps; ++i) {
               const int t = t0 + i * kTokens, key = key0 + t;
-              uint4 u = *reinterpret_cast<const uint4*>(smem + from_of(t));
+              uint4 u = *reinterpret_cast<const uint4*>(smem + from_of(pos, t));
               const bool out = key < it.lo || key >= it.hi || sv[t >> a.block_shift] == 0.f;
               // some row may take part with this token and some not: a NaN goes into P of those that do
               const bool nan = !every && !out && (__vcmpeq4(u.x & 0x7f7f7f7fu, 0x7f7f7f7fu) | __vcmpeq4(u.y & 0x7f7f7f7fu, 0x7f7f7f7fu) |
@@ -276,7 +273,7 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           __syncwarp();
           if (lane == 0) {
             mbar_arrive(bar_base + 8u * (L::B_V_READY + half));
-            if (half == 1) mbar_arrive(bar_base + 8u * L::B_V_EMPTY);
+            if (half == 1) mbar_arrive(bar_base + 8u * (L::B_V_EMPTY + pos % L::kVStages));
           }
         }
       }
@@ -290,7 +287,8 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const int r = qt * kTile + quarter * 32 + lane;  // row of the item
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_rows = tmem_base + qt * kTile + lane_base, o_tmem = tmem_base + 256 + qt * kTile + lane_base;
-    uint32_t pos = 0, q_pos = 0, done = 0;  // tiles, items with tiles, tiles of this row tile
+    uint32_t pos = 0, done = 0;  // tiles, tiles of this row tile
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows' factors are read below
     while (true) {
       const PagedItem it = cta.take_item(ST_ROLE_ACT);
       if (named_bar_or(3, 32 * L::kActWarps, it.h < 0)) break;
@@ -307,10 +305,7 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       const KeyRange rf = keys_of(it.row0 / a.group, it.q_len, it.len, a.causal, a.window),
                      rl = keys_of((it.row0 + it.rows - 1) / a.group, it.q_len, it.len, a.causal, a.window);
       const int all_lo = max(rf.lo, rl.lo), all_hi = min(rf.hi, rl.hi);
-      const uint32_t buf = q_pos & 1u;
-      PAGED_WAIT_ON(L::B_Q_FULL + buf, (q_pos >> 1) & 1u);
-      ++q_pos;
-      const float qa = reinterpret_cast<const float*>(smem + L::kQaOff)[buf * kRows + r];
+      const float qa = __ldcg(a.qa + (static_cast<long long>(it.h) * a.total_q + it.q_start) * a.group + it.row0 + min(r, it.rows - 1));
       float ref = SOFTMAX ? kNoMax : 1.2676506e30f, l = 0.f;  // running maximum / multiplier; sum of P
       for (int j = 0; j < it.tiles; ++j, ++pos) {
         const uint32_t stage = pos % L::kStages, phase = (pos / L::kStages) & 1u;
@@ -362,16 +357,17 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             const float before = ref;
             bool again = masked || first;
             if (!again) {
-              uint32_t s[2][16];
-              tmem_ld16(s_tmem, s[0]);
+              uint32_t s[4][16];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) tmem_ld16(s_tmem + i * 16, s[i]);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 4; ++i) tmem_regs_ready(s[i]);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 float kf, vs, y[16];
-                tmem_wait_ld();
-                tmem_regs_ready(s[i & 1]);
-                if (i < 3) tmem_ld16(s_tmem + (i + 1) * 16, s[(i + 1) & 1]);
                 factors(i, kf, vs);
-                products(s[i & 1], kf, vs, y);
+                products(s[i], kf, vs, y);
                 const float part = sum_of(y);
                 sum += part;
                 if constexpr (SOFTMAX) weights = fmaf(part, __fdividef(1.f, vs * L::kTarget), weights);
@@ -454,7 +450,6 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         ++done;
       }
       // ---- the end of the stretch
-      if (lane == 0) mbar_arrive(bar_base + 8u * (L::B_Q_EMPTY + buf));
       const bool cut = it.pieces > 1;
       const int part = 2 * blockIdx.x + (static_cast<int>(blockIdx.x) == it.first ? 1 : 0);
       if (warp_live) {

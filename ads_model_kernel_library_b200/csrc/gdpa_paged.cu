@@ -20,8 +20,8 @@
 // taken and O rescaled, a vote of the warpgroup per tile and group of columns otherwise.  The exact value of a row's reference does
 // not enter the result.
 //
-// Work: units are tiles; the units of all (request, K / V head, row tile) items in order are cut into equal stretches, one per CTA
-// (one persistent CTA per SM), whatever the requests' lengths.  An item that is cut leaves partial sums in a workspace, and the
+// Work: units are tiles, and four for an item's beginning and end; the units of all (request, K / V head, row tile) items in order are cut into equal stretches, one per CTA
+// (persistent ones, as many as are resident), whatever the requests' lengths.  An item that is cut leaves partial sums in a workspace, and the
 // CTA that finishes it last (an atomic count per item) joins them in the order of the pieces, so the result does not depend on who
 // was last.  No CTA waits for another.
 //

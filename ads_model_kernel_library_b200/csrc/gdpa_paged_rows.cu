@@ -16,11 +16,11 @@
 // whole test.  Then, for the first tokens of a stretch and where a mask leaves tokens out, the scores, which are still there, are gone through
 // again: once for the sum and maximum under the masks, once for P.  Both forms do the same arithmetic, so no row's bits depend on its neighbours.
 //
-// Measured (one B200, caches cold): causal chunks of 256 to 1024 queries 427 us, candidates (64 to 1024, SiLU) 724 us; the transposed form with
+// Measured (one B200, caches cold): causal chunks of 256 to 1024 queries 396 us, candidates (64 to 1024, SiLU) 629 us; the transposed form with
 // 128 rows 757 and 917, this form with P in two e4m3 values 478 and 815.  128 tokens against 256 rows take 2.4 to 2.5 us whatever the
 // activation, against 128 rows 1.85 (2.2 with one place for V as it comes from the cache: its next tile then waited for the conversion).
 // No pipe is near its end (tensor 23 %, ALU 28 %, issue 39 % on chunks); what bounds it is the way of 64 tokens from the products with Q to
-// those with V and back, with two warps on a scheduler.  No faster: an MMA warp for each row tile (429, 743); a row tile's two halves one
+// those with V and back, with two warps on a scheduler.  No faster (against 427, 724 then): an MMA warp for each row tile (429, 743); a row tile's two halves one
 // after the other (433, 735); scores of 128 tokens at once (438, 730); the row tiles' warps taking strict turns (507, 967); 16 element-wise
 // warps, half a row each, with two converting V, who are then late (600, 1110).
 //
@@ -44,7 +44,7 @@ struct RowsShape {
   static constexpr int kVStages = 2;
   static constexpr int kActWarps = 8, kConvertWarps = 4, kWarps = kActWarps + 2 + kConvertWarps, kThreads = 32 * kWarps;
   static constexpr int kLoadWarp = kActWarps, kMmaWarp = kActWarps + 1, kConvertWarp = kActWarps + 2;
-  static constexpr int kItemUnits = 2;  // beginning and end, in tiles; 2 : 3 for tiles of one and of two row tiles: candidates 916 us, not 815
+  static constexpr int kItemUnits = 4;  // beginning and end, in tiles.  Chunks / candidates, us: 1 454 / 803, 2 427 / 724, 3 410 / 682, 4 396 / 629, 6 399 / 642, 10 410 / 669
   static constexpr float kTarget = 64.f;
   static constexpr int kKvOff = 0;                                 // [stage] K
   static constexpr int kVOff = kStages * kTileBytes;               // [V stage] V as it is in the cache

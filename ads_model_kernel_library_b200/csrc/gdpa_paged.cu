@@ -226,7 +226,12 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (it.h == -2) goto role_done;
         break;
       }
-      if (it.tiles == 0) continue;
+      if (it.tiles == 0) {
+        // nothing of it is multiplied, but the element-wise warps take no further item before they have what is owed: a few items without keys in
+        // a row fill the ring, and the next item with keys would never come
+        if (owed.any && !issue_pv()) goto role_done;
+        continue;
+      }
       const int n16 = (it.rows + L::kCols - 1) / L::kCols * (L::kCols / 16);  // whole warpgroups' columns
       const uint32_t q_buf = q_pos & 1u;
       PAGED_WAIT(L::B_Q_FULL + q_buf, (q_pos >> 1) & 1u, ST_ROLE_MMA);

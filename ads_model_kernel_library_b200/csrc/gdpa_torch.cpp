@@ -78,6 +78,10 @@ void check_rows(const char* name, const at::Tensor& t) {
   TORCH_CHECK_VALUE(!misaligned(t, 2), name,
                     " must have a contiguous head dimension and 16-byte aligned row / head strides (a contiguous tensor, or a slice of a "
                     "packed QKV / KV tensor along the last dimension)");
+  // an expanded tensor among them: the C ABI takes a stride of 0 for the contiguous one
+  for (int i = 0; i < 2; ++i)
+    TORCH_CHECK_VALUE(t.numel() == 0 || t.size(i) <= 1 || t.stride(i) >= t.size(2), name, " must have rows and heads of its own, got strides ", t.strides(),
+                      " (an expanded tensor: make it contiguous)");
 }
 
 void check_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs, const at::Tensor& like) {
@@ -121,6 +125,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> build_block_tables(co
   check_vector("num_free", num_free, cached_lens, 1);
   check_block_size(block_size);
   check_table(block_tables, cached_lens, batch, block_size);
+  TORCH_CHECK_VALUE(batch <= 1 || block_tables.stride(0) >= block_tables.size(1), "block_tables must have rows of its own: they are written to");
   TORCH_CHECK_VALUE(batch < int64_t{1} << 31, "too many requests");
   TORCH_CHECK_VALUE(total_new >= 0 && total_new < int64_t{1} << 31, "total_new must be in [0, 2^31), got ", total_new);
   const c10::cuda::CUDAGuard guard(cached_lens.device());

@@ -50,3 +50,45 @@ def test_positions_before_the_first_key(queries):
     # causal, more queries than tokens: whole row tiles without a key in requests that have some
     lens = [(50 * b) % 700 for b in range(200)]
     check_empty_requests(lens, [queries if n % 100 else 64 for n in lens], 4, 4, 64, 16, causal=True)
+
+
+# ------------------------------------------------------------------------------------------ tensors that share their memory
+
+
+def test_expanded_inputs_are_refused():
+    f8, tokens, heads, dim = torch.float8_e4m3fn, 6, 4, 64
+    cache = [torch.zeros(2, 16, heads, dim, dtype=torch.uint8, device=DEV).view(f8) for _ in range(2)] + [torch.ones(2, heads, device=DEV) for _ in range(2)]
+    slots = torch.arange(tokens, device=DEV)
+    full = torch.randn(tokens, heads, dim, device=DEV).bfloat16()
+    row = torch.randn(tokens * heads * dim, device=DEV).bfloat16()
+    shared = [full[:, :1].expand(-1, heads, -1),                            # one head for all
+              full[:1].expand(tokens, -1, -1),                              # one token for all
+              full[:1, :1].expand(tokens, heads, -1),
+              torch.as_strided(row, (tokens, heads, dim), (heads * dim, dim // 2, 1))]  # heads that overlap
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    attend = lambda q: G.generalized_dot_product_attention_paged_fp8(q, *cache, i32([[0, 1]]), i32([0, tokens]), i32([20]), tokens)  # noqa: E731
+    for x in shared:
+        for key, value in ((x, full), (full, x)):
+            with pytest.raises(ValueError):
+                G.append_kv_cache_fp8(key, value, *cache, slots)
+        with pytest.raises(ValueError):
+            attend(x)
+        assert torch.isfinite(attend(x.contiguous())).all()
+    # a dimension of one entry has no stride that matters
+    one = full[:1, :1].expand(1, 1, dim)
+    narrow = [c[:, :, :1] for c in cache[:2]] + [c[:, :1].contiguous() for c in cache[2:]]
+    G.append_kv_cache_fp8(one, one, *narrow, slots[:1])
+    # the heads before the tokens in memory
+    swapped = full.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(attend(swapped), attend(full))
+
+
+def test_a_shared_table_is_read_but_not_written():
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    table = i32([[0, 1, -1]]).expand(3, -1)
+    with pytest.raises(ValueError):
+        G.build_block_tables(table, i32([5, 5, 5]), i32([1, 1, 1]), i32([2, 3]), i32([2]), 16, 3)
+    batch = Batch([30], [2], 4, 2, 64, 16)
+    alone = batch.run(0.1)
+    batch.lens, batch.offsets, batch.q, batch.table = [30] * 3, [0, 2, 4, 6], batch.q.repeat(3, 1, 1), batch.table.expand(3, -1)
+    assert torch.equal(batch.run(0.1), alone.repeat(3, 1, 1))

@@ -10,10 +10,17 @@
 // The cache bytes go from HBM through TMA into the tensor cores without a conversion, the 128-row side of the MMA is always full, and
 // N is as small as the rows are few (16 or 64), where the untransposed form would compute 128 rows for one query.
 //
-// Both small operands have to be e4m3 as well, and one e4m3 value has four significant bits.  So Q and P are each the sum of two:
+// Both small operands have to be e4m3 as well, and one e4m3 value has four significant bits, none of them below 2^-9.  So Q is the sum of two:
 // hi = e4m3(x), lo = e4m3(x - hi), both multiplied into the same accumulator.  For a bf16 Q (eight significant bits) scaled by a
-// power of two per row the sum is exact (down to 2^-19 of the row's largest element); for P it leaves 2^-8 of a value at most
-// (7e-4 rms), like the rounding to bf16 elsewhere.  The second product costs tensor time that a cache-bound call has to spare.
+// power of two per row the sum is exact (down to 2^-19 of the row's largest element).
+//
+// P is the sum of three, a = e4m3(x), b = e4m3(16 (x - a)), c = e4m3(32 (16 (x - a) - b)): each remainder is brought up to where the format has its
+// bits (16 * 16 and 32 * 8 are the most that fit below 448), and has an accumulator of its own, O = A + B / 16 + C / 512: the parts are columns of
+// one product, beside one another for each warpgroup.  That is float16's precision, and steps of 2^-18 where the row's largest is 64.  With hi and lo
+// as for Q, what was 2^-16 of the largest P was zero and what is just above it off by a half, while the row's sum took it in full: a key 12 (nats) ahead of
+// 4095 others, 0.97 of the weight, took 0.25 of the others' share away, one 13 ahead 0.55.  Two parts with their own accumulators would take 112 us
+// where three take 116 (256 requests of up to 4096 tokens), but have steps of 2^-13, an eighth of what lies 12 below.  c only where a is subnormal,
+// or multiplied only in tiles that have one: no faster.
 //
 // P^T is scaled per row so that its largest element (times V's block scale) lies at kTarget.  The scale, for the softmax the
 // running maximum, is kept until a product would pass 448 (e4m3's largest): only then, and for the first tile, is the exact maximum
@@ -25,9 +32,9 @@
 // CTA that finishes it last (an atomic count per item) joins them in the order of the pieces, so the result does not depend on who
 // was last.  No CTA waits for another.
 //
-// Measured (one B200, us a pass of both kernels, calls back to back): 256 requests of up to 4096 tokens, a query each, 32 heads on 4: 112 (5.0 TB/s
-// of cache); six of 32768 to 262144 tokens 80 (5.1 TB/s); one of 1500 tokens 14.3, most of it the host; up to four draft queries of 96 requests,
-// head_dim 64, window 1024: 47, a chain of latencies per item.
+// Measured (one B200, us a pass of both kernels, calls back to back): 256 requests of up to 4096 tokens, a query each, 32 heads on 4: 116 (4.8 TB/s
+// of cache); six of 32768 to 262144 tokens 81 (5.0 TB/s); one of 1500 tokens 14.3, most of it the host; up to four draft queries of 96 requests,
+// head_dim 64, window 1024: 50, a chain of latencies per item.
 //
 // Roles: kGroups warpgroups (element-wise work, epilogue), one warp of TMA loads, one warp that issues MMAs.  A small kernel before this one
 // splits Q and zeroes the items' counters; this one's beginning (barriers, tensor memory, the scan of the lengths) overlaps it.
@@ -53,15 +60,15 @@ struct PagedShape {
   static constexpr int kWarps = 4 * kGroups + 2;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kLoadWarp = 4 * kGroups, kMmaWarp = kLoadWarp + 1;
-  static constexpr int kTmemCols = NMAX <= 16 ? 64 : 256;  // S0, S1, O of NMAX columns each
+  static constexpr int kTmemCols = NMAX <= 16 ? 128 : 512;  // S0, S1 of NMAX columns each, O: [warpgroup][part]
   static constexpr bool kOwnV = false;  // a stage has K and V
   static constexpr int kItemUnits = 4;                 // beginning and end, in tiles; 2 to 8: the same within 3 %, 4 the best by a little
   static constexpr float kTarget = 64.f;
 
   static constexpr int kKvOff = 0;                                  // [stage]{K, V}
   static constexpr int kQOff = kKvOff + kStages * 2 * kTileBytes;   // [2]{hi, lo}
-  static constexpr int kPOff = kQOff + 2 * 2 * kQBytes;             // {hi, lo}
-  static constexpr int kScaleOff = kPOff + 2 * kPBytes;             // float[stage][16]: K scales of up to 8 blocks, V scales
+  static constexpr int kPOff = kQOff + 2 * 2 * kQBytes;             // [warpgroup][part of P]
+  static constexpr int kScaleOff = kPOff + 3 * kPBytes;             // float[stage][16]: K scales of up to 8 blocks, V scales
   static constexpr int kQaOff = kScaleOff + kStages * 64;           // float[2][NMAX]: factor of a row's scores
   static constexpr int kRefOff = kQaOff + 2 * NMAX * 4;             // float[NMAX]: minus the running maximum / multiplier of a row
   static constexpr int kFacOff = kRefOff + NMAX * 4;                // float[NMAX]
@@ -207,14 +214,11 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (!__all_sync(kFull, ok)) return false;
       ++pv_pos;
       tc_fence_after();
-      const uint32_t idesc = umma_idesc(0, 0, 1, 1, kTile, 16 * owed.n16);
+      const uint32_t idesc = umma_idesc(0, 0, 1, 1, kTile, 3 * 16 * owed.n16);
       const uint64_t dv = umma_desc_advance(dv0, owed.stage * 2 * L::kTileBytes);
 #pragma unroll
-      for (int kk = 0; kk < kTile / 32; ++kk) {
-        const uint64_t dvk = umma_desc_advance(dv, kk * 32 * D);
-        umma_ss_f8(tmem_base + 2 * NMAX, dvk, umma_desc_advance(dp0, kk * 512), idesc, owed.accumulate || kk > 0 ? 1u : 0u);
-        umma_ss_f8(tmem_base + 2 * NMAX, dvk, umma_desc_advance(dp0, L::kPBytes + kk * 512), idesc, 1u);
-      }
+      for (int kk = 0; kk < kTile / 32; ++kk)
+        umma_ss_f8(tmem_base + 2 * NMAX, umma_desc_advance(dv, kk * 32 * D), umma_desc_advance(dp0, kk * 512), idesc, owed.accumulate || kk > 0 ? 1u : 0u);
       tc_commit(bar_base + 8u * (L::B_KV_EMPTY + owed.stage));
       tc_commit(bar_base + 8u * L::B_PV_DONE);
       owed.any = false;
@@ -264,7 +268,7 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     static_assert(L::kTarget == 64.f, "kHeadroom");
     const int wg = warp >> 2, tid = threadIdx.x & 127, quarter = warp & 3, c0 = wg * C;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t o_tmem = tmem_base + 2 * NMAX + lane_base + c0;
+    const uint32_t o_tmem = tmem_base + 2 * NMAX + lane_base + 3 * c0;
     float* const ref = reinterpret_cast<float*>(smem + L::kRefOff) + c0;
     float* const fac = reinterpret_cast<float*>(smem + L::kFacOff) + c0;
     float* const red = reinterpret_cast<float*>(smem + L::kRedOff) + c0;  // [quarter * NMAX + column]
@@ -435,47 +439,60 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
             named_bar_sync(bar_wg, 128);
             if (!first) {
-              uint32_t raw[C];
-              tmem_ld_cols(o_tmem, raw);
-              tmem_wait_ld();
-              tmem_regs_ready(raw);
+              if constexpr (SOFTMAX) {
 #pragma unroll
-              for (int i = 0; i < C; i += 2) {
-                const float2 f = *reinterpret_cast<const float2*>(fac + i);
-                raw[i] = __float_as_uint(__uint_as_float(raw[i]) * f.x);
-                raw[i + 1] = __float_as_uint(__uint_as_float(raw[i + 1]) * f.y);
-                if constexpr (SOFTMAX) l[i / 2] = mul_f32x2(l[i / 2], pack_f32x2(f.x, f.y));
+                for (int i = 0; i < C; i += 2) l[i / 2] = mul_f32x2(l[i / 2], pack_f32x2(fac[i], fac[i + 1]));
               }
-              tmem_st_cols(o_tmem, raw);
+#pragma unroll 1
+              for (int part = 0; part < 3; ++part) {
+                uint32_t raw[C];
+                tmem_ld_cols(o_tmem + part * C, raw);
+                tmem_wait_ld();
+                tmem_regs_ready(raw);
+#pragma unroll
+                for (int i = 0; i < C; i += 2) {
+                  const float2 f = *reinterpret_cast<const float2*>(fac + i);
+                  raw[i] = __float_as_uint(__uint_as_float(raw[i]) * f.x);
+                  raw[i + 1] = __float_as_uint(__uint_as_float(raw[i + 1]) * f.y);
+                }
+                tmem_st_cols(o_tmem + part * C, raw);
+              }
               tmem_wait_st();
             }
             compute();
           }
-          // P, times V's scale, as the sum of two e4m3 values
-          uint32_t w_hi[C / 4], w_lo[C / 4];
+          // P, times V's scale, as the sum of three e4m3 values (see the top of this file)
+          uint32_t w[3][C / 4], h[C / 2];
           const uint64_t m2 = pack_f32x2(m, m);
 #pragma unroll
-          for (int i = 0; i < C / 4; ++i) {
-            uint16_t eh[2], el[2];
+          for (int i = 0; i < C / 2; ++i) {
+            const uint64_t x = pack_f32x2(p[2 * i], p[2 * i + 1]);
+            if constexpr (SOFTMAX) l[i] = add_f32x2(l[i], x);
+            float y0, y1;
+            unpack_f32x2(mul_f32x2(x, m2), y0, y1);
+            h[i] = pack_f16x2(y0, y1);
+          }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint64_t x = pack_f32x2(p[4 * i + 2 * e], p[4 * i + 2 * e + 1]);
-              if constexpr (SOFTMAX) l[2 * i + e] = add_f32x2(l[2 * i + e], x);
-              float y0, y1;
-              unpack_f32x2(mul_f32x2(x, m2), y0, y1);
-              const uint32_t h = pack_f16x2(y0, y1);
-              eh[e] = e4m3x2_from_f16x2(h);
-              el[e] = e4m3x2_from_f16x2(sub_f16x2(h, f16x2_from_e4m3x2(eh[e])));
+          for (int part = 0; part < 3; ++part) {
+            const uint32_t up = part == 0 ? 0x4c004c00u : 0x50005000u, down = up | 0x80008000u;  // 16, 32; exact, and so is what is left
+#pragma unroll
+            for (int i = 0; i < C / 4; ++i) {
+              const uint16_t e0 = e4m3x2_from_f16x2(h[2 * i]), e1 = e4m3x2_from_f16x2(h[2 * i + 1]);
+              w[part][i] = static_cast<uint32_t>(e0) | (static_cast<uint32_t>(e1) << 16);
+              if (part < 2) {
+                h[2 * i] = fma_f16x2(f16x2_from_e4m3x2(e0), down, mul_f16x2(h[2 * i], up));
+                h[2 * i + 1] = fma_f16x2(f16x2_from_e4m3x2(e1), down, mul_f16x2(h[2 * i + 1], up));
+              }
             }
-            w_hi[i] = static_cast<uint32_t>(eh[0]) | (static_cast<uint32_t>(eh[1]) << 16);
-            w_lo[i] = static_cast<uint32_t>(el[0]) | (static_cast<uint32_t>(el[1]) << 16);
           }
           if (pos > 0) PAGED_WAIT_ON(L::B_PV_DONE, (pos - 1) & 1u);  // P's buffer is free
-          uint8_t* const dst = smem + L::kPOff + c0 * kTile + tid * 16;
+          uint8_t* const dst = smem + L::kPOff + 3 * c0 * kTile + tid * 16;
 #pragma unroll
           for (int c = 0; c < C / 16; ++c) {
-            *reinterpret_cast<uint4*>(dst + c * 16 * kTile) = make_uint4(w_hi[4 * c], w_hi[4 * c + 1], w_hi[4 * c + 2], w_hi[4 * c + 3]);
-            *reinterpret_cast<uint4*>(dst + L::kPBytes + c * 16 * kTile) = make_uint4(w_lo[4 * c], w_lo[4 * c + 1], w_lo[4 * c + 2], w_lo[4 * c + 3]);
+#pragma unroll
+            for (int part = 0; part < 3; ++part)
+              *reinterpret_cast<uint4*>(dst + (part * C + c * 16) * kTile) =
+                  make_uint4(w[part][4 * c], w[part][4 * c + 1], w[part][4 * c + 2], w[part][4 * c + 3]);
           }
         } else if (pos > 0) {
           // a warpgroup without columns waits too: its arrival for the next tile must not count for this one
@@ -512,16 +529,18 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
       named_bar_sync(bar_wg, 128);
       if (rows > 0) {
-        uint32_t raw[C];
-        tmem_ld_cols(o_tmem, raw);
+        uint32_t raw[3][C];
+#pragma unroll
+        for (int part = 0; part < 3; ++part) tmem_ld_cols(o_tmem + part * C, raw[part]);
         tmem_wait_ld();
-        tmem_regs_ready(raw);
+#pragma unroll
+        for (int part = 0; part < 3; ++part) tmem_regs_ready(raw[part]);
         if (tid < D) {
           float* const po = a.part_o + (static_cast<long long>(part) * NMAX + c0) * D + tid;
 #pragma unroll
           for (int i = 0; i < C; ++i) {
             if (i < rows) {
-              const float v = __uint_as_float(raw[i]) * fac[i];
+              const float v = fmaf(fmaf(__uint_as_float(raw[2][i]), 1.f / 32.f, __uint_as_float(raw[1][i])), 1.f / 16.f, __uint_as_float(raw[0][i])) * fac[i];
               if (cut) po[i * D] = v;
               else a.o[row_at[i] + tid] = __float2bfloat16_rn(v);
             }

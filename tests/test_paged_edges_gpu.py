@@ -92,3 +92,71 @@ def test_a_shared_table_is_read_but_not_written():
     alone = batch.run(0.1)
     batch.lens, batch.offsets, batch.q, batch.table = [30] * 3, [0, 2, 4, 6], batch.q.repeat(3, 1, 1), batch.table.expand(3, -1)
     assert torch.equal(batch.run(0.1), alone.repeat(3, 1, 1))
+
+
+# ------------------------------------------------------------------------------------------ one key far ahead of the others
+
+
+def peaked(gap, tokens, queries, heads, kv_heads, dim, seed=0, tail=None):
+    """A batch of one request whose token `tokens // 3` is `gap` (a softmax's scale included) ahead of the others' mean, with values of zero; the
+    others' scores are normal, or all the same, and their values positive."""
+    batch = Batch([tokens], [queries], heads, kv_heads, dim, 64, seed=seed)
+    g = torch.Generator(device=DEV).manual_seed(seed + 1)
+    u = torch.randint(0, 2, (dim,), generator=g, device=DEV) * 2.0 - 1
+    batch.q = (u + 0.02 * torch.randn(batch.q.shape, generator=g, device=DEV)).bfloat16()
+    batch.v = (batch.v & 0x7F) if tail is None else torch.full_like(batch.v, 0x38)  # |v|, or ones (times the scale)
+    if tail is not None:
+        batch.k[:] = 0
+    at = tokens // 3
+    blk, row = int(batch.table[0, at // 64]), at % 64
+    batch.k[blk, row] = (u * gap / dim ** 0.5 * 64).to(torch.float8_e4m3fn).view(torch.uint8)
+    batch.v[blk, row] = 0
+    return batch
+
+
+def check_copies(batch, copies, scale, activation="softmax"):
+    """One request many times over, so that a CTA goes through a whole history (one alone is cut into pieces, each with a reference of its own)."""
+    want, tol = batch.want(scale, activation)
+    queries = len(batch.q)
+    batch.lens, batch.offsets = batch.lens * copies, [queries * i for i in range(copies + 1)]
+    batch.q, batch.table = batch.q.repeat(copies, 1, 1), batch.table.expand(copies, -1)
+    o = batch.run(scale, activation).double().view(copies, *want.shape)
+    assert G.kernel_status() == 0
+    assert bool(torch.isfinite(o).all())
+    over = ((o - want).abs() - tol).amax(0)
+    assert float(over.max()) <= 0, (f"{int((over > 0).sum())} of {over.numel()} elements too far, worst by {float((over / tol).max()):.3g} tolerances; "
+                                    f"the row's output off by {float(((o - want).norm(dim=3) / want.norm(dim=2)).max()):.3g} of it")
+
+
+@pytest.mark.parametrize("queries,heads,kv_heads", [(1, 8, 2), (5, 16, 2), (70, 4, 2)])
+@pytest.mark.parametrize("gap,tokens", [(8, 4096), (10, 4096), (11, 4096), (12, 4096), (13, 4096), (11, 32768), (12, 32768), (13, 32768), (14, 32768)])
+def test_the_tail_of_a_peaked_softmax(gap, tokens, queries, heads, kv_heads):
+    for dim in (64, 128):
+        check_copies(peaked(gap, tokens, queries, heads, kv_heads, dim), 250, dim ** -0.5)
+        peaked(gap, tokens, queries, heads, kv_heads, dim).check(dim ** -0.5)
+
+
+@pytest.mark.parametrize("queries", [1, 12, 70])
+@pytest.mark.parametrize("gap,tokens", [(11.25, 32768), (12, 100000), (12, 200000), (14, 200000)])
+def test_a_tail_of_equal_scores(gap, tokens, queries):
+    # all P of the tail are rounded the same way
+    for dim in (64, 128):
+        check_copies(peaked(gap, tokens, queries, 4, 1, dim, tail="equal"), 250, dim ** -0.5)
+
+
+@pytest.mark.parametrize("queries", [1, 5, 70])
+@pytest.mark.parametrize("activation", ["relu_square", "raw", "silu"])
+def test_one_product_far_ahead(activation, queries):
+    for dim in (64, 128):
+        batch = peaked(12, 4096, queries, 8, 2, dim)
+        blk = int(batch.table[0, (4096 // 3) // 64])
+        batch.ks[blk] *= 256  # the scores of that block
+        check_copies(batch, 250, 1 / 4096, activation)
+
+
+def test_a_peak_that_comes_late():
+    # the row's reference moves at the last tile, and everything before it with the reference
+    for queries in (1, 12, 70):
+        batch = peaked(12, 8192, queries, 4, 1, 128)
+        batch.table = batch.table.roll(128 - 8192 // 3 // 64 - 1, 1).contiguous()
+        check_copies(batch, 250, 128 ** -0.5)

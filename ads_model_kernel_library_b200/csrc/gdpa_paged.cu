@@ -312,18 +312,18 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const float* const sc = reinterpret_cast<const float*>(smem + L::kScaleOff) + stage * 16 + (tid >> a.block_shift);
         const float ks = sc[0];
         float vs = sc[8];
-        const bool out = key < it.lo || key >= it.hi || vs == 0.f;  // no row takes part with this token
-        vs = fmaxf(vs, kLeastScale);
+        const bool out = key < it.lo || key >= it.hi || no_block(vs);  // no row takes part with this token
+        bool poisoned = !out && !(vs <= 3.4028235e38f);                // a scale that is no number makes NaN of all rows that do
+        if (out || poisoned) vs = 0.f;
         const bool every = key0 >= all_lo && key0 + kTile <= all_hi;  // the tile needs no mask but that of `out`
-        const bool masked = !every || __any_sync(kFull, out);
+        const bool masked = !every || __any_sync(kFull, out || poisoned);
         PAGED_WAIT_ON(L::B_S_FULL + (pos & 1u), (pos >> 1) & 1u);
         tc_fence_after();
-        bool poisoned = false;
         if (masked) {
           // P of a token that takes no part is 0, and 0 times what its V row holds (an unused row, NaN) has to be 0
           PAGED_WAIT_ON(L::B_KV_FULL + stage, phase);
           uint4* const v_row = reinterpret_cast<uint4*>(smem + L::kKvOff + (2 * stage + 1) * L::kTileBytes + tid * D);
-          if (!every && !out) {
+          if (!every && !out && !poisoned) {
             // some row may take part and some not: a NaN goes into P of those that do
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
@@ -396,7 +396,7 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             // the exact reference of every column, and O and the row sums moved to it
             scores(false);
             if constexpr (SOFTMAX) {
-              const float lv = log2f(vs);
+              const float lv = log2f(fmaxf(vs, kLeastScale));
 #pragma unroll
               for (int i = 0; i < C; ++i) p[i] += lv;
             } else {
@@ -425,7 +425,7 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
               if constexpr (SOFTMAX) {
                 const float old = -ref[tid];
                 const float next = first || now - old > kHeadroom ? fmaxf(old, fminf(now, 3.0e38f)) : old;
-                fac[tid] = first ? 0.f : ex2_approx(old - next);
+                fac[tid] = first ? 0.f : ex2_approx(0.5f * (old - next));  // its root, taken twice: a row's sum is large where V's scales were small
                 ref[tid] = -next;
               } else {
                 // the largest power of two that keeps |P| times V's scale at or below the target; 2^100 for a row of zeros
@@ -441,7 +441,10 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             if (!first) {
               if constexpr (SOFTMAX) {
 #pragma unroll
-                for (int i = 0; i < C; i += 2) l[i / 2] = mul_f32x2(l[i / 2], pack_f32x2(fac[i], fac[i + 1]));
+                for (int i = 0; i < C; i += 2) {
+                  const uint64_t f = pack_f32x2(fac[i], fac[i + 1]);
+                  l[i / 2] = mul_f32x2(mul_f32x2(l[i / 2], f), f);
+                }
               }
 #pragma unroll 1
               for (int part = 0; part < 3; ++part) {
@@ -451,7 +454,8 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 tmem_regs_ready(raw);
 #pragma unroll
                 for (int i = 0; i < C; i += 2) {
-                  const float2 f = *reinterpret_cast<const float2*>(fac + i);
+                  float2 f = *reinterpret_cast<const float2*>(fac + i);
+                  if constexpr (SOFTMAX) f = make_float2(f.x * f.x, f.y * f.y);
                   raw[i] = __float_as_uint(__uint_as_float(raw[i]) * f.x);
                   raw[i + 1] = __float_as_uint(__uint_as_float(raw[i + 1]) * f.y);
                 }

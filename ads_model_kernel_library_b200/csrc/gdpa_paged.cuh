@@ -14,7 +14,11 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kItemSlots = 4;
 constexpr float kMax8 = 448.f;
 constexpr float kNoMax = -3.0e38f;     // running maximum of a row that has seen no key
-constexpr float kLeastScale = 7.888609e-31f;  // 2^-100
+constexpr float kLeastScale = 7.888609e-31f;  // 2^-100, the least scale that the append writes
+// What stands in the place of V's scale for a block that the table has not: a NaN that no arithmetic makes.
+constexpr uint32_t kNoBlock = 0xffffffffu;
+__device__ const uint32_t g_no_block = kNoBlock;
+__device__ __forceinline__ bool no_block(float v_scale) { return __float_as_uint(v_scale) == kNoBlock; }
 
 // One stretch of tiles of one item, as the loader publishes it.
 struct PagedItem {
@@ -333,12 +337,12 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
           tma_load_4d(dst, &tm_k, bar, 0, 0, it.h, blk);
           if constexpr (!L::kOwnV) tma_load_4d(dst + L::kTileBytes, &tm_v, bar, 0, 0, it.h, blk);
         }
-        // a block that is not there has scale 0, which tells the others
+        // a block that is not there has a mark in the place of V's scale, which tells the others
         if (lane < per_tile) {
           const uint32_t sc = smem_base + L::kScaleOff + stage * 64 + lane * 4;
           const long long si = valid ? static_cast<long long>(blk) * a.kv_heads + it.h : 0;
           cp_async4(sc, a.k_scales + si, valid);
-          cp_async4(sc + 32, a.v_scales + si, valid);
+          cp_async4(sc + 32, valid ? static_cast<const void*>(a.v_scales + si) : &g_no_block, true);
         }
         cp_async_mbar_arrive(bar_base + 8u * (L::B_SC_FULL + stage));
         loaded = pos + 1;
@@ -402,8 +406,9 @@ __device__ __forceinline__ void paged_join(const PagedArgs& a, const PagedItem& 
         if constexpr (SOFTMAX) {
           const float* const ml = a.part_ml + slot_of(k0 + min(lane, n - 1)) * 2 * NMAX + row[x];
           const float m = __ldcg(ml), l = __ldcg(ml + NMAX);
-          w[x] *= ex2_approx(m - m_all[x]);
-          if (lane < n) l_all[x] += w[x] * l;
+          const float half = ex2_approx(0.5f * (m - m_all[x]));  // twice: l is large where V's scales are small, and must not be lost before it is scaled
+          w[x] *= half * half;
+          if (lane < n) l_all[x] = fmaf(l * half, half, l_all[x]);
         }
       }
       for (int i0 = 0; i0 < n; i0 += kAhead) {

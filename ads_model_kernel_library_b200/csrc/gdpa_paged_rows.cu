@@ -8,8 +8,9 @@
 //
 // P in one float16 instead of two e4m3 values: the products take as long (half the rate, once instead of twice) and leave 2^-11 of a value,
 // and P takes one conversion for two elements, not four; V, which then has to be float16, is one conversion of 128 x D elements for all rows
-// of a tile, by warps of their own.  A token's scales are the same for a whole row of threads: the score's factor and the logarithm of V's
-// scale are two registers for 16 tokens, so that P times V's scale is one FMA and one exponential.
+// of a tile, by warps of their own.  A token's scales are the same for a whole row of threads, two registers
+// for 16 tokens.  P is an FMA, an exponential and, for the product, V's scale; the row's sum is taken without it, so that blocks of small values (of zeros
+// above all, whose scale is the least there is) keep their weight beside blocks of large ones.
 //
 // The reference of a row (the running maximum; for the other activations a power of two that P is multiplied by) is set so that the largest P
 // lies in (32, 64], and moves when 64 tokens' |P| sum up to 65504, float16's largest, or more: the sum that the softmax takes anyhow is the
@@ -240,7 +241,7 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         PAGED_WAIT(L::B_V_FULL + pos % L::kVStages, (pos / L::kVStages) & 1u, ST_ROLE_FIX);
         const float* const sv = reinterpret_cast<const float*>(smem + L::kScaleOff) + stage * 16 + 8;
         const bool every = key0 >= all_lo && key0 + kTile <= all_hi;
-        const bool checks = !every || __any_sync(kFull, lane < kTile >> a.block_shift && sv[lane & 7] == 0.f);
+        const bool checks = !every || __any_sync(kFull, lane < kTile >> a.block_shift && no_block(sv[lane & 7]));
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
           const int t0 = half * 64 + w * 16 + t_lane;
@@ -257,7 +258,7 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             for (int i = 0; i < kSteps; ++i) {
               const int t = t0 + i * kTokens, key = key0 + t;
               uint4 u = *reinterpret_cast<const uint4*>(smem + from_of(pos, t));
-              const bool out = key < it.lo || key >= it.hi || sv[t >> a.block_shift] == 0.f;
+              const bool out = key < it.lo || key >= it.hi || no_block(sv[t >> a.block_shift]);
               // some row may take part with this token and some not: a NaN goes into P of those that do
               const bool nan = !every && !out && (__vcmpeq4(u.x & 0x7f7f7f7fu, 0x7f7f7f7fu) | __vcmpeq4(u.y & 0x7f7f7f7fu, 0x7f7f7f7fu) |
                                                   __vcmpeq4(u.z & 0x7f7f7f7fu, 0x7f7f7f7fu) | __vcmpeq4(u.w & 0x7f7f7f7fu, 0x7f7f7f7fu)) != 0u;
@@ -315,7 +316,7 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         const float* const sc = reinterpret_cast<const float*>(smem + L::kScaleOff) + stage * 16;
         const bool every = key0 >= all_lo && key0 + kTile <= all_hi;
         // ... or a block that the table has not
-        const bool masked = !every || __any_sync(kFull, lane < kTile >> a.block_shift && sc[8 + (lane & 7)] == 0.f);
+        const bool masked = !every || __any_sync(kFull, lane < kTile >> a.block_shift && no_block(sc[8 + (lane & 7)]));
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
           PAGED_WAIT_ON(L::B_S_FULL + 2 * qt + half, done & 1u);
@@ -330,19 +331,29 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             auto factors = [&](int i, float& kf, float& vs) {
               const int b = (half * (kTile / 2) + i * 16) >> a.block_shift;
               kf = sc[b] * qa;
-              vs = fmaxf(sc[8 + b], kLeastScale);
+              vs = no_block(sc[8 + b]) ? 0.f : sc[8 + b];
             };
             auto first_bits = [](int n) { return n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u; };
             auto part_of = [&](int i) -> uint32_t {  // a bit for each of the 16
-              return sc[8 + ((half * (kTile / 2) + i * 16) >> a.block_shift)] == 0.f ? 0u : first_bits(to - i * 16) & ~first_bits(from - i * 16);
+              return no_block(sc[8 + ((half * (kTile / 2) + i * 16) >> a.block_shift)]) ? 0u : first_bits(to - i * 16) & ~first_bits(from - i * 16);
             };
-            // P of 16 scores, and its sum (of |P|), the same in both forms below: no row's bits depend on what another row asks for
+            // P of 16 scores (for the softmax without V's scale: its sum is of these), and its sum (of |P|), the same in both forms below: no row's
+            // bits depend on what another row asks for
             auto products = [&](const uint32_t (&s)[16], float kf, float vs, float (&y)[16]) {
-              const float off = SOFTMAX ? __log2f(vs) + kLogTarget - ref : 0.f, m = a.scale * vs * ref;
+              const float off = kLogTarget - ref;
+              float m = a.scale * vs * ref;
+              if (fabsf(m) > 3.4028235e38f) m = copysignf(3.4028235e38f, m);  // a row of zeros stays one
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
                 const float x = __uint_as_float(s[e]);
                 y[e] = SOFTMAX ? ex2_approx(fmaf(x, kf, off)) : act_one<ACT>(x * kf, m);
+              }
+            };
+            auto scaled = [&](float (&y)[16], float vs) {
+              if constexpr (SOFTMAX) {
+                const uint64_t v2 = pack_f32x2(vs, vs);
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) unpack_f32x2(mul_f32x2(pack_f32x2(y[e], y[e + 1]), v2), y[e], y[e + 1]);
               }
             };
             auto sum_of = [&](const float (&y)[16]) {
@@ -369,8 +380,9 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                 factors(i, kf, vs);
                 products(s[i], kf, vs, y);
                 const float part = sum_of(y);
-                sum += part;
-                if constexpr (SOFTMAX) weights = fmaf(part, __fdividef(1.f, vs * L::kTarget), weights);
+                sum = SOFTMAX ? fmaf(part, vs, sum) : sum + part;
+                if constexpr (SOFTMAX) weights = fmaf(part, 1.f / L::kTarget, weights);
+                scaled(y, vs);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) w[8 * i + e] = pack_f16x2(y[2 * e], y[2 * e + 1]);
               }
@@ -397,15 +409,21 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                     y[e] = (bad >> e) & 1u ? __uint_as_float(0x7fffffffu) : y[e];
                   }
                   const float part = sum_of(y);
-                  sum += part;
-                  if constexpr (SOFTMAX) weights = fmaf(part, __fdividef(1.f, vs * L::kTarget), weights);
+                  const bool number = fabsf(vs) <= 3.4028235e38f;  // a scale that is none makes NaN of the rows that take part, and of no other
+                  sum = SOFTMAX ? fmaf(part, number ? vs : 0.f, sum) : sum + part;
+                  if constexpr (SOFTMAX) weights = fmaf(part, 1.f / L::kTarget, weights);
                   if (keep) {
+                    scaled(y, vs);
+                    if (!number) {
+#pragma unroll
+                      for (int e = 0; e < 16; ++e) y[e] = (in >> e) & 1u ? y[e] : 0.f;
+                    }
                     uint32_t p[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) p[e] = pack_f16x2(y[2 * e], y[2 * e + 1]);
                     tmem_st8(s_tmem + i * 8, p);
                   } else {
-                    const float log_vs = __log2f(vs);
+                    const float log_vs = __log2f(fmaxf(vs, kLeastScale));
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                       const float x = __uint_as_float(s[e]) * kf, t = SOFTMAX ? x + log_vs : fabsf(act_one<ACT>(x, a.scale)) * vs;
@@ -425,7 +443,10 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             } else {
               tmem_st32(s_tmem, w);
             }
-            if constexpr (SOFTMAX) l = fmaf(l, ex2_approx(before - ref), weights);
+            if constexpr (SOFTMAX) {
+              const float root = ex2_approx(0.5f * (before - ref));  // twice: the sum is large where V's scales were small
+              l = fmaf(l * root, root, weights);
+            }
             if (!first && __any_sync(kFull, ref != before)) {
               const float f = SOFTMAX ? ex2_approx(before - ref) : ref / before;
               PAGED_WAIT_ON(L::B_PV_DONE + 2 * qt + (half ^ 1), (half ? done : done - 1) & 1u);  // O holds every token before these

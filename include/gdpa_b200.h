@@ -428,7 +428,8 @@ int gdpa_append_kv_cache_fp8(const GdpaCacheAppendParams* params, gdpa_stream_t 
 /* GDPA forward over the cache.  Query i of request b (rows q_offsets[b] + i) has position
  * seq_lens[b] - q_len + i; it takes part with keys j < seq_lens[b], with `causal` j <= position, with a
  * window |j - position| <= window; a row without keys gives zeros.  Tokens of a block that the table has not (an entry outside
- * [0, num_blocks)) take no part.  Scales must be positive.  O is [total_q, heads, head_dim] bf16. */
+ * [0, num_blocks)) take no part.  V's scales are not negative; a block with a scale of 0 holds zeros, and its
+ * tokens take part.  O is [total_q, heads, head_dim] bf16. */
 typedef struct GdpaPagedParams {
   uint32_t struct_size;        /* sizeof(GdpaPagedParams) */
   int32_t activation;

@@ -160,3 +160,60 @@ def test_a_peak_that_comes_late():
         batch = peaked(12, 8192, queries, 4, 1, 128)
         batch.table = batch.table.roll(128 - 8192 // 3 // 64 - 1, 1).contiguous()
         check_copies(batch, 250, 128 ** -0.5)
+
+
+# ------------------------------------------------------------------------------------------ scales of V
+
+
+@pytest.mark.parametrize("queries", [1, 12, 70])
+@pytest.mark.parametrize("activation", ["softmax", "silu", "relu"])
+def test_blocks_with_a_scale_of_zero(activation, queries):
+    # their values are zeros; their tokens take part like any others (a softmax's sum has them)
+    for dim in (64, 128):
+        batch = Batch([700, 64, 130, 1000], [queries] * 4, 4, 2, dim, 32, seed=queries)
+        for b, j in ((0, 0), (0, 3), (0, 21), (1, 0), (1, 1), (2, 4), (3, 0), (3, 1), (3, 2), (3, 3), (3, 4)):
+            batch.vs[int(batch.table[b, j])] = 0.0
+        batch.vs[int(batch.table[0, 5]), 1] = 0.0
+        scale = 0.1 if activation == "softmax" else 1e-3
+        o = batch.check(scale, activation)
+        assert bool((o[batch.offsets[1]:batch.offsets[2]] == 0).all())
+        batch.check(scale, activation, causal=True)
+
+
+@pytest.mark.parametrize("queries", [1, 12, 70])
+@pytest.mark.parametrize("power", [0, 24, 60, 100])
+def test_scales_far_apart(power, queries):
+    # a token whose values are large is 8 ahead of 4095 whose values are zeros (so that their scale is the least there is): these have 0.58 of the weight
+    for dim in (64, 128):
+        batch = peaked(8, 4096, queries, 4, 2, dim)
+        blk = int(batch.table[0, (4096 // 3) // 64])
+        batch.v[:], batch.vs[:] = 0, 2.0 ** -100
+        batch.v[blk, 4096 // 3 % 64], batch.vs[blk] = 0x40, 2.0 ** power
+        batch.check(dim ** -0.5)
+
+
+@pytest.mark.parametrize("queries", [1, 12, 70])
+def test_products_of_zero_with_large_scales(queries):
+    # no score above zero in the first tiles, or anywhere
+    for dim in (64, 128):
+        batch = Batch([500], [queries], 4, 2, dim, 64)
+        batch.q, batch.vs[:] = batch.q.abs(), 2.0 ** 60
+        batch.k |= 0x80
+        assert bool((batch.check(1e-3, "relu") == 0).all())
+        batch.k[int(batch.table[0, 6])] &= 0x7F
+        batch.k[int(batch.table[0, 6])] &= 0x5F  # (a byte of 0x7F is NaN)
+        batch.check(1e-3, "relu")
+        batch.check(1e-3, "relu_square")
+
+
+@pytest.mark.parametrize("queries", [1, 12, 70])
+def test_a_nan_scale_stays_where_it_is(queries):
+    for dim, activation in ((64, "softmax"), (128, "silu")):
+        batch = Batch([300, 300], [queries] * 2, 4, 2, dim, 64)
+        clean = batch.run(0.1, activation, causal=True)
+        batch.vs[int(batch.table[0, 4]), 1] = float("nan")  # tokens 256 .. 299
+        dirty = batch.run(0.1, activation, causal=True)
+        sees = torch.zeros(2 * queries, 4, dtype=torch.bool, device=DEV)
+        sees[max(0, queries - 44):queries, 2:] = True
+        assert bool(dirty[sees].isnan().all()) and torch.equal(dirty[~sees], clean[~sees])
+        assert G.kernel_status() == 0

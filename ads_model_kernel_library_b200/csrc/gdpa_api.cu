@@ -626,6 +626,8 @@ int gdpa_fwd_paged_fp8(const GdpaPagedParams* p, gdpa_stream_t stream) {
   a.o = static_cast<__nv_bfloat16*>(p->o);
   a.k_scales = p->k_scales;
   a.v_scales = p->v_scales;
+  a.v_cache = static_cast<const uint8_t*>(p->v_cache);
+  for (int i = 0; i < 3; ++i) a.v_strides[i] = vs[i];
   a.block_tables = p->block_tables;
   a.table_stride = p->table_stride;
   a.table_width = p->table_width;

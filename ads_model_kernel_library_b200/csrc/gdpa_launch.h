@@ -223,6 +223,8 @@ struct PagedArgs {
   __nv_bfloat16* o;        // [total_q, heads, head_dim]
   const float* k_scales;   // [blocks, kv_heads]
   const float* v_scales;
+  const uint8_t* v_cache;  // as tm_v has it, for a NaN that has to be found again
+  long long v_strides[3];  // block, row, head
   const int* block_tables;
   long long table_stride;
   int table_width;

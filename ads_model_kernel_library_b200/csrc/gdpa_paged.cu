@@ -90,7 +90,7 @@ struct PagedShape {
     B_ITEM_EMPTY = B_ITEM_FULL + kItemSlots,
     B_COUNT = B_ITEM_EMPTY + kItemSlots
   };
-  static constexpr int kMiscOff = kBarOff + B_COUNT * 8;  // tmem address, abort flag, last-arrival flag, pad; then the scan's scratch
+  static constexpr int kMiscOff = kBarOff + B_COUNT * 8;  // tmem address, abort flag, last-arrival flag, nan_item; then the scan's scratch
   static constexpr int kScanOff = kMiscOff + 16;          // long long[32] + start state
   static constexpr int kBytes = kScanOff + 32 * 8 + 48;
   static constexpr int kDynBytes = kBytes + 1024;
@@ -129,7 +129,7 @@ __device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)
 template <int D, int NMAX, bool SOFTMAX>
 __global__ void __launch_bounds__(PagedShape<D, NMAX>::kThreads, PagedShape<D, NMAX>::kCtasPerSm)
 gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                  const PagedArgs a) {
+                  const __grid_constant__ PagedArgs a) {
   using L = PagedShape<D, NMAX>;
   constexpr int kGroups = L::kGroups;
   extern __shared__ uint8_t smem_raw[];
@@ -139,6 +139,7 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   volatile uint32_t* const tmem_ptr = reinterpret_cast<volatile uint32_t*>(smem + L::kMiscOff);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
   volatile int* const last_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 8);
+  volatile uint32_t* const nan_item = reinterpret_cast<volatile uint32_t*>(smem + L::kMiscOff + 12);  // the last item that had NaNs taken out of V, from 1
   const int warp = warp_uniform(threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
 
@@ -153,6 +154,7 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       mbar_init(bar_base + 8u * i, n);
     }
     *abort_flag = 0;
+    *nan_item = 0;
     mbar_fence_init();
   }
   if (warp == L::kMmaWarp) {
@@ -319,24 +321,20 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const bool masked = !every || __any_sync(kFull, out || poisoned);
         PAGED_WAIT_ON(L::B_S_FULL + (pos & 1u), (pos >> 1) & 1u);
         tc_fence_after();
-        if (masked) {
+        if (masked && wg == 0) {
           // P of a token that takes no part is 0, and 0 times what its V row holds (an unused row, NaN) has to be 0
           PAGED_WAIT_ON(L::B_KV_FULL + stage, phase);
           uint4* const v_row = reinterpret_cast<uint4*>(smem + L::kKvOff + (2 * stage + 1) * L::kTileBytes + tid * D);
-          if (!every && !out && !poisoned) {
-            // some row may take part and some not: a NaN goes into P of those that do
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              const uint4 u = v_row[i];
-              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) poisoned |= __vcmpeq4(w[e] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0u;
-            }
-          }
-          if (kGroups > 1 && !every) named_bar_sync(3, 128 * kGroups);  // all warpgroups have looked
-          if (wg == 0 && (out || poisoned)) {
+          if (out || poisoned) {
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) v_row[i] = make_uint4(0, 0, 0, 0);
+          } else if (!every) {
+            // some row may take part and some not: a NaN is put into the columns of those that do at the stretch's end
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              uint4 u = v_row[i];
+              if (drop_nans(u)) v_row[i] = u, *nan_item = q_pos;
+            }
           }
         }
         if (rows > 0) {
@@ -549,7 +547,15 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
               else a.o[row_at[i] + tid] = __float2bfloat16_rn(v);
             }
           }
+          if (*nan_item == q_pos) {
+            for (int i = 0; i < rows; ++i) {
+              if (((nan_columns(a, it.b, it.h, it.tile0, it.tiles, range[i].x, range[i].y, all_lo, all_hi, tid & ~31) >> (tid & 31)) & 1u) == 0u) continue;
+              if (cut) po[i * D] = __uint_as_float(0x7fffffffu);
+              else a.o[row_at[i] + tid] = __ushort_as_bfloat16(0x7fffu);
+            }
+          }
         }
+        __syncwarp();
       }
       tc_fence_before();
       if (!cut) {

@@ -32,6 +32,7 @@ struct PagedItem {
   int tile0, tiles;
   int pieces;   // stretches the item is cut into
   int first;    // CTA of the first of them
+  int b;        // request
 };
 
 // One more of the CTAs of an item: how many came before.  Release and acquire: what the caller's CTA wrote before its barrier is seen by
@@ -64,6 +65,40 @@ __device__ __forceinline__ KeyRange keys_of_any(int i0, int i1, int q_len, int l
   return r;
 }
 __device__ __forceinline__ int tiles_of(const KeyRange& r) { return r.hi > r.lo ? (r.hi + kTile - 1) / kTile - r.lo / kTile : 0; }
+
+// A NaN in V makes NaN of its column of O, for the rows that take part with its token.  Where all rows of a tile do, the products see to that; where
+// some do not, the NaNs leave V before them (0 times NaN is NaN), and a stretch that had any asks here at its end: a bit for each of 32
+// columns, c0 on, that holds a NaN at one of a row's keys [lo, hi) in those of the tiles that not all rows take part with ([all_lo, all_hi)).  From
+// the cache once more: rare, and no place to remember it in (256 rows of 128 columns).
+static __device__ __noinline__ uint32_t nan_columns(const PagedArgs& a, int b, int h, int tile0, int tiles, int lo, int hi, int all_lo, int all_hi, int c0) {
+  const int* const table = a.block_tables + static_cast<long long>(b) * a.table_stride;
+  uint32_t bits = 0;
+  for (int t = tile0; t < tile0 + tiles; ++t) {
+    if (t * kTile >= all_lo && (t + 1) * kTile <= all_hi) continue;
+    for (int key = max(lo, t * kTile); key < min(hi, (t + 1) * kTile); ++key) {
+      const int blk = table[key >> a.block_shift];
+      if (blk < 0 || blk >= a.num_blocks) continue;
+      const uint4* const v = reinterpret_cast<const uint4*>(a.v_cache + blk * a.v_strides[0] + (key & ((1 << a.block_shift) - 1)) * a.v_strides[1] +
+                                                            h * a.v_strides[2] + c0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint4 u = v[i];
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          bits |= (((__vcmpeq4(w[e] & 0x7f7f7f7fu, 0x7f7f7f7fu) & 0x08040201u) * 0x01010101u) >> 24) << (16 * i + 4 * e);
+      }
+    }
+  }
+  return bits;
+}
+// Sixteen bytes of V without their NaNs; whether there were any.
+__device__ __forceinline__ bool drop_nans(uint4& u) {
+  const uint32_t x = __vcmpeq4(u.x & 0x7f7f7f7fu, 0x7f7f7f7fu), y = __vcmpeq4(u.y & 0x7f7f7f7fu, 0x7f7f7f7fu),
+                 z = __vcmpeq4(u.z & 0x7f7f7f7fu, 0x7f7f7f7fu), w = __vcmpeq4(u.w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+  u = make_uint4(u.x & ~x, u.y & ~y, u.z & ~z, u.w & ~w);
+  return (x | y | z | w) != 0u;
+}
 
 struct Request {
   int q_start, q_len, len;
@@ -193,8 +228,9 @@ struct PagedCta {
     it.h = -2;
     if (!wait(L::B_ITEM_FULL + item_pos % kItemSlots, (item_pos / kItemSlots) & 1u, role)) return it;
     const int4 x = slot()[0], y = slot()[1], z = slot()[2];
+    const int b = slot()[3].x;
     it = PagedItem{warp_uniform(x.x), warp_uniform(x.y), warp_uniform(x.z), warp_uniform(x.w), warp_uniform(y.x), warp_uniform(y.y),
-                   warp_uniform(y.z), warp_uniform(y.w), warp_uniform(z.x), warp_uniform(z.y), warp_uniform(z.z), warp_uniform(z.w)};
+                   warp_uniform(y.z), warp_uniform(y.w), warp_uniform(z.x), warp_uniform(z.y), warp_uniform(z.z), warp_uniform(z.w), warp_uniform(b)};
     __syncwarp();
     if (lane == 0) mbar_arrive(bar_base + 8u * (L::B_ITEM_EMPTY + item_pos % kItemSlots));
     ++item_pos;
@@ -206,6 +242,7 @@ struct PagedCta {
       slot()[0] = make_int4(it.h, it.q_start, it.q_len, it.row0);
       slot()[1] = make_int4(it.rows, it.len, it.lo, it.hi);
       slot()[2] = make_int4(it.tile0, it.tiles, it.pieces, it.first);
+      slot()[3].x = it.b;
       mbar_arrive(bar_base + 8u * (L::B_ITEM_FULL + item_pos % kItemSlots));
     }
     ++item_pos;
@@ -272,8 +309,8 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
     int wb = start->b - 1, wh = a.kv_heads, wt = 0, w_nt = 0, w_rows = 0;
     long long at = start->before;
     Request rq{0, 0, 0};
-    // the next item of which this CTA has tiles, published; h = -1 at the end.  Its request is `b_of`.
-    auto next_item = [&](PagedItem& it, int& b_of) -> bool {
+    // the next item of which this CTA has tiles, published; h = -1 at the end
+    auto next_item = [&](PagedItem& it) -> bool {
       it = PagedItem{};
       it.h = -1;
       while (at < u1) {
@@ -302,21 +339,19 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
         // the CTA that has unit u is the largest c with all * c / ctas <= u
         const int first = static_cast<int>(((s + 1) * ctas - 1) / all_units);
         const int pieces = static_cast<int>(((s + n1) * ctas - 1) / all_units) - first + 1;
-        it = PagedItem{wh, rq.q_start, rq.q_len, row0, rows, rq.len, r.lo, r.hi, r.lo / kTile + from, n == 0 ? 0 : to - from, pieces, first};
-        b_of = wb;
+        it = PagedItem{wh, rq.q_start, rq.q_len, row0, rows, rq.len, r.lo, r.hi, r.lo / kTile + from, n == 0 ? 0 : to - from, pieces, first, wb};
         break;
       }
       return cta.publish(it);
     };
     PagedItem it, ahead;
-    int b = 0, b_ahead = 0;
-    if (!next_item(it, b)) return false;
+    if (!next_item(it)) return false;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (it.h >= 0 && it.tiles > 0 && !load_q(it)) return false;
-    for (; it.h >= 0; it = ahead, b = b_ahead) {
-      if (!next_item(ahead, b_ahead)) return false;
+    for (; it.h >= 0; it = ahead) {
+      if (!next_item(ahead)) return false;
       const int n_blocks = min((it.len + block_size - 1) >> a.block_shift, a.table_width);
-      const int* const table = a.block_tables + static_cast<long long>(b) * a.table_stride;
+      const int* const table = a.block_tables + static_cast<long long>(it.b) * a.table_stride;
       int cached = 0, cached_at = -1;  // 32 entries of the table, from entry cached_at on
       for (int j = 0; j < it.tiles; ++j, ++pos) {
         const uint32_t stage = pos % L::kStages;

@@ -82,7 +82,7 @@ struct RowsShape {
 template <int D, int ACT>
 __global__ void __launch_bounds__(RowsShape<D>::kThreads, 1)
 gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                       const PagedArgs a) {
+                       const __grid_constant__ PagedArgs a) {
   using L = RowsShape<D>;
   constexpr bool SOFTMAX = ACT == ACT_SOFTMAX;
   extern __shared__ uint8_t smem_raw[];
@@ -259,12 +259,9 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               const int t = t0 + i * kTokens, key = key0 + t;
               uint4 u = *reinterpret_cast<const uint4*>(smem + from_of(pos, t));
               const bool out = key < it.lo || key >= it.hi || no_block(sv[t >> a.block_shift]);
-              // some row may take part with this token and some not: a NaN goes into P of those that do
-              const bool nan = !every && !out && (__vcmpeq4(u.x & 0x7f7f7f7fu, 0x7f7f7f7fu) | __vcmpeq4(u.y & 0x7f7f7f7fu, 0x7f7f7f7fu) |
-                                                  __vcmpeq4(u.z & 0x7f7f7f7fu, 0x7f7f7f7fu) | __vcmpeq4(u.w & 0x7f7f7f7fu, 0x7f7f7f7fu)) != 0u;
-              const bool bad = ((__ballot_sync(kFull, nan) >> (t_lane * kChunks)) & ((1u << kChunks) - 1u)) != 0u;
-              if (bad) poison |= 1u << (i * kTokens + t_lane);
-              if (out || bad) u = make_uint4(0, 0, 0, 0);
+              // some row may take part with this token and some not: a NaN is put into the columns of those that do at the stretch's end
+              if (!every && !out && drop_nans(u)) poison |= 1u << (i * kTokens + t_lane);
+              if (out) u = make_uint4(0, 0, 0, 0);
               put(t, u);
             }
             poison = __reduce_or_sync(kFull, poison);
@@ -308,6 +305,7 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       const int all_lo = max(rf.lo, rl.lo), all_hi = min(rf.hi, rl.hi);
       const float qa = __ldcg(a.qa + (static_cast<long long>(it.h) * a.total_q + it.q_start) * a.group + it.row0 + min(r, it.rows - 1));
       float ref = SOFTMAX ? kNoMax : 1.2676506e30f, l = 0.f;  // running maximum / multiplier; sum of P
+      bool nan_seen = false;                                  // a token of this row had NaNs taken out of V
       for (int j = 0; j < it.tiles; ++j, ++pos) {
         const uint32_t stage = pos % L::kStages, phase = (pos / L::kStages) & 1u;
         if (!tile_live) continue;  // neither S nor P of this row tile in the item
@@ -395,7 +393,8 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                 float top = SOFTMAX ? kNoMax : 0.f;  // the largest |P| without the reference (softmax: its logarithm)
 #pragma unroll 1
                 for (int i = 0; i < 4; ++i) {
-                  const uint32_t in = masked ? part_of(i) : 0xffffu, bad = every ? 0u : poison[i] & in;
+                  const uint32_t in = masked ? part_of(i) : 0xffffu;
+                  if (!every && (poison[i] & in) != 0u) nan_seen = true;
                   uint32_t s[16];
                   float kf, vs, y[16];
                   tmem_ld16(s_tmem + i * 16, s);
@@ -404,10 +403,7 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                   factors(i, kf, vs);
                   products(s, kf, vs, y);
 #pragma unroll
-                  for (int e = 0; e < 16; ++e) {
-                    y[e] = (in >> e) & 1u ? y[e] : 0.f;
-                    y[e] = (bad >> e) & 1u ? __uint_as_float(0x7fffffffu) : y[e];
-                  }
+                  for (int e = 0; e < 16; ++e) y[e] = (in >> e) & 1u ? y[e] : 0.f;
                   const float part = sum_of(y);
                   const bool number = fabsf(vs) <= 3.4028235e38f;  // a scale that is none makes NaN of the rows that take part, and of no other
                   sum = SOFTMAX ? fmaf(part, number ? vs : 0.f, sum) : sum + part;
@@ -507,6 +503,16 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             }
           }
         }
+        if (nan_seen) {
+          for (int c = 0; c < D; c += 32) {
+            for (uint32_t nans = nan_columns(a, it.b, it.h, it.tile0, it.tiles, rg.lo, rg.hi, all_lo, all_hi, c); nans != 0u; nans &= nans - 1u) {
+              const int e = c + __ffs(nans) - 1;
+              if (cut) a.part_o[(static_cast<long long>(part) * kRows + r) * D + e] = __uint_as_float(0x7fffffffu);
+              else o_row[e] = __ushort_as_bfloat16(0x7fffu);
+            }
+          }
+        }
+        __syncwarp();
         tc_fence_before();
       }
       if (cut) {

@@ -217,3 +217,28 @@ def test_a_nan_scale_stays_where_it_is(queries):
         sees[max(0, queries - 44):queries, 2:] = True
         assert bool(dirty[sees].isnan().all()) and torch.equal(dirty[~sees], clean[~sees])
         assert G.kernel_status() == 0
+
+
+# ------------------------------------------------------------------------------------------ NaN in V
+
+
+@pytest.mark.parametrize("queries", [1, 6, 30, 70, 300])
+@pytest.mark.parametrize("activation", ["softmax", "silu"])
+@pytest.mark.parametrize("causal,window", [(False, None), (True, None), (True, 40), (False, 0), (False, 700)])
+def test_a_nan_in_v_is_its_column_s(causal, window, activation, queries):
+    # whether the tile it lies in has a mask or not, whether the item is cut or not: the element is NaN for the queries that see the token, and
+    # nothing else changes
+    for dim, lens in ((64, [900, 400, 130]), (128, [300, 5000, 64])):
+        batch = Batch(lens, [queries] * 3, 4, 2, dim, 32, seed=queries)
+        clean = batch.run(0.1, activation, causal, window)
+        bad = torch.zeros(clean.shape, dtype=torch.bool, device=DEV)
+        for b, pos, head, column in ((0, 5, 0, 3), (0, lens[0] - 1, 1, 40), (0, lens[0] - 1, 1, dim - 1), (1, lens[1] - 2, 0, 31), (1, 250, 1, 0), (2, 60, 0, 17)):
+            batch.v[int(batch.table[b, pos // 32]), pos % 32, head, column] = 0x7F if column % 2 else 0xFF
+            for i in range(queries):
+                p = lens[b] - queries + i
+                if (not causal or pos <= p) and (window is None or abs(pos - p) <= window):
+                    bad[batch.offsets[b] + i, 2 * head:2 * head + 2, column] = True
+        dirty = batch.run(0.1, activation, causal, window)
+        assert G.kernel_status() == 0
+        assert torch.equal(dirty.isnan(), bad)
+        assert torch.equal(dirty[~bad], clean[~bad])

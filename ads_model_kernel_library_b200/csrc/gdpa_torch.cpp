@@ -26,10 +26,27 @@ struct EntryPoints {
   const char* (*strerror)(int);
 } g_call{};
 constexpr int kMaxDevices = 64;
-std::atomic<int32_t*> g_status[kMaxDevices];  // of each device, or null
+// The word of each device into which a kernel writes when a wait of it runs out, or null as long as nobody has asked for it.  Python has it: the
+// call returns it and, where it is set, clears it and says what happened in `message`.
+std::atomic<int32_t*> g_status[kMaxDevices];
+using StatusLook = int32_t* (*)(int device, char* message, int size);
+std::atomic<StatusLook> g_look{nullptr};
 std::atomic<void*> g_timing[2];               // events around the attention's kernel, or null
 
 void check(int code, const char* what) { TORCH_CHECK(code == GDPA_OK, what, ": ", g_call.strerror(code), " (code ", code, ")"); }
+
+// The status word for a call on `device`; an error if a wait of an earlier call's kernel ran out.  Here, not in Python, so that a traced call does it too.
+int32_t* status_of(int device) {
+  if (device < 0 || device >= kMaxDevices) return nullptr;
+  int32_t* word = g_status[device].load();
+  if (word != nullptr && *static_cast<volatile int32_t*>(word) == 0) return word;
+  const StatusLook look = g_look.load();
+  if (look == nullptr) return word;
+  char message[512] = "";
+  g_status[device].store(word = look(device, message, sizeof(message)));
+  TORCH_CHECK(message[0] == '\0', message);
+  return word;
+}
 
 void check_cuda(const char* name, const at::Tensor& t) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor: this operator has no CPU path");
@@ -194,6 +211,7 @@ at::Tensor attend_paged_fp8(const at::Tensor& query, const at::Tensor& k_cache, 
                             const at::Tensor& v_scales, const at::Tensor& block_tables, const at::Tensor& query_offset, const at::Tensor& seq_lens,
                             int64_t max_seq_len_q, double qk_scale, int64_t activation, bool is_causal, int64_t window_size) {
   check_cuda("query", query);
+  int32_t* const status = status_of(query.get_device());
   check_type("query", query, at::kBFloat16);
   check_rows("query", query);
   check_cache(k_cache, v_cache, k_scales, v_scales, query);
@@ -246,8 +264,7 @@ at::Tensor attend_paged_fp8(const at::Tensor& query, const at::Tensor& k_cache, 
   p.window_plus_one = static_cast<int32_t>(window_size + 1);
   p.workspace = workspace.mutable_data_ptr();
   p.workspace_bytes = static_cast<int64_t>(bytes);
-  const int device = query.get_device();
-  p.status = device >= 0 && device < kMaxDevices ? g_status[device].load() : nullptr;
+  p.status = status;
   p.timing_start_event = g_timing[0].load();
   p.timing_stop_event = g_timing[1].load();
   check(g_call.attend(&p, c10::cuda::getCurrentCUDAStream().stream()), "gdpa_fwd_paged_fp8");
@@ -264,9 +281,10 @@ extern "C" __attribute__((visibility("default"))) void gdpa_torch_init(void* tab
   g_call.attend = reinterpret_cast<decltype(g_call.attend)>(attend);
   g_call.strerror = reinterpret_cast<decltype(g_call.strerror)>(error);
 }
-// The status word of a device, and the events around the next calls' kernel (null: none).
-extern "C" __attribute__((visibility("default"))) void gdpa_torch_set_status(int device, void* word) {
-  if (device >= 0 && device < kMaxDevices) g_status[device].store(static_cast<int32_t*>(word));
+// Who has the status words, and the events around the next calls' kernel (null: none).
+extern "C" __attribute__((visibility("default"))) void gdpa_torch_set_status_look(void* look) {
+  for (auto& word : g_status) word.store(nullptr);
+  g_look.store(reinterpret_cast<StatusLook>(look));
 }
 extern "C" __attribute__((visibility("default"))) void gdpa_torch_set_timing(void* start, void* stop) {
   g_timing[0].store(start);

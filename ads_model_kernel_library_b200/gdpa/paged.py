@@ -27,6 +27,19 @@ __all__ = ["build_block_tables", "append_kv_cache_fp8", "generalized_dot_product
 LIB_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "libgdpa_b200_torch.so")
 
 
+@C.CFUNCTYPE(C.c_void_p, C.c_int, C.POINTER(C.c_char), C.c_int)
+def _look_at_status(device: int, message, size: int):
+    """The address of a device's status word, for the operators' C++ side: called for a device's first call, and when the word is set."""
+    where = torch.device("cuda", device)
+    word = ops._status_word(where).data_ptr()
+    try:
+        ops._raise_if_wait_ran_out(where)
+    except RuntimeError as e:
+        text = str(e).encode()[:size - 1] + b"\0"
+        C.memmove(message, text, len(text))
+    return word
+
+
 class _Operators:
     """The three torch operators, which libgdpa_b200_torch.so registers (checks, outputs and launch in C++: a step of generation is host
     time), with their fake kernels."""
@@ -42,7 +55,7 @@ class _Operators:
         entries = (lib.gdpa_build_block_tables, lib.gdpa_append_kv_cache_fp8, lib.gdpa_paged_workspace_bytes, lib.gdpa_fwd_paged_fp8, lib.gdpa_strerror)
         self.native.gdpa_torch_init(*(C.cast(f, C.c_void_p) for f in entries))
         self.native.gdpa_torch_set_timing.argtypes = [C.c_void_p, C.c_void_p]
-        self.native.gdpa_torch_set_status.argtypes = [C.c_int, C.c_void_p]
+        self.native.gdpa_torch_set_status_look(_look_at_status)
         if first:
             torch.library.register_fake("gdpa::build_block_tables", _fake_tables)
             torch.library.register_fake("gdpa::append_kv_cache_fp8", lambda *args: None)
@@ -51,15 +64,6 @@ class _Operators:
         self.tables = torch.ops.gdpa.build_block_tables.default
         self.append = torch.ops.gdpa.append_kv_cache_fp8.default
         self.attend = torch.ops.gdpa.generalized_dot_product_attention_paged_fp8.default
-        self.has_status = set()
-
-    def look_at_status(self, device: int) -> None:
-        """Raise if a wait of an earlier call's kernel ran out; a device's first call gives it its status word."""
-        if device not in self.has_status:
-            self.native.gdpa_torch_set_status(device, ops._status_word(torch.device("cuda", device)).data_ptr())
-            self.has_status.add(device)
-        if ops._status_views[device].value:
-            ops._raise_if_wait_ran_out(torch.device("cuda", device))
 
 
 _operators: Optional[_Operators] = None
@@ -176,11 +180,8 @@ def generalized_dot_product_attention_paged_fp8(
     trusted like the offsets of the other operators (clamped in the kernel, checked on the host with offset validation on).
     """
     call = _operators or _load()
-    if not torch.compiler.is_compiling():
-        if query.is_cuda:
-            call.look_at_status(query.get_device())
-        if ops._validate_offsets:
-            _check_lengths(query, k_cache, block_tables, query_offset, seq_lens)
+    if ops._validate_offsets and not torch.compiler.is_compiling():
+        _check_lengths(query, k_cache, block_tables, query_offset, seq_lens)
     args = (query, k_cache, v_cache, k_scales, v_scales, block_tables, query_offset, seq_lens, max_seq_len_q,
             1.0 if qk_scale is None else qk_scale, activation_string_to_int(activation), is_causal, -1 if window_size is None else window_size)
     events = ops._timing_events["fwd"]

@@ -1,8 +1,13 @@
 """Edges of the paged 8-bit cache on the GPU: batches and values at which its operators can go wrong."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
 import ads_model_kernel_library_b200.gdpa as G
+from ads_model_kernel_library_b200.gdpa import ops
 from tests._paged_batches import Batch
 
 pytestmark = pytest.mark.gpu
@@ -242,3 +247,44 @@ def test_a_nan_in_v_is_its_column_s(causal, window, activation, queries):
         assert G.kernel_status() == 0
         assert torch.equal(dirty.isnan(), bad)
         assert torch.equal(dirty[~bad], clean[~bad])
+
+
+# ------------------------------------------------------------------------------------------ a wait that ran out
+
+
+def test_a_wait_that_ran_out_is_said_by_the_next_call():
+    batch = Batch([100], [2], 4, 2, 64, 16)
+    clean = batch.run(0.1)
+    word = ops._status_word(torch.device("cuda", torch.cuda.current_device()))
+    torch.cuda.synchronize()
+    word[0] = 0x1703  # what a kernel writes
+    with pytest.raises(RuntimeError, match="wait ran out .*0x1703"):
+        batch.run(0.1)
+    assert torch.equal(batch.run(0.1), clean) and G.kernel_status() == 0
+
+
+_TRACED = """
+import torch
+import ads_model_kernel_library_b200.gdpa as G
+from ads_model_kernel_library_b200.gdpa import ops
+from tests._paged_batches import Batch
+b = Batch([100], [2], 4, 2, 64, 16)
+args = (b.q, b.k.view(torch.float8_e4m3fn), b.v.view(torch.float8_e4m3fn), b.ks, b.vs, b.table, b.int32(b.offsets), b.int32(b.lens))
+step = torch.compile(lambda *a: G.generalized_dot_product_attention_paged_fp8(*a, 2, qk_scale=0.1), backend="aot_eager")
+first = step(*args)
+torch.cuda.synchronize()
+ops._status_word(torch.device("cuda", 0))[0] = 0x1703
+try:
+    step(*args)
+except RuntimeError as e:
+    assert "0x1703" in str(e), e
+    assert torch.equal(step(*args), first) and G.kernel_status() == 0
+    print("said")
+"""
+
+
+def test_a_traced_call_has_the_status_word_too():
+    # in a process of its own, in which no call was made before the traced one
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _TRACED], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0 and "said" in r.stdout, r.stdout + r.stderr

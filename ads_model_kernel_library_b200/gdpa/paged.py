@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import threading
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -67,11 +68,14 @@ class _Operators:
 
 
 _operators: Optional[_Operators] = None
+_loading = threading.Lock()
 
 
 def _load() -> _Operators:
     global _operators
-    _operators = _Operators()
+    with _loading:  # first calls of two threads: the operators are registered once
+        if _operators is None:
+            _operators = _Operators()
     return _operators
 
 

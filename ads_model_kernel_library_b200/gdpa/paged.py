@@ -256,3 +256,11 @@ class PagedKVCache:
         self.num_free = self.num_free.clamp_min(0) + held.sum().to(torch.int32)
         self.block_tables[rows] = -1
         self.seq_lens[rows] = 0
+
+
+# The libraries are loaded here if they are built, so that a compiler that traces a first call finds the operators; if that fails, the first call says why.
+if os.path.exists(LIB_PATH) and os.path.exists(_cabi.LIB_PATH):
+    try:
+        _load()
+    except OSError:
+        pass

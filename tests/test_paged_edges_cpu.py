@@ -11,6 +11,34 @@ def in_a_process_of_its_own(code):
     assert r.returncode == 0 and "ok" in r.stdout, r.stdout + r.stderr
 
 
+def test_a_step_traces_as_one_graph_before_any_other_call():
+    in_a_process_of_its_own("""
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+import ads_model_kernel_library_b200.gdpa as G
+
+def step(q, k, v, k8, v8, ks, vs, table, cached, new, free, num_free):
+    slots, offsets, lens, left = G.build_block_tables(table, cached, new, free, num_free, 16, q.shape[0])
+    G.append_kv_cache_fp8(k, v, k8, v8, ks, vs, slots)
+    return G.generalized_dot_product_attention_paged_fp8(q, k8, v8, ks, vs, table, offsets, lens, 2, is_causal=True), lens, left
+
+calls = []
+def backend(graph, inputs):
+    calls.append([str(n.target) for n in graph.graph.nodes if n.op == "call_function" and "gdpa" in str(n.target)])
+    return graph.forward
+
+with FakeTensorMode(allow_non_fake_inputs=True):
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+    x = lambda h: torch.zeros(3, h, 64, dtype=torch.bfloat16, device="cuda")
+    f8 = lambda: torch.zeros(8, 16, 2, 64, dtype=torch.float8_e4m3fn, device="cuda")
+    s = lambda: torch.ones(8, 2, device="cuda")
+    out, lens, left = torch.compile(step, backend=backend, fullgraph=True)(x(4), x(2), x(2), f8(), f8(), s(), s(), i(2, 4), i(2), i(2), i(8), i(1))
+assert out.shape == (3, 4, 64) and out.dtype == torch.bfloat16 and lens.shape == (2,) and left.shape == (1,)
+assert calls == [["gdpa.build_block_tables.default", "gdpa.append_kv_cache_fp8.default", "gdpa.generalized_dot_product_attention_paged_fp8.default"]], calls
+print("ok")
+""")
+
+
 def test_first_calls_of_several_threads_load_the_operators_once():
     in_a_process_of_its_own("""
 import threading

@@ -14,6 +14,7 @@ and makes the three calls.  Nothing here synchronises with the host, and there a
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import os
 import threading
 from typing import Optional, Sequence, Tuple
@@ -243,8 +244,13 @@ class PagedKVCache:
         return self.attend(query, self.append(key, value, new_lens), max_seq_len_q, **{"is_causal": True, **options})
 
     def release(self, requests: Sequence[int]) -> None:
-        """Give back the blocks of these requests (rows of the tables), which are empty afterwards."""
-        rows = torch.tensor(sorted(set(requests)), dtype=torch.int64, device=self.block_tables.device)
+        """Give back the blocks of these requests (rows of the tables, negative ones from the end), which are empty afterwards."""
+        batch = self.block_tables.shape[0]
+        asked = [operator.index(r) for r in requests]
+        for r in asked:  # on the host: an index out of range would be an assertion on the GPU, whose context is lost with it
+            if not -batch <= r < batch:
+                raise IndexError(f"request {r} is not one of this cache's {batch}")
+        rows = torch.tensor(sorted({r % batch for r in asked}), dtype=torch.int64, device=self.block_tables.device)
         table = self.block_tables[rows]
         held = torch.arange(table.shape[1], device=table.device) < ((self.seq_lens[rows] + self.block_size - 1) // self.block_size)[:, None]
         held &= table >= 0

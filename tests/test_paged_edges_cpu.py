@@ -3,6 +3,11 @@ import os
 import subprocess
 import sys
 
+import pytest
+import torch
+
+import ads_model_kernel_library_b200.gdpa as G
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
@@ -63,3 +68,38 @@ threads = [threading.Thread(target=first) for _ in range(8)]
 assert not errors and len(made) == 1, (errors, len(made))
 print("ok")
 """)
+
+
+def held_cache():
+    """A cache of five requests on the CPU, of which the first four hold 1 to 4 blocks."""
+    cache = G.PagedKVCache(20, 16, 1, 64, 5, 128, device="cpu")
+    for b in range(4):
+        n = b + 1
+        cache.block_tables[b, :n] = cache.free_blocks[int(cache.num_free) - n:int(cache.num_free)]
+        cache.seq_lens[b], cache.num_free = 16 * n - 3, cache.num_free - n
+    return cache
+
+
+def free(cache):
+    return sorted(cache.free_blocks[:int(cache.num_free)].tolist())
+
+
+@pytest.mark.parametrize("requests", [[5], [-6], [0, 99], [2 ** 40], [1, -1000]])
+def test_release_of_a_request_that_is_not_there(requests):
+    cache = held_cache()
+    before = [t.clone() for t in (cache.block_tables, cache.seq_lens, cache.free_blocks, cache.num_free)]
+    with pytest.raises(IndexError, match="is not one of this cache's 5"):
+        cache.release(requests)
+    assert all(torch.equal(a, b) for a, b in zip(before, (cache.block_tables, cache.seq_lens, cache.free_blocks, cache.num_free)))
+    with pytest.raises(TypeError):
+        cache.release([1.5])
+
+
+def test_release_of_a_request_by_two_names():
+    cache = held_cache()
+    cache.release([3, -2, 3, 1])  # 3 and -2 are the same one
+    assert int(cache.num_free) == 16 and len(set(free(cache))) == 16
+    assert cache.seq_lens.tolist() == [13, 0, 45, 0, 0] and cache.block_tables[[1, 3]].eq(-1).all()
+    cache.release([])
+    cache.release([0, 1, 2, 3, 4])
+    assert free(cache) == list(range(20))

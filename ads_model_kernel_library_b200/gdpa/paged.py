@@ -250,7 +250,9 @@ class PagedKVCache:
         for r in asked:  # on the host: an index out of range would be an assertion on the GPU, whose context is lost with it
             if not -batch <= r < batch:
                 raise IndexError(f"request {r} is not one of this cache's {batch}")
-        rows = torch.tensor(sorted({r % batch for r in asked}), dtype=torch.int64, device=self.block_tables.device)
+        rows = torch.tensor(sorted({r % batch for r in asked}), dtype=torch.int64)
+        if self.block_tables.is_cuda:  # from pinned memory: a copy from pageable memory waits for the stream
+            rows = rows.pin_memory().to(self.block_tables.device, non_blocking=True)
         table = self.block_tables[rows]
         held = torch.arange(table.shape[1], device=table.device) < ((self.seq_lens[rows] + self.block_size - 1) // self.block_size)[:, None]
         held &= table >= 0
@@ -260,8 +262,8 @@ class PagedKVCache:
         stack[torch.where(held.flatten(), place, self.free_blocks.numel())] = table.flatten()
         self.free_blocks = stack[:-1]
         self.num_free = self.num_free.clamp_min(0) + held.sum().to(torch.int32)
-        self.block_tables[rows] = -1
-        self.seq_lens[rows] = 0
+        self.block_tables.index_fill_(0, rows, -1)
+        self.seq_lens.index_fill_(0, rows, 0)
 
 
 # The libraries are loaded here if they are built, so that a compiler that traces a first call finds the operators; if that fails, the first call says why.

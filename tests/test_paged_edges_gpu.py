@@ -288,3 +288,29 @@ def test_a_traced_call_has_the_status_word_too():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", _TRACED], capture_output=True, text=True, timeout=300, cwd=root)
     assert r.returncode == 0 and "said" in r.stdout, r.stdout + r.stderr
+
+
+# ------------------------------------------------------------------------------------------ a cache's steps
+
+
+def test_a_step_and_a_release_do_not_wait_for_the_gpu():
+    cache = G.PagedKVCache(40, 16, 2, 64, 5, 128)
+    new = torch.tensor([20, 1, 0, 33, 5], dtype=torch.int32, device=DEV)
+    q, kv = torch.randn(59, 4, 64, device=DEV).bfloat16(), torch.randn(59, 2, 64, device=DEV).bfloat16()
+    cache.step(q, kv, kv, new, 33)
+    cache.release([2])
+    torch.cuda.synchronize()
+    mode = torch.cuda.get_sync_debug_mode()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        cache.step(q, kv, kv, new, 33)
+        cache.release([0, 3])
+        cache.step(q, kv, kv, new, 33)
+    finally:
+        torch.cuda.set_sync_debug_mode(mode)
+    assert cache.seq_lens.tolist() == [20, 3, 0, 33, 15]
+    assert int(cache.num_free) == 40 - 2 - 1 - 0 - 3 - 1
+    table = cache.block_tables[cache.block_tables >= 0].tolist()
+    assert len(set(table) | set(cache.free_blocks[:int(cache.num_free)].tolist())) == 40
+    with pytest.raises(IndexError):
+        cache.release([5])

@@ -145,11 +145,9 @@ def _check_slots(slot_mapping: torch.Tensor, cache: torch.Tensor) -> None:
     """The host's look at a slot map (offset validation): every block's tokens are one run."""
     blocks, size = cache.shape[:2]
     s = slot_mapping.detach().to("cpu")
-    s = s[(s >= 0) & (s < blocks * size)]
-    if s.numel() == 0:
-        return
-    begins = torch.ones_like(s, dtype=torch.bool)
-    begins[1:] = (s[1:] != s[:-1] + 1) | (s[1:] % size == 0)
+    held = (s >= 0) & (s < blocks * size)
+    begins = held.clone()  # a token that is skipped ends a run, as any other slot than the next does
+    begins[1:] &= ~held[:-1] | (s[1:] != s[:-1] + 1) | (s[1:] % size == 0)
     runs = s[begins] // size
     if runs.unique().numel() != runs.numel():
         raise ValueError("slot_mapping must hold the tokens of a block one after the other, with consecutive slots")

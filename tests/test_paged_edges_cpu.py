@@ -103,3 +103,18 @@ def test_release_of_a_request_by_two_names():
     cache.release([])
     cache.release([0, 1, 2, 3, 4])
     assert free(cache) == list(range(20))
+
+
+@pytest.mark.parametrize("slots,good", [
+    ([], True), ([-1, -1], True), ([3], True), ([14, 15, 16, 17], True), ([0, 1, -1, 32, 33], True), ([-1, 4, 5, -1], True), ([10 ** 12, 0, 1], True),
+    ([48, 49, 10 ** 12, 0], True), ([63, 64, 65], True),
+    ([5, -1, 6], False), ([5, 10 ** 12, 6], False), ([5, 64, 6], False), ([-1, 5, -1, 6, -1], False), ([0, 1, 16, 2], False), ([1, 0], False), ([3, 3], False),
+])
+def test_what_the_check_of_slots_says(slots, good):
+    # of a cache of four blocks of 16
+    cache = torch.zeros(4, 16, 1, 64, dtype=torch.uint8)
+    if good:
+        G.paged._check_slots(torch.tensor(slots, dtype=torch.int64), cache)
+    else:
+        with pytest.raises(ValueError):
+            G.paged._check_slots(torch.tensor(slots, dtype=torch.int64), cache)

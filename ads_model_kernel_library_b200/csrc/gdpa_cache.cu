@@ -33,8 +33,30 @@ __device__ __forceinline__ int clamp_len(const void* p, int b, int flags) {
   return static_cast<int>(clamp_ll(load_offset(p, b, flags), 0, 0x3fffff00));  // two of them and a block fit in an int
 }
 
+// Where there are more tokens than slots: the new blocks that begin with a token without one, by one CTA.  For itself and at the kernel's end: not
+// what a caller should do, and a call within the rounds cost the usual case 1.3 us.  A thread has a stretch of requests, and the sums before it.
+__device__ __noinline__ void blocks_without_slots(const BlockTableArgs& a, long long have) {
+  const int S = 1 << a.block_shift;
+  const int per = (a.batch + blockDim.x - 1) / blockDim.x;
+  const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
+  long long tok = 0, blk = 0;
+  for (int b = 0; b < b1; ++b) {
+    const int cached = clamp_len(a.cached_lens, b, a.lens_are_int64), n = clamp_len(a.new_lens, b, a.lens_are_int64);
+    const int held = min((cached + S - 1) >> a.block_shift, a.table_width), after = min((cached + n + S - 1) >> a.block_shift, a.table_width);
+    if (b >= b0) {
+      for (int j = held; j < after; ++j) {
+        const long long at = have - 1 - (blk + (j - held));
+        if (tok + ((static_cast<long long>(j) << a.block_shift) - cached) >= a.total_new)
+          a.block_tables[static_cast<long long>(b) * a.table_stride + j] = at >= 0 ? a.free_blocks[at] : -1;
+      }
+    }
+    tok += n;
+    blk += after - held;
+  }
+}
+
 template <int kTableThreads, int PER>
-__global__ void __launch_bounds__(kTableThreads) gdpa_block_tables_kernel(const BlockTableArgs a) {
+__global__ void __launch_bounds__(kTableThreads) gdpa_block_tables_kernel(const __grid_constant__ BlockTableArgs a) {
   constexpr int kWarps = kTableThreads / 32;
   // of the round's requests: new tokens and blocks before them (from the start of the round), cached tokens
   extern __shared__ unsigned s_tokens[];
@@ -100,6 +122,8 @@ __global__ void __launch_bounds__(kTableThreads) gdpa_block_tables_kernel(const 
       a.query_offset[b0 + i] = static_cast<int>(tok0 + s_tokens[i]);
       a.seq_lens[b0 + i] = static_cast<int>(min(static_cast<long long>(s_cached[i]) + (end - s_tokens[i]), 0x7fffffffll));
     }
+    // tokens that have a slot to write: all, if total_new is what the lengths add up to, which bounds the walk whatever they say
+    const unsigned n_walk = static_cast<unsigned>(clamp_ll(a.total_new - tok0, 0, n_tok));
     // A warp takes 128 tokens at a time, four of each lane's at once.  The last request that begins at or before a token has it (one
     // without tokens begins where the next does): looked for among all requests by the whole warp for the first and the last
     // of the 128, between these two by each lane.
@@ -112,14 +136,14 @@ __global__ void __launch_bounds__(kTableThreads) gdpa_block_tables_kernel(const 
       }
       return lo;
     };
-    for (unsigned k0 = (blockIdx.x * kWarps + wp) * 128u; k0 < n_tok; k0 += gridDim.x * kWarps * 128u) {
-      const int from = owner_by_warp(k0), to = owner_by_warp(min(k0 + 127u, n_tok - 1)) + 1;
+    for (unsigned k0 = (blockIdx.x * kWarps + wp) * 128u; k0 < n_walk; k0 += gridDim.x * kWarps * 128u) {
+      const int from = owner_by_warp(k0), to = owner_by_warp(min(k0 + 127u, n_walk - 1)) + 1;
       int owner[4], blk[4];
       long long p[4];
       bool begins[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const unsigned k = min(k0 + 32u * i + lane, n_tok - 1);
+        const unsigned k = min(k0 + 32u * i + lane, n_walk - 1);
         int lo = from, hi = to;
         while (hi - lo > 1) {
           const int mid = (lo + hi) >> 1;
@@ -143,9 +167,9 @@ __global__ void __launch_bounds__(kTableThreads) gdpa_block_tables_kernel(const 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const unsigned k = k0 + 32u * i + lane;
-        if (k >= n_tok) continue;
+        if (k >= n_walk) continue;
         if (begins[i]) a.block_tables[static_cast<long long>(b0 + owner[i]) * a.table_stride + (p[i] >> a.block_shift)] = blk[i];
-        if (tok0 + k < a.total_new) a.slots[tok0 + k] = blk[i] < 0 ? -1ll : (static_cast<long long>(blk[i]) << a.block_shift) + (p[i] & (S - 1));
+        a.slots[tok0 + k] = blk[i] < 0 ? -1ll : (static_cast<long long>(blk[i]) << a.block_shift) + (p[i] & (S - 1));
       }
     }
     tok0 += n_tok;
@@ -157,6 +181,7 @@ __global__ void __launch_bounds__(kTableThreads) gdpa_block_tables_kernel(const 
     a.query_offset[a.batch] = static_cast<int>(min(tok0, 0x7fffffffll));
     *a.num_free_after = static_cast<int>(clamp_ll(have - blk0, -0x7fffffff, 0x7fffffff));
   }
+  if (blockIdx.x == 0 && tok0 > a.total_new) blocks_without_slots(a, have);
 }
 
 // ------------------------------------------------------------------------------------------ new keys and values

@@ -8,6 +8,7 @@ import torch
 
 import ads_model_kernel_library_b200.gdpa as G
 from ads_model_kernel_library_b200.gdpa import ops
+from tests import _paged_oracle as ref
 from tests._paged_batches import Batch
 
 pytestmark = pytest.mark.gpu
@@ -267,6 +268,7 @@ _TRACED = """
 import torch
 import ads_model_kernel_library_b200.gdpa as G
 from ads_model_kernel_library_b200.gdpa import ops
+from tests import _paged_oracle as ref
 from tests._paged_batches import Batch
 b = Batch([100], [2], 4, 2, 64, 16)
 args = (b.q, b.k.view(torch.float8_e4m3fn), b.v.view(torch.float8_e4m3fn), b.ks, b.vs, b.table, b.int32(b.offsets), b.int32(b.lens))
@@ -314,3 +316,42 @@ def test_a_step_and_a_release_do_not_wait_for_the_gpu():
     assert len(set(table) | set(cache.free_blocks[:int(cache.num_free)].tolist())) == 40
     with pytest.raises(IndexError):
         cache.release([5])
+
+
+# ------------------------------------------------------------------------------------------ block tables
+
+
+@pytest.mark.parametrize("batch", [5, 300, 9000])
+@pytest.mark.parametrize("share", [0.0, 0.3, 0.99])
+def test_tables_with_fewer_slots_than_tokens(batch, share):
+    # the tables, lengths and offsets are the same; the slots are the first ones
+    g = torch.Generator().manual_seed(batch)
+    cached, new = torch.randint(0, 60, (batch,), generator=g).tolist(), torch.randint(0, 90, (batch,), generator=g).tolist()
+    free, table = torch.randperm(batch * 8, generator=g).int(), torch.full((batch, 8), -1, dtype=torch.int32)
+    at = 0
+    for b, c in enumerate(cached):
+        n = -(-c // 16)
+        table[b, :n] = torch.arange(at, at + n) + 10 ** 6
+        at += n
+    total, short = sum(new), int(sum(new) * share)
+    want = ref.tables(table, cached, new, free, len(free) - 3, 16, total)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    mine = table.to(DEV)
+    slots, offsets, lens, left = G.build_block_tables(mine, i32(cached), i32(new), free.to(DEV), i32([len(free) - 3]), 16, short)
+    assert torch.equal(mine.cpu(), want[0]) and torch.equal(slots.cpu(), want[1][:short])
+    assert torch.equal(offsets.cpu().long(), want[2]) and torch.equal(lens.cpu().long(), want[3].long()) and int(left) == want[4]
+
+
+@pytest.mark.parametrize("batch", [6, 400, 3000])
+@pytest.mark.parametrize("length", [2 ** 30, 2 ** 31 - 1, 2 ** 40])
+def test_tables_of_lengths_that_are_nonsense(batch, length):
+    # what they say is unspecified; the call ends, writes nothing but its outputs, and the first request's tokens have their slots
+    dtype = torch.int64 if length > 2 ** 31 else torch.int32
+    wide = torch.full((batch, 9), 77, dtype=torch.int32, device=DEV)
+    free = torch.arange(100, dtype=torch.int32, device=DEV)
+    new = torch.full((batch,), length, dtype=dtype, device=DEV)
+    slots, offsets, lens, left = G.build_block_tables(wide[:, :4], torch.zeros_like(new), new, free, torch.tensor([100], dtype=torch.int32, device=DEV), 16, 40)
+    torch.cuda.synchronize()
+    assert bool((wide[:, 4:] == 77).all()) and wide[0, :4].tolist() == [99, 98, 97, 96]
+    assert slots.tolist() == [(99 - i // 16) * 16 + i % 16 for i in range(40)]
+    assert bool(((wide[:, :4] >= -1) & (wide[:, :4] < 100)).all())

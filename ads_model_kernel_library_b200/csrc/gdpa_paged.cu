@@ -285,7 +285,7 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (tid < C) {
         const int g = it.row0 + c0 + tid, i = g / a.group;
         row_at[tid] = ((it.q_start + static_cast<long long>(i)) * a.heads + it.h * a.group + (g - i * a.group)) * D;
-        const KeyRange r = tid < rows ? keys_of(i, it.q_len, it.len, a.causal, a.window) : KeyRange{0, 0};
+        const KeyRange r = tid < rows ? keys_of(i, it.past, it.len, a.causal, a.window) : KeyRange{0, 0};
         range[tid] = make_int2(r.lo, r.hi);
         ref[tid] = SOFTMAX ? -kNoMax : 1.f;
       }
@@ -302,7 +302,7 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
       for (int i = 0; i < C / 2; ++i) l[i] = 0ull;
       const int i0 = it.row0 / a.group, i1 = (it.row0 + it.rows - 1) / a.group;
-      const KeyRange r0 = keys_of(i0, it.q_len, it.len, a.causal, a.window), r1 = keys_of(i1, it.q_len, it.len, a.causal, a.window);
+      const KeyRange r0 = keys_of(i0, it.past, it.len, a.causal, a.window), r1 = keys_of(i1, it.past, it.len, a.causal, a.window);
       const int all_lo = max(r0.lo, r1.lo), all_hi = min(r0.hi, r1.hi);  // keys that every row takes part with (if any)
       PAGED_WAIT_ON(L::B_Q_FULL + q_buf, (q_pos >> 1) & 1u);
       ++q_pos;

@@ -24,7 +24,7 @@ __device__ __forceinline__ bool no_block(float v_scale) { return __float_as_uint
 struct PagedItem {
   int h;        // K / V head; -1 ends the walk, -2: a wait ran out
   int q_start;  // first query row of the request
-  int q_len;
+  int past;     // position of its first query
   int row0;     // first (query, head of the group) row of the tile
   int rows;
   int len;      // tokens of the request
@@ -46,9 +46,9 @@ __device__ __forceinline__ int count_arrival(int* counter) {
 struct KeyRange {
   int lo, hi;
 };
-// keys that query i takes part with; the queries are the last q_len positions of the request
-__device__ __forceinline__ KeyRange keys_of(int i, int q_len, int len, int causal, int window) {
-  const int p = len - q_len + i;
+// keys that query i takes part with; the first one's position is `past`
+__device__ __forceinline__ KeyRange keys_of(int i, int past, int len, int causal, int window) {
+  const int p = past + i;
   KeyRange r{0, len};
   if (causal) r.hi = min(r.hi, p + 1);
   if (window >= 0) r.lo = max(0, p - window), r.hi = min(r.hi, p + window + 1);
@@ -56,8 +56,8 @@ __device__ __forceinline__ KeyRange keys_of(int i, int q_len, int len, int causa
   return r;
 }
 // ... and any of queries i0 .. i1
-__device__ __forceinline__ KeyRange keys_of_any(int i0, int i1, int q_len, int len, int causal, int window) {
-  const int p0 = len - q_len + i0, p1 = len - q_len + i1;
+__device__ __forceinline__ KeyRange keys_of_any(int i0, int i1, int past, int len, int causal, int window) {
+  const int p0 = past + i0, p1 = past + i1;
   KeyRange r{0, len};
   if (causal) r.hi = min(r.hi, p1 + 1);
   if (window >= 0) r.lo = max(0, p0 - window), r.hi = min(r.hi, p1 + window + 1);
@@ -101,7 +101,9 @@ __device__ __forceinline__ bool drop_nans(uint4& u) {
 }
 
 struct Request {
-  int q_start, q_len, len;
+  int q_start, q_len;
+  int len;   // tokens that the table can hold, at most
+  int past;  // position of the first query: the queries are the request's last tokens, those that the table has no place for among them
 };
 __device__ __forceinline__ Request load_request(const PagedArgs& a, int b) {
   long long q0 = load_offset(a.q_off, b, a.off64), q1 = load_offset(a.q_off, b + 1, a.off64);
@@ -111,7 +113,9 @@ __device__ __forceinline__ Request load_request(const PagedArgs& a, int b) {
   Request r;
   r.q_start = static_cast<int>(q0);
   r.q_len = static_cast<int>(min(q1 - q0, static_cast<long long>(a.max_q)));
-  r.len = static_cast<int>(clamp_ll(load_offset(a.seq_lens, b, a.lens64), 0, most));
+  const long long len = clamp_ll(load_offset(a.seq_lens, b, a.lens64), 0, 1 << 30);
+  r.len = static_cast<int>(min(len, most));
+  r.past = static_cast<int>(len) - r.q_len;
   return r;
 }
 
@@ -130,7 +134,7 @@ __device__ __forceinline__ long long units_of(const PagedArgs& a, const Request&
   long long n = 0;
   for (int t = 0; t < nt; ++t) {
     const int last = min(rows, (t + 1) * NMAX);
-    n += units_of_item<L>(tiles_of(keys_of_any(t * NMAX / a.group, (last - 1) / a.group, r.q_len, r.len, a.causal, a.window)));
+    n += units_of_item<L>(tiles_of(keys_of_any(t * NMAX / a.group, (last - 1) / a.group, r.past, r.len, a.causal, a.window)));
   }
   return n;
 }
@@ -239,7 +243,7 @@ struct PagedCta {
   __device__ __forceinline__ bool publish(const PagedItem& it) {
     if (!wait(L::B_ITEM_EMPTY + item_pos % kItemSlots, ((item_pos / kItemSlots) & 1u) ^ 1u, ST_ROLE_LOAD)) return false;
     if (lane == 0) {
-      slot()[0] = make_int4(it.h, it.q_start, it.q_len, it.row0);
+      slot()[0] = make_int4(it.h, it.q_start, it.past, it.row0);
       slot()[1] = make_int4(it.rows, it.len, it.lo, it.hi);
       slot()[2] = make_int4(it.tile0, it.tiles, it.pieces, it.first);
       slot()[3].x = it.b;
@@ -308,7 +312,7 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
     // the walk: request, head and row tile that come next, units before them
     int wb = start->b - 1, wh = a.kv_heads, wt = 0, w_nt = 0, w_rows = 0;
     long long at = start->before;
-    Request rq{0, 0, 0};
+    Request rq{0, 0, 0, 0};
     // the next item of which this CTA has tiles, published; h = -1 at the end
     auto next_item = [&](PagedItem& it) -> bool {
       it = PagedItem{};
@@ -328,7 +332,7 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
         }
         const int row0 = wt * NMAX, rows = min(NMAX, w_rows - row0);
         ++wt;
-        const KeyRange r = keys_of_any(row0 / a.group, (row0 + rows - 1) / a.group, rq.q_len, rq.len, a.causal, a.window);
+        const KeyRange r = keys_of_any(row0 / a.group, (row0 + rows - 1) / a.group, rq.past, rq.len, a.causal, a.window);
         const int n = tiles_of(r), n1 = max(1, n);
         const long long s = at + L::kItemUnits;  // where the tiles' units begin
         at = s + n1;
@@ -339,7 +343,7 @@ __device__ __forceinline__ void paged_load(PagedCta<L>& cta, const PagedStart* s
         // the CTA that has unit u is the largest c with all * c / ctas <= u
         const int first = static_cast<int>(((s + 1) * ctas - 1) / all_units);
         const int pieces = static_cast<int>(((s + n1) * ctas - 1) / all_units) - first + 1;
-        it = PagedItem{wh, rq.q_start, rq.q_len, row0, rows, rq.len, r.lo, r.hi, r.lo / kTile + from, n == 0 ? 0 : to - from, pieces, first, wb};
+        it = PagedItem{wh, rq.q_start, rq.past, row0, rows, rq.len, r.lo, r.hi, r.lo / kTile + from, n == 0 ? 0 : to - from, pieces, first, wb};
         break;
       }
       return cta.publish(it);

@@ -231,8 +231,8 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         if (it.h == -2) goto role_done;
         break;
       }
-      const KeyRange r0 = keys_of(it.row0 / a.group, it.q_len, it.len, a.causal, a.window),
-                     r1 = keys_of((it.row0 + it.rows - 1) / a.group, it.q_len, it.len, a.causal, a.window);
+      const KeyRange r0 = keys_of(it.row0 / a.group, it.past, it.len, a.causal, a.window),
+                     r1 = keys_of((it.row0 + it.rows - 1) / a.group, it.past, it.len, a.causal, a.window);
       const int all_lo = max(r0.lo, r1.lo), all_hi = min(r0.hi, r1.hi);  // keys that every row takes part with (if any)
       for (int j = 0; j < it.tiles; ++j, ++pos) {
         const uint32_t stage = pos % L::kStages;
@@ -299,9 +299,9 @@ gdpa_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         continue;
       }
       const bool tile_live = qt * kTile < it.rows, warp_live = qt * kTile + quarter * 32 < it.rows;
-      const KeyRange rg = live ? keys_of(i, it.q_len, it.len, a.causal, a.window) : KeyRange{0, 0};
-      const KeyRange rf = keys_of(it.row0 / a.group, it.q_len, it.len, a.causal, a.window),
-                     rl = keys_of((it.row0 + it.rows - 1) / a.group, it.q_len, it.len, a.causal, a.window);
+      const KeyRange rg = live ? keys_of(i, it.past, it.len, a.causal, a.window) : KeyRange{0, 0};
+      const KeyRange rf = keys_of(it.row0 / a.group, it.past, it.len, a.causal, a.window),
+                     rl = keys_of((it.row0 + it.rows - 1) / a.group, it.past, it.len, a.causal, a.window);
       const int all_lo = max(rf.lo, rl.lo), all_hi = min(rf.hi, rl.hi);
       const float qa = __ldcg(a.qa + (static_cast<long long>(it.h) * a.total_q + it.q_start) * a.group + it.row0 + min(r, it.rows - 1));
       float ref = SOFTMAX ? kNoMax : 1.2676506e30f, l = 0.f;  // running maximum / multiplier; sum of P

@@ -177,8 +177,8 @@ def generalized_dot_product_attention_paged_fp8(
     The queries of request ``b`` are the rows ``query_offset[b]:query_offset[b + 1]`` of ``query`` (at most ``max_seq_len_q``), its keys the
     first ``seq_lens[b]`` tokens of its row of ``block_tables``.  Query ``i`` of ``n`` has position ``seq_lens[b] - n + i``: with ``is_causal`` it
     takes part with keys up to its position, with ``window_size`` with those at most that far from it.  Without either every query sees all
-    keys (candidates of a request that attend to its history).  A row without keys gives zeros.  Tokens past ``seq_lens[b]``, and blocks
-    that the table has not (-1), take no part, whatever their memory holds.  Scales are finite, V's not negative (a block whose scale is 0
+    keys (candidates of a request that attend to its history).  A row without keys gives zeros.  Tokens past ``seq_lens[b]``, those past
+    the table's width and those of blocks that the table has not (-1) take no part, whatever their memory holds.  Scales are finite, V's not negative (a block whose scale is 0
     holds zeros, and its tokens take part).  ``seq_lens`` and ``query_offset`` are
     trusted like the offsets of the other operators (clamped in the kernel, checked on the host with offset validation on).
     """

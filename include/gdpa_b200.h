@@ -448,7 +448,7 @@ typedef struct GdpaPagedParams {
   int32_t block_size;
   int64_t num_blocks;
   const void* q_offsets;       /* [batch + 1] */
-  const void* seq_lens;        /* [batch], clamped to table_width * block_size */
+  const void* seq_lens;        /* [batch]; tokens from table_width * block_size on have no place and take no part */
   int32_t offsets_are_int64;
   int32_t lens_are_int64;
   int32_t batch;

@@ -65,10 +65,11 @@ class Batch:
             if hi == lo or n == 0:
                 continue
             (k8, sk), (v8, sv) = (ref.gather(c, s, self.table[b], n) for c, s in ((self.k, self.ks), (self.v, self.vs)))
+            n = len(k8)  # no more than the table can hold; the queries are the last of all tokens
             k, v = (t.repeat_interleave(self.group, 1).transpose(0, 1) for t in (k8 * sk[..., None], v8 * sv[..., None]))
             sv = sv.repeat_interleave(self.group, 1).T[:, None]
             x = self.q[lo:hi].double().transpose(0, 1) @ k.transpose(1, 2)
-            p0, j = torch.arange(n - (hi - lo), n, device=x.device)[:, None], torch.arange(n, device=x.device)
+            p0, j = torch.arange(self.lens[b] - (hi - lo), self.lens[b], device=x.device)[:, None], torch.arange(n, device=x.device)
             off = torch.zeros(hi - lo, n, dtype=torch.bool, device=x.device)
             if causal:
                 off |= j > p0

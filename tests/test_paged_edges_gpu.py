@@ -355,3 +355,32 @@ def test_tables_of_lengths_that_are_nonsense(batch, length):
     assert bool((wide[:, 4:] == 77).all()) and wide[0, :4].tolist() == [99, 98, 97, 96]
     assert slots.tolist() == [(99 - i // 16) * 16 + i % 16 for i in range(40)]
     assert bool(((wide[:, :4] >= -1) & (wide[:, :4] < 100)).all())
+
+
+# ------------------------------------------------------------------------------------------ requests longer than their tables
+
+
+@pytest.mark.parametrize("queries,more", [(1, 1), (1, 300), (12, 5), (12, 12), (12, 400), (100, 30), (100, 700)])
+@pytest.mark.parametrize("causal,window", [(True, None), (True, 50), (False, 0), (False, 200), (False, None)])
+def test_attend_past_the_end_of_the_table(causal, window, queries, more):
+    # tokens without a place take no part; the queries keep their positions
+    for dim in (64, 128):
+        batch = Batch([320, 64, 192], [queries] * 3, 4, 2, dim, 32)
+        batch.lens[0] += more  # the table is as wide as the first needs
+        batch.check(0.1, causal=causal, window=window)
+        batch.check(1e-3, "silu", causal=causal, window=window)
+
+
+def test_a_cache_that_is_full_goes_on():
+    # the second step brings tokens that the first request has no place for
+    cache = G.PagedKVCache(20, 16, 2, 64, 2, 64)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    q, kv = torch.randn(70, 4, 64, device=DEV).bfloat16(), torch.randn(70, 2, 64, device=DEV).bfloat16()
+    cache.step(q, kv, kv, i32([60, 10]), 60)
+    o = cache.step(q[:12], kv[:12], kv[:12], i32([10, 2]), 10, qk_scale=0.1)
+    assert cache.seq_lens.tolist() == [70, 12] and G.kernel_status() == 0
+    seen = Batch([70], [10], 4, 2, 64, 16)
+    seen.q, seen.table, seen.k, seen.v, seen.ks, seen.vs = (q[:10], cache.block_tables[:1], cache.k_cache.view(torch.uint8), cache.v_cache.view(torch.uint8),
+                                                           cache.k_scales, cache.v_scales)
+    want, tol = seen.want(0.1, causal=True)
+    assert bool(((o[:10].double() - want).abs() <= tol).all())

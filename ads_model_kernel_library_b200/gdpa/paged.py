@@ -225,9 +225,11 @@ class PagedKVCache:
 
     def append(self, key: torch.Tensor, value: torch.Tensor, new_lens: torch.Tensor) -> torch.Tensor:
         """Store the keys and values of ``new_lens[b]`` (int32) new tokens of each request; returns their offsets ``[B + 1]``."""
-        slots, query_offset, self.seq_lens, self.num_free = build_block_tables(
+        slots, query_offset, seq_lens, num_free = build_block_tables(
             self.block_tables, self.seq_lens, new_lens, self.free_blocks, self.num_free, self.block_size, key.shape[0])
         append_kv_cache_fp8(key, value, self.k_cache, self.v_cache, self.k_scales, self.v_scales, slots)
+        # not before: keys or values that were refused are not in the cache (the blocks that the tables have for them count as free)
+        self.seq_lens, self.num_free = seq_lens, num_free
         return query_offset
 
     def attend(self, query: torch.Tensor, query_offset: torch.Tensor, max_seq_len_q: int, **options) -> torch.Tensor:

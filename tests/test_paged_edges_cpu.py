@@ -118,3 +118,16 @@ def test_what_the_check_of_slots_says(slots, good):
     else:
         with pytest.raises(ValueError):
             G.paged._check_slots(torch.tensor(slots, dtype=torch.int64), cache)
+
+
+def test_tokens_that_are_refused_are_not_counted(monkeypatch):
+    cache = held_cache()
+    monkeypatch.setattr(G.paged, "build_block_tables", lambda tables, cached, new, *args: (torch.zeros(3), torch.zeros(6), cached + new, torch.zeros(1)))
+    monkeypatch.setattr(G.paged, "append_kv_cache_fp8", lambda *args: (_ for _ in ()).throw(ValueError("refused")))
+    lens, left = cache.seq_lens.tolist(), int(cache.num_free)
+    with pytest.raises(ValueError, match="refused"):
+        cache.append(torch.zeros(3, 1, 64), torch.zeros(3, 1, 32), torch.tensor([1, 1, 1, 0, 0], dtype=torch.int32))
+    assert cache.seq_lens.tolist() == lens and int(cache.num_free) == left
+    monkeypatch.setattr(G.paged, "append_kv_cache_fp8", lambda *args: None)
+    cache.append(torch.zeros(3, 1, 64), torch.zeros(3, 1, 64), torch.tensor([1, 1, 1, 0, 0], dtype=torch.int32))
+    assert cache.seq_lens.tolist() == [14, 30, 46, 61, 0] and int(cache.num_free) == 0

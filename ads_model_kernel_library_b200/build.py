@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -22,6 +23,7 @@ CSRC = os.path.join(PKG, "csrc")
 OUT = os.path.join(PKG, "libgdpa_b200.so")
 TORCH_SRC = os.path.join(CSRC, "gdpa_torch.cpp")
 TORCH_OUT = os.path.join(PKG, "libgdpa_b200_torch.so")
+TORCH_STAMP = os.path.join(CSRC, "build", "gdpa_torch.stamp")  # which torch it was built for
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17", "--expt-relaxed-constexpr",
@@ -47,11 +49,21 @@ def _newest_header() -> float:
 
 
 def _build_torch_ops(force: bool, verbose: bool) -> None:
+    """The torch operators, for the torch that is installed: again when it is another one than at the last build.  Without torch or g++ they are left
+    out (the kernel library needs neither; the operators' first call says that they are missing)."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or shutil.which("g++") is None:
+        sys.stderr.write(f"{'torch' if spec is None else 'g++'} is not there: {os.path.basename(TORCH_OUT)} is not built\n")
+        return
+    torch = os.path.dirname(spec.origin)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    built_for = f"torch {importlib.metadata.version('torch')} in {torch}\n"
     header = os.path.join(os.path.dirname(PKG), "include", "gdpa_b200.h")
     if not force and os.path.exists(TORCH_OUT) and os.path.getmtime(TORCH_OUT) >= max(os.path.getmtime(TORCH_SRC), os.path.getmtime(header)):
-        return
-    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
-    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+        if os.path.exists(TORCH_STAMP):
+            with open(TORCH_STAMP) as f:
+                if f.read() == built_for:
+                    return
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-I{torch}/include", f"-I{cuda}/include", TORCH_SRC,
            "-o", TORCH_OUT, f"-L{torch}/lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -59,11 +71,13 @@ def _build_torch_ops(force: bool, verbose: bool) -> None:
         sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
     if r.returncode != 0:
         raise RuntimeError("g++ failed; see output above")
+    os.makedirs(os.path.dirname(TORCH_STAMP), exist_ok=True)
+    with open(TORCH_STAMP, "w") as f:
+        f.write(built_for)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
     nvcc = _nvcc()
-    _build_torch_ops(force, verbose)
     objdir = os.path.join(CSRC, "build")
     os.makedirs(objdir, exist_ok=True)
     hdr_time = _newest_header()
@@ -96,6 +110,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link of libgdpa_b200.so failed")
+    _build_torch_ops(force, verbose)
     return OUT
 
 

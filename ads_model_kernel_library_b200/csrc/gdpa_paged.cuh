@@ -168,28 +168,6 @@ __device__ __forceinline__ void act_any(int act, float (&x)[N], float m) {
   }
 }
 
-// Sixteen values -> the sum of two e4m3 values each, hi = e4m3(x) and lo = e4m3(x - hi), packed four to a register.  Stage after stage over
-// all of them, in an order that the volatile statements keep, so that the chains of conversions run beside one another.
-__device__ __forceinline__ void split_e4m3(const float (&x)[16], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-  uint32_t u[8], v[8];
-  uint16_t h[8], l[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) asm volatile("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h[i]) : "r"(u[i]));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) asm volatile("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(v[i]) : "h"(h[i]));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) asm volatile("sub.f16x2 %0, %0, %1;" : "+r"(u[i]) : "r"(v[i]));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) asm volatile("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l[i]) : "r"(u[i]));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    hi[i] = __byte_perm(h[2 * i], h[2 * i + 1], 0x5410);
-    lo[i] = __byte_perm(l[2 * i], l[2 * i + 1], 0x5410);
-  }
-}
-
 // Where a CTA's walk over the items begins.
 struct PagedStart {
   long long all, before;  // all units; units before request b

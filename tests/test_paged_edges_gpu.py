@@ -384,3 +384,40 @@ def test_a_cache_that_is_full_goes_on():
                                                            cache.k_scales, cache.v_scales)
     want, tol = seen.want(0.1, causal=True)
     assert bool(((o[:10].double() - want).abs() <= tol).all())
+
+
+# ------------------------------------------------------------------------------------------ traced
+
+
+def test_the_append_traces():
+    f8 = torch.float8_e4m3fn
+    cache = [torch.zeros(2, 16, 2, 64, dtype=torch.uint8, device=DEV).view(f8) for _ in range(2)] + [torch.ones(2, 2, device=DEV) for _ in range(2)]
+    kv = torch.randn(5, 2, 64, device=DEV).bfloat16()
+    torch.library.opcheck(torch.ops.gdpa.append_kv_cache_fp8.default, (kv, kv, *cache, torch.arange(5, device=DEV)), test_utils=("test_faketensor",))
+
+
+def test_a_compiled_step_is_the_step():
+    f8 = torch.float8_e4m3fn
+
+    def step(q, k, v, k8, v8, ks, vs, table, cached, new, free, num_free):
+        slots, offsets, lens, left = G.build_block_tables(table, cached, new, free, num_free, 16, q.shape[0])
+        G.append_kv_cache_fp8(k * 2, v + 1, k8, v8, ks, vs, slots)
+        return G.generalized_dot_product_attention_paged_fp8(q, k8, v8, ks, vs, table, offsets, lens, 30, qk_scale=0.1, is_causal=True) * 3, lens, left
+
+    def state():
+        cache = [torch.zeros(12, 16, 2, 64, dtype=torch.uint8, device=DEV).view(f8) for _ in range(2)] + [torch.ones(12, 2, device=DEV) for _ in range(2)]
+        return [*cache, torch.full((3, 8), -1, dtype=torch.int32, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV),
+                torch.arange(12, dtype=torch.int32, device=DEV), torch.tensor([12], dtype=torch.int32, device=DEV)]
+
+    compiled = torch.compile(step, backend="aot_eager", fullgraph=True)
+    mine, theirs = state(), state()
+    for new in ([20, 3, 30], [1, 1, 1], [0, 2, 1]):
+        q, k, v = (torch.randn(sum(new), h, 64, device=DEV).bfloat16() for h in (4, 2, 2))
+        new = torch.tensor(new, dtype=torch.int32, device=DEV)
+        results = []
+        for f, s in ((step, mine), (compiled, theirs)):
+            o, s[5], s[7] = f(q, k, v, *s[:5], s[5], new, s[6], s[7])
+            results.append(o)
+        assert torch.equal(*results)
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(mine, theirs))
+    assert G.kernel_status() == 0

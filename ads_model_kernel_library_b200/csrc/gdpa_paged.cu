@@ -32,7 +32,7 @@
 // CTA that finishes it last (an atomic count per item) joins them in the order of the pieces, so the result does not depend on who
 // was last.  No CTA waits for another.
 //
-// Measured (one B200, us a pass of both kernels, calls back to back): 256 requests of up to 4096 tokens, a query each, 32 heads on 4: 116 (4.8 TB/s
+// Measured (one B200, us a pass of both kernels, calls back to back): 256 requests of up to 4096 tokens, a query each, 32 heads on 4: 117 (4.8 TB/s
 // of cache); six of 32768 to 262144 tokens 81 (5.0 TB/s); one of 1500 tokens 14.3, most of it the host; up to four draft queries of 96 requests,
 // head_dim 64, window 1024: 50, a chain of latencies per item.
 //
@@ -388,9 +388,14 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             for (int i = 0; i < C; i += 2) most = SOFTMAX ? max3(most, p[i], p[i + 1]) : max3(most, fabsf(p[i]), fabsf(p[i + 1]));
             return most * m <= kMax8;
           };
-          bool fits = true;
-          if (!first) fits = compute();
-          if (first || named_bar_or(bar_wg, 128, !fits)) {
+          // With head_dim 64 the code of compute is there once, with 128 twice: three CTAs an SM are short of instructions, two wait for the
+          // cache (draft_window 49.5 us and 52, decode_ragged 118 and 114.5).
+#pragma unroll 1
+          for (bool moved = false, next = !first;; next = moved = true) {
+            if (next) {
+              const bool fits = compute();
+              if (moved || !named_bar_or(bar_wg, 128, !fits)) break;
+            }
             // the exact reference of every column, and O and the row sums moved to it
             scores(false);
             if constexpr (SOFTMAX) {
@@ -461,7 +466,10 @@ gdpa_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
               }
               tmem_wait_st();
             }
-            compute();
+            if constexpr (D == 128) {
+              compute();
+              break;
+            }
           }
           // P, times V's scale, as the sum of three e4m3 values (see the top of this file)
           uint32_t w[3][C / 4], h[C / 2];

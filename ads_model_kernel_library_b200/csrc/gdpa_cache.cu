@@ -28,7 +28,7 @@ constexpr unsigned kFull = 0xffffffffu;
 //
 // Latency is all of it: three trips to memory one after the other (lengths, free blocks, slots) between a launch and its end.  PER is the
 // number of requests a thread has in one round, in registers; the small form (64 requests: 4.9 -> 4.0 us) has neither the
-// unrolled code nor the threads of the large one.  Alone: 64 requests with a token each 4.0 us, 512 new ones (1.2 M tokens) 11.6, 8192 9.5.
+// unrolled code nor the threads of the large one.  Alone: 64 requests with a token each 4.0 us, 512 new ones (1.2 M tokens) 11.4, 8192 9.2.
 __device__ __forceinline__ int clamp_len(const void* p, int b, int flags) {
   return static_cast<int>(clamp_ll(load_offset(p, b, flags), 0, 0x3fffff00));  // two of them and a block fit in an int
 }

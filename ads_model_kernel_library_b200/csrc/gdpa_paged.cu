@@ -33,7 +33,7 @@
 // was last.  No CTA waits for another.
 //
 // Measured (one B200, us a pass of both kernels, calls back to back): 256 requests of up to 4096 tokens, a query each, 32 heads on 4: 117 (4.8 TB/s
-// of cache); six of 32768 to 262144 tokens 81 (5.0 TB/s); one of 1500 tokens 14.3, most of it the host; up to four draft queries of 96 requests,
+// of cache); six of 32768 to 262144 tokens 81 (5.0 TB/s); one of 1500 tokens 14.3, a chain of trips to memory; up to four draft queries of 96 requests,
 // head_dim 64, window 1024: 50, a chain of latencies per item.
 //
 // Roles: kGroups warpgroups (element-wise work, epilogue), one warp of TMA loads, one warp that issues MMAs.  A small kernel before this one

@@ -17,16 +17,16 @@
 // whole test.  Then, for the first tokens of a stretch and where a mask leaves tokens out, the scores, which are still there, are gone through
 // again: once for the sum and maximum under the masks, once for P.  Both forms do the same arithmetic, so no row's bits depend on its neighbours.
 //
-// Measured (one B200, caches cold): causal chunks of 256 to 1024 queries 396 us, candidates (64 to 1024, SiLU) 629 us; the transposed form with
+// Measured (one B200, caches cold): causal chunks of 256 to 1024 queries 373 us, candidates (64 to 1024, SiLU) 655 us; the transposed form with
 // 128 rows 757 and 917, this form with P in two e4m3 values 478 and 815.  128 tokens against 256 rows take 2.4 to 2.5 us whatever the
 // activation, against 128 rows 1.85 (2.2 with one place for V as it comes from the cache: its next tile then waited for the conversion).
-// No pipe is near its end (tensor 23 %, ALU 28 %, issue 39 % on chunks); what bounds it is the way of 64 tokens from the products with Q to
+// No pipe is near its end (exponentials 30 %, tensor 25 %, ALU 25 %, issue 39 % on chunks); what bounds it is the way of 64 tokens from the products with Q to
 // those with V and back, with two warps on a scheduler.  No faster (against 427, 724 then): an MMA warp for each row tile (429, 743); a row tile's two halves one
 // after the other (433, 735); scores of 128 tokens at once (438, 730); the row tiles' warps taking strict turns (507, 967); 16 element-wise
 // warps, half a row each, with two converting V, who are then late (600, 1110).
 //
 // Roles: warps 0-3 and 4-7 the element-wise work and epilogue of row tiles 0 and 1, warp 8 TMA loads and the walk, warp 9 MMAs, warps 10-13
-// V to float16, with zeros for tokens that no query may see (0 times NaN is NaN).
+// V to float16, with zeros for tokens that no query may see (0 times NaN is NaN), and for NaNs where some see the token and some do not.
 #include <cuda_bf16.h>
 
 #include "gdpa_paged.cuh"

@@ -21,7 +21,7 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 OUT = os.path.join(PKG, "libgdpa_b200.so")
-TORCH_SRC = os.path.join(CSRC, "gdpa_torch.cpp")
+TORCH_SRCS = [os.path.join(CSRC, f) for f in ("gdpa_torch.cpp", "gdpa_torch_heads.cpp")]
 TORCH_OUT = os.path.join(PKG, "libgdpa_b200_torch.so")
 TORCH_STAMP = os.path.join(CSRC, "build", "gdpa_torch.stamp")  # which torch it was built for
 NVCC_FLAGS = [
@@ -58,13 +58,14 @@ def _build_torch_ops(force: bool, verbose: bool) -> None:
     torch = os.path.dirname(spec.origin)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
     built_for = f"torch {importlib.metadata.version('torch')} in {torch}\n"
-    header = os.path.join(os.path.dirname(PKG), "include", "gdpa_b200.h")
-    if not force and os.path.exists(TORCH_OUT) and os.path.getmtime(TORCH_OUT) >= max(os.path.getmtime(TORCH_SRC), os.path.getmtime(header)):
+    read = [*TORCH_SRCS, os.path.join(CSRC, "gdpa_torch.h"), os.path.join(os.path.dirname(PKG), "include", "gdpa_b200.h")]
+    if not force and os.path.exists(TORCH_OUT) and os.path.getmtime(TORCH_OUT) >= max(os.path.getmtime(f) for f in read):
         if os.path.exists(TORCH_STAMP):
             with open(TORCH_STAMP) as f:
                 if f.read() == built_for:
                     return
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-I{torch}/include", f"-I{cuda}/include", TORCH_SRC,
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-I{torch}/include", f"-I{torch}/include/torch/csrc/api/include",
+           f"-I{cuda}/include", *TORCH_SRCS,
            "-o", TORCH_OUT, f"-L{torch}/lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or r.returncode != 0:

@@ -541,13 +541,13 @@ int gdpa_build_block_tables(const GdpaBlockTableParams* p, gdpa_stream_t stream)
   return rc;
 }
 
-int gdpa_append_kv_cache_fp8(const GdpaCacheAppendParams* p, gdpa_stream_t stream) {
-  if (p == nullptr || p->struct_size != sizeof(GdpaCacheAppendParams)) return GDPA_ERR_BAD_ARG;
+namespace {
+// The checks of an append, and what its kernel is given; `rows` false: nothing to do.
+int cache_append_args(const GdpaCacheAppendParams* p, CacheAppendArgs& a, bool& rows) {
   const int shift = block_shift_of(p->block_size);
   if (shift < 0 || p->tokens < 0 || p->num_blocks < 0 || p->kv_heads <= 0) return GDPA_ERR_BAD_ARG;
   if (p->head_dim != 64 && p->head_dim != 128) return GDPA_ERR_UNSUPPORTED_DIM;
   if (p->tokens > 32ll * 0x7fffffffll || p->kv_heads > (1 << 20)) return GDPA_ERR_BAD_ARG;
-  CacheAppendArgs a;
   std::memset(&a, 0, sizeof(a));
   const int elem = p->x_is_fp32 != 0 ? 4 : 2;
   int rc;
@@ -555,13 +555,15 @@ int gdpa_append_kv_cache_fp8(const GdpaCacheAppendParams* p, gdpa_stream_t strea
   if ((rc = row_strides(p->value_strides, p->kv_heads, p->head_dim, elem, a.value_strides)) != GDPA_OK) return rc;
   if ((rc = cache_strides(p->k_cache_strides, p->block_size, p->kv_heads, p->head_dim, a.k_cache_strides)) != GDPA_OK) return rc;
   if ((rc = cache_strides(p->v_cache_strides, p->block_size, p->kv_heads, p->head_dim, a.v_cache_strides)) != GDPA_OK) return rc;
-  if (p->tokens == 0 || p->num_blocks == 0) return GDPA_OK;
+  rows = p->tokens > 0 && p->num_blocks > 0;
+  a.tokens = p->tokens;
+  a.heads = p->kv_heads;
+  a.block_shift = shift;
+  if (!rows) return GDPA_OK;
   if (p->key == nullptr || p->value == nullptr || p->k_cache == nullptr || p->v_cache == nullptr || p->k_scales == nullptr ||
       p->v_scales == nullptr || p->slot_mapping == nullptr)
     return GDPA_ERR_BAD_ARG;
   if (!aligned16(p->key, p->value) || !aligned16(p->k_cache, p->v_cache)) return GDPA_ERR_MISALIGNED;
-  DeviceInfo di;
-  if ((rc = device_info(&di)) != GDPA_OK) return rc;
   a.key = p->key;
   a.value = p->value;
   a.k_cache = static_cast<uint8_t*>(p->k_cache);
@@ -569,10 +571,19 @@ int gdpa_append_kv_cache_fp8(const GdpaCacheAppendParams* p, gdpa_stream_t strea
   a.k_scales = p->k_scales;
   a.v_scales = p->v_scales;
   a.slot_mapping = reinterpret_cast<const long long*>(p->slot_mapping);
-  a.tokens = p->tokens;
   a.num_blocks = p->num_blocks;
-  a.block_shift = shift;
-  a.heads = p->kv_heads;
+  return GDPA_OK;
+}
+}  // namespace
+
+int gdpa_append_kv_cache_fp8(const GdpaCacheAppendParams* p, gdpa_stream_t stream) {
+  if (p == nullptr || p->struct_size != sizeof(GdpaCacheAppendParams)) return GDPA_ERR_BAD_ARG;
+  CacheAppendArgs a;
+  bool rows = false;
+  int rc = cache_append_args(p, a, rows);
+  if (rc != GDPA_OK || !rows) return rc;
+  DeviceInfo di;
+  if ((rc = device_info(&di)) != GDPA_OK) return rc;
   rc = launch_cache_append(a, p->head_dim, p->x_is_fp32 != 0, di.sm_count, static_cast<cudaStream_t>(stream));
   if (rc == 0) g_launches.fetch_add(1);
   return rc;
@@ -658,6 +669,242 @@ int gdpa_fwd_paged_fp8(const GdpaPagedParams* p, gdpa_stream_t stream) {
   rc = launch_paged(l, p->head_dim);
   if (p->timing_stop_event != nullptr) cudaEventRecord(static_cast<cudaEvent_t>(p->timing_stop_event), l.stream);
   if (rc == 0) g_launches.fetch_add(2);
+  return rc;
+}
+
+namespace {
+int rotary_spec(const GdpaRotarySpec& p, int head_dim, RotarySpec& r) {
+  std::memset(&r, 0, sizeof(r));
+  if (p.pairs < 0 || p.pairs % 8 != 0 || p.pairs > head_dim / 2 || p.axes < 1 || p.axes > kMaxAxes) return GDPA_ERR_BAD_ARG;
+  if (p.pairs > 0 && p.inv_freq == nullptr) return GDPA_ERR_BAD_ARG;
+  if (p.norm != 0 && !(p.eps >= 0.f && p.eps < 3.0e38f)) return GDPA_ERR_BAD_ARG;
+  for (int i = 0; i < p.axes && p.axes > 1; ++i) {
+    if (p.section_ends[i] < (i > 0 ? p.section_ends[i - 1] : 0)) return GDPA_ERR_BAD_ARG;
+    r.ends[i] = p.section_ends[i];
+  }
+  if (p.axes > 1 && p.section_ends[p.axes - 1] != p.pairs) return GDPA_ERR_BAD_ARG;
+  r.inv_freq = p.inv_freq;
+  r.inv_freq_is_fp64 = p.inv_freq_is_fp64 != 0;
+  r.pairs = p.pairs;
+  r.interleaved = p.interleaved != 0;
+  r.axes = p.axes;
+  r.norm = p.norm != 0;
+  r.eps = p.eps;
+  return GDPA_OK;
+}
+
+int rotary_tensor(const GdpaRotaryTensor& p, const RotarySpec& r, int head_dim, int elem, bool backward, RotaryTensor& t) {
+  if (p.tokens < 0 || p.tokens >= (1ll << 30) || p.heads < 0 || p.heads > (1 << 20) || p.position_stride < 0) return GDPA_ERR_BAD_ARG;
+  int rc;
+  if ((rc = row_strides(p.x_strides, p.heads, head_dim, elem, t.x_strides)) != GDPA_OK) return rc;
+  if (backward && (rc = row_strides(p.dy_strides, p.heads, head_dim, elem, t.dy_strides)) != GDPA_OK) return rc;
+  t.heads = p.heads;
+  t.tokens = p.heads > 0 ? p.tokens : 0;
+  t.dweight = backward && r.norm ? p.dweight : nullptr;
+  t.weight_is_bf16 = p.weight_is_bf16 != 0;
+  if (t.tokens == 0) return GDPA_OK;
+  const bool reads_x = !backward || r.norm;
+  if ((reads_x && p.x == nullptr) || p.y == nullptr || (backward && p.dy == nullptr) || (r.pairs > 0 && p.positions == nullptr)) return GDPA_ERR_BAD_ARG;
+  if (!aligned16(reads_x ? p.x : nullptr, p.y) || !aligned16(backward ? p.dy : nullptr, nullptr)) return GDPA_ERR_MISALIGNED;
+  t.x = p.x;
+  t.y = p.y;
+  t.dy = p.dy;
+  t.weight = r.norm ? p.weight : nullptr;
+  t.positions = p.positions;
+  t.position_stride = p.position_stride;
+  t.positions_are_int64 = p.positions_are_int64 != 0;
+  return GDPA_OK;
+}
+
+int run_rotary(const GdpaRotaryParams* p, bool backward, gdpa_stream_t stream) {
+  if (p == nullptr || p->struct_size != sizeof(GdpaRotaryParams)) return GDPA_ERR_BAD_ARG;
+  if (p->head_dim != 64 && p->head_dim != 128) return GDPA_ERR_UNSUPPORTED_DIM;
+  RotaryArgs a;
+  std::memset(&a, 0, sizeof(a));
+  const int elem = p->is_fp32 != 0 ? 4 : 2;
+  int rc;
+  if ((rc = rotary_spec(p->rotary, p->head_dim, a.rotary)) != GDPA_OK) return rc;
+  if ((rc = rotary_tensor(p->query, a.rotary, p->head_dim, elem, backward, a.t[0])) != GDPA_OK) return rc;
+  if ((rc = rotary_tensor(p->key, a.rotary, p->head_dim, elem, backward, a.t[1])) != GDPA_OK) return rc;
+  const bool sums = a.t[0].dweight != nullptr || a.t[1].dweight != nullptr;
+  if (a.t[0].tokens == 0 && a.t[1].tokens == 0 && !sums) return GDPA_OK;
+  if (sums && p->workspace == nullptr) return GDPA_ERR_BAD_ARG;
+  if (sums && !aligned16(p->workspace, nullptr)) return GDPA_ERR_MISALIGNED;
+  DeviceInfo di;
+  if ((rc = device_info(&di)) != GDPA_OK) return rc;
+  if (!backward) {
+    rc = launch_rotary(a, p->head_dim, p->is_fp32 != 0, di.sm_count, static_cast<cudaStream_t>(stream));
+    if (rc == 0) g_launches.fetch_add(1);
+    return rc;
+  }
+  if (sums) {
+    if (p->workspace_bytes < static_cast<int64_t>(gdpa_rotary_workspace_bytes(p->head_dim))) return GDPA_ERR_CAPACITY;
+    a.partial = static_cast<float*>(p->workspace);
+  }
+  rc = launch_rotary_bwd(a, p->head_dim, p->is_fp32 != 0, di.sm_count, static_cast<cudaStream_t>(stream));
+  if (rc < 0) return -rc;
+  g_launches.fetch_add(rc);
+  return GDPA_OK;
+}
+}  // namespace
+
+size_t gdpa_rotary_workspace_bytes(int32_t head_dim) {
+  DeviceInfo di;
+  if (head_dim <= 0 || device_info(&di) != GDPA_OK) return 0;
+  return static_cast<size_t>(rotary_bwd_ctas(di.sm_count)) * 2 * head_dim * sizeof(float);
+}
+
+int gdpa_qk_norm_rotary(const GdpaRotaryParams* p, gdpa_stream_t stream) { return run_rotary(p, false, stream); }
+int gdpa_qk_norm_rotary_bwd(const GdpaRotaryParams* p, gdpa_stream_t stream) { return run_rotary(p, true, stream); }
+
+int gdpa_append_rotated_kv_cache_fp8(const GdpaRotatedAppendParams* p, gdpa_stream_t stream) {
+  if (p == nullptr || p->struct_size != sizeof(GdpaRotatedAppendParams) || p->cache.struct_size != sizeof(GdpaCacheAppendParams)) return GDPA_ERR_BAD_ARG;
+  RotatedAppendArgs a;
+  std::memset(&a, 0, sizeof(a));
+  bool rows = false;
+  int rc = cache_append_args(&p->cache, a.cache, rows);
+  if (rc != GDPA_OK) return rc;
+  if ((rc = rotary_spec(p->rotary, p->cache.head_dim, a.rotary)) != GDPA_OK) return rc;
+  const int elem = p->cache.x_is_fp32 != 0 ? 4 : 2;
+  if (p->heads <= 0 || p->heads > (1 << 20) || p->cache.tokens >= (1ll << 30) || p->batch < 0 || p->position_stride < 0) return GDPA_ERR_BAD_ARG;
+  if ((rc = row_strides(p->query_strides, p->heads, p->cache.head_dim, elem, a.query_strides)) != GDPA_OK) return rc;
+  if (p->cache.tokens == 0) return GDPA_OK;
+  if (p->query == nullptr || p->query_out == nullptr) return GDPA_ERR_BAD_ARG;
+  if (p->positions == nullptr && p->batch > 0 && (p->q_offsets == nullptr || p->seq_lens == nullptr)) return GDPA_ERR_BAD_ARG;
+  if (!aligned16(p->query, p->query_out)) return GDPA_ERR_MISALIGNED;
+  DeviceInfo di;
+  if ((rc = device_info(&di)) != GDPA_OK) return rc;
+  a.query = p->query;
+  a.query_out = p->query_out;
+  a.heads = p->heads;
+  a.query_weight = a.rotary.norm ? p->query_weight : nullptr;
+  a.key_weight = a.rotary.norm ? p->key_weight : nullptr;
+  a.query_weight_is_bf16 = p->query_weight_is_bf16 != 0;
+  a.key_weight_is_bf16 = p->key_weight_is_bf16 != 0;
+  a.positions = p->positions;
+  a.position_stride = p->position_stride;
+  a.positions_are_int64 = p->positions_are_int64 != 0;
+  a.q_off = p->q_offsets;
+  a.seq_lens = p->seq_lens;
+  a.off64 = p->offsets_are_int64 != 0 ? kOffsets64 : 0;
+  a.lens64 = p->lens_are_int64 != 0 ? kOffsets64 : 0;
+  a.batch = p->batch;
+  rc = launch_rotated_append(a, p->cache.head_dim, p->cache.x_is_fp32 != 0, di.sm_count, static_cast<cudaStream_t>(stream));
+  if (rc == 0) g_launches.fetch_add(1);
+  return rc;
+}
+
+int gdpa_read_kv_cache_fp8(const GdpaCacheReadParams* p, gdpa_stream_t stream) {
+  if (p == nullptr || p->struct_size != sizeof(GdpaCacheReadParams)) return GDPA_ERR_BAD_ARG;
+  if (p->head_dim != 64 && p->head_dim != 128) return GDPA_ERR_UNSUPPORTED_DIM;
+  const int shift = block_shift_of(p->block_size);
+  if (shift < 0 || p->batch < 0 || p->kv_heads <= 0 || p->kv_heads > (1 << 16) || p->total < 0 || p->total >= (1ll << 36)) return GDPA_ERR_BAD_ARG;
+  if (p->table_width < 0 || p->table_stride < 0 || p->num_blocks < 0 || p->num_blocks > 0x7fffffffll) return GDPA_ERR_BAD_ARG;
+  if ((static_cast<long long>(p->table_width) << shift) > (1ll << 30)) return GDPA_ERR_BAD_ARG;
+  CacheReadArgs a;
+  std::memset(&a, 0, sizeof(a));
+  int rc;
+  if ((rc = cache_strides(p->k_cache_strides, p->block_size, p->kv_heads, p->head_dim, a.k_cache_strides)) != GDPA_OK) return rc;
+  if ((rc = cache_strides(p->v_cache_strides, p->block_size, p->kv_heads, p->head_dim, a.v_cache_strides)) != GDPA_OK) return rc;
+  if (p->total == 0) return GDPA_OK;
+  if (p->key == nullptr || p->value == nullptr) return GDPA_ERR_BAD_ARG;
+  if (p->batch > 0 && (p->offsets == nullptr || (p->table_width > 0 && p->block_tables == nullptr))) return GDPA_ERR_BAD_ARG;
+  if (p->num_blocks > 0 && (p->k_cache == nullptr || p->v_cache == nullptr || p->k_scales == nullptr || p->v_scales == nullptr)) return GDPA_ERR_BAD_ARG;
+  if (!aligned16(p->k_cache, p->v_cache) || !aligned16(p->key, p->value)) return GDPA_ERR_MISALIGNED;
+  DeviceInfo di;
+  if ((rc = device_info(&di)) != GDPA_OK) return rc;
+  a.k_cache = static_cast<const uint8_t*>(p->k_cache);
+  a.v_cache = static_cast<const uint8_t*>(p->v_cache);
+  a.k_scales = p->k_scales;
+  a.v_scales = p->v_scales;
+  a.block_tables = p->block_tables;
+  a.table_stride = p->table_stride;
+  a.table_width = p->table_width;
+  a.block_shift = shift;
+  a.num_blocks = p->num_blocks;
+  a.offsets = p->offsets;
+  a.first = p->first;
+  a.off64 = p->offsets_are_int64 != 0 ? kOffsets64 : 0;
+  a.first64 = p->first_is_int64 != 0 ? kOffsets64 : 0;
+  a.batch = p->batch;
+  a.heads = p->kv_heads;
+  a.total = p->total;
+  a.key = p->key;
+  a.value = p->value;
+  rc = launch_cache_read(a, p->head_dim, p->out_is_fp32 != 0, di.sm_count, static_cast<cudaStream_t>(stream));
+  if (rc == 0) g_launches.fetch_add(1);
+  return rc;
+}
+
+int gdpa_verify_draft_tokens(const GdpaVerifyParams* p, gdpa_stream_t stream) {
+  if (p == nullptr || p->struct_size != sizeof(GdpaVerifyParams)) return GDPA_ERR_BAD_ARG;
+  if (p->rows < 0 || p->drafts < 0 || p->vocab < 1 || p->vocab > verify_most_vocab() || p->batch < 0 || p->batch > (1 << 27)) return GDPA_ERR_BAD_ARG;
+  if (p->max_drafts < 0 || p->max_drafts > (1 << 20) || p->target_stride < 0 || p->draft_stride < 0) return GDPA_ERR_BAD_ARG;
+  if (p->batch == 0) return GDPA_OK;
+  if (p->row_offsets == nullptr || p->draft_offsets == nullptr || p->sample == nullptr || p->out_tokens == nullptr || p->accepted == nullptr ||
+      p->refused == nullptr)
+    return GDPA_ERR_BAD_ARG;
+  if (p->rows > 0 && p->target == nullptr) return GDPA_ERR_BAD_ARG;
+  if (p->drafts > 0 && (p->tokens == nullptr || p->accept == nullptr)) return GDPA_ERR_BAD_ARG;
+  DeviceInfo di;
+  int rc = device_info(&di);
+  if (rc != GDPA_OK) return rc;
+  VerifyArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.target = p->target;
+  a.draft = p->draft;
+  a.target_stride = p->target_stride;
+  a.draft_stride = p->draft_stride;
+  a.rows = p->rows;
+  a.drafts = p->drafts;
+  a.vocab = p->vocab;
+  a.tokens = p->tokens;
+  a.tokens64 = p->tokens_are_int64 != 0;
+  a.row_offsets = p->row_offsets;
+  a.draft_offsets = p->draft_offsets;
+  a.off64 = p->offsets_are_int64 != 0 ? kOffsets64 : 0;
+  a.accept = p->accept;
+  a.sample = p->sample;
+  a.batch = p->batch;
+  a.max_drafts = p->max_drafts;
+  a.out_tokens = p->out_tokens;
+  a.accepted = p->accepted;
+  a.refused = p->refused;
+  rc = launch_verify(a, p->is_bf16 != 0, di.sm_count, static_cast<cudaStream_t>(stream));
+  if (rc == 0) g_launches.fetch_add(1);
+  return rc;
+}
+
+int gdpa_drop_cached_tokens(const GdpaDropParams* p, gdpa_stream_t stream) {
+  if (p == nullptr || p->struct_size != sizeof(GdpaDropParams)) return GDPA_ERR_BAD_ARG;
+  const int shift = block_shift_of(p->block_size);
+  if (shift < 0 || p->batch < 0 || p->batch > 0x7ffffff0 || p->table_width < 0 || p->table_stride < 0 || p->free_capacity < 0) return GDPA_ERR_BAD_ARG;
+  if ((static_cast<long long>(p->table_width) << shift) > (1ll << 30)) return GDPA_ERR_BAD_ARG;
+  if (p->num_free == nullptr || p->num_free_after == nullptr || p->num_free == p->num_free_after) return GDPA_ERR_BAD_ARG;
+  if (p->batch > 0 && (p->seq_lens == nullptr || p->dropped == nullptr || p->seq_lens_after == nullptr)) return GDPA_ERR_BAD_ARG;
+  if (p->batch > 0 && p->table_width > 0 && p->block_tables == nullptr) return GDPA_ERR_BAD_ARG;
+  if (p->free_capacity > 0 && p->free_blocks == nullptr) return GDPA_ERR_BAD_ARG;
+  DeviceInfo di;
+  int rc = device_info(&di);
+  if (rc != GDPA_OK) return rc;
+  DropArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.block_tables = p->block_tables;
+  a.table_stride = p->table_stride;
+  a.table_width = p->table_width;
+  a.block_shift = shift;
+  a.seq_lens = p->seq_lens;
+  a.dropped = p->dropped;
+  a.lens64 = p->lens_are_int64 != 0 ? kOffsets64 : 0;
+  a.dropped64 = p->dropped_is_int64 != 0 ? kOffsets64 : 0;
+  a.batch = p->batch;
+  a.free_blocks = p->free_blocks;
+  a.free_capacity = p->free_capacity;
+  a.num_free = p->num_free;
+  a.seq_lens_after = p->seq_lens_after;
+  a.num_free_after = p->num_free_after;
+  rc = launch_drop(a, static_cast<cudaStream_t>(stream));
+  if (rc == 0) g_launches.fetch_add(1);
   return rc;
 }
 

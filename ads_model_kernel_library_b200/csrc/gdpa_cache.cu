@@ -12,6 +12,7 @@
 
 #include "gdpa_common.cuh"
 #include "gdpa_launch.h"
+#include "gdpa_pieces.cuh"
 
 namespace gdpa {
 
@@ -199,49 +200,6 @@ __global__ void __launch_bounds__(kTableThreads) gdpa_block_tables_kernel(const 
 // their runs with a vote; a window's triples are dealt out to gridDim.y CTAs.  Measured: 128 histories of 512 to 4096 tokens, 8 heads of 128
 // values, 318 us (5.8 TB/s; a warp to a run 577), one token for 256 requests 4.1, 300 ragged runs of fp32 7.0.
 constexpr int kAppendWarps = 4;
-
-template <class T>
-struct Piece;  // 16 bytes of a row
-template <>
-struct Piece<__nv_bfloat16> {
-  static constexpr int kElems = 8;
-  static __device__ __forceinline__ void unpack(const uint4& u, float (&v)[8]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-  // the largest magnitude's bits, in two halves / whole, as long as it goes on; then as bits of fp32
-  static __device__ __forceinline__ uint32_t magnitude(uint32_t top, const uint4& u) {
-    top = max_u16x2(max_u16x2(top, u.x & 0x7fff7fffu), u.y & 0x7fff7fffu);
-    return max_u16x2(max_u16x2(top, u.z & 0x7fff7fffu), u.w & 0x7fff7fffu);
-  }
-  static __device__ __forceinline__ uint32_t whole(uint32_t top) { return max(top & 0xffffu, top >> 16) << 16; }
-};
-template <>
-struct Piece<float> {
-  static constexpr int kElems = 4;
-  static __device__ __forceinline__ void unpack(const uint4& u, float (&v)[4]) {
-    v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y), v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
-  }
-  static __device__ __forceinline__ uint32_t magnitude(uint32_t top, const uint4& u) {
-    top = max(max(top, u.x & 0x7fffffffu), u.y & 0x7fffffffu);
-    return max(max(top, u.z & 0x7fffffffu), u.w & 0x7fffffffu);
-  }
-  static __device__ __forceinline__ uint32_t whole(uint32_t top) { return top; }
-};
-
-__device__ __forceinline__ float2 e4m3x2_values(uint32_t v) {
-  const uint32_t h = f16x2_from_e4m3x2(static_cast<uint16_t>(v));
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
-}
-
-// exponent k of the smallest power of two with amax / 2^k <= 448 = 1.75 * 2^8, at least -100; `bits` of a finite fp32 >= 0
-__device__ __forceinline__ int scale_exponent(uint32_t bits) {
-  const int k = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return max(k, -100);
-}
-
-constexpr uint32_t kInfBits = 0x7f800000u;
 
 // W warps (1 or kAppendWarps) quantise one run of one head; `w` is this warp's number among them.  `top_of` makes a maximum over the
 // lanes of all W warps of the fp32 bits it is given.  The first HOLD pieces of a lane stay in registers, further ones are read again.

@@ -1,0 +1,122 @@
+// What a paged cache of 8-bit values holds, read back as packed keys and values: token i of request b is its cached token first[b] + i.
+//
+// value = e4m3 * scale, in fp32, rounded once (a power of two times e4m3 is a bf16 number: then nothing is rounded).  A token
+// without a block (one beyond the table, an entry outside the cache) and a row that no request has are zeros.
+//
+// HBM-bound: a byte in, two or four out.  A warp takes a window of 32 tokens; its lanes find their requests and blocks, then the warp walks
+// over the window's rows, keys and values, eight values a lane (8 bytes in, 16 out; four and 16 for fp32), several at once.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "gdpa_common.cuh"
+#include "gdpa_launch.h"
+#include "gdpa_pieces.cuh"
+
+namespace gdpa {
+
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kReadWarps = 4;
+
+template <class T, int D>
+__global__ void __launch_bounds__(kReadWarps * 32) gdpa_cache_read_kernel(const __grid_constant__ CacheReadArgs a) {
+  constexpr int E = Piece<T>::kElems;  // values of a lane at a time: 16 bytes of the output
+  constexpr int P = D / E;             // lanes of a head
+  constexpr int U = 8;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // a warp's share: 32 tokens, one part of their (token, key or value, head) rows
+  const long long base = (static_cast<long long>(blockIdx.x) * kReadWarps + warp) * 32;
+  if (base >= a.total) return;
+  const int tokens = static_cast<int>(min(32ll, a.total - base));
+  // where the lane's token is: its block (-1: nowhere) and row
+  int lo = 0, hi = a.batch;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const unsigned below = __ballot_sync(kFull, at < hi && load_offset(a.offsets, at, a.off64) <= base);
+    lo += (below == 0 ? 0 : __popc(below) - 1) * step;
+    hi = min(hi, lo + step);
+  }
+  int owner = lo;
+  for (int b = lo + 1; b < a.batch; b += 32) {
+    const long long begin = b + lane < a.batch ? load_offset(a.offsets, b + lane, a.off64) : 0x7fffffffffffffffll;
+    int count = 0;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) count += __shfl_sync(kFull, begin, count + s - 1) <= base + lane ? s : 0;
+    count += __shfl_sync(kFull, begin, count) <= base + lane;
+    owner += count;
+    if (__shfl_sync(kFull, begin, 31) > base + 31) break;
+  }
+  int block = -1, row = 0;
+  if (a.batch > 0 && lane < tokens) {
+    const long long begin = load_offset(a.offsets, owner, a.off64), end = load_offset(a.offsets, owner + 1, a.off64);
+    const long long p = (a.first != nullptr ? load_offset(a.first, owner, a.first64) : 0) + (base + lane - begin);
+    if (base + lane >= begin && base + lane < end && p >= 0 && (p >> a.block_shift) < a.table_width) {
+      block = a.block_tables[owner * a.table_stride + (p >> a.block_shift)];
+      row = static_cast<int>(p & ((1 << a.block_shift) - 1));
+      if (block < 0 || block >= a.num_blocks) block = -1;
+    }
+  }
+  // rows of the window in the order of the output: all tokens' keys, then their values
+  const int pieces = a.heads * P, all = tokens * pieces;
+  for (int kv = 0; kv < 2; ++kv) {
+    const uint8_t* const cache = kv == 0 ? a.k_cache : a.v_cache;
+    const long long* const cs = kv == 0 ? a.k_cache_strides : a.v_cache_strides;
+    const float* const scales = kv == 0 ? a.k_scales : a.v_scales;
+    T* const out = static_cast<T*>(kv == 0 ? a.key : a.value) + base * a.heads * D;
+    for (int i0 = 0; i0 < all; i0 += 32 * U) {
+      uint32_t u[U][E / 4];
+      float scale[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int i = i0 + 32 * k + lane;
+        const int t = min(i / pieces, 31), piece = i - t * pieces, h = piece / P, e = piece % P;
+        const int blk = __shfl_sync(kFull, block, t), r = __shfl_sync(kFull, row, t);
+        scale[k] = 0;
+#pragma unroll
+        for (int j = 0; j < E / 4; ++j) u[k][j] = 0;
+        if (i < all && blk >= 0) {
+          const uint8_t* const p = cache + blk * cs[0] + r * cs[1] + h * cs[2] + e * E;
+          scale[k] = __ldg(scales + static_cast<long long>(blk) * a.heads + h);
+          if constexpr (E == 8) {
+            const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+            u[k][0] = x.x, u[k][1] = x.y;
+          } else {
+            u[k][0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int i = i0 + 32 * k + lane;
+        float v[E];
+#pragma unroll
+        for (int j = 0; j < E / 4; ++j) {
+          const float2 x = e4m3x2_values(u[k][j] & 0xffffu), y = e4m3x2_values(u[k][j] >> 16);
+          v[4 * j] = x.x * scale[k], v[4 * j + 1] = x.y * scale[k], v[4 * j + 2] = y.x * scale[k], v[4 * j + 3] = y.y * scale[k];
+        }
+        if (i < all) reinterpret_cast<uint4*>(out)[i] = Piece<T>::pack(v);
+      }
+    }
+  }
+}
+
+}  // namespace
+
+int launch_cache_read(const CacheReadArgs& a, int head_dim, int out_is_fp32, int, cudaStream_t stream) {
+  if (a.total == 0) return 0;
+  const long long grid = (a.total + kReadWarps * 32 - 1) / (kReadWarps * 32);
+  auto launch = [&](auto type, auto dim) {
+    gdpa_cache_read_kernel<decltype(type), decltype(dim)::value><<<static_cast<unsigned>(grid), kReadWarps * 32, 0, stream>>>(a);
+  };
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
+  if (out_is_fp32) head_dim == 128 ? launch(float{}, D128{}) : launch(float{}, D64{});
+  else head_dim == 128 ? launch(__nv_bfloat16{}, D128{}) : launch(__nv_bfloat16{}, D64{});
+  return cudaGetLastError() == cudaSuccess ? 0 : GDPA_ERR_LAUNCH_;
+}
+
+}  // namespace gdpa

@@ -258,6 +258,124 @@ struct PagedLaunch {
   cudaStream_t stream;
 };
 
+// How heads are rotated: pair i < pairs turns by position[axis of i] * inv_freq[i]; `ends` are the axes' ends among the pairs.
+constexpr int kMaxAxes = 4;
+struct RotarySpec {
+  const void* inv_freq;  // [pairs], radians a position
+  int inv_freq_is_fp64;
+  int pairs;             // a multiple of 8, at most head_dim / 2
+  int interleaved;       // pairs (2 i, 2 i + 1), else (i, i + pairs)
+  int axes;
+  int ends[kMaxAxes];
+  int norm;              // RMS norm of the head before it is rotated
+  float eps;
+};
+
+struct RotaryTensor {
+  const void* x;
+  long long x_strides[2];  // token, head; in elements
+  void* y;                 // contiguous: the output, or the gradient of x
+  const void* dy;          // gradient of the output
+  long long dy_strides[2];
+  const void* weight;      // [head_dim], or null
+  int weight_is_bf16;
+  int heads;
+  long long tokens;
+  const void* positions;   // [axes, tokens]
+  long long position_stride;
+  int positions_are_int64;
+  void* dweight;           // [head_dim] of the weight's type, or null
+  int per_item;            // heads of an item, a multiple of a warp's
+  int chunks;              // items of a token
+};
+
+struct RotaryArgs {
+  RotarySpec rotary;
+  RotaryTensor t[2];  // queries, keys
+  float* partial;     // backward: [grid][2][head_dim] sums of the weights' gradients, or null
+};
+
+struct RotatedAppendArgs {
+  CacheAppendArgs cache;  // its key and value are the new ones
+  RotarySpec rotary;
+  const void* query;
+  long long query_strides[2];
+  void* query_out;        // contiguous
+  int heads;
+  const void* query_weight;
+  const void* key_weight;
+  int query_weight_is_bf16, key_weight_is_bf16;
+  const void* positions;  // [axes, tokens], or null: they follow from the lengths
+  long long position_stride;
+  int positions_are_int64;
+  const void* q_off;      // [batch + 1]
+  const void* seq_lens;   // [batch]
+  int off64, lens64;
+  int batch;
+  // the grid: kv_windows * kv_parts CTAs for keys and values, then those for queries
+  int kv_windows, kv_parts;
+  int per_item, chunks;   // as in RotaryTensor
+  long long items_per_warp;
+};
+
+struct CacheReadArgs {
+  const uint8_t* k_cache;
+  const uint8_t* v_cache;
+  long long k_cache_strides[3];  // block, row, head; in elements
+  long long v_cache_strides[3];
+  const float* k_scales;
+  const float* v_scales;
+  const int* block_tables;
+  long long table_stride;
+  int table_width;
+  int block_shift;
+  long long num_blocks;
+  const void* offsets;   // [batch + 1]
+  const void* first;     // [batch], or null: zeros
+  int off64, first64;
+  int batch;
+  int heads;
+  long long total;
+  void* key;
+  void* value;
+};
+
+struct VerifyArgs {
+  const void* target;      // [rows, vocab]
+  const void* draft;       // [drafts, vocab], or null
+  long long target_stride, draft_stride;
+  long long rows, drafts;
+  int vocab;
+  const void* tokens;      // [drafts]
+  int tokens64;
+  const void* row_offsets;    // [batch + 1]
+  const void* draft_offsets;  // [batch + 1]
+  int off64;
+  const float* accept;     // [drafts]
+  const float* sample;     // [batch]
+  int batch;
+  int max_drafts;
+  void* out_tokens;        // [batch, max_drafts + 1], as tokens
+  int* accepted;
+  int* refused;
+};
+
+struct DropArgs {
+  const int* block_tables;
+  long long table_stride;
+  int table_width;
+  int block_shift;
+  const void* seq_lens;
+  const void* dropped;
+  int lens64, dropped64;
+  int batch;
+  int* free_blocks;
+  long long free_capacity;
+  const int* num_free;
+  int* seq_lens_after;
+  int* num_free_after;
+};
+
 }  // namespace gdpa
 struct GdpaFwdParams;
 namespace gdpa {
@@ -280,6 +398,14 @@ int launch_norm_rows_bwd(const NormBwdArgs& a, int mode, cudaStream_t stream);
 int launch_build_schedule(const SchedArgs& a, cudaStream_t stream);
 int launch_block_tables(const BlockTableArgs& a, int sm_count, cudaStream_t stream);
 int launch_cache_append(const CacheAppendArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream);
+int launch_rotary(RotaryArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream);
+int launch_rotary_bwd(RotaryArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream);  // kernels launched, or -(an error)
+int rotary_bwd_ctas(int sm_count);  // CTAs that have a row of RotaryArgs::partial each
+int launch_rotated_append(RotatedAppendArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream);
+int launch_cache_read(const CacheReadArgs& a, int head_dim, int out_is_fp32, int sm_count, cudaStream_t stream);
+int launch_verify(const VerifyArgs& a, int is_bf16, int sm_count, cudaStream_t stream);
+int verify_most_vocab();
+int launch_drop(const DropArgs& a, cudaStream_t stream);
 int launch_paged(const PagedLaunch& l, int head_dim);
 int launch_paged_rows(const PagedLaunch& l, int head_dim);  // of launch_paged, for row tiles of 256
 int paged_ctas_per_sm(int rows, int head_dim);  // resident CTAs of the kernel for row tiles of `rows`: a launch has that many

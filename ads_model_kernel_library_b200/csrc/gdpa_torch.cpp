@@ -4,17 +4,13 @@
 // the three calls took 28, 29 and 46 us, their kernels 3 to 18.  The operators have no gradient and only a CUDA kernel; their fake
 // kernels are registered in Python.  The C ABI stays free of torch types: its entry points are handed over by address
 // (gdpa_torch_init), so that this library needs no particular copy of it.
-#include <ATen/ATen.h>
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
-#include <torch/library.h>
 
 #include <atomic>
-#include <tuple>
 
-#include "../../include/gdpa_b200.h"
+#include "gdpa_torch.h"
+
+using namespace gdpa_torch;
 
 namespace {
 
@@ -23,7 +19,6 @@ struct EntryPoints {
   int (*append)(const GdpaCacheAppendParams*, gdpa_stream_t);
   size_t (*workspace_bytes)(int64_t, int32_t, int32_t, int32_t, int32_t);
   int (*attend)(const GdpaPagedParams*, gdpa_stream_t);
-  const char* (*strerror)(int);
 } g_call{};
 constexpr int kMaxDevices = 64;
 // The word of each device into which a kernel writes when a wait of it runs out, or null as long as nobody has asked for it.  Python has it: the
@@ -32,8 +27,6 @@ std::atomic<int32_t*> g_status[kMaxDevices];
 using StatusLook = int32_t* (*)(int device, char* message, int size);
 std::atomic<StatusLook> g_look{nullptr};
 std::atomic<void*> g_timing[2];               // events around the attention's kernel, or null
-
-void check(int code, const char* what) { TORCH_CHECK(code == GDPA_OK, what, ": ", g_call.strerror(code), " (code ", code, ")"); }
 
 // The status word for a call on `device`; an error if a wait of an earlier call's kernel ran out.  Here, not in Python, so that a traced call does it too.
 int32_t* status_of(int device) {
@@ -46,85 +39,6 @@ int32_t* status_of(int device) {
   g_status[device].store(word = look(device, message, sizeof(message)));
   TORCH_CHECK(message[0] == '\0', message);
   return word;
-}
-
-void check_cuda(const char* name, const at::Tensor& t) {
-  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor: this operator has no CPU path");
-}
-void check_device(const char* name, const at::Tensor& t, const at::Tensor& like) {
-  TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", got ", t.device());
-}
-void check_type(const char* name, const at::Tensor& t, at::ScalarType type) {
-  TORCH_CHECK_TYPE(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
-}
-bool check_int(const char* name, const at::Tensor& t) {  // whether it is 64 bits wide
-  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64, got ", t.scalar_type());
-  return t.scalar_type() == at::kLong;
-}
-void check_vector(const char* name, const at::Tensor& t, const at::Tensor& like, int64_t length) {
-  check_device(name, t, like);
-  TORCH_CHECK_VALUE(t.dim() == 1 && t.is_contiguous(), name, " must be a contiguous 1-D tensor");
-  TORCH_CHECK_VALUE(length < 0 || t.numel() == length, name, " must have ", length, " entries, got ", t.numel());
-}
-void check_block_size(int64_t size) {
-  TORCH_CHECK_NOT_IMPLEMENTED(size == 16 || size == 32 || size == 64 || size == 128, "a block size of ", size,
-                              " is not supported (supported: 16, 32, 64, 128)");
-}
-void check_table(const at::Tensor& t, const at::Tensor& like, int64_t batch, int64_t size) {
-  check_device("block_tables", t, like);
-  check_type("block_tables", t, at::kInt);
-  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == batch, "block_tables must be [", batch, ", width], got ", t.sizes());
-  TORCH_CHECK_VALUE(t.size(1) <= 1 || t.stride(1) == 1, "block_tables must have contiguous rows");
-  TORCH_CHECK_VALUE(t.size(1) * size <= (int64_t{1} << 30), "block_tables: a request can hold 2^30 tokens at most");
-}
-
-bool misaligned(const at::Tensor& t, int dims) {  // of the strides that matter, in bytes, and the address
-  if (t.numel() == 0) return false;
-  if (t.stride(dims) != 1 && t.size(dims) > 1) return true;
-  for (int i = 0; i < dims; ++i)
-    if (t.size(i) > 1 && (t.stride(i) < 0 || t.stride(i) * t.element_size() % 16 != 0)) return true;
-  return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 != 0;
-}
-// a dimension of one entry has no stride that matters: the contiguous one is taken (0)
-template <int N>
-void strides(int64_t (&field)[N], const at::Tensor& t) {
-  for (int i = 0; i < N; ++i) field[i] = t.size(i) > 1 ? t.stride(i) : 0;
-}
-void check_rows(const char* name, const at::Tensor& t) {
-  TORCH_CHECK_VALUE(t.dim() == 3, name, " must be [total_tokens, H, D], got ", t.sizes());
-  TORCH_CHECK_VALUE(!misaligned(t, 2), name,
-                    " must have a contiguous head dimension and 16-byte aligned row / head strides (a contiguous tensor, or a slice of a "
-                    "packed QKV / KV tensor along the last dimension)");
-  // an expanded tensor among them: the C ABI takes a stride of 0 for the contiguous one
-  for (int i = 0; i < 2; ++i)
-    TORCH_CHECK_VALUE(t.numel() == 0 || t.size(i) <= 1 || t.stride(i) >= t.size(2), name, " must have rows and heads of its own, got strides ", t.strides(),
-                      " (an expanded tensor: make it contiguous)");
-}
-
-void check_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs, const at::Tensor& like) {
-  for (auto& [name, t] : {std::pair<const char*, const at::Tensor&>("k_cache", k), {"v_cache", v}}) {
-    check_device(name, t, like);
-    check_type(name, t, at::kFloat8_e4m3fn);
-    TORCH_CHECK_VALUE(t.dim() == 4, name, " must be [num_blocks, block_size, H_kv, D], got ", t.sizes());
-    bool bad = misaligned(t, 3);
-    for (int i = 0; i < 3; ++i) bad |= t.size(i) > 1 && t.stride(i) <= 0;
-    TORCH_CHECK_VALUE(!bad, name, " must have a contiguous head dimension and 16-byte aligned strides");
-  }
-  TORCH_CHECK_VALUE(k.sizes() == v.sizes(), "k_cache and v_cache must have the same shape");
-  check_block_size(k.size(1));
-  TORCH_CHECK_NOT_IMPLEMENTED(k.size(3) == 64 || k.size(3) == 128, "head_dim ", k.size(3), " is not supported (supported: 64, 128)");
-  TORCH_CHECK_VALUE(k.size(2) >= 1, "a cache must have at least one head");
-  for (auto& [name, t] : {std::pair<const char*, const at::Tensor&>("k_scales", ks), {"v_scales", vs}}) {
-    check_device(name, t, like);
-    check_type(name, t, at::kFloat);
-    TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == k.size(0) && t.size(1) == k.size(2) && t.is_contiguous(), name, " must be a contiguous [",
-                      k.size(0), ", ", k.size(2), "] tensor");
-  }
-}
-
-// From the caching allocator, without the dispatcher.
-at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
-  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> build_block_tables(const at::Tensor& block_tables, const at::Tensor& cached_lens,
@@ -273,13 +187,13 @@ at::Tensor attend_paged_fp8(const at::Tensor& query, const at::Tensor& k_cache, 
 
 }  // namespace
 
-// The entry points of the kernel library (in the order of EntryPoints).
+// The entry points of the kernel library (in the order of EntryPoints), and its error texts.
 extern "C" __attribute__((visibility("default"))) void gdpa_torch_init(void* tables, void* append, void* workspace, void* attend, void* error) {
   g_call.build_block_tables = reinterpret_cast<decltype(g_call.build_block_tables)>(tables);
   g_call.append = reinterpret_cast<decltype(g_call.append)>(append);
   g_call.workspace_bytes = reinterpret_cast<decltype(g_call.workspace_bytes)>(workspace);
   g_call.attend = reinterpret_cast<decltype(g_call.attend)>(attend);
-  g_call.strerror = reinterpret_cast<decltype(g_call.strerror)>(error);
+  strerror_of = reinterpret_cast<const char* (*)(int)>(error);
 }
 // Who has the status words, and the events around the next calls' kernel (null: none).
 extern "C" __attribute__((visibility("default"))) void gdpa_torch_set_status_look(void* look) {

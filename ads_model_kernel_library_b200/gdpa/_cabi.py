@@ -39,6 +39,13 @@ EXPORTS = (
     "gdpa_append_kv_cache_fp8",
     "gdpa_paged_workspace_bytes",
     "gdpa_fwd_paged_fp8",
+    "gdpa_qk_norm_rotary",
+    "gdpa_qk_norm_rotary_bwd",
+    "gdpa_rotary_workspace_bytes",
+    "gdpa_append_rotated_kv_cache_fp8",
+    "gdpa_read_kv_cache_fp8",
+    "gdpa_verify_draft_tokens",
+    "gdpa_drop_cached_tokens",
     "gdpa_bwd_workspace_bytes",
     "gdpa_bwd",
     "gdpa_strerror",
@@ -311,6 +318,152 @@ class GdpaPagedParams(C.Structure):
     ]
 
 
+class GdpaRotarySpec(C.Structure):
+    _fields_ = [
+        ("inv_freq", C.c_void_p),
+        ("inv_freq_is_fp64", C.c_int32),
+        ("pairs", C.c_int32),
+        ("interleaved", C.c_int32),
+        ("axes", C.c_int32),
+        ("section_ends", C.c_int32 * 4),
+        ("norm", C.c_int32),
+        ("eps", C.c_float),
+    ]
+
+
+class GdpaRotaryTensor(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("x_strides", C.c_int64 * 2),
+        ("y", C.c_void_p),
+        ("dy", C.c_void_p),
+        ("dy_strides", C.c_int64 * 2),
+        ("weight", C.c_void_p),
+        ("weight_is_bf16", C.c_int32),
+        ("heads", C.c_int32),
+        ("tokens", C.c_int64),
+        ("positions", C.c_void_p),
+        ("position_stride", C.c_int64),
+        ("positions_are_int64", C.c_int32),
+        ("reserved", C.c_int32),
+        ("dweight", C.c_void_p),
+    ]
+
+
+class GdpaRotaryParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("is_fp32", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("reserved", C.c_int32),
+        ("rotary", GdpaRotarySpec),
+        ("query", GdpaRotaryTensor),
+        ("key", GdpaRotaryTensor),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+    ]
+
+
+class GdpaRotatedAppendParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("heads", C.c_int32),
+        ("cache", GdpaCacheAppendParams),
+        ("rotary", GdpaRotarySpec),
+        ("query", C.c_void_p),
+        ("query_strides", C.c_int64 * 2),
+        ("query_out", C.c_void_p),
+        ("query_weight", C.c_void_p),
+        ("key_weight", C.c_void_p),
+        ("query_weight_is_bf16", C.c_int32),
+        ("key_weight_is_bf16", C.c_int32),
+        ("positions", C.c_void_p),
+        ("position_stride", C.c_int64),
+        ("positions_are_int64", C.c_int32),
+        ("batch", C.c_int32),
+        ("q_offsets", C.c_void_p),
+        ("seq_lens", C.c_void_p),
+        ("offsets_are_int64", C.c_int32),
+        ("lens_are_int64", C.c_int32),
+    ]
+
+
+class GdpaCacheReadParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("out_is_fp32", C.c_int32),
+        ("k_cache", C.c_void_p),
+        ("v_cache", C.c_void_p),
+        ("k_cache_strides", C.c_int64 * 3),
+        ("v_cache_strides", C.c_int64 * 3),
+        ("k_scales", C.c_void_p),
+        ("v_scales", C.c_void_p),
+        ("block_tables", C.c_void_p),
+        ("table_stride", C.c_int64),
+        ("table_width", C.c_int32),
+        ("block_size", C.c_int32),
+        ("num_blocks", C.c_int64),
+        ("offsets", C.c_void_p),
+        ("first", C.c_void_p),
+        ("offsets_are_int64", C.c_int32),
+        ("first_is_int64", C.c_int32),
+        ("batch", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("reserved", C.c_int32),
+        ("total", C.c_int64),
+        ("key", C.c_void_p),
+        ("value", C.c_void_p),
+    ]
+
+
+class GdpaVerifyParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("is_bf16", C.c_int32),
+        ("target", C.c_void_p),
+        ("draft", C.c_void_p),
+        ("target_stride", C.c_int64),
+        ("draft_stride", C.c_int64),
+        ("rows", C.c_int64),
+        ("drafts", C.c_int64),
+        ("vocab", C.c_int32),
+        ("tokens_are_int64", C.c_int32),
+        ("tokens", C.c_void_p),
+        ("row_offsets", C.c_void_p),
+        ("draft_offsets", C.c_void_p),
+        ("offsets_are_int64", C.c_int32),
+        ("batch", C.c_int32),
+        ("accept", C.c_void_p),
+        ("sample", C.c_void_p),
+        ("max_drafts", C.c_int32),
+        ("reserved", C.c_int32),
+        ("out_tokens", C.c_void_p),
+        ("accepted", C.c_void_p),
+        ("refused", C.c_void_p),
+    ]
+
+
+class GdpaDropParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("block_size", C.c_int32),
+        ("block_tables", C.c_void_p),
+        ("table_stride", C.c_int64),
+        ("table_width", C.c_int32),
+        ("batch", C.c_int32),
+        ("seq_lens", C.c_void_p),
+        ("dropped", C.c_void_p),
+        ("lens_are_int64", C.c_int32),
+        ("dropped_is_int64", C.c_int32),
+        ("free_blocks", C.c_void_p),
+        ("free_capacity", C.c_int64),
+        ("num_free", C.c_void_p),
+        ("seq_lens_after", C.c_void_p),
+        ("num_free_after", C.c_void_p),
+    ]
+
+
 def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -343,11 +496,16 @@ def _load() -> C.CDLL:
     lib.gdpa_bwd.restype = C.c_int
     lib.gdpa_bwd.argtypes = [C.POINTER(GdpaBwdParams), C.c_void_p]
     for fn, params in ((lib.gdpa_build_block_tables, GdpaBlockTableParams), (lib.gdpa_append_kv_cache_fp8, GdpaCacheAppendParams),
-                       (lib.gdpa_fwd_paged_fp8, GdpaPagedParams)):
+                       (lib.gdpa_fwd_paged_fp8, GdpaPagedParams), (lib.gdpa_qk_norm_rotary, GdpaRotaryParams),
+                       (lib.gdpa_qk_norm_rotary_bwd, GdpaRotaryParams), (lib.gdpa_append_rotated_kv_cache_fp8, GdpaRotatedAppendParams),
+                       (lib.gdpa_read_kv_cache_fp8, GdpaCacheReadParams), (lib.gdpa_verify_draft_tokens, GdpaVerifyParams),
+                       (lib.gdpa_drop_cached_tokens, GdpaDropParams)):
         fn.restype = C.c_int
         fn.argtypes = [C.POINTER(params), C.c_void_p]
     lib.gdpa_paged_workspace_bytes.restype = C.c_size_t
     lib.gdpa_paged_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32]
+    lib.gdpa_rotary_workspace_bytes.restype = C.c_size_t
+    lib.gdpa_rotary_workspace_bytes.argtypes = [C.c_int32]
     lib.gdpa_strerror.restype = C.c_char_p
     lib.gdpa_strerror.argtypes = [C.c_int]
     lib.gdpa_launch_count.restype = C.c_int64

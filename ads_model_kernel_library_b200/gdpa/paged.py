@@ -8,8 +8,10 @@ between calls, as e4m3 values in blocks of 16, 32, 64 or 128 tokens with one fp3
     block_tables        [B, width]                         int32: the blocks of a request's tokens, in order
 
 One step of a batch is :func:`build_block_tables` (blocks and slots of the new tokens), :func:`append_kv_cache_fp8` (their keys
-and values) and :func:`generalized_dot_product_attention_paged_fp8` (their queries).  :class:`PagedKVCache` holds the tensors
-and makes the three calls.  Nothing here synchronises with the host, and there are no gradients.
+and values) and :func:`generalized_dot_product_attention_paged_fp8` (their queries).  :func:`append_rotated_kv_cache_fp8` norms and rotates queries
+and keys on the way, :func:`read_kv_cache_fp8` gives packed keys and values back, :func:`drop_cached_tokens` takes tokens out again (drafts
+that were refused).  :class:`PagedKVCache` holds the tensors and makes the calls.  Nothing here synchronises with the host, and there are no
+gradients.
 """
 from __future__ import annotations
 
@@ -24,7 +26,8 @@ import torch
 from . import _cabi, ops
 from .math import activation_string_to_int
 
-__all__ = ["build_block_tables", "append_kv_cache_fp8", "generalized_dot_product_attention_paged_fp8", "PagedKVCache"]
+__all__ = ["build_block_tables", "append_kv_cache_fp8", "append_rotated_kv_cache_fp8", "generalized_dot_product_attention_paged_fp8", "read_kv_cache_fp8",
+           "drop_cached_tokens", "PagedKVCache"]
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "libgdpa_b200_torch.so")
 
@@ -43,7 +46,7 @@ def _look_at_status(device: int, message, size: int):
 
 
 class _Operators:
-    """The three torch operators, which libgdpa_b200_torch.so registers (checks, outputs and launch in C++: a step of generation is host
+    """The torch operators that libgdpa_b200_torch.so registers (checks, outputs and launch in C++: a step of generation is host
     time), with their fake kernels."""
 
     def __init__(self):
@@ -56,6 +59,9 @@ class _Operators:
         self.native = C.CDLL(LIB_PATH)
         entries = (lib.gdpa_build_block_tables, lib.gdpa_append_kv_cache_fp8, lib.gdpa_paged_workspace_bytes, lib.gdpa_fwd_paged_fp8, lib.gdpa_strerror)
         self.native.gdpa_torch_init(*(C.cast(f, C.c_void_p) for f in entries))
+        entries = (lib.gdpa_qk_norm_rotary, lib.gdpa_qk_norm_rotary_bwd, lib.gdpa_rotary_workspace_bytes, lib.gdpa_append_rotated_kv_cache_fp8,
+                   lib.gdpa_read_kv_cache_fp8, lib.gdpa_verify_draft_tokens, lib.gdpa_drop_cached_tokens)
+        self.native.gdpa_torch_init_heads((C.c_void_p * len(entries))(*(C.cast(f, C.c_void_p) for f in entries)))
         self.native.gdpa_torch_set_timing.argtypes = [C.c_void_p, C.c_void_p]
         self.native.gdpa_torch_set_status_look(_look_at_status)
         if first:
@@ -63,9 +69,21 @@ class _Operators:
             torch.library.register_fake("gdpa::append_kv_cache_fp8", lambda *args: None)
             torch.library.register_fake("gdpa::generalized_dot_product_attention_paged_fp8",
                                         lambda query, *args: torch.empty(query.shape, dtype=torch.bfloat16, device=query.device))
+            torch.library.register_fake("gdpa::qk_norm_rotary", lambda query, key, *args: (_packed(query), _packed(key)))
+            torch.library.register_fake("gdpa::qk_norm_rotary_backward", _fake_rotary_backward)
+            torch.library.register_fake("gdpa::append_rotated_kv_cache_fp8", lambda query, *args: _packed(query))
+            torch.library.register_fake("gdpa::read_kv_cache_fp8", _fake_read)
+            torch.library.register_fake("gdpa::verify_draft_tokens", _fake_verify)
+            torch.library.register_fake("gdpa::drop_cached_tokens",
+                                        lambda table, lens, *args: (torch.empty_like(lens, dtype=torch.int32), lens.new_empty(1, dtype=torch.int32)))
         self.tables = torch.ops.gdpa.build_block_tables.default
         self.append = torch.ops.gdpa.append_kv_cache_fp8.default
         self.attend = torch.ops.gdpa.generalized_dot_product_attention_paged_fp8.default
+        self.rotary = torch.ops.gdpa.qk_norm_rotary.default
+        self.append_rotated = torch.ops.gdpa.append_rotated_kv_cache_fp8.default
+        self.read = torch.ops.gdpa.read_kv_cache_fp8.default
+        self.verify = torch.ops.gdpa.verify_draft_tokens.default
+        self.drop = torch.ops.gdpa.drop_cached_tokens.default
 
 
 _operators: Optional[_Operators] = None
@@ -86,6 +104,27 @@ def _fake_tables(block_tables, cached_lens, new_lens, free_blocks, num_free, blo
 
     batch = cached_lens.shape[0]
     return empty(total_new, torch.int64), empty(batch + 1, torch.int32), empty(batch, torch.int32), empty(1, torch.int32)
+
+
+def _packed(x):
+    return x.new_empty(x.shape)
+
+
+def _fake_rotary_backward(query_grad, key_grad, query, key, inv_freq, query_positions, key_positions, query_weight, key_weight, eps, norm, interleaved, sections,
+                          weight_grads):
+    def of(weight):
+        return query.new_empty(0, dtype=torch.float32) if weight is None or not (weight_grads and norm) else weight.new_empty(weight.shape)
+
+    return _packed(query), _packed(key), of(query_weight), of(key_weight)
+
+
+def _fake_read(k_cache, v_cache, k_scales, v_scales, block_tables, key_offset, total_tokens, first_tokens, dtype):
+    return tuple(torch.empty((total_tokens, *k_cache.shape[2:]), dtype=dtype, device=k_cache.device) for _ in range(2))
+
+
+def _fake_verify(target_probs, draft_probs, draft_tokens, query_offset, draft_offset, accept_uniform, sample_uniform, max_drafts):
+    batch = sample_uniform.shape[0]
+    return draft_tokens.new_empty((batch, max_drafts + 1)), *(draft_tokens.new_empty(batch, dtype=torch.int32) for _ in range(2))
 
 
 # ------------------------------------------------------------------------------------------ block tables, slot maps
@@ -204,6 +243,91 @@ def _check_lengths(query, k_cache, block_tables, query_offset, seq_lens) -> None
         raise ValueError("seq_lens has entries outside [0, width of block_tables * block size]")
 
 
+# ------------------------------------------------------------------------------------------ queries and keys on their way in
+
+
+def append_rotated_kv_cache_fp8(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_scales: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    query_offset: torch.Tensor,
+    seq_lens: torch.Tensor,
+    inv_freq: torch.Tensor,
+    positions: Optional[torch.Tensor] = None,
+    query_weight: Optional[torch.Tensor] = None,
+    key_weight: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    norm: bool = True,
+    interleaved: bool = False,
+    sections: Optional[Sequence[int]] = None,
+) -> torch.Tensor:
+    """:func:`~.rotary.qk_norm_rotary` of a step's queries and keys and :func:`append_kv_cache_fp8` of the rotated keys and the values, in one
+    kernel; returns the rotated queries for the attention.
+
+    ``query`` ``[tokens, H, D]``, ``key`` and ``value`` ``[tokens, H_kv, D]`` (bf16 or fp32, strided as slices of one packed projection are).
+    ``positions`` (``[tokens]``, or ``[axes, tokens]`` with ``sections``) may be left out: token ``i`` of the ``n`` that request ``b`` has, rows
+    ``query_offset[b]:query_offset[b + 1]``, is at ``seq_lens[b] - n + i`` (``seq_lens`` with the new tokens, as :func:`build_block_tables` returns
+    it), on every axis.  Rotated keys go from fp32 to e4m3: they are rounded once, where the two operators one after the other round to bf16
+    in between.  A query whose token has no slot (-1) is rotated all the same; what holds for the slots holds as in the append.
+    """
+    if ops._validate_offsets and not torch.compiler.is_compiling():
+        _check_slots(slot_mapping, k_cache)
+        ops._check_offsets("query_offset", query_offset, query.shape[0], False)
+    return (_operators or _load()).append_rotated(
+        query, key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping, query_offset, seq_lens, inv_freq, positions, query_weight, key_weight, eps, norm,
+        interleaved, () if sections is None else sections)
+
+
+# ------------------------------------------------------------------------------------------ what the cache holds
+
+
+def read_kv_cache_fp8(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_scales: torch.Tensor,
+    block_tables: torch.Tensor,
+    key_offset: torch.Tensor,
+    total_tokens: int,
+    first_tokens: Optional[torch.Tensor] = None,
+    dtype: torch.dtype = torch.bfloat16,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The cached keys and values of a batch as packed ``[total_tokens, H_kv, D]`` tensors (bf16 or fp32), as the operators that have no paged form
+    take them.
+
+    Rows ``key_offset[b]:key_offset[b + 1]`` are request ``b``'s tokens ``first_tokens[b]``, ``first_tokens[b] + 1``, ... (from 0 without
+    ``first_tokens``; both int32 or int64).  A value is e4m3 times scale in fp32, rounded once: with scales that the append made (powers of two)
+    bf16 holds it exactly.  Tokens past the table's width, those of blocks that the table has not (-1) and rows that no request has are zeros.
+    ``key_offset`` is trusted like the offsets of the other operators.
+    """
+    if ops._validate_offsets and not torch.compiler.is_compiling():
+        ops._check_offsets("key_offset", key_offset, total_tokens, False)
+    return (_operators or _load()).read(k_cache, v_cache, k_scales, v_scales, block_tables, key_offset, total_tokens, first_tokens, dtype)
+
+
+def drop_cached_tokens(
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    dropped: torch.Tensor,
+    free_blocks: torch.Tensor,
+    num_free: torch.Tensor,
+    block_size: int,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The last ``dropped[b]`` tokens of each request leave the cache (drafts that were refused; all of them: the request is done), in one kernel.
+
+    Blocks that none of a request's remaining tokens needs go onto the stack ``free_blocks[:num_free]`` (int32, changed in place), in the order of the
+    requests and of their tables; entries that are no block (-1) do not.  ``dropped`` is clamped to what a request has, a negative ``num_free``
+    counts as 0.  Returns ``(seq_lens_after, num_free_after)``, int32 ``[B]`` and ``[1]``.  The tables are left as they are: what lies behind
+    a request's length is not looked at, and :func:`build_block_tables` writes over it.
+    """
+    return (_operators or _load()).drop(block_tables, seq_lens, dropped, free_blocks, num_free, block_size)
+
+
 class PagedKVCache:
     """The cache of a batch of requests, with its free blocks, and the three calls of a step.
 
@@ -232,6 +356,23 @@ class PagedKVCache:
         self.seq_lens, self.num_free = seq_lens, num_free
         return query_offset
 
+    def append_rotated(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, new_lens: torch.Tensor, rotary: dict):
+        """As :meth:`append`, with queries and keys normed and rotated on the way (``rotary``: :func:`append_rotated_kv_cache_fp8`'s arguments from
+        ``inv_freq`` on); returns ``(queries, offsets)``."""
+        slots, query_offset, seq_lens, num_free = build_block_tables(
+            self.block_tables, self.seq_lens, new_lens, self.free_blocks, self.num_free, self.block_size, key.shape[0])
+        query = append_rotated_kv_cache_fp8(query, key, value, self.k_cache, self.v_cache, self.k_scales, self.v_scales, slots, query_offset, seq_lens, **rotary)
+        self.seq_lens, self.num_free = seq_lens, num_free  # not before, as in append
+        return query, query_offset
+
+    def read(self, key_offset: torch.Tensor, total_tokens: int, first_tokens: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16):
+        """:func:`read_kv_cache_fp8` of what the cache holds."""
+        return read_kv_cache_fp8(self.k_cache, self.v_cache, self.k_scales, self.v_scales, self.block_tables, key_offset, total_tokens, first_tokens, dtype)
+
+    def drop(self, dropped: torch.Tensor) -> None:
+        """Take the last ``dropped[b]`` tokens of each request out of the cache, and their blocks back (:func:`drop_cached_tokens`)."""
+        self.seq_lens, self.num_free = drop_cached_tokens(self.block_tables, self.seq_lens, dropped, self.free_blocks, self.num_free, self.block_size)
+
     def attend(self, query: torch.Tensor, query_offset: torch.Tensor, max_seq_len_q: int, **options) -> torch.Tensor:
         """:func:`generalized_dot_product_attention_paged_fp8` over what the cache holds."""
         return generalized_dot_product_attention_paged_fp8(
@@ -239,9 +380,14 @@ class PagedKVCache:
             **options)
 
     def step(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, new_lens: torch.Tensor, max_seq_len_q: int,
-             **options) -> torch.Tensor:
-        """Append, then attend with the new tokens' queries (causal unless ``is_causal=False`` is given)."""
-        return self.attend(query, self.append(key, value, new_lens), max_seq_len_q, **{"is_causal": True, **options})
+             rotary: Optional[dict] = None, **options) -> torch.Tensor:
+        """Append, then attend with the new tokens' queries (causal unless ``is_causal=False`` is given); with ``rotary``, queries and keys are
+        normed and rotated first (:meth:`append_rotated`)."""
+        if rotary is None:
+            query_offset = self.append(key, value, new_lens)
+        else:
+            query, query_offset = self.append_rotated(query, key, value, new_lens, rotary)
+        return self.attend(query, query_offset, max_seq_len_q, **{"is_causal": True, **options})
 
     def release(self, requests: Sequence[int]) -> None:
         """Give back the blocks of these requests (rows of the tables, negative ones from the end), which are empty afterwards."""

@@ -473,6 +473,172 @@ size_t gdpa_paged_workspace_bytes(int64_t total_q, int32_t heads, int32_t kv_hea
 int gdpa_fwd_paged_fp8(const GdpaPagedParams* params, gdpa_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Queries and keys between the projections and the attention: the RMS norm of every head and its rotation
+ * by the token's position.  For head x, weight w, position p (one for each axis) and pair i < pairs:
+ *   n = x * rsqrt(mean(x^2) + eps) * w  (norm = 0: n = x),  angle = p[axis of i] * inv_freq[i],
+ *   (y_a, y_b) = (n_a cos - n_b sin, n_b cos + n_a sin), (a, b) = (i, i + pairs) or, interleaved, (2i, 2i + 1);
+ * values behind the pairs are n.  Angles are taken in 64 bits, everything else in fp32, rounded once.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct GdpaRotarySpec {
+  const void* inv_freq;        /* [pairs] radians a position, fp32 or fp64 */
+  int32_t inv_freq_is_fp64;
+  int32_t pairs;               /* a multiple of 8, at most head_dim / 2; 0 = no rotation */
+  int32_t interleaved;
+  int32_t axes;                /* 1 to 4 */
+  int32_t section_ends[4];     /* pairs [ends[a - 1], ends[a]) turn with axis a; ends[axes - 1] = pairs.  Not read for one axis */
+  int32_t norm;
+  float eps;
+} GdpaRotarySpec;
+
+typedef struct GdpaRotaryTensor {
+  const void* x;               /* [tokens, heads, head_dim] */
+  int64_t x_strides[2];        /* token, head; 0 = contiguous.  Multiples of 16 bytes */
+  void* y;                     /* out, contiguous: forward the result, backward the gradient of x */
+  const void* dy;              /* backward: gradient of the result */
+  int64_t dy_strides[2];
+  const void* weight;          /* [head_dim] fp32 or bf16, or null (ones) */
+  int32_t weight_is_bf16;
+  int32_t heads;
+  int64_t tokens;
+  const void* positions;       /* [axes, tokens], int32 or int64 */
+  int64_t position_stride;     /* between axes */
+  int32_t positions_are_int64;
+  int32_t reserved;
+  void* dweight;               /* backward: [head_dim] of the weight's type, or null */
+} GdpaRotaryTensor;
+
+typedef struct GdpaRotaryParams {
+  uint32_t struct_size;        /* sizeof(GdpaRotaryParams) */
+  int32_t is_fp32;             /* type of x, y and dy: 0 bf16, 1 fp32 */
+  int32_t head_dim;            /* 64 or 128 */
+  int32_t reserved;
+  GdpaRotarySpec rotary;
+  GdpaRotaryTensor query;
+  GdpaRotaryTensor key;        /* its tokens and positions may be others */
+  void* workspace;             /* backward with a dweight: gdpa_rotary_workspace_bytes(), 16-byte aligned, one per call in flight */
+  int64_t workspace_bytes;
+} GdpaRotaryParams;
+
+int gdpa_qk_norm_rotary(const GdpaRotaryParams* params, gdpa_stream_t stream);
+/* dx = r (g - x r^2 mean(g x)) and dw = sum(dn x r) with dn the result's gradient turned back, g = dn w, r the norm's factor.  The sums'
+ * order does not vary: the same inputs give the same bits on the same GPU. */
+int gdpa_qk_norm_rotary_bwd(const GdpaRotaryParams* params, gdpa_stream_t stream);
+/* Bytes of the backward's workspace on the current device; 0 if there is none. */
+size_t gdpa_rotary_workspace_bytes(int32_t head_dim);
+
+/* A serving step: queries and keys normed and rotated as above, keys and values quantised into their slots as
+ * gdpa_append_kv_cache_fp8 does (the keys from fp32: they are rounded once, to e4m3), queries written for the attention. */
+typedef struct GdpaRotatedAppendParams {
+  uint32_t struct_size;        /* sizeof(GdpaRotatedAppendParams) */
+  int32_t heads;               /* of the queries */
+  GdpaCacheAppendParams cache; /* its struct_size set too; x_is_fp32 is the queries' type as well */
+  GdpaRotarySpec rotary;
+  const void* query;           /* [tokens, heads, head_dim] */
+  int64_t query_strides[2];
+  void* query_out;             /* out, contiguous */
+  const void* query_weight;
+  const void* key_weight;
+  int32_t query_weight_is_bf16;
+  int32_t key_weight_is_bf16;
+  const void* positions;       /* [axes, tokens], or null: token i of n of request b is at seq_lens[b] - n + i on every axis */
+  int64_t position_stride;
+  int32_t positions_are_int64;
+  int32_t batch;
+  const void* q_offsets;       /* [batch + 1] */
+  const void* seq_lens;        /* [batch], the new tokens counted */
+  int32_t offsets_are_int64;
+  int32_t lens_are_int64;
+} GdpaRotatedAppendParams;
+
+int gdpa_append_rotated_kv_cache_fp8(const GdpaRotatedAppendParams* params, gdpa_stream_t stream);
+
+/* What a cache holds, as packed keys and values: rows offsets[b] .. offsets[b + 1) are request b's tokens first[b], first[b] + 1, ...
+ * (e4m3 * scale in fp32, rounded once).  Tokens without a block and rows of no request become zeros. */
+typedef struct GdpaCacheReadParams {
+  uint32_t struct_size;        /* sizeof(GdpaCacheReadParams) */
+  int32_t out_is_fp32;         /* 0 bf16, 1 fp32 */
+  const void* k_cache;
+  const void* v_cache;
+  int64_t k_cache_strides[3];  /* block, row, head; 0 = contiguous */
+  int64_t v_cache_strides[3];
+  const float* k_scales;
+  const float* v_scales;
+  const int32_t* block_tables;
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t block_size;
+  int64_t num_blocks;
+  const void* offsets;         /* [batch + 1] */
+  const void* first;           /* [batch], or null: zeros */
+  int32_t offsets_are_int64;
+  int32_t first_is_int64;
+  int32_t batch;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t reserved;
+  int64_t total;               /* rows of key and value */
+  void* key;                   /* out [total, kv_heads, head_dim], contiguous */
+  void* value;
+} GdpaCacheReadParams;
+
+int gdpa_read_kv_cache_fp8(const GdpaCacheReadParams* params, gdpa_stream_t stream);
+
+/* Drafted tokens against the target's probabilities.  Request b has rows row_offsets[b] .. of target and drafts draft_offsets[b] .. (n of them: at
+ * most max_drafts and one less than its rows).  Draft j is accepted if accept[j] * draft[j, x_j] < target[row j, x_j] (draft null: the
+ * factor is one) and all before it are; with a of them accepted, the next token is the first at which the partial sum of
+ * max(target - draft, 0) (a = n: of target; draft null: of target without the refused token) exceeds sample[b] times its total, where there is
+ * no total, that of target; -1 if that has none either.  Shares that are not positive finite numbers count as zero; sums are in 64 bits. */
+typedef struct GdpaVerifyParams {
+  uint32_t struct_size;        /* sizeof(GdpaVerifyParams) */
+  int32_t is_bf16;             /* type of target and draft: 0 fp32, 1 bf16 */
+  const void* target;          /* [rows, vocab], contiguous in a row */
+  const void* draft;           /* [drafts, vocab], or null */
+  int64_t target_stride;       /* between rows */
+  int64_t draft_stride;
+  int64_t rows;
+  int64_t drafts;
+  int32_t vocab;               /* 1 to 2^20 */
+  int32_t tokens_are_int64;    /* type of tokens and out_tokens */
+  const void* tokens;          /* [drafts] */
+  const void* row_offsets;     /* [batch + 1] */
+  const void* draft_offsets;   /* [batch + 1] */
+  int32_t offsets_are_int64;
+  int32_t batch;
+  const float* accept;         /* [drafts], in [0, 1) */
+  const float* sample;         /* [batch], in [0, 1) */
+  int32_t max_drafts;
+  int32_t reserved;
+  void* out_tokens;            /* out [batch, max_drafts + 1]: the accepted drafts, the next token, then -1; a request without rows: -1 */
+  int32_t* accepted;           /* out [batch] */
+  int32_t* refused;            /* out [batch]: n - a */
+} GdpaVerifyParams;
+
+int gdpa_verify_draft_tokens(const GdpaVerifyParams* params, gdpa_stream_t stream);
+
+/* The last dropped[b] tokens (clamped to [0, seq_lens[b]]) of each request leave the cache: blocks that none of its tokens needs go onto the stack
+ * free_blocks[0 .. *num_free), in the order of the requests and their tables; entries that are no block do not, nor those that the stack has
+ * no place for.  Tables are only read. */
+typedef struct GdpaDropParams {
+  uint32_t struct_size;        /* sizeof(GdpaDropParams) */
+  int32_t block_size;
+  const int32_t* block_tables;
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t batch;
+  const void* seq_lens;        /* [batch] */
+  const void* dropped;         /* [batch] */
+  int32_t lens_are_int64;
+  int32_t dropped_is_int64;
+  int32_t* free_blocks;        /* in / out */
+  int64_t free_capacity;
+  const int32_t* num_free;     /* device; negative counts as 0 */
+  int32_t* seq_lens_after;     /* out [batch] */
+  int32_t* num_free_after;     /* out [1], not the word num_free points to */
+} GdpaDropParams;
+
+int gdpa_drop_cached_tokens(const GdpaDropParams* params, gdpa_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Backward.  Replaces torch.ops.gdpa.generalized_dot_product_attention_backward
  * (gdpa/triton/triton_generalized_dot_product_attention.py:3461-3788) and _flash_attn_bwd
  * (gdpa/src/interface.py:1257-1685): S and P are recomputed, dQ, dK, dV come out of one

@@ -764,26 +764,29 @@ int gdpa_append_rotated_kv_cache_fp8(const GdpaRotatedAppendParams* p, gdpa_stre
   bool rows = false;
   int rc = cache_append_args(&p->cache, a.cache, rows);
   if (rc != GDPA_OK) return rc;
-  if ((rc = rotary_spec(p->rotary, p->cache.head_dim, a.rotary)) != GDPA_OK) return rc;
+  RotarySpec& r = a.queries.rotary;
+  RotaryTensor &q = a.queries.t[0], &k = a.queries.t[1];
+  if ((rc = rotary_spec(p->rotary, p->cache.head_dim, r)) != GDPA_OK) return rc;
   const int elem = p->cache.x_is_fp32 != 0 ? 4 : 2;
   if (p->heads <= 0 || p->heads > (1 << 20) || p->cache.tokens >= (1ll << 30) || p->batch < 0 || p->position_stride < 0) return GDPA_ERR_BAD_ARG;
-  if ((rc = row_strides(p->query_strides, p->heads, p->cache.head_dim, elem, a.query_strides)) != GDPA_OK) return rc;
+  if ((rc = row_strides(p->query_strides, p->heads, p->cache.head_dim, elem, q.x_strides)) != GDPA_OK) return rc;
   if (p->cache.tokens == 0) return GDPA_OK;
   if (p->query == nullptr || p->query_out == nullptr) return GDPA_ERR_BAD_ARG;
   if (p->positions == nullptr && p->batch > 0 && (p->q_offsets == nullptr || p->seq_lens == nullptr)) return GDPA_ERR_BAD_ARG;
   if (!aligned16(p->query, p->query_out)) return GDPA_ERR_MISALIGNED;
   DeviceInfo di;
   if ((rc = device_info(&di)) != GDPA_OK) return rc;
-  a.query = p->query;
-  a.query_out = p->query_out;
-  a.heads = p->heads;
-  a.query_weight = a.rotary.norm ? p->query_weight : nullptr;
-  a.key_weight = a.rotary.norm ? p->key_weight : nullptr;
-  a.query_weight_is_bf16 = p->query_weight_is_bf16 != 0;
-  a.key_weight_is_bf16 = p->key_weight_is_bf16 != 0;
-  a.positions = p->positions;
-  a.position_stride = p->position_stride;
-  a.positions_are_int64 = p->positions_are_int64 != 0;
+  q.x = p->query;
+  q.y = p->query_out;
+  q.heads = p->heads;
+  q.tokens = p->cache.tokens;
+  q.positions = p->positions;
+  q.position_stride = p->position_stride;
+  q.positions_are_int64 = p->positions_are_int64 != 0;
+  q.weight = r.norm ? p->query_weight : nullptr;
+  q.weight_is_bf16 = p->query_weight_is_bf16 != 0;
+  k.weight = r.norm ? p->key_weight : nullptr;
+  k.weight_is_bf16 = p->key_weight_is_bf16 != 0;
   a.q_off = p->q_offsets;
   a.seq_lens = p->seq_lens;
   a.off64 = p->offsets_are_int64 != 0 ? kOffsets64 : 0;

@@ -9,7 +9,7 @@
 // token is -1.
 //
 // Sums are in 64 bits: a vocabulary's partial sums in fp32 would be off by more than most tokens' shares, and what comes out is a whole
-// number.  A request needs two rows at most, one pass over them: a cluster of CTAs sums stretches of 1024 tokens, and the stretch in which the
+// number.  A request needs two rows at most, one pass over them: a cluster of CTAs sums stretches of 256 or 1024 tokens, and the stretch in which the
 // sum passes its mark is looked at again (it is in the L2 cache).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -27,15 +27,17 @@ namespace gdpa {
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32;
-constexpr int kStretch = 1024;          // tokens of a stretch
-constexpr int kMostStretches = 1024;    // of a vocabulary
+constexpr int kVerifyThreads = 256, kVerifyWarps = kVerifyThreads / 32;
+constexpr int kVerifyCtas = 4;          // resident on an SM
+constexpr int kMostVocab = 1 << 20;
+constexpr int kMostStretches = kMostVocab / 1024;  // of a vocabulary
 constexpr int kMaxCluster = 8;
 
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-__device__ __forceinline__ double share(double x) { return x > 0 && x <= 1.7976931348623157e308 ? x : 0; }
+// positive finite numbers, as they are; anything else is 0
+__device__ __forceinline__ float share(float x) { return __float_as_uint(x) < 0x7f800000u ? x : 0.f; }
 
 __device__ __forceinline__ double warp_sum(double x) {
 #pragma unroll
@@ -47,21 +49,61 @@ __device__ __forceinline__ double warp_sum(double x) {
 template <class T>
 struct Left {
   const T* p;
-  const T* q;       // or null
-  long long without;  // or -1
-  __device__ __forceinline__ double at(float pv, float qv, int i) const {
-    double x = pv;
-    if (q != nullptr) x -= fmax(static_cast<double>(qv), 0.0);
-    return i == without ? 0 : share(x);
+  const T* q;  // or null
+  int without;  // or -1
+  __device__ __forceinline__ double operator()(int i) const {
+    const float pv = share(as_float(p[i])), qv = q != nullptr ? fmaxf(as_float(q[i]), 0.f) : 0.f;
+    return i != without && pv > qv ? static_cast<double>(pv) - static_cast<double>(qv) : 0;
   }
-  __device__ __forceinline__ double operator()(int i) const { return at(as_float(p[i]), q != nullptr ? as_float(q[i]) : 0.f, i); }
+  // the sum of 32 U tokens from i0 on, by a warp; WHOLE: they are all there
+  template <int U, bool WHOLE>
+  __device__ __forceinline__ double sum(int i0, int vocab) const {
+    constexpr int B = U < 16 ? U : 16;
+    double sums[2] = {0, 0};
+    const int lane = threadIdx.x & 31;
+    const T *const pp = p + i0 + lane, *const qq = q + i0 + lane;
+#pragma unroll
+    for (int u0 = 0; u0 < U; u0 += B) {
+      T a[B], b[B];
+#pragma unroll
+      for (int u = 0; u < B; ++u) a[u] = WHOLE || i0 + lane + (u0 + u) * 32 < vocab ? pp[(u0 + u) * 32] : static_cast<T>(0.f);
+      if (q != nullptr) {
+#pragma unroll
+        for (int u = 0; u < B; ++u) b[u] = WHOLE || i0 + lane + (u0 + u) * 32 < vocab ? qq[(u0 + u) * 32] : static_cast<T>(0.f);
+#pragma unroll
+        for (int u = 0; u < B; ++u) {
+          const float pv = share(as_float(a[u])), qv = fmaxf(as_float(b[u]), 0.f);
+          const double d = static_cast<double>(pv) - static_cast<double>(qv);
+          if (pv > qv) sums[u & 1] += d;
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < B; ++u) sums[u & 1] += static_cast<double>(share(as_float(a[u])));
+      }
+    }
+    double s = sums[0] + sums[1];
+    // the token that was refused, if it is one of the lane's
+    const int at = without - i0 - lane;
+    if (without >= 0 && at >= 0 && at < 32 * U && at % 32 == 0) s = sum_without(i0, U, vocab);
+    return warp_sum(s);
+  }
+  __device__ __noinline__ double sum_without(int i0, int U, int vocab) const {
+    double s = 0;
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + (threadIdx.x & 31) + u * 32;
+      if (i < vocab) s += (*this)(i);
+    }
+    return s;
+  }
 };
 
-template <class T>
-__global__ void __launch_bounds__(kVerifyThreads) gdpa_verify_kernel(const __grid_constant__ VerifyArgs a) {
+// U * 32 tokens are a stretch.
+template <class T, int U>
+__global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas) gdpa_verify_kernel(const __grid_constant__ VerifyArgs a) {
+  constexpr int kStretch = 32 * U;
   __shared__ double s_sum[kMostStretches];  // of a stretch; then up to its end
   __shared__ double s_total;                // of this CTA, for the cluster
-  __shared__ double s_share[32 * 33];
+  __shared__ double s_share[32 * (U + 1)];
   __shared__ int s_accepted, s_stretch;
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
@@ -116,7 +158,7 @@ __global__ void __launch_bounds__(kVerifyThreads) gdpa_verify_kernel(const __gri
   Left<T> left{target + (row0 + accepted) * a.target_stride, nullptr, -1};
   if (accepted < n) {
     if (draft != nullptr) left.q = draft + (d0 + accepted) * a.draft_stride;
-    else left.without = token_of(d0 + accepted);
+    else left.without = static_cast<int>(clamp_ll(token_of(d0 + accepted), -1, a.vocab));
   }
   // this CTA's stretches
   const int stretches = (a.vocab + kStretch - 1) / kStretch;
@@ -126,21 +168,8 @@ __global__ void __launch_bounds__(kVerifyThreads) gdpa_verify_kernel(const __gri
   int owner;
   for (;;) {
     for (int k = warp; k < mine; k += kVerifyWarps) {
-      double sum[2] = {0, 0};
-      const int i0 = (k0 + k) * kStretch + lane;
-#pragma unroll
-      for (int u0 = 0; u0 < kStretch / 32; u0 += 8) {
-        float p[8], q[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int i = i0 + (u0 + u) * 32;
-          p[u] = i < a.vocab ? as_float(left.p[i]) : 0.f;
-          q[u] = left.q != nullptr && i < a.vocab ? as_float(left.q[i]) : 0.f;
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) sum[u & 1] += left.at(p[u], q[u], i0 + (u0 + u) * 32);
-      }
-      const double s = warp_sum(sum[0] + sum[1]);
+      const int i0 = (k0 + k) * kStretch;
+      const double s = i0 + kStretch <= a.vocab ? left.template sum<U, true>(i0, a.vocab) : left.template sum<U, false>(i0, a.vocab);
       if (lane == 0) s_sum[k] = s;
     }
     __syncthreads();
@@ -199,13 +228,14 @@ __global__ void __launch_bounds__(kVerifyThreads) gdpa_verify_kernel(const __gri
   const int k = s_stretch;
   for (int i = threadIdx.x; i < kStretch; i += kVerifyThreads) {
     const int at = (k0 + k) * kStretch + i;
-    s_share[i / 32 * 33 + i % 32] = at < a.vocab ? left(at) : 0;
+    s_share[i / U * (U + 1) + i % U] = at < a.vocab ? left(at) : 0;
   }
   __syncthreads();
   if (warp != 0) return;
-  // 32 tokens of the stretch for each lane, then one
+  // U tokens of the stretch for each lane, then one
   double sum = 0;
-  for (int i = 0; i < 32; ++i) sum += s_share[lane * 33 + i];
+#pragma unroll
+  for (int i = 0; i < U; ++i) sum += s_share[lane * (U + 1) + i];
   double up_to = sum;
 #pragma unroll
   for (int s = 1; s < 32; s <<= 1) {
@@ -216,7 +246,7 @@ __global__ void __launch_bounds__(kVerifyThreads) gdpa_verify_kernel(const __gri
   unsigned with = __ballot_sync(kFull, sum > 0), those = __ballot_sync(kFull, sum > 0 && at_start + up_to > mark);
   const int row = those != 0 ? __ffs(those) - 1 : with != 0 ? 31 - __clz(with) : 0;
   const double at_row = at_start + __shfl_sync(kFull, up_to - sum, row);
-  const double mine_here = s_share[row * 33 + lane];
+  const double mine_here = lane < U ? s_share[row * (U + 1) + lane] : 0;
   up_to = mine_here;
 #pragma unroll
   for (int s = 1; s < 32; s <<= 1) {
@@ -225,7 +255,7 @@ __global__ void __launch_bounds__(kVerifyThreads) gdpa_verify_kernel(const __gri
   }
   with = __ballot_sync(kFull, mine_here > 0), those = __ballot_sync(kFull, mine_here > 0 && at_row + up_to > mark);
   const int column = those != 0 ? __ffs(those) - 1 : with != 0 ? 31 - __clz(with) : 0;
-  if (lane == 0) put(accepted, (k0 + k) * kStretch + row * 32 + column);
+  if (lane == 0) put(accepted, (k0 + k) * kStretch + row * U + column);
 }
 
 // ------------------------------------------------------------------------------------------ tokens that leave the cache
@@ -234,12 +264,12 @@ __global__ void __launch_bounds__(kVerifyThreads) gdpa_verify_kernel(const __gri
 // the order of the requests and of their tables (entries that are no block, -1, do not).  Tables are left as they are: what lies behind a
 // request's length is not looked at.
 //
-// Latency is all of it.  A warp has eight requests, whose entries it walks over 128 at a time: once to count them, once, when a
+// Latency is all of it.  A warp looks at four requests at a time, up to 128 entries of each, all asked for at once: first to count them, then, when a
 // cluster of CTAs has added up what comes before, to put them on the stack.
-constexpr int kDropWarps = 32, kDropRequests = 8;
+constexpr int kDropWarps = 32, kDropRequests = 4;
 
 __global__ void __launch_bounds__(kDropWarps * 32) gdpa_drop_kernel(const __grid_constant__ DropArgs a) {
-  __shared__ long long s_count[kDropWarps];
+  __shared__ int s_count[kDropWarps];
   __shared__ long long s_total;
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
@@ -248,57 +278,67 @@ __global__ void __launch_bounds__(kDropWarps * 32) gdpa_drop_kernel(const __grid
   const long long have = clamp_ll(*a.num_free, 0, a.free_capacity);
   // this warp's requests
   const int groups = (a.batch + kDropRequests - 1) / kDropRequests, all = ranks * kDropWarps, me = rank * kDropWarps + warp;
-  const int g0 = static_cast<int>(static_cast<long long>(groups) * me / all), g1 = static_cast<int>(static_cast<long long>(groups) * (me + 1) / all);
-  // all entries of the warp's requests, in order: body(lane has one, the entry, votes of the lanes that have one)
+  const int first = static_cast<int>(static_cast<long long>(groups) * me / all) * kDropRequests;
+  const int last = min(static_cast<int>(static_cast<long long>(groups) * (me + 1) / all) * kDropRequests, a.batch);
+  // all their entries that may go, in order: body(the lane's entry or -1, votes of the lanes that have one)
   auto walk = [&](bool write_lens, auto body) {
-    for (int g = g0; g < g1; ++g) {
-      const int b = g * kDropRequests + lane;
-      int keep = 0, count = 0;
-      if (lane < kDropRequests && b < a.batch) {
-        const long long len = clamp_ll(load_offset(a.seq_lens, b, a.lens64), 0, 0x7fffff00);
-        const long long after = len - clamp_ll(load_offset(a.dropped, b, a.dropped64), 0, len);
-        if (write_lens) a.seq_lens_after[b] = static_cast<int>(after);
+    for (int b0 = first; b0 < last; b0 += 32) {
+      int keep = 0, held = 0;
+      if (b0 + lane < last) {
+        const long long len = clamp_ll(load_offset(a.seq_lens, b0 + lane, a.lens64), 0, 0x7fffff00);
+        const long long after = len - clamp_ll(load_offset(a.dropped, b0 + lane, a.dropped64), 0, len);
+        if (write_lens) a.seq_lens_after[b0 + lane] = static_cast<int>(after);
         keep = static_cast<int>(min((after + S - 1) >> a.block_shift, static_cast<long long>(a.table_width)));
-        count = static_cast<int>(min((len + S - 1) >> a.block_shift, static_cast<long long>(a.table_width))) - keep;
+        held = static_cast<int>(min((len + S - 1) >> a.block_shift, static_cast<long long>(a.table_width)));
       }
-      long long up_to = count;
+      for (int g = 0; g < 32 && b0 + g < last; g += kDropRequests) {
+        int from[kDropRequests], to[kDropRequests], entry[kDropRequests][4];
 #pragma unroll
-      for (int s = 1; s < kDropRequests; s <<= 1) {
-        const long long o = __shfl_up_sync(kFull, up_to, s);
-        if (lane >= s) up_to += o;
-      }
-      const long long entries = __shfl_sync(kFull, up_to, kDropRequests - 1), before = up_to - count;
-      for (long long e0 = 0; e0 < entries; e0 += 128) {
-        int entry[4];
+        for (int i = 0; i < kDropRequests; ++i) {
+          from[i] = __shfl_sync(kFull, keep, g + i), to[i] = __shfl_sync(kFull, held, g + i);
+          const int* const row = a.block_tables + static_cast<long long>(b0 + g + i) * a.table_stride;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const long long e = e0 + 32 * u + lane;
-          int owner = 0;  // requests whose entries all lie before this one
-#pragma unroll
-          for (int s = kDropRequests / 2; s > 0; s >>= 1) owner += __shfl_sync(kFull, up_to, owner + s - 1) <= e ? s : 0;
-          const long long j = __shfl_sync(kFull, keep, owner) + e - __shfl_sync(kFull, before, owner);
-          entry[u] = e < entries ? a.block_tables[static_cast<long long>(g * kDropRequests + owner) * a.table_stride + j] : -1;
+          for (int u = 0; u < 4; ++u) {
+            const int j = from[i] + 32 * u + lane;
+            entry[i][u] = j < to[i] ? row[j] : -1;
+          }
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) body(entry[u], __ballot_sync(kFull, entry[u] >= 0));
+        for (int i = 0; i < kDropRequests; ++i) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (from[i] + 32 * u < to[i]) body(entry[i][u], __ballot_sync(kFull, entry[i][u] >= 0));
+          }
+          // a request with more
+          const int* const row = a.block_tables + static_cast<long long>(b0 + g + i) * a.table_stride;
+          for (int j = from[i] + 128 + lane; j - lane < to[i]; j += 32) {
+            const int e = j < to[i] ? row[j] : -1;
+            body(e, __ballot_sync(kFull, e >= 0));
+          }
+        }
       }
     }
   };
   long long count = 0;
   walk(true, [&](int, unsigned those) { count += __popc(those); });
-  if (lane == 0) s_count[warp] = count;
+  if (lane == 0) s_count[warp] = static_cast<int>(min(count, 0x3fffffffll));  // a stack has fewer places
   __syncthreads();
-  long long place = have, cta = 0;
-  for (int w = 0; w < kDropWarps; ++w) {
-    if (w < warp) place += s_count[w];
-    cta += s_count[w];
+  const int of_lane = s_count[lane];
+  long long up_to = of_lane;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const long long o = __shfl_up_sync(kFull, up_to, s);
+    if (lane >= s) up_to += o;
   }
-  if (threadIdx.x == 0) s_total = cta;
+  long long place = have + __shfl_sync(kFull, up_to - of_lane, warp);
+  if (warp == 0 && lane == 31) s_total = up_to;
   cluster.sync();
+  const long long of_rank = lane < ranks ? *cluster.map_shared_rank(&s_total, lane) : 0;
   long long total = 0;
   for (int r = 0; r < ranks; ++r) {
+    const long long x = __shfl_sync(kFull, of_rank, r);
     if (r == rank) place += total;
-    total += *cluster.map_shared_rank(&s_total, r);
+    total += x;
   }
   cluster.sync();  // before a CTA ends
   if (rank == 0 && threadIdx.x == 0) *a.num_free_after = static_cast<int>(clamp_ll(have + total, 0, a.free_capacity));
@@ -325,15 +365,21 @@ int launch_cluster(K kernel, const A& args, unsigned grid, unsigned threads, uns
 
 }  // namespace
 
-int verify_most_vocab() { return kMostStretches * kStretch; }
+int verify_most_vocab() { return kMostVocab; }
 
 int launch_verify(const VerifyArgs& a, int is_bf16, int sm_count, cudaStream_t stream) {
-  // CTAs of a request: until there are a few for each SM, and as long as each has several stretches
+  // CTAs of a request: as many as are resident at once with all requests', and as long as each has a few hundred tokens for each warp
   unsigned ranks = 1;
-  while (ranks < kMaxCluster && static_cast<long long>(a.batch) * ranks < 8ll * sm_count && a.vocab >= static_cast<int>(ranks) * 2 * 2 * kStretch) ranks *= 2;
+  while (ranks < kMaxCluster && 2ll * a.batch * ranks <= static_cast<long long>(kVerifyCtas) * sm_count && a.vocab > static_cast<int>(ranks) * kVerifyThreads * 8)
+    ranks *= 2;
   const unsigned grid = static_cast<unsigned>(a.batch) * ranks;
-  return is_bf16 ? launch_cluster(gdpa_verify_kernel<__nv_bfloat16>, a, grid, kVerifyThreads, ranks, stream)
-                 : launch_cluster(gdpa_verify_kernel<float>, a, grid, kVerifyThreads, ranks, stream);
+  auto launch = [&](auto type) {
+    using T = decltype(type);
+    // stretches of 256 tokens where long ones would leave warps without one
+    if (a.vocab < static_cast<int>(ranks) * kVerifyWarps * 1024) return launch_cluster(gdpa_verify_kernel<T, 8>, a, grid, kVerifyThreads, ranks, stream);
+    return launch_cluster(gdpa_verify_kernel<T, 32>, a, grid, kVerifyThreads, ranks, stream);
+  };
+  return is_bf16 ? launch(__nv_bfloat16{}) : launch(float{});
 }
 
 int launch_drop(const DropArgs& a, cudaStream_t stream) {

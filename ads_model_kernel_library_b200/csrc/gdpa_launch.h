@@ -285,37 +285,26 @@ struct RotaryTensor {
   long long position_stride;
   int positions_are_int64;
   void* dweight;           // [head_dim] of the weight's type, or null
-  int per_item;            // heads of an item, a multiple of a warp's
-  int chunks;              // items of a token
 };
 
 struct RotaryArgs {
   RotarySpec rotary;
   RotaryTensor t[2];  // queries, keys
   float* partial;     // backward: [grid][2][head_dim] sums of the weights' gradients, or null
+  // items: of queries, then of keys; or, where both have the same tokens and positions, of both at once
+  int paired;
+  int item_tokens[2], per[2], chunks[2];
+  unsigned items[2];
 };
 
 struct RotatedAppendArgs {
   CacheAppendArgs cache;  // its key and value are the new ones
-  RotarySpec rotary;
-  const void* query;
-  long long query_strides[2];
-  void* query_out;        // contiguous
-  int heads;
-  const void* query_weight;
-  const void* key_weight;
-  int query_weight_is_bf16, key_weight_is_bf16;
-  const void* positions;  // [axes, tokens], or null: they follow from the lengths
-  long long position_stride;
-  int positions_are_int64;
+  RotaryArgs queries;     // t[0]: the queries; t[1] has no tokens, its weight is the keys'.  Positions null: they follow from the lengths
   const void* q_off;      // [batch + 1]
   const void* seq_lens;   // [batch]
   int off64, lens64;
   int batch;
-  // the grid: kv_windows * kv_parts CTAs for keys and values, then those for queries
-  int kv_windows, kv_parts;
-  int per_item, chunks;   // as in RotaryTensor
-  long long items_per_warp;
+  int kv_windows, kv_parts;  // the grid's first kv_windows * kv_parts CTAs are for keys and values
 };
 
 struct CacheReadArgs {
@@ -338,6 +327,7 @@ struct CacheReadArgs {
   long long total;
   void* key;
   void* value;
+  int warp_tokens;  // rows of a warp, 32 at most
 };
 
 struct VerifyArgs {
@@ -402,7 +392,7 @@ int launch_rotary(RotaryArgs& a, int head_dim, int is_fp32, int sm_count, cudaSt
 int launch_rotary_bwd(RotaryArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream);  // kernels launched, or -(an error)
 int rotary_bwd_ctas(int sm_count);  // CTAs that have a row of RotaryArgs::partial each
 int launch_rotated_append(RotatedAppendArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream);
-int launch_cache_read(const CacheReadArgs& a, int head_dim, int out_is_fp32, int sm_count, cudaStream_t stream);
+int launch_cache_read(CacheReadArgs& a, int head_dim, int out_is_fp32, int sm_count, cudaStream_t stream);
 int launch_verify(const VerifyArgs& a, int is_bf16, int sm_count, cudaStream_t stream);
 int verify_most_vocab();
 int launch_drop(const DropArgs& a, cudaStream_t stream);

@@ -20,25 +20,10 @@ namespace gdpa {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kFwdCtas = 12;  // of an SM, at most
-constexpr int kBwdCtas = 4;
-
-// Item `i` of queries (0) or keys (1).
-struct Item {
-  int which, head0, head1;
-  long long token;
-};
-__device__ __forceinline__ Item item_at(const RotaryArgs& a, unsigned i, unsigned query_items) {
-  Item it;
-  it.which = i >= query_items;
-  const RotaryTensor& t = a.t[it.which];
-  if (it.which) i -= query_items;
-  const unsigned token = t.chunks == 1 ? i : i / static_cast<unsigned>(t.chunks);
-  it.token = token;
-  it.head0 = static_cast<int>(i - token * static_cast<unsigned>(t.chunks)) * t.per_item;
-  it.head1 = min(it.head0 + t.per_item, t.heads);
-  return it;
-}
+constexpr int kFwdCtas = 5;  // resident on an SM
+constexpr int kBwdCtas = 3;
+constexpr int kFwdRing = 6;  // units of a warp on their way
+constexpr int kBwdRing = 4;
 
 __device__ __forceinline__ long long position_at(const RotaryTensor& t, int axis, long long token) {
   const long long i = axis * t.position_stride + token;
@@ -46,190 +31,109 @@ __device__ __forceinline__ long long position_at(const RotaryTensor& t, int axis
 }
 
 template <class T, int D>
-__device__ __forceinline__ void take_weight(const HeadLanes<T, D>& h, const RotaryTensor& t, float (&w)[HeadLanes<T, D>::V]) {
-  constexpr int E = HeadLanes<T, D>::E;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    w[e] = weight_at(t.weight, t.weight_is_bf16, h.g0 * E + e);
-    w[E + e] = weight_at(t.weight, t.weight_is_bf16, h.g1 * E + e);
-  }
-}
-
-template <class T, int D>
-__global__ void __launch_bounds__(kWarps * 32) gdpa_rotary_kernel(const __grid_constant__ RotaryArgs a) {
-  using Lanes = HeadLanes<T, D>;
-  constexpr int E = Lanes::E, V = Lanes::V, U = 2;  // U warp-wide heads at once
-  __shared__ float4 s_angles[kWarps][2][D / 8];
+__global__ void __launch_bounds__(kWarps * 32, kFwdCtas) gdpa_rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  extern __shared__ uint4 s_ring[];  // [warp][kFwdRing] units
+  __shared__ float4 s_tables[kWarps][kItemTokens][D / 4];
+  __shared__ float4 s_weight[2][D / 4];
   const int warp = threadIdx.x >> 5;
-  const Lanes lanes(a.rotary);
-  const WarpAngles<T, D> angles(a.rotary);
-  float* const s_cos = reinterpret_cast<float*>(s_angles[warp][0]);
-  float* const s_sin = reinterpret_cast<float*>(s_angles[warp][1]);
-  const unsigned nq = static_cast<unsigned>(a.t[0].tokens * a.t[0].chunks), n = nq + static_cast<unsigned>(a.t[1].tokens * a.t[1].chunks);
-  int held = -1;  // whose weight this is
-  float w[V];
-  for (unsigned i = blockIdx.x * kWarps + warp; i < n; i += gridDim.x * kWarps) {
-    const Item it = item_at(a, i, nq);
-    const RotaryTensor& t = a.t[it.which];
-    const T* const x = static_cast<const T*>(t.x) + it.token * t.x_strides[0];
-    T* const y = static_cast<T*>(t.y) + it.token * t.heads * D;
-    uint4 u[U][2];
-    auto load = [&](int head0) {
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int head = head0 + k * Lanes::H + lanes.sub;
-        u[k][0] = u[k][1] = make_uint4(0, 0, 0, 0);
-        if (head < it.head1) {
-          const T* const p = x + head * t.x_strides[1];
-          u[k][0] = __ldg(reinterpret_cast<const uint4*>(p) + lanes.g0);
-          u[k][1] = __ldg(reinterpret_cast<const uint4*>(p) + lanes.g1);
-        }
-      }
-    };
-    load(it.head0);
-    if (held != it.which) {
-      held = it.which;
-      take_weight<T, D>(lanes, t, w);
-    }
-    __syncwarp();  // the last item's angles have been read
-    angles.write(s_cos, s_sin, [&](int axis) { return position_at(t, axis, it.token); });
-    __syncwarp();
-    float c[E], s[E];
-    if (lanes.rotated) lanes.take(s_cos, c), lanes.take(s_sin, s);
-    for (int head0 = it.head0;;) {
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int head = head0 + k * Lanes::H + lanes.sub;
-        float v[V];
-        Lanes::unpack(u[k], v);
-        if (a.rotary.norm) {
-          float ss = 0;
-#pragma unroll
-          for (int e = 0; e < V; ++e) ss += v[e] * v[e];
-          const float r = rsqrtf(Lanes::sum(ss) * (1.f / D) + a.rotary.eps);
-#pragma unroll
-          for (int e = 0; e < V; ++e) v[e] = v[e] * r * w[e];
-        }
-        lanes.template turn<false>(a.rotary.interleaved, c, s, v);
-        if (head < it.head1) {
-          uint4* const p = reinterpret_cast<uint4*>(y + static_cast<long long>(head) * D);
-          p[lanes.g0] = Piece<T>::pack(v);
-          p[lanes.g1] = Piece<T>::pack(v + E);
-        }
-      }
-      head0 += U * Lanes::H;
-      if (head0 >= it.head1) break;
-      load(head0);
-    }
-  }
+  rotate_items<T, D, kFwdRing>(a, s_ring + warp * kFwdRing * kUnitPieces, reinterpret_cast<float*>(s_tables[warp]), reinterpret_cast<float*>(s_weight), 2,
+                               blockIdx.x * kWarps + warp, gridDim.x * kWarps,
+                               [&](int k, int axis, long long token) { return position_at(a.t[k], axis, token); }, [](long long) {});
 }
 
-// dx, and the sums of dn x r of this CTA's items.  The sums are made twice over: a lane's over a few heads first, then those.  One sum over all of a
-// lane's heads would carry an error of 2^-24 sqrt(heads / 2), which long batches see.
+// dx, and the sums of dn x r of this CTA's items.  The sums are made twice over: a lane's over an item's heads in registers, then, in shared memory,
+// over its items.  One sum over all of a lane's heads would carry an error of 2^-24 sqrt(heads / 2), which long batches see.
 template <class T, int D>
 __global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gdpa_rotary_bwd_kernel(const __grid_constant__ RotaryArgs a) {
   using Lanes = HeadLanes<T, D>;
-  constexpr int E = Lanes::E, V = Lanes::V;
-  __shared__ float4 s_angles[kWarps][2][D / 8];
-  __shared__ float s_dw[kWarps][2][D];
+  constexpr int C = Lanes::C, E = Lanes::E;
+  extern __shared__ uint4 s_ring[];  // [warp][kBwdRing][x, dy] units; then, for the weights' gradients, sums [warp][2][2 C][32]
+  __shared__ float4 s_tables[kWarps][kItemTokens][D / 4];
+  __shared__ float4 s_weight[2][D / 4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Lanes lanes(a.rotary);
+  const unsigned n = a.items[0] + a.items[1], first = blockIdx.x * kWarps + warp;
+  uint4* const ring = s_ring + warp * kBwdRing * 2 * kUnitPieces;
+  Stream<T, D, 2, kBwdRing> stream(a, lanes, ring, first, gridDim.x * kWarps);
   const WarpAngles<T, D> angles(a.rotary);
-  float* const s_cos = reinterpret_cast<float*>(s_angles[warp][0]);
-  float* const s_sin = reinterpret_cast<float*>(s_angles[warp][1]);
-  const unsigned nq = static_cast<unsigned>(a.t[0].tokens * a.t[0].chunks), n = nq + static_cast<unsigned>(a.t[1].tokens * a.t[1].chunks);
-  int held = -1, few = 0;
-  float w[V], sum[V], part[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) sum[e] = part[e] = 0;
+  float* const tables = reinterpret_cast<float*>(s_tables[warp]);
+  uint64_t* const all_sums = reinterpret_cast<uint64_t*>(s_ring + kWarps * kBwdRing * 2 * kUnitPieces);
+  uint64_t* const sums = all_sums + warp * 2 * 2 * C * 32 + lane;
+  if (warp < 2) lanes.write_weight(reinterpret_cast<float*>(s_weight[warp]), a.t[warp].weight, a.t[warp].weight_is_bf16);
   if (a.partial != nullptr) {
-    for (int i = lane; i < 2 * D; i += 32) s_dw[warp][i / D][i % D] = 0;
-    __syncwarp();
+    for (int e = 0; e < 2 * 2 * C; ++e) sums[e * 32] = 0;
   }
-  auto flush = [&]() {  // a warp's sums of one tensor
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float x = sum[e] + part[e];
-#pragma unroll
-      for (int s = Lanes::L; s < 32; s <<= 1) x += __shfl_xor_sync(kAllLanes, x, s);
-      if (lanes.sub == 0) s_dw[warp][held][(e < E ? lanes.g0 : lanes.g1) * E + e % E] = x;
-      sum[e] = part[e] = 0;
-    }
-  };
-  for (unsigned i = blockIdx.x * kWarps + warp; i < n; i += gridDim.x * kWarps) {
-    const Item it = item_at(a, i, nq);
-    const RotaryTensor& t = a.t[it.which];
-    const T* const x = static_cast<const T*>(t.x) + it.token * t.x_strides[0];
-    const T* const dy = static_cast<const T*>(t.dy) + it.token * t.dy_strides[0];
-    T* const dx = static_cast<T*>(t.y) + it.token * t.heads * D;
-    uint4 ux[2], ug[2];
-    auto load = [&](int head0) {
-      const int head = head0 + lanes.sub;
-      ux[0] = ux[1] = ug[0] = ug[1] = make_uint4(0, 0, 0, 0);
-      if (head < it.head1) {
-        const T* const p = dy + head * t.dy_strides[1];
-        ug[0] = __ldg(reinterpret_cast<const uint4*>(p) + lanes.g0);
-        ug[1] = __ldg(reinterpret_cast<const uint4*>(p) + lanes.g1);
-        if (a.rotary.norm) {
-          const T* const q = x + head * t.x_strides[1];
-          ux[0] = __ldg(reinterpret_cast<const uint4*>(q) + lanes.g0);
-          ux[1] = __ldg(reinterpret_cast<const uint4*>(q) + lanes.g1);
-        }
-      }
-    };
-    load(it.head0);
-    if (held != it.which) {
-      if (held >= 0 && a.partial != nullptr) flush();
-      held = it.which;
-      take_weight<T, D>(lanes, t, w);
-    }
+  __syncthreads();
+  unsigned slot = 0;
+  for (unsigned i = first; i < n; i += gridDim.x * kWarps) {
+    const Item it = item_at(a, i);
     __syncwarp();
-    angles.write(s_cos, s_sin, [&](int axis) { return position_at(t, axis, it.token); });
+    for (int j = 0; j < it.tokens; ++j) angles.write(tables + j * D, [&](int axis) { return position_at(a.t[it.first], axis, it.token + j); });
     __syncwarp();
-    float c[E], s[E];
-    if (lanes.rotated) lanes.take(s_cos, c), lanes.take(s_sin, s);
-    for (int head0 = it.head0;;) {
-      const int head = head0 + lanes.sub;
-      float v[V], g[V];
-      Lanes::unpack(ux, v);
-      Lanes::unpack(ug, g);
-      head0 += Lanes::H;
-      if (head0 < it.head1) load(head0);
-      lanes.template turn<true>(a.rotary.interleaved, c, s, g);
-      if (a.rotary.norm) {
-        float ss = 0, gx = 0;
+    for (int k = it.first; k <= it.last; ++k) {
+      const RotaryTensor& t = a.t[k];
+      int u0, u1;
+      units_of(a, it, k, Lanes::H, u0, u1);
+      if (u0 >= u1) continue;
+      HeadWalk<T, D> dx;
+      dx.begin(static_cast<T*>(t.y), static_cast<long long>(t.heads) * D, D, lanes, it.token, u0, u1);
+      const float* const weight = reinterpret_cast<const float*>(s_weight[k]);
+      uint64_t part[2 * C];
 #pragma unroll
-        for (int e = 0; e < V; ++e) ss += v[e] * v[e], gx += g[e] * w[e] * v[e];
-        const float r = rsqrtf(Lanes::sum(ss) * (1.f / D) + a.rotary.eps);
-        const float m = Lanes::sum(gx) * (1.f / D) * r * r;
-        if (head < it.head1) {
+      for (int e = 0; e < 2 * C; ++e) part[e] = 0;
+      for (int j = 0; j < it.tokens; ++j) {
+        uint64_t c[C], s[C];
+        if (lanes.rotated) lanes.take(tables + j * D, c), lanes.take(tables + j * D + D / 2, s);
+        for (int u = u0; u < u1; ++u) {
+          stream.fetch();
+          fetch_wait<kBwdRing - 1>();
+          const uint4* const from = ring + slot * 2 * kUnitPieces;
+          slot = slot + 1 == kBwdRing ? 0 : slot + 1;
+          uint4 p[2];
+          fetched(from + kUnitPieces, p);
+          uint64_t g[2 * C];
+          Lanes::unpack(p, g);
+          if (lanes.rotated) Lanes::template turn<true>(a.rotary.interleaved, c, s, g);
+          const bool there = u * Lanes::H + lanes.sub < t.heads;
+          if (a.rotary.norm) {
+            uint64_t v[2 * C], gw[2 * C];
+            fetched(from, p);
+            Lanes::unpack(p, v);
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            part[e] += g[e] * (v[e] * r);
-            g[e] = r * (g[e] * w[e] - v[e] * m);
+            for (int e = 0; e < 2 * C; ++e) gw[e] = g[e];
+            lanes.times(weight, gw);
+            const float r = rsqrtf(Lanes::sum(Lanes::dot(v, v)) * (1.f / D) + a.rotary.eps);
+            const float m = Lanes::sum(Lanes::dot(gw, v)) * (1.f / D) * r * r;
+            Lanes::times(r, v);  // the normed head, without its weight
+            const uint64_t r2 = pack_f32x2(r, r), m2 = pack_f32x2(-m, -m);
+#pragma unroll
+            for (int e = 0; e < 2 * C; ++e) {
+              if (there) part[e] = fma_f32x2(g[e], v[e], part[e]);
+              g[e] = fma_f32x2(gw[e], r2, mul_f32x2(v[e], m2));  // r gw - x r m
+            }
           }
+          if (there) dx.store(lanes, g);
+          dx.next(u + 1 == u1);
         }
-        if (++few == 16) {
-          few = 0;
+      }
+      if (t.dweight != nullptr) {
 #pragma unroll
-          for (int e = 0; e < V; ++e) sum[e] += part[e], part[e] = 0;
-        }
+        for (int e = 0; e < 2 * C; ++e) sums[(k * 2 * C + e) * 32] = add_f32x2(sums[(k * 2 * C + e) * 32], part[e]);
       }
-      if (head < it.head1) {
-        uint4* const p = reinterpret_cast<uint4*>(dx + static_cast<long long>(head) * D);
-        p[lanes.g0] = Piece<T>::pack(g);
-        p[lanes.g1] = Piece<T>::pack(g + E);
-      }
-      if (head0 >= it.head1) break;
     }
   }
   if (a.partial != nullptr) {
-    if (held >= 0) flush();
+    // value i of a head: piece, and the lanes that have it in each of the warp's heads
     __syncthreads();
+    const int np = a.rotary.pairs / E;
     for (int i = threadIdx.x; i < 2 * D; i += kWarps * 32) {
+      const int k = i / D, g = i % D / E, e = i % E;
+      const int l = g < np ? g : g < 2 * np ? g - np : g / 2, second = g < np ? 0 : g < 2 * np ? 1 : g % 2;
       float x = 0;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) x += s_dw[k][i / D][i % D];
+      for (int w = 0; w < kWarps; ++w) {
+        for (int h = 0; h < Lanes::H; ++h)
+          x += reinterpret_cast<const float*>(all_sums)[2 * (((w * 2 + k) * 2 * C + second * C + e / 2) * 32 + h * Lanes::L + l) + e % 2];
+      }
       a.partial[static_cast<long long>(blockIdx.x) * 2 * D + i] = x;
     }
   }
@@ -263,15 +167,8 @@ int by_type(int head_dim, int is_fp32, F launch) {
   return cudaGetLastError() == cudaSuccess ? 0 : GDPA_ERR_LAUNCH_;
 }
 
-// Items for about `warps` warps, and CTAs for them, `most` at most.
-unsigned plan(RotaryArgs& a, int head_dim, int is_fp32, long long warps, long long most) {
-  const int a_warp = is_fp32 ? 256 / head_dim : 512 / head_dim;
-  long long items = 0;
-  for (RotaryTensor& t : a.t) {
-    split_heads(t.tokens, t.heads, a_warp, warps, t.per_item, t.chunks);
-    items += t.tokens * t.chunks;
-  }
-  const long long grid = (items + kWarps - 1) / kWarps;
+unsigned ctas(const RotaryArgs& a, long long most) {
+  const long long grid = (static_cast<long long>(a.items[0]) + a.items[1] + kWarps - 1) / kWarps;
   return static_cast<unsigned>(grid < most ? grid : most);
 }
 
@@ -280,18 +177,24 @@ unsigned plan(RotaryArgs& a, int head_dim, int is_fp32, long long warps, long lo
 int rotary_bwd_ctas(int sm_count) { return kBwdCtas * sm_count; }
 
 int launch_rotary(RotaryArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream) {
-  const unsigned grid = plan(a, head_dim, is_fp32, 16ll * sm_count, static_cast<long long>(kFwdCtas) * sm_count);
+  plan_items(a, head_dim, is_fp32, 16ll * sm_count);
+  const unsigned grid = ctas(a, static_cast<long long>(kFwdCtas) * sm_count);
   if (grid == 0) return 0;
   return by_type(head_dim, is_fp32, [&](auto type, auto dim) {
-    gdpa_rotary_kernel<decltype(type), decltype(dim)::value><<<grid, kWarps * 32, 0, stream>>>(a);
+    gdpa_rotary_kernel<decltype(type), decltype(dim)::value><<<grid, kWarps * 32, kWarps * kFwdRing * kUnitPieces * 16, stream>>>(a);
   });
 }
 
 int launch_rotary_bwd(RotaryArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream) {
-  const unsigned grid = plan(a, head_dim, is_fp32, 16ll * sm_count, rotary_bwd_ctas(sm_count));
+  plan_items(a, head_dim, is_fp32, static_cast<long long>(kBwdCtas) * kWarps * sm_count);
+  const unsigned grid = ctas(a, rotary_bwd_ctas(sm_count));
   if (grid > 0) {
+    // the ring, and a lane's sums of both tensors
+    const int smem = kWarps * kBwdRing * 2 * kUnitPieces * 16 + (a.partial != nullptr ? kWarps * 2 * (is_fp32 ? 8 : 16) * 32 * static_cast<int>(sizeof(float)) : 0);
     const int rc = by_type(head_dim, is_fp32, [&](auto type, auto dim) {
-      gdpa_rotary_bwd_kernel<decltype(type), decltype(dim)::value><<<grid, kWarps * 32, 0, stream>>>(a);
+      auto kernel = gdpa_rotary_bwd_kernel<decltype(type), decltype(dim)::value>;
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return;  // the launch then fails, and says so
+      kernel<<<grid, kWarps * 32, smem, stream>>>(a);
     });
     if (rc != 0) return -rc;
   }

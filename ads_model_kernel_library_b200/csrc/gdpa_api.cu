@@ -878,6 +878,8 @@ int gdpa_verify_draft_tokens(const GdpaVerifyParams* p, gdpa_stream_t stream) {
   return rc;
 }
 
+size_t gdpa_drop_workspace_bytes(int32_t batch) { return batch > 0 ? static_cast<size_t>(drop_workspace_ints(batch)) * sizeof(int) : 0; }
+
 int gdpa_drop_cached_tokens(const GdpaDropParams* p, gdpa_stream_t stream) {
   if (p == nullptr || p->struct_size != sizeof(GdpaDropParams)) return GDPA_ERR_BAD_ARG;
   const int shift = block_shift_of(p->block_size);
@@ -887,6 +889,10 @@ int gdpa_drop_cached_tokens(const GdpaDropParams* p, gdpa_stream_t stream) {
   if (p->batch > 0 && (p->seq_lens == nullptr || p->dropped == nullptr || p->seq_lens_after == nullptr)) return GDPA_ERR_BAD_ARG;
   if (p->batch > 0 && p->table_width > 0 && p->block_tables == nullptr) return GDPA_ERR_BAD_ARG;
   if (p->free_capacity > 0 && p->free_blocks == nullptr) return GDPA_ERR_BAD_ARG;
+  const size_t bytes = gdpa_drop_workspace_bytes(p->batch);
+  if (bytes > 0 && p->workspace == nullptr) return GDPA_ERR_BAD_ARG;
+  if (p->workspace_bytes < static_cast<int64_t>(bytes)) return GDPA_ERR_CAPACITY;
+  if (!aligned16(p->workspace, nullptr)) return GDPA_ERR_MISALIGNED;
   DeviceInfo di;
   int rc = device_info(&di);
   if (rc != GDPA_OK) return rc;
@@ -906,8 +912,9 @@ int gdpa_drop_cached_tokens(const GdpaDropParams* p, gdpa_stream_t stream) {
   a.num_free = p->num_free;
   a.seq_lens_after = p->seq_lens_after;
   a.num_free_after = p->num_free_after;
+  a.counts = static_cast<int*>(p->workspace);
   rc = launch_drop(a, static_cast<cudaStream_t>(stream));
-  if (rc == 0) g_launches.fetch_add(1);
+  if (rc == 0) g_launches.fetch_add(bytes > 0 ? 2 : 1);
   return rc;
 }
 

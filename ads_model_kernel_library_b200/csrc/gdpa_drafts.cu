@@ -55,30 +55,40 @@ struct Left {
     const float pv = share(as_float(p[i])), qv = q != nullptr ? fmaxf(as_float(q[i]), 0.f) : 0.f;
     return i != without && pv > qv ? static_cast<double>(pv) - static_cast<double>(qv) : 0;
   }
-  // the sum of 32 U tokens from i0 on, by a warp; WHOLE: they are all there
+  // The sum of 32 U tokens from i0 on, by a warp; WHOLE: they are all there.  Some of them are on their way while others are added.
   template <int U, bool WHOLE>
   __device__ __forceinline__ double sum(int i0, int vocab) const {
-    constexpr int B = U < 16 ? U : 16;
+    constexpr int B = 8;
     double sums[2] = {0, 0};
     const int lane = threadIdx.x & 31;
-    const T *const pp = p + i0 + lane, *const qq = q + i0 + lane;
+    const T* const pp = p + i0 + lane;
+    auto load = [&](const T* from, int u0, T (&x)[B]) {
 #pragma unroll
-    for (int u0 = 0; u0 < U; u0 += B) {
-      T a[B], b[B];
+      for (int u = 0; u < B; ++u) x[u] = WHOLE || i0 + lane + (u0 + u) * 32 < vocab ? from[(u0 + u) * 32] : static_cast<T>(0.f);
+    };
+    T a[2][B];
+    load(pp, 0, a[0]);
+    if (q != nullptr) {
+      const T* const qq = q + i0 + lane;
+      T b[2][B];
+      load(qq, 0, b[0]);
 #pragma unroll
-      for (int u = 0; u < B; ++u) a[u] = WHOLE || i0 + lane + (u0 + u) * 32 < vocab ? pp[(u0 + u) * 32] : static_cast<T>(0.f);
-      if (q != nullptr) {
-#pragma unroll
-        for (int u = 0; u < B; ++u) b[u] = WHOLE || i0 + lane + (u0 + u) * 32 < vocab ? qq[(u0 + u) * 32] : static_cast<T>(0.f);
+      for (int u0 = 0; u0 < U; u0 += B) {
+        const int now = u0 / B & 1;
+        if (u0 + B < U) load(pp, u0 + B, a[now ^ 1]), load(qq, u0 + B, b[now ^ 1]);
 #pragma unroll
         for (int u = 0; u < B; ++u) {
-          const float pv = share(as_float(a[u])), qv = fmaxf(as_float(b[u]), 0.f);
-          const double d = static_cast<double>(pv) - static_cast<double>(qv);
-          if (pv > qv) sums[u & 1] += d;
+          const float qv = fmaxf(as_float(b[now][u]), 0.f), larger = fmaxf(share(as_float(a[now][u])), qv);
+          sums[u & 1] += static_cast<double>(larger) - static_cast<double>(qv);
         }
-      } else {
+      }
+    } else {
 #pragma unroll
-        for (int u = 0; u < B; ++u) sums[u & 1] += static_cast<double>(share(as_float(a[u])));
+      for (int u0 = 0; u0 < U; u0 += B) {
+        const int now = u0 / B & 1;
+        if (u0 + B < U) load(pp, u0 + B, a[now ^ 1]);
+#pragma unroll
+        for (int u = 0; u < B; ++u) sums[u & 1] += static_cast<double>(share(as_float(a[now][u])));
       }
     }
     double s = sums[0] + sums[1];
@@ -264,91 +274,118 @@ __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas) gdpa_verify_kerne
 // the order of the requests and of their tables (entries that are no block, -1, do not).  Tables are left as they are: what lies behind a
 // request's length is not looked at.
 //
-// Latency is all of it.  A warp looks at four requests at a time, up to 128 entries of each, all asked for at once: first to count them, then, when a
-// cluster of CTAs has added up what comes before, to put them on the stack.
-constexpr int kDropWarps = 32, kDropRequests = 4;
+// Latency is all of it.  A warp has four requests, up to 128 entries of each, all asked for at once and kept in registers until it is known how many go
+// before them.  Up to 256 requests, a cluster of CTAs adds that up in shared memory.  More of them: one kernel counts, another, whose loads the end
+// of the first overlaps, adds up the counts of the CTAs before its own; 4096 requests with 64 entries each 48 us in one cluster, 9 so.
+constexpr int kDropWarps = 8, kDropRequests = 4;
 
+enum DropWay { kDropCluster, kDropCount, kDropStore };
+
+template <DropWay WAY>
 __global__ void __launch_bounds__(kDropWarps * 32) gdpa_drop_kernel(const __grid_constant__ DropArgs a) {
   __shared__ int s_count[kDropWarps];
-  __shared__ long long s_total;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  __shared__ int s_total;
+  __shared__ long long s_before[kDropWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int S = 1 << a.block_shift;
-  const long long have = clamp_ll(*a.num_free, 0, a.free_capacity);
-  // this warp's requests
-  const int groups = (a.batch + kDropRequests - 1) / kDropRequests, all = ranks * kDropWarps, me = rank * kDropWarps + warp;
-  const int first = static_cast<int>(static_cast<long long>(groups) * me / all) * kDropRequests;
-  const int last = min(static_cast<int>(static_cast<long long>(groups) * (me + 1) / all) * kDropRequests, a.batch);
-  // all their entries that may go, in order: body(the lane's entry or -1, votes of the lanes that have one)
-  auto walk = [&](bool write_lens, auto body) {
-    for (int b0 = first; b0 < last; b0 += 32) {
-      int keep = 0, held = 0;
-      if (b0 + lane < last) {
-        const long long len = clamp_ll(load_offset(a.seq_lens, b0 + lane, a.lens64), 0, 0x7fffff00);
-        const long long after = len - clamp_ll(load_offset(a.dropped, b0 + lane, a.dropped64), 0, len);
-        if (write_lens) a.seq_lens_after[b0 + lane] = static_cast<int>(after);
-        keep = static_cast<int>(min((after + S - 1) >> a.block_shift, static_cast<long long>(a.table_width)));
-        held = static_cast<int>(min((len + S - 1) >> a.block_shift, static_cast<long long>(a.table_width)));
-      }
-      for (int g = 0; g < 32 && b0 + g < last; g += kDropRequests) {
-        int from[kDropRequests], to[kDropRequests], entry[kDropRequests][4];
+  const int b0 = (blockIdx.x * kDropWarps + warp) * kDropRequests;
+  // the warp's requests, and those of their entries that may go
+  int keep = 0, held = 0;
+  if (lane < kDropRequests && b0 + lane < a.batch) {
+    const long long len = clamp_ll(load_offset(a.seq_lens, b0 + lane, a.lens64), 0, 0x7fffff00);
+    const long long after = len - clamp_ll(load_offset(a.dropped, b0 + lane, a.dropped64), 0, len);
+    if (WAY != kDropCount) a.seq_lens_after[b0 + lane] = static_cast<int>(after);
+    keep = static_cast<int>(min((after + S - 1) >> a.block_shift, static_cast<long long>(a.table_width)));
+    held = static_cast<int>(min((len + S - 1) >> a.block_shift, static_cast<long long>(a.table_width)));
+  }
+  int entry[kDropRequests][4];
 #pragma unroll
-        for (int i = 0; i < kDropRequests; ++i) {
-          from[i] = __shfl_sync(kFull, keep, g + i), to[i] = __shfl_sync(kFull, held, g + i);
-          const int* const row = a.block_tables + static_cast<long long>(b0 + g + i) * a.table_stride;
+  for (int i = 0; i < kDropRequests; ++i) {
+    const int from = __shfl_sync(kFull, keep, i), to = __shfl_sync(kFull, held, i);
+    const int* const row = a.block_tables + static_cast<long long>(b0 + i) * a.table_stride;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int j = from[i] + 32 * u + lane;
-            entry[i][u] = j < to[i] ? row[j] : -1;
-          }
-        }
+    for (int u = 0; u < 4; ++u) {
+      const int j = from + 32 * u + lane;
+      entry[i][u] = j < to ? row[j] : -1;
+    }
+  }
+  // all of them in order: body(the lane's entry or -1, votes of the lanes that have one)
+  auto walk = [&](auto body) {
 #pragma unroll
-        for (int i = 0; i < kDropRequests; ++i) {
+    for (int i = 0; i < kDropRequests; ++i) {
+      const int from = __shfl_sync(kFull, keep, i), to = __shfl_sync(kFull, held, i);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if (from[i] + 32 * u < to[i]) body(entry[i][u], __ballot_sync(kFull, entry[i][u] >= 0));
-          }
-          // a request with more
-          const int* const row = a.block_tables + static_cast<long long>(b0 + g + i) * a.table_stride;
-          for (int j = from[i] + 128 + lane; j - lane < to[i]; j += 32) {
-            const int e = j < to[i] ? row[j] : -1;
-            body(e, __ballot_sync(kFull, e >= 0));
-          }
-        }
+      for (int u = 0; u < 4; ++u) body(entry[i][u], __ballot_sync(kFull, entry[i][u] >= 0));
+      // a request with more
+      const int* const row = a.block_tables + static_cast<long long>(b0 + i) * a.table_stride;
+      for (int j = from + 128 + lane; j - lane < to; j += 32) {
+        const int e = j < to ? row[j] : -1;
+        body(e, __ballot_sync(kFull, e >= 0));
       }
     }
   };
-  long long count = 0;
-  walk(true, [&](int, unsigned those) { count += __popc(those); });
-  if (lane == 0) s_count[warp] = static_cast<int>(min(count, 0x3fffffffll));  // a stack has fewer places
-  __syncthreads();
-  const int of_lane = s_count[lane];
-  long long up_to = of_lane;
+  if (WAY != kDropStore) {
+    long long count = 0;
+    walk([&](int, unsigned those) { count += __popc(those); });
+    if (lane == 0) s_count[warp] = static_cast<int>(min(count, 0x0fffffffll));  // more than a stack that holds them once has places
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int total = 0;
+      for (int w = 0; w < kDropWarps; ++w) {
+        const int n = s_count[w];
+        s_count[w] = total;
+        total += n;
+      }
+      s_total = total;
+    }
+    __syncthreads();
+  }
+  if (WAY == kDropCount) {
+    int* const counts = a.counts + blockIdx.x * (kDropWarps + 1);
+    if (threadIdx.x < kDropWarps) counts[1 + threadIdx.x] = s_count[threadIdx.x];
+    if (threadIdx.x == 0) counts[0] = s_total;
+    return;
+  }
+  const long long have = clamp_ll(*a.num_free, 0, a.free_capacity);
+  long long place = have, total = 0;
+  if (WAY == kDropCluster) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    cluster.sync();
+    const int of_rank = lane < ranks ? *cluster.map_shared_rank(&s_total, lane) : 0;
+    for (int r = 0; r < ranks; ++r) {
+      const int n = __shfl_sync(kFull, of_rank, r);
+      if (r == rank) place += total;
+      total += n;
+    }
+    place += s_count[warp];
+    cluster.sync();  // before a CTA ends
+  } else {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // for the counts
+    long long before = 0;
+    for (int c = threadIdx.x; c < static_cast<int>(gridDim.x); c += kDropWarps * 32) {
+      const int n = a.counts[c * (kDropWarps + 1)];
+      total += n;
+      before += c < static_cast<int>(blockIdx.x) ? n : 0;
+    }
 #pragma unroll
-  for (int s = 1; s < 32; s <<= 1) {
-    const long long o = __shfl_up_sync(kFull, up_to, s);
-    if (lane >= s) up_to += o;
+    for (int s = 16; s > 0; s >>= 1) total += __shfl_xor_sync(kFull, total, s), before += __shfl_xor_sync(kFull, before, s);
+    __shared__ long long s_all[kDropWarps];
+    if (lane == 0) s_before[warp] = before, s_all[warp] = total;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < kDropWarps; ++w) place += s_before[w], total += s_all[w];
+    place += a.counts[blockIdx.x * (kDropWarps + 1) + 1 + warp];
   }
-  long long place = have + __shfl_sync(kFull, up_to - of_lane, warp);
-  if (warp == 0 && lane == 31) s_total = up_to;
-  cluster.sync();
-  const long long of_rank = lane < ranks ? *cluster.map_shared_rank(&s_total, lane) : 0;
-  long long total = 0;
-  for (int r = 0; r < ranks; ++r) {
-    const long long x = __shfl_sync(kFull, of_rank, r);
-    if (r == rank) place += total;
-    total += x;
-  }
-  cluster.sync();  // before a CTA ends
-  if (rank == 0 && threadIdx.x == 0) *a.num_free_after = static_cast<int>(clamp_ll(have + total, 0, a.free_capacity));
-  walk(false, [&](int entry, unsigned those) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.num_free_after = static_cast<int>(clamp_ll(have + total, 0, a.free_capacity));
+  walk([&](int entry_here, unsigned those) {
     const long long at = place + __popc(those & ((1u << lane) - 1));
-    if (entry >= 0 && at < a.free_capacity) a.free_blocks[at] = entry;
+    if (entry_here >= 0 && at < a.free_capacity) a.free_blocks[at] = entry_here;
     place += __popc(those);
   });
 }
 
+// `ranks`: CTAs of a cluster; 0: none, and the kernel before it on the stream may still run.
 template <class K, class A>
 int launch_cluster(K kernel, const A& args, unsigned grid, unsigned threads, unsigned ranks, cudaStream_t stream) {
   cudaLaunchConfig_t c = {};
@@ -356,8 +393,13 @@ int launch_cluster(K kernel, const A& args, unsigned grid, unsigned threads, uns
   c.blockDim = dim3(threads);
   c.stream = stream;
   cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = ranks, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  if (ranks > 0) {
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = ranks, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  } else {
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+  }
   c.attrs = at;
   c.numAttrs = 1;
   return cudaLaunchKernelEx(&c, kernel, args) == cudaSuccess ? 0 : GDPA_ERR_LAUNCH_;
@@ -382,9 +424,21 @@ int launch_verify(const VerifyArgs& a, int is_bf16, int sm_count, cudaStream_t s
   return is_bf16 ? launch(__nv_bfloat16{}) : launch(float{});
 }
 
+namespace {
+unsigned drop_ctas(long long batch) { return static_cast<unsigned>((batch + kDropWarps * kDropRequests - 1) / (kDropWarps * kDropRequests)); }
+}  // namespace
+
+long long drop_workspace_ints(long long batch) {
+  const unsigned ctas = drop_ctas(batch);
+  return ctas <= kMaxCluster ? 0 : static_cast<long long>(ctas) * (kDropWarps + 1);
+}
+
 int launch_drop(const DropArgs& a, cudaStream_t stream) {
-  const unsigned ranks = a.batch > kDropWarps * kDropRequests ? kMaxCluster : 1;
-  return launch_cluster(gdpa_drop_kernel, a, ranks, kDropWarps * 32, ranks, stream);
+  const unsigned ctas = a.batch > 0 ? drop_ctas(a.batch) : 1;
+  if (ctas <= kMaxCluster) return launch_cluster(gdpa_drop_kernel<kDropCluster>, a, ctas, kDropWarps * 32, ctas, stream);
+  gdpa_drop_kernel<kDropCount><<<ctas, kDropWarps * 32, 0, stream>>>(a);
+  if (cudaGetLastError() != cudaSuccess) return GDPA_ERR_LAUNCH_;
+  return launch_cluster(gdpa_drop_kernel<kDropStore>, a, ctas, kDropWarps * 32, 0, stream);
 }
 
 }  // namespace gdpa

@@ -291,9 +291,10 @@ struct RotaryArgs {
   RotarySpec rotary;
   RotaryTensor t[2];  // queries, keys
   float* partial;     // backward: [grid][2][head_dim] sums of the weights' gradients, or null
-  // items: of queries, then of keys; or, where both have the same tokens and positions, of both at once
+  // How the work is dealt out: of queries, then of keys; or, where both have the same tokens and positions, of both at once.
   int paired;
-  int item_tokens[2], per[2], chunks[2];
+  int item_tokens;        // tokens of an item
+  int per[2], chunks[2];  // units (the heads that a warp has at once) of an item, items of a token (1: some tokens are an item)
   unsigned items[2];
 };
 
@@ -364,6 +365,7 @@ struct DropArgs {
   const int* num_free;
   int* seq_lens_after;
   int* num_free_after;
+  int* counts;  // drop_workspace_ints
 };
 
 }  // namespace gdpa
@@ -395,6 +397,7 @@ int launch_rotated_append(RotatedAppendArgs& a, int head_dim, int is_fp32, int s
 int launch_cache_read(CacheReadArgs& a, int head_dim, int out_is_fp32, int sm_count, cudaStream_t stream);
 int launch_verify(const VerifyArgs& a, int is_bf16, int sm_count, cudaStream_t stream);
 int verify_most_vocab();
+long long drop_workspace_ints(long long batch);
 int launch_drop(const DropArgs& a, cudaStream_t stream);
 int launch_paged(const PagedLaunch& l, int head_dim);
 int launch_paged_rows(const PagedLaunch& l, int head_dim);  // of launch_paged, for row tiles of 256

@@ -20,25 +20,30 @@ namespace gdpa {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kFwdCtas = 5;  // resident on an SM
+constexpr int kFwdCtas = 4;  // resident on an SM
 constexpr int kBwdCtas = 3;
-constexpr int kFwdRing = 6;  // units of a warp on their way
+constexpr int kFwdRing = 3;  // groups of units of a warp on their way
 constexpr int kBwdRing = 4;
+constexpr int kBwdTokens = 6;  // of an item
 
-__device__ __forceinline__ long long position_at(const RotaryTensor& t, int axis, long long token) {
-  const long long i = axis * t.position_stride + token;
+// The lane's position of an item's.
+__device__ __forceinline__ long long position_of(const RotaryArgs& a, const Item& it) {
+  const RotaryTensor& t = a.t[it.first];
+  const int lane = threadIdx.x & 31, axis = lane / kMostItemTokens, j = lane % kMostItemTokens;
+  if (axis >= a.rotary.axes || j >= it.tokens || a.rotary.pairs == 0) return 0;
+  const long long i = axis * t.position_stride + it.token + j;
   return t.positions_are_int64 ? static_cast<const long long*>(t.positions)[i] : static_cast<const int*>(t.positions)[i];
 }
 
 template <class T, int D>
 __global__ void __launch_bounds__(kWarps * 32, kFwdCtas) gdpa_rotary_kernel(const __grid_constant__ RotaryArgs a) {
-  extern __shared__ uint4 s_ring[];  // [warp][kFwdRing] units
-  __shared__ float4 s_tables[kWarps][kItemTokens][D / 4];
+  extern __shared__ uint4 s_ring[];  // [warp][kFwdRing][kTogether] units
+  __shared__ float4 s_tables[kWarps][kTokens][D / 4];
   __shared__ float4 s_weight[2][D / 4];
   const int warp = threadIdx.x >> 5;
-  rotate_items<T, D, kFwdRing>(a, s_ring + warp * kFwdRing * kUnitPieces, reinterpret_cast<float*>(s_tables[warp]), reinterpret_cast<float*>(s_weight), 2,
-                               blockIdx.x * kWarps + warp, gridDim.x * kWarps,
-                               [&](int k, int axis, long long token) { return position_at(a.t[k], axis, token); }, [](long long) {});
+  auto positions = [&](const Item& it) { return position_of(a, it); };
+  rotate_items<T, D, kFwdRing>(a, s_ring + warp * kFwdRing * kTogether * kUnitPieces, reinterpret_cast<float*>(s_tables[warp]), reinterpret_cast<float*>(s_weight), 2,
+                               Cursor(blockIdx.x * kWarps + warp, gridDim.x * kWarps), positions);
 }
 
 // dx, and the sums of dn x r of this CTA's items.  The sums are made twice over: a lane's over an item's heads in registers, then, in shared memory,
@@ -48,13 +53,16 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gdpa_rotary_bwd_kernel(
   using Lanes = HeadLanes<T, D>;
   constexpr int C = Lanes::C, E = Lanes::E;
   extern __shared__ uint4 s_ring[];  // [warp][kBwdRing][x, dy] units; then, for the weights' gradients, sums [warp][2][2 C][32]
-  __shared__ float4 s_tables[kWarps][kItemTokens][D / 4];
+  __shared__ float4 s_tables[kWarps][kBwdTokens][D / 4];
   __shared__ float4 s_weight[2][D / 4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Lanes lanes(a.rotary);
-  const unsigned n = a.items[0] + a.items[1], first = blockIdx.x * kWarps + warp;
+  Cursor cursor(blockIdx.x * kWarps + warp, gridDim.x * kWarps);
   uint4* const ring = s_ring + warp * kBwdRing * 2 * kUnitPieces;
-  Stream<T, D, 2, kBwdRing> stream(a, lanes, ring, first, gridDim.x * kWarps);
+  Stream<T, D, 2, 1, kBwdRing> stream(a, lanes, ring, cursor);
+  Item it, next;
+  bool more = cursor.next(a, next);
+  long long next_position = more ? position_of(a, next) : 0;
   const WarpAngles<T, D> angles(a.rotary);
   float* const tables = reinterpret_cast<float*>(s_tables[warp]);
   uint64_t* const all_sums = reinterpret_cast<uint64_t*>(s_ring + kWarps * kBwdRing * 2 * kUnitPieces);
@@ -65,18 +73,18 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gdpa_rotary_bwd_kernel(
   }
   __syncthreads();
   unsigned slot = 0;
-  for (unsigned i = first; i < n; i += gridDim.x * kWarps) {
-    const Item it = item_at(a, i);
-    __syncwarp();
-    for (int j = 0; j < it.tokens; ++j) angles.write(tables + j * D, [&](int axis) { return position_at(a.t[it.first], axis, it.token + j); });
-    __syncwarp();
+  while (more) {
+    it = next;
+    const long long its_position = next_position;
+    if ((more = cursor.next(a, next))) next_position = position_of(a, next);
+    angles.template write_all<kBwdTokens>(tables, it.tokens, its_position);
     for (int k = it.first; k <= it.last; ++k) {
       const RotaryTensor& t = a.t[k];
       int u0, u1;
       units_of(a, it, k, Lanes::H, u0, u1);
       if (u0 >= u1) continue;
       HeadWalk<T, D> dx;
-      dx.begin(static_cast<T*>(t.y), static_cast<long long>(t.heads) * D, D, lanes, it.token, u0, u1);
+      dx.begin(static_cast<T*>(t.y), static_cast<long long>(t.heads) * D, D, lanes, it.token, u0, u1, 1);
       const float* const weight = reinterpret_cast<const float*>(s_weight[k]);
       uint64_t part[2 * C];
 #pragma unroll
@@ -96,14 +104,20 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gdpa_rotary_bwd_kernel(
           if (lanes.rotated) Lanes::template turn<true>(a.rotary.interleaved, c, s, g);
           const bool there = u * Lanes::H + lanes.sub < t.heads;
           if (a.rotary.norm) {
-            uint64_t v[2 * C], gw[2 * C];
+            uint64_t v[2 * C], weighed[1][2 * C];
+            uint64_t(&gw)[2 * C] = weighed[0];
             fetched(from, p);
             Lanes::unpack(p, v);
 #pragma unroll
             for (int e = 0; e < 2 * C; ++e) gw[e] = g[e];
-            lanes.times(weight, gw);
-            const float r = rsqrtf(Lanes::sum(Lanes::dot(v, v)) * (1.f / D) + a.rotary.eps);
-            const float m = Lanes::sum(Lanes::dot(gw, v)) * (1.f / D) * r * r;
+            lanes.times(weight, weighed);
+            float sums_of[2] = {Lanes::dot(v, v), Lanes::dot(gw, v)};
+#pragma unroll
+            for (int l = 1; l < Lanes::L; l <<= 1) {
+#pragma unroll
+              for (int x = 0; x < 2; ++x) sums_of[x] += __shfl_xor_sync(kAllLanes, sums_of[x], l);
+            }
+            const float r = rsqrtf(sums_of[0] * (1.f / D) + a.rotary.eps), m = sums_of[1] * (1.f / D) * r * r;
             Lanes::times(r, v);  // the normed head, without its weight
             const uint64_t r2 = pack_f32x2(r, r), m2 = pack_f32x2(-m, -m);
 #pragma unroll
@@ -112,7 +126,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gdpa_rotary_bwd_kernel(
               g[e] = fma_f32x2(gw[e], r2, mul_f32x2(v[e], m2));  // r gw - x r m
             }
           }
-          if (there) dx.store(lanes, g);
+          if (there) dx.store(lanes, 0, g);
           dx.next(u + 1 == u1);
         }
       }
@@ -125,10 +139,10 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gdpa_rotary_bwd_kernel(
   if (a.partial != nullptr) {
     // value i of a head: piece, and the lanes that have it in each of the warp's heads
     __syncthreads();
-    const int np = a.rotary.pairs / E;
     for (int i = threadIdx.x; i < 2 * D; i += kWarps * 32) {
       const int k = i / D, g = i % D / E, e = i % E;
-      const int l = g < np ? g : g < 2 * np ? g - np : g / 2, second = g < np ? 0 : g < 2 * np ? 1 : g % 2;
+      bool second;
+      const int l = Lanes::lane_of_piece(a.rotary, g, second);
       float x = 0;
       for (int w = 0; w < kWarps; ++w) {
         for (int h = 0; h < Lanes::H; ++h)
@@ -177,16 +191,16 @@ unsigned ctas(const RotaryArgs& a, long long most) {
 int rotary_bwd_ctas(int sm_count) { return kBwdCtas * sm_count; }
 
 int launch_rotary(RotaryArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream) {
-  plan_items(a, head_dim, is_fp32, 16ll * sm_count);
+  plan_items(a, head_dim, is_fp32, static_cast<long long>(kFwdCtas) * kWarps * sm_count, kTokens);
   const unsigned grid = ctas(a, static_cast<long long>(kFwdCtas) * sm_count);
   if (grid == 0) return 0;
   return by_type(head_dim, is_fp32, [&](auto type, auto dim) {
-    gdpa_rotary_kernel<decltype(type), decltype(dim)::value><<<grid, kWarps * 32, kWarps * kFwdRing * kUnitPieces * 16, stream>>>(a);
+    gdpa_rotary_kernel<decltype(type), decltype(dim)::value><<<grid, kWarps * 32, kWarps * kFwdRing * kTogether * kUnitPieces * 16, stream>>>(a);
   });
 }
 
 int launch_rotary_bwd(RotaryArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream) {
-  plan_items(a, head_dim, is_fp32, static_cast<long long>(kBwdCtas) * kWarps * sm_count);
+  plan_items(a, head_dim, is_fp32, static_cast<long long>(kBwdCtas) * kWarps * sm_count, kBwdTokens);
   const unsigned grid = ctas(a, rotary_bwd_ctas(sm_count));
   if (grid > 0) {
     // the ring, and a lane's sums of both tensors

@@ -7,7 +7,7 @@
 //
 // A lane has two pieces of 16 bytes of a head: those that hold both halves of its pairs, so that nothing but the norm's sum crosses lanes.
 // With R a multiple of a piece's E values, lane l < R / E has the pieces l and l + R / E (both styles of pairs lie within these two), the
-// other lanes have two neighbouring pieces behind the rotated ones.  A head is L = D / 2E lanes: 8 for 128 values of bf16, so a
+// other lanes have two of those behind them, so that neighbouring lanes have neighbouring pieces.  A head is L = D / 2E lanes: 8 for 128 values of bf16, so a
 // warp-wide load is four heads' 128-byte halves.
 //
 // Angles: the product of position and frequency is taken in 64 bits and loses its whole turns there, 2 pi in two parts, before it becomes fp32 (a
@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "gdpa_common.cuh"
 #include "gdpa_launch.h"
@@ -27,6 +28,8 @@
 namespace gdpa {
 
 constexpr unsigned kAllLanes = 0xffffffffu;
+constexpr int kMostItemTokens = 8;  // tokens of a warp at a time
+static_assert(kMaxAxes * kMostItemTokens <= 32, "a lane has one of their positions");
 
 __device__ __forceinline__ float weight_at(const void* w, int is_bf16, int i) {
   if (w == nullptr) return 1.f;
@@ -48,14 +51,20 @@ struct HeadLanes {
     const int lane = threadIdx.x & 31, np = r.pairs / E;
     l = lane % L, sub = lane / L;
     rotated = l < np;
-    g0 = rotated ? l : 2 * l;  // behind the 2 np rotated pieces: 2 np + 2 (l - np)
-    g1 = rotated ? l + np : 2 * l + 1;
+    g0 = rotated ? l : np + l;  // behind the 2 np rotated pieces, in two halves: 2 np + (l - np)
+    g1 = rotated ? l + np : L + l;
   }
   // the sum over a head's lanes
   static __device__ __forceinline__ float sum(float x) {
 #pragma unroll
     for (int s = 1; s < L; s <<= 1) x += __shfl_xor_sync(kAllLanes, x, s);
     return x;
+  }
+  // Which lane of a head has piece g, and whether as its second one.
+  static __device__ __forceinline__ int lane_of_piece(const RotarySpec& r, int g, bool& second) {
+    const int np = r.pairs / E;
+    second = g < 2 * np ? g >= np : g >= np + L;
+    return g < np ? g : g < np + L ? g - np : g - L;
   }
   // Where a table of D / 2 values has value e of lane l: the lanes' 16-byte reads are neighbours.
   static __device__ __forceinline__ int slot(int l, int e) { return ((e >> 2) * L + l) * 4 + (e & 3); }
@@ -81,13 +90,17 @@ struct HeadLanes {
       table[D / 2 + slot(l, e)] = weight_at(weight, is_bf16, g1 * E + e);
     }
   }
-  __device__ __forceinline__ void times(const float* table, uint64_t (&v)[2 * C]) const {
+  template <int N>
+  __device__ __forceinline__ void times(const float* table, uint64_t (&v)[N][2 * C]) const {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       uint64_t w[C];
       take(table + p * (D / 2), w);
 #pragma unroll
-      for (int k = 0; k < C; ++k) v[p * C + k] = mul_f32x2(v[p * C + k], w[k]);
+      for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int k = 0; k < C; ++k) v[n][p * C + k] = mul_f32x2(v[n][p * C + k], w[k]);
+      }
     }
   }
   static __device__ __forceinline__ void times(float f, uint64_t (&v)[2 * C]) {
@@ -118,10 +131,25 @@ struct HeadLanes {
     for (int e = 0; e < C; ++e) unpack_f32x2(v[e], p[2 * e], p[2 * e + 1]);
     return Piece<T>::pack(p);
   }
+  // The norms of N heads; `weight` as above.  The factor comes before the weight: a head whose squares overflow is zeros, whatever its weight.
+  template <int N>
+  __device__ __forceinline__ void norm(const RotarySpec& r, const float* weight, uint64_t (&v)[N][2 * C]) const {
+    if (!r.norm) return;
+    float f[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) f[n] = dot(v[n], v[n]);
+#pragma unroll
+    for (int i = 1; i < L; i <<= 1) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) f[n] += __shfl_xor_sync(kAllLanes, f[n], i);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) times(rsqrtf(f[n] * (1.f / D) + r.eps), v[n]);
+    times(weight, v);
+  }
   // The lane's values turned by its angles (not to be called for a lane whose values are not rotated); `back`: the other way.
   template <bool back>
   static __device__ __forceinline__ void turn(bool interleaved, const uint64_t (&c)[C], const uint64_t (&s)[C], uint64_t (&v)[2 * C]) {
-    constexpr uint64_t kSigns = 0x8000000080000000ull;
     if (interleaved) {
 #pragma unroll
       for (int k = 0; k < C; ++k) {
@@ -138,9 +166,9 @@ struct HeadLanes {
     } else {
 #pragma unroll
       for (int k = 0; k < C; ++k) {
-        const uint64_t a = v[k], b = v[C + k], minus = s[k] ^ kSigns;
-        v[k] = fma_f32x2(a, c[k], mul_f32x2(b, back ? s[k] : minus));
-        v[C + k] = fma_f32x2(b, c[k], mul_f32x2(a, back ? minus : s[k]));
+        const uint64_t a = v[k], b = v[C + k];
+        v[k] = back ? fma_f32x2(a, c[k], mul_f32x2(b, s[k])) : sub_f32x2(mul_f32x2(a, c[k]), mul_f32x2(b, s[k]));
+        v[C + k] = back ? sub_f32x2(mul_f32x2(b, c[k]), mul_f32x2(a, s[k])) : fma_f32x2(b, c[k], mul_f32x2(a, s[k]));
       }
     }
   }
@@ -185,8 +213,19 @@ struct WarpAngles {
   __device__ __forceinline__ void write(float* table, F position) const {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      if (at[k] >= 0) sin_cos<T>(frequency[k], position(axis[k]), table[D / 2 + at[k]], table[at[k]]);
+      const long long p = position(axis[k]);
+      if (at[k] >= 0) sin_cos<T>(frequency[k], p, table[D / 2 + at[k]], table[at[k]]);
     }
+  }
+  // Tables of an item's tokens, TOKENS at most.  `mine`: lane axis * kMostItemTokens + j has token j's position on the axis.
+  template <int TOKENS>
+  __device__ __forceinline__ void write_all(float* tables, int tokens, long long mine) const {
+    __syncwarp();  // the last item's have been read
+#pragma unroll
+    for (int j = 0; j < TOKENS; ++j) {
+      if (j < tokens) write(tables + j * D, [&](int axis) { return __shfl_sync(kAllLanes, mine, axis * kMostItemTokens + j); });
+    }
+    __syncwarp();
   }
 };
 
@@ -194,24 +233,28 @@ struct WarpAngles {
 template <class T, int D>
 struct HeadWalk {
   T* at = nullptr;
-  long long unit = 0, token = 0;  // steps to the next unit; to the next token, from its last unit
-  __device__ __forceinline__ void begin(T* x, long long token_stride, long long head_stride, const HeadLanes<T, D>& lanes, long long t0, int u0, int u1) {
+  long long unit = 0, step = 0, token = 0;  // to the next unit; to the unit after the next `together`; to the next token, instead of the last such step
+  __device__ __forceinline__ void begin(T* x, long long token_stride, long long head_stride, const HeadLanes<T, D>& lanes, long long t0, int u0, int u1,
+                                        int together) {
     at = x + t0 * token_stride + (u0 * HeadLanes<T, D>::H + lanes.sub) * head_stride;
     unit = HeadLanes<T, D>::H * head_stride;
-    token = token_stride - (u1 - u0 - 1) * unit;
+    step = together * unit;
+    token = token_stride - (u1 - u0 - 1) / together * step;
   }
-  __device__ __forceinline__ void next(bool last) { at += last ? token : unit; }
+  __device__ __forceinline__ void next(bool last) { at += last ? token : step; }
   // into the lane's place of a unit's kilobyte of shared memory; zeros where there is no head
-  __device__ __forceinline__ void fetch(const HeadLanes<T, D>& lanes, uint4* to, bool there) const {
+  __device__ __forceinline__ void fetch(const HeadLanes<T, D>& lanes, int i, uint4* to, bool there) const {
     const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(to)) + (threadIdx.x & 31) * 16;
-    const uint4 *p = reinterpret_cast<const uint4*>(at) + lanes.g0, *q = reinterpret_cast<const uint4*>(at) + lanes.g1;
+    const uint4* const row = reinterpret_cast<const uint4*>(at + i * unit);
+    const uint4 *p = row + lanes.g0, *q = row + lanes.g1;
     const int size = there ? 16 : 0;
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(p), "r"(size) : "memory");
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s + 512), "l"(q), "r"(size) : "memory");
   }
-  __device__ __forceinline__ void store(const HeadLanes<T, D>& lanes, const uint64_t (&v)[2 * HeadLanes<T, D>::C]) const {
-    reinterpret_cast<uint4*>(at)[lanes.g0] = HeadLanes<T, D>::pack(v);
-    reinterpret_cast<uint4*>(at)[lanes.g1] = HeadLanes<T, D>::pack(v + HeadLanes<T, D>::C);
+  __device__ __forceinline__ void store(const HeadLanes<T, D>& lanes, int i, const uint64_t (&v)[2 * HeadLanes<T, D>::C]) const {
+    uint4* const row = reinterpret_cast<uint4*>(at + i * unit);
+    row[lanes.g0] = HeadLanes<T, D>::pack(v);
+    row[lanes.g1] = HeadLanes<T, D>::pack(v + HeadLanes<T, D>::C);
   }
 };
 
@@ -222,38 +265,38 @@ __device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_g
 template <int N>
 __device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// A unit's heads, normed and turned.
-template <class T, int D>
-__device__ __forceinline__ void rotate_unit(const RotarySpec& r, const HeadLanes<T, D>& lanes, const float* weight, const uint64_t (&c)[HeadLanes<T, D>::C],
-                                            const uint64_t (&s)[HeadLanes<T, D>::C], uint64_t (&v)[2 * HeadLanes<T, D>::C]) {
-  using Lanes = HeadLanes<T, D>;
-  float f = 1;
-  if (r.norm) {
-    f = rsqrtf(Lanes::sum(Lanes::dot(v, v)) * (1.f / D) + r.eps);
-    lanes.times(weight, v);
-  }
-  if (lanes.rotated) Lanes::template turn<false>(r.interleaved, c, s, v);
-  if (r.norm) Lanes::times(f, v);
-}
-
 // Some tokens and units: of queries, of keys, or, paired, of both (a token's units are then its queries' and behind them its keys').
 struct Item {
   long long token;
   int tokens, u0, u1;
   int first, last;  // tensors
 };
-__device__ __forceinline__ Item item_at(const RotaryArgs& a, unsigned i) {
-  Item it;
-  const int k = i >= a.items[0];
-  if (k) i -= a.items[0];
-  const unsigned group = a.chunks[k] == 1 ? i : i / static_cast<unsigned>(a.chunks[k]);
-  it.token = static_cast<long long>(group) * a.item_tokens[k];
-  it.tokens = static_cast<int>(min(static_cast<long long>(a.item_tokens[k]), a.t[k].tokens - it.token));
-  it.u0 = static_cast<int>(i - group * static_cast<unsigned>(a.chunks[k])) * a.per[k];
-  it.u1 = it.u0 + a.per[k];
-  it.first = k, it.last = a.paired ? 1 : k;
-  return it;
-}
+// A warp's items, the w-th of every n: what the warps have in hand at a time lies close together.
+struct Cursor {
+  unsigned w, n;
+  int k = -1;  // queries or keys
+  unsigned at = 0, end = 0;
+  __device__ __forceinline__ Cursor(unsigned warp, unsigned warps) : w(warp), n(warps) {}
+  __device__ __forceinline__ bool next(const RotaryArgs& a, Item& it) {
+    while (at >= end) {
+      if (++k > (a.paired ? 0 : 1)) return false;
+      at = w, end = a.items[k];
+    }
+    it.first = k, it.last = a.paired ? 1 : k;
+    it.u0 = 0, it.u1 = a.per[k];
+    if (a.chunks[k] == 1) {
+      it.token = static_cast<long long>(at) * a.item_tokens;
+      it.tokens = static_cast<int>(min(a.t[k].tokens - it.token, static_cast<long long>(a.item_tokens)));
+    } else {
+      it.token = at / static_cast<unsigned>(a.chunks[k]);
+      it.tokens = 1;
+      it.u0 = static_cast<int>(at - static_cast<unsigned>(it.token) * a.chunks[k]) * a.per[k];
+      it.u1 += it.u0;
+    }
+    at += n;
+    return true;
+  }
+};
 // The units of an item that are tensor k's, [u0, u1) of its own; none: u0 >= u1.
 __device__ __forceinline__ void units_of(const RotaryArgs& a, const Item& it, int k, int heads_a_unit, int& u0, int& u1) {
   const int before = k > it.first ? (a.t[0].heads + heads_a_unit - 1) / heads_a_unit : 0;
@@ -261,141 +304,149 @@ __device__ __forceinline__ void units_of(const RotaryArgs& a, const Item& it, in
   u1 = min(it.u1 - before, (a.t[k].heads + heads_a_unit - 1) / heads_a_unit);
 }
 
-// The units of a warp's items, one after the other, fetched ahead of their use: of x, and (N = 2) behind it of dy.
-template <class T, int D, int N, int RING>
+// The units of a warp's items, U of a token at a time, fetched ahead of their use: of x, and (N = 2) behind them those of dy.  RING: such groups on
+// their way.
+template <class T, int D, int N, int U, int RING>
 struct Stream {
   using Lanes = HeadLanes<T, D>;
   const RotaryArgs& a;
   const Lanes& lanes;
   uint4* const ring;
-  const unsigned items, step;
-  unsigned item, slot = 0;
+  Cursor cursor;
+  unsigned slot = 0;
   Item it;
-  int k = 0, u = 0, u0 = 0, u1 = 0, left = 0;  // tensor, the unit that is fetched next, of [u0, u1); units left of this tensor
+  int k = 0, u = 0, u0 = 0, u1 = 0, left = 0;  // tensor, the unit that is fetched next, of [u0, u1); tokens left of this tensor
   HeadWalk<T, D> walk[N];
 
-  __device__ __forceinline__ Stream(const RotaryArgs& args, const Lanes& l, uint4* r, unsigned first, unsigned s)
-      : a(args), lanes(l), ring(r), items(args.items[0] + args.items[1]), step(s), item(first) {
-    if (item < items) it = item_at(a, item), k = it.first - 1, next_tensor();
+  __device__ __forceinline__ Stream(const RotaryArgs& args, const Lanes& l, uint4* r, const Cursor& c) : a(args), lanes(l), ring(r), cursor(c) {
+    it.last = -1;
+    next_tensor();
 #pragma unroll
     for (int i = 0; i + 1 < RING; ++i) fetch();
   }
   __device__ __forceinline__ void next_tensor() {
     while (left == 0) {
       if (++k > it.last) {
-        item += step;
-        if (item >= items) return;
-        it = item_at(a, item), k = it.first;
+        if (!cursor.next(a, it)) return;
+        k = it.first;
       }
       units_of(a, it, k, Lanes::H, u0, u1);
       if (u0 >= u1) continue;
-      left = it.tokens * (u1 - u0), u = u0;
+      left = it.tokens, u = u0;
       const RotaryTensor& t = a.t[k];
-      walk[0].begin(static_cast<T*>(const_cast<void*>(t.x)), t.x_strides[0], t.x_strides[1], lanes, it.token, u0, u1);
-      if constexpr (N == 2) walk[1].begin(static_cast<T*>(const_cast<void*>(t.dy)), t.dy_strides[0], t.dy_strides[1], lanes, it.token, u0, u1);
+      walk[0].begin(static_cast<T*>(const_cast<void*>(t.x)), t.x_strides[0], t.x_strides[1], lanes, it.token, u0, u1, U);
+      if constexpr (N == 2) walk[1].begin(static_cast<T*>(const_cast<void*>(t.dy)), t.dy_strides[0], t.dy_strides[1], lanes, it.token, u0, u1, U);
     }
   }
   __device__ __forceinline__ void fetch() {
     if (left > 0) {
-      const bool there = u * Lanes::H + lanes.sub < a.t[k].heads, last = u + 1 == u1;
+      const int heads = a.t[k].heads;
+      const bool last = u + U >= u1;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (N == 1 || i == 1 || a.rotary.norm) walk[i].fetch(lanes, ring + (slot * N + i) * kUnitPieces, there);
+        if (N == 1 || i == 1 || a.rotary.norm) {
+#pragma unroll
+          for (int j = 0; j < U; ++j) {
+            if (j == 0 || u + j < u1) walk[i].fetch(lanes, j, ring + ((slot * N + i) * U + j) * kUnitPieces, (u + j) * Lanes::H + lanes.sub < heads);
+          }
+        }
         walk[i].next(last);
       }
-      u = last ? u0 : u + 1;
-      if (--left == 0) next_tensor();
+      u = last ? u0 : u + U;
+      if (last && --left == 0) next_tensor();
     }
     fetch_commit();
     slot = slot + 1 == RING ? 0 : slot + 1;
   }
 };
 
-// All of a warp's items: first, first + step, ...  `weights`: of the tensors, `n_weights` of them, D values each, for the whole CTA; `position`: of a
-// tensor's token on an axis, after the whole warp's `look` at the token.
-template <class T, int D, int RING, class F, class G>
-__device__ __forceinline__ void rotate_items(const RotaryArgs& a, uint4* ring, float* tables, float* weights, int n_weights, unsigned first, unsigned step, F position, G look) {
+constexpr int kTogether = 2;  // units of a token at once
+constexpr int kTokens = 2;    // tokens of an item
+
+// All of a warp's items.  `weights`: of the tensors, `n_weights` of them, D values each, for the whole CTA; `positions`: the lane's of an item's
+// (WarpAngles::write_all), by the whole warp.
+template <class T, int D, int RING, class F>
+__device__ __forceinline__ void rotate_items(const RotaryArgs& a, uint4* ring, float* tables, float* weights, int n_weights, Cursor cursor, F& positions) {
   using Lanes = HeadLanes<T, D>;
-  constexpr int C = Lanes::C;
+  constexpr int C = Lanes::C, U = kTogether;
   const Lanes lanes(a.rotary);
-  Stream<T, D, 1, RING> stream(a, lanes, ring, first, step);
+  Stream<T, D, 1, U, RING> stream(a, lanes, ring, cursor);
+  Item it, next;
+  bool more = cursor.next(a, next);
+  long long next_positions = more ? positions(next) : 0;
   const WarpAngles<T, D> angles(a.rotary);
   const int warp = threadIdx.x >> 5;
   if (warp < n_weights) lanes.write_weight(weights + warp * D, a.t[warp].weight, a.t[warp].weight_is_bf16);
   __syncthreads();
-  const unsigned n = a.items[0] + a.items[1];
   unsigned slot = 0;
-  for (unsigned i = first; i < n; i += step) {
-    const Item it = item_at(a, i);
-    __syncwarp();  // the last item's angles have been read
-    for (int j = 0; j < it.tokens; ++j) {
-      look(it.token + j);
-      angles.write(tables + j * D, [&](int axis) { return position(it.first, axis, it.token + j); });
-    }
-    __syncwarp();
+  while (more) {
+    it = next;
+    const long long its_positions = next_positions;
+    if ((more = cursor.next(a, next))) next_positions = positions(next);
+    angles.template write_all<kTokens>(tables, it.tokens, its_positions);
     for (int k = it.first; k <= it.last; ++k) {
       const RotaryTensor& t = a.t[k];
       int u0, u1;
       units_of(a, it, k, Lanes::H, u0, u1);
       if (u0 >= u1) continue;
       HeadWalk<T, D> y;
-      y.begin(static_cast<T*>(t.y), static_cast<long long>(t.heads) * D, D, lanes, it.token, u0, u1);
+      y.begin(static_cast<T*>(t.y), static_cast<long long>(t.heads) * D, D, lanes, it.token, u0, u1, U);
+      const float* const weight = weights + k * D;
       for (int j = 0; j < it.tokens; ++j) {
         uint64_t c[C], s[C];
         if (lanes.rotated) lanes.take(tables + j * D, c), lanes.take(tables + j * D + D / 2, s);
-        for (int u = u0; u < u1; ++u) {
+        for (int u = u0; u < u1; u += U) {
           stream.fetch();
           fetch_wait<RING - 1>();
-          uint4 p[2];
-          fetched(ring + slot * kUnitPieces, p);
+          const uint4* const from = ring + slot * U * kUnitPieces;
           slot = slot + 1 == RING ? 0 : slot + 1;
-          uint64_t v[2 * C];
-          Lanes::unpack(p, v);
-          rotate_unit<T, D>(a.rotary, lanes, weights + k * D, c, s, v);
-          if (u * Lanes::H + lanes.sub < t.heads) y.store(lanes, v);
-          y.next(u + 1 == u1);
+          auto work = [&](auto together) {
+            constexpr int N = decltype(together)::value;
+            uint64_t v[N][2 * C];
+#pragma unroll
+            for (int x = 0; x < N; ++x) {
+              uint4 p[2];
+              fetched(from + x * kUnitPieces, p);
+              Lanes::unpack(p, v[x]);
+            }
+            lanes.template norm<N>(a.rotary, weight, v);
+            if (lanes.rotated) {
+#pragma unroll
+              for (int x = 0; x < N; ++x) Lanes::template turn<false>(a.rotary.interleaved, c, s, v[x]);
+            }
+#pragma unroll
+            for (int x = 0; x < N; ++x)
+              if ((u + x) * Lanes::H + lanes.sub < t.heads) y.store(lanes, x, v[x]);
+          };
+          if (u + 1 < u1) work(std::integral_constant<int, U>{});
+          else work(std::integral_constant<int, 1>{});
+          y.next(u + U >= u1);
         }
       }
     }
   }
 }
 
-// How `tokens` tokens of `units` units each are dealt out to about `warps` warps: some tokens to an item, eight at most, or, with too few tokens for that,
-// some units of one.  A token's angles are made once for each of its items.
-constexpr int kItemTokens = 8;
-struct Split {
-  int tokens;  // of an item
-  int per;     // units of an item
-  int chunks;  // items of a token
-  long long items;
-};
-__host__ inline Split split_tokens(long long tokens, long long units, long long warps) {
-  Split s{1, 1, 1, 0};
-  if (tokens <= 0 || units <= 0) return s;
-  const long long n = tokens / warps;
-  s.tokens = static_cast<int>(n < 1 ? 1 : n > kItemTokens ? kItemTokens : n);
-  long long per = (tokens * units + warps - 1) / warps;
-  per = per > units ? units : per;
-  s.chunks = static_cast<int>((units + per - 1) / per);
-  s.per = static_cast<int>((units + s.chunks - 1) / s.chunks);
-  s.chunks = static_cast<int>((units + s.per - 1) / s.per);
-  s.items = (tokens + s.tokens - 1) / s.tokens * s.chunks;
-  return s;
-}
-
-// Items for about `warps` warps: of both tensors at once where they have the same positions.
-__host__ inline void plan_items(RotaryArgs& a, int head_dim, int is_fp32, long long warps) {
+// What is dealt out to about `warps` warps: whole tokens, whose angles are then made once, or, with fewer tokens than warps, parts of some units.
+// Of both tensors at once where they have the same positions.
+__host__ inline void plan_items(RotaryArgs& a, int head_dim, int is_fp32, long long warps, int item_tokens) {
   const int a_warp = is_fp32 ? 256 / head_dim : 512 / head_dim;
   auto units = [&](int k) { return (a.t[k].heads + a_warp - 1) / a_warp; };
-  auto take = [&](int k, const Split& s) { a.item_tokens[k] = s.tokens, a.per[k] = s.per, a.chunks[k] = s.chunks, a.items[k] = static_cast<unsigned>(s.items); };
+  auto deal = [&](int k, long long tokens, long long n) {
+    a.per[k] = a.chunks[k] = 1, a.items[k] = 0;
+    if (tokens <= 0 || n <= 0) return;
+    long long per = (tokens * n + warps - 1) / warps;  // whole tokens, some to an item, once there are enough for that
+    per = per > n ? n : per;
+    per = (n + (n + per - 1) / per - 1) / ((n + per - 1) / per);  // as even as it goes
+    a.per[k] = static_cast<int>(per);
+    a.chunks[k] = static_cast<int>((n + per - 1) / per);
+    a.items[k] = static_cast<unsigned>(a.chunks[k] == 1 ? (tokens + item_tokens - 1) / item_tokens : tokens * a.chunks[k]);
+  };
+  a.item_tokens = item_tokens;
   a.paired = a.t[0].tokens == a.t[1].tokens && a.t[0].positions == a.t[1].positions && a.t[0].position_stride == a.t[1].position_stride &&
              a.t[0].positions_are_int64 == a.t[1].positions_are_int64;
-  if (a.paired) {
-    take(0, split_tokens(a.t[0].tokens, units(0) + units(1), warps));
-    take(1, Split{1, 1, 1, 0});
-  } else {
-    for (int k = 0; k < 2; ++k) take(k, split_tokens(a.t[k].tokens, units(k), warps));
-  }
+  deal(0, a.t[0].tokens, a.paired ? units(0) + units(1) : units(0));
+  deal(1, a.paired ? 0 : a.t[1].tokens, units(1));
 }
 
 }  // namespace gdpa

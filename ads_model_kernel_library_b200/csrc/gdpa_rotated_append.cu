@@ -42,185 +42,164 @@ __device__ __forceinline__ long long given_position(const RotatedAppendArgs& a, 
   return q.positions_are_int64 ? static_cast<const long long*>(q.positions)[i] : static_cast<const int*>(q.positions)[i];
 }
 
-// One run of one head, keys (KEY) or values, by the lanes that hold its rows r0, r0 + step, ...; the first HOLD of them come as they are in `u` and
-// stay in registers, further ones (ALL: there are none) are read and made again.  `angles(row, c, s)` gives a lane its angles; `top_of` makes a maximum over all the
-// run's lanes.  Lanes without a run have len 0; every lane of a warp comes along.  `first`: whether this lane writes the scale.
-template <class T, int D, int HOLD, bool ALL, bool KEY, class Angles, class Top>
-__device__ __forceinline__ void store_run(const RotatedAppendArgs& a, const HeadLanes<T, D>& lanes, const float* s_weight, const uint4 (&u)[HOLD][2], int r0, int step,
-                                          int h, long long t0, long long blk, int o, int len, bool first, Angles angles, Top top_of) {
+// The largest of `top` and a row's magnitudes; a NaN is none, nor, if they are to be finite, an infinity.
+template <int N>
+__device__ __forceinline__ float largest(float top, const uint64_t (&v)[N], bool finite) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    float lo, hi;
+    unpack_f32x2(v[e], lo, hi);
+    if (finite) {
+      lo = fabsf(lo) < INFINITY ? lo : 0.f;
+      hi = fabsf(hi) < INFINITY ? hi : 0.f;
+    }
+    top = max3_abs(top, lo, hi);
+  }
+  return top;
+}
+
+// A row's values times `inv`, in 8 bits.
+template <class T, int D>
+__device__ __forceinline__ void store_row(const HeadLanes<T, D>& lanes, uint8_t* row, uint64_t (&v)[2 * HeadLanes<T, D>::C], float inv) {
   using Lanes = HeadLanes<T, D>;
   constexpr int E = Lanes::E, C = Lanes::C;
+  Lanes::times(inv, v);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    uint32_t q[E / 4];
+#pragma unroll
+    for (int e = 0; e < E / 4; ++e) {
+      float f[4];
+      unpack_f32x2(v[k * C + 2 * e], f[0], f[1]);
+      unpack_f32x2(v[k * C + 2 * e + 1], f[2], f[3]);
+      q[e] = pack_e4m3x4(f[0], f[1], f[2], f[3]);
+    }
+    uint8_t* const at = row + (k == 0 ? lanes.g0 : lanes.g1) * E;
+    if constexpr (E == 8) *reinterpret_cast<uint2*>(at) = make_uint2(q[0], q[1]);
+    else *reinterpret_cast<uint32_t*>(at) = q[0];
+  }
+}
+
+// A run's scale from its largest finite magnitude, and, where it has grown, the rows before the run rescaled: r0, r0 + step, ... of them by these lanes.
+template <class T, int D>
+__device__ __forceinline__ float scale_of_run(const HeadLanes<T, D>& lanes, float top, float old, uint8_t* block, long long row_stride, int o, int r0, int step) {
+  using Lanes = HeadLanes<T, D>;
+  const float fresh = __uint_as_float(static_cast<uint32_t>(scale_exponent(__float_as_uint(top)) + 127) << 23);
+  const float scale = old > fresh ? old : fresh;
+  if (o > 0 && scale != old) {
+    const float ratio = old / scale;
+    constexpr int P = D / 16;  // 16-byte pieces of a row, over the lanes of a head
+    constexpr int K = (P + Lanes::L - 1) / Lanes::L, AT_ONCE = 4;
+    for (int r = r0; r < o; r += AT_ONCE * step) {
+      uint4 held[AT_ONCE][K];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (r + i * step < o && k * Lanes::L + lanes.l < P)
+            held[i][k] = reinterpret_cast<const uint4*>(block + (r + i * step) * row_stride)[k * Lanes::L + lanes.l];
+      }
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (r + i * step >= o || k * Lanes::L + lanes.l >= P) continue;
+          uint32_t q[4] = {held[i][k].x, held[i][k].y, held[i][k].z, held[i][k].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 lo = e4m3x2_values(q[j] & 0xffffu), hi = e4m3x2_values(q[j] >> 16);
+            q[j] = pack_e4m3x4(lo.x * ratio, lo.y * ratio, hi.x * ratio, hi.y * ratio);
+          }
+          reinterpret_cast<uint4*>(block + (r + i * step) * row_stride)[k * Lanes::L + lanes.l] = make_uint4(q[0], q[1], q[2], q[3]);
+        }
+      }
+    }
+  }
+  return scale;
+}
+
+// One run of one head, keys (KEY) or values, by the lanes that have its rows r0, r0 + step, ...; the first stays in registers, further ones are read
+// and made again.  `angles(row, c, s)` gives a lane its angles; `top_of` makes a maximum over all the run's lanes.
+// Lanes without a run have len 0; every lane of a warp comes along.  `first`: whether this lane writes the scale.
+template <class T, int D, bool KEY, class Angles, class Top>
+__device__ __forceinline__ void store_run(const RotatedAppendArgs& a, const HeadLanes<T, D>& lanes, const float* s_weight, int r0, int step, int h,
+                                          long long t0, long long blk, int o, int len, bool first, Angles angles, Top top_of) {
+  using Lanes = HeadLanes<T, D>;
+  constexpr int C = Lanes::C;
   const CacheAppendArgs& ca = a.cache;
-  const RotarySpec& spec = a.queries.rotary;
   const long long row_stride = KEY ? ca.key_strides[0] : ca.value_strides[0];
   const T* const x = static_cast<const T*>(KEY ? ca.key : ca.value) + t0 * row_stride + h * (KEY ? ca.key_strides[1] : ca.value_strides[1]);
   float* const scale_at = (KEY ? ca.k_scales : ca.v_scales) + blk * ca.heads + h;
   const long long* const cs = KEY ? ca.k_cache_strides : ca.v_cache_strides;
   uint8_t* const out = (KEY ? ca.k_cache : ca.v_cache) + blk * cs[0] + h * cs[2];
-  auto values = [&](int r, const uint4 (&p)[2], uint64_t (&v)[2 * C]) {
-    Lanes::unpack(p, v);
+  auto values = [&](int r, uint64_t (&v)[1][2 * C]) {
+    uint4 p[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (r < len) {
+      const uint4* const at = reinterpret_cast<const uint4*>(x + r * row_stride);
+      p[0] = __ldg(at + lanes.g0), p[1] = __ldg(at + lanes.g1);
+    }
+    Lanes::unpack(p, v[0]);
     if constexpr (KEY) {
-      uint64_t c[C], s[C];
-      if (lanes.rotated) angles(r < len ? r : 0, c, s);
-      rotate_unit<T, D>(spec, lanes, s_weight, c, s, v);
+      lanes.template norm<1>(a.queries.rotary, s_weight, v);
+      if (lanes.rotated) {
+        uint64_t c[C], s[C];
+        angles(r < len ? r : 0, c, s);
+        Lanes::template turn<false>(a.queries.rotary.interleaved, c, s, v[0]);
+      }
     }
-  };
-  auto largest = [](uint32_t top, const uint64_t (&v)[2 * C], bool finite) {
-#pragma unroll
-    for (int e = 0; e < 2 * C; ++e) {
-      float lo, hi;
-      unpack_f32x2(v[e], lo, hi);
-      const uint32_t p = __float_as_uint(lo) & 0x7fffffffu, q = __float_as_uint(hi) & 0x7fffffffu;
-      top = max(top, finite && p >= kInfBits ? 0u : p);
-      top = max(top, finite && q >= kInfBits ? 0u : q);
-    }
-    return top;
   };
   const float old = o > 0 && len > 0 ? *scale_at : 0.f;
-  uint64_t v[HOLD][2 * C];
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < HOLD; ++i) values(r0 + i * step, u[i], v[i]);
-  float scale = 0, inv = 0;
-  auto store = [&](int r, const uint64_t (&given)[2 * C]) {
-    uint8_t* const p = out + (o + r) * cs[1];
-    uint64_t w[2 * C];
-#pragma unroll
-    for (int e = 0; e < 2 * C; ++e) w[e] = given[e];
-    Lanes::times(inv, w);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      uint32_t q[E / 4];
-#pragma unroll
-      for (int e = 0; e < E / 4; ++e) {
-        float f[4];
-        unpack_f32x2(w[k * C + 2 * e], f[0], f[1]);
-        unpack_f32x2(w[k * C + 2 * e + 1], f[2], f[3]);
-        q[e] = pack_e4m3x4(f[0], f[1], f[2], f[3]);
-      }
-      uint8_t* const at = p + (k == 0 ? lanes.g0 : lanes.g1) * E;
-      if constexpr (E == 8) *reinterpret_cast<uint2*>(at) = make_uint2(q[0], q[1]);
-      else *reinterpret_cast<uint32_t*>(at) = q[0];
-    }
-  };
-  // Three passes over the rows: their maximum; if it is none, an infinity or NaN among them (rare), that of the others; their conversion.
+  uint64_t held[1][2 * C];
+  values(r0, held);
+  float top = 0, scale = 0, inv = 0;
+  // Three passes over the rows: their maximum; if it is infinite (rare), that of the others; their conversion.
   for (int pass = 0;;) {
-#pragma unroll
-    for (int i = 0; i < HOLD; ++i) {
-      if (pass < 2) top = largest(top, v[i], pass == 1);
-      else if (r0 + i * step < len) store(r0 + i * step, v[i]);
-    }
-    if constexpr (!ALL) {
-      for (int r = r0 + HOLD * step; __any_sync(kAllLanes, r < len); r += step) {
-        uint4 p[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-        if (r < len) {
-          const uint4* const at = reinterpret_cast<const uint4*>(x + r * row_stride);
-          p[0] = __ldg(at + lanes.g0), p[1] = __ldg(at + lanes.g1);
-        }
-        uint64_t w[2 * C];
-        values(r, p, w);
-        if (r >= len) continue;
-        if (pass < 2) top = largest(top, w, pass == 1);
-        else store(r, w);
-      }
+    if (pass < 2) top = largest(top, held[0], pass == 1);
+    else if (r0 < len) store_row<T, D>(lanes, out + (o + r0) * cs[1], held[0], inv);
+    for (int r = r0 + step; __any_sync(kAllLanes, r < len); r += step) {
+      uint64_t w[1][2 * C];
+      values(r, w);
+      if (r >= len) continue;
+      if (pass < 2) top = largest(top, w[0], pass == 1);
+      else store_row<T, D>(lanes, out + (o + r) * cs[1], w[0], inv);
     }
     if (pass == 2) break;
     top = top_of(top);
-    if (pass == 0 && __any_sync(kAllLanes, top >= kInfBits)) {
+    if (pass == 0 && __any_sync(kAllLanes, top == INFINITY)) {
       pass = 1, top = 0;
       continue;
     }
     pass = 2;
-    const float fresh = __uint_as_float(static_cast<uint32_t>(scale_exponent(top) + 127) << 23);
-    scale = old > fresh ? old : fresh;
+    scale = scale_of_run<T, D>(lanes, top, old, out, cs[1], len > 0 ? o : 0, r0, step);
     inv = 1.f / scale;
-    if (o > 0 && len > 0 && scale != old) {
-      // the rows before the run, rescaled
-      const float ratio = old / scale;
-      constexpr int P = D / 16;  // 16-byte pieces of a row, over the lanes of a head
-      for (int r = r0; r < o; r += step) {
-#pragma unroll
-        for (int k = 0; k < (P + Lanes::L - 1) / Lanes::L; ++k) {
-          if (k * Lanes::L + lanes.l >= P) continue;
-          uint4* const p = reinterpret_cast<uint4*>(out + r * cs[1]) + k * Lanes::L + lanes.l;
-          const uint4 held = *p;
-          uint32_t q[4] = {held.x, held.y, held.z, held.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 lo = e4m3x2_values(q[i] & 0xffffu), hi = e4m3x2_values(q[i] >> 16);
-            q[i] = pack_e4m3x4(lo.x * ratio, lo.y * ratio, hi.x * ratio, hi.y * ratio);
-          }
-          *p = make_uint4(q[0], q[1], q[2], q[3]);
-        }
-      }
-    }
   }
   if (first && len > 0 && scale != old) *scale_at = scale;
 }
 
-// A warp's share of a CTA's shared memory: its ring of units; and of its tables, which for keys and values are those of a block's rows.
-template <int HOLD>
-constexpr int kRing = 2 * HOLD > 6 ? 2 * HOLD : 6;
+// Where a window of 32 tokens has its runs, as every warp of a CTA sees it.
+struct Window {
+  const RotatedAppendArgs& a;
+  long long base, slot;  // its first token; the lane's slot, or -1
+  unsigned leaders;      // lanes whose token begins a run
 
-// W warps of a CTA; HOLD rows of a lane when all of them are on one run, so that a whole block is held.
-template <class T, int D, int W, int HOLD>
-__global__ void __launch_bounds__(W * 32, 16 / W) gdpa_rotated_append_kernel(const __grid_constant__ RotatedAppendArgs a) {
-  using Lanes = HeadLanes<T, D>;
-  constexpr int C = Lanes::C, RING = kRing<HOLD>;
-  extern __shared__ uint4 s_dynamic[];
-  __shared__ float4 s_weight4[D / 4];
-  __shared__ double s_frequency[D / 2];  // of the pairs, in a lane's order
-  __shared__ int s_axis[D / 2];
-  __shared__ uint32_t s_top[2][W];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float* const s_weight = reinterpret_cast<float*>(s_weight4);
-  uint4* const ring = s_dynamic + warp * RING * kUnitPieces;
-  float* const tables = reinterpret_cast<float*>(s_dynamic + W * RING * kUnitPieces);
-  const bool given = a.queries.t[0].positions != nullptr;
-  const int kv_ctas = a.kv_windows * a.kv_parts;
-  if (static_cast<int>(blockIdx.x) >= kv_ctas) {
-    long long origin = 0, begin = 0, end = -1;  // of the request at hand: its first token and the one behind its last
-    rotate_items<T, D, RING>(a.queries, ring, tables + warp * kItemTokens * D, s_weight, 1, (blockIdx.x - kv_ctas) * W + warp, (gridDim.x - kv_ctas) * W,
-                             [&](int, int axis, long long t) -> long long {
-      return given ? given_position(a, axis, t) : origin + t;
-    }, [&](long long t) {
-      if (given || (t >= begin && t < end)) return;
-      const int owner = owner_of(a, t);
-      origin = origin_of(a, owner);
-      begin = a.batch == 0 ? 0 : load_offset(a.q_off, owner, a.off64);
-      end = a.batch == 0 ? 0x7fffffffffffffffll : load_offset(a.q_off, owner + 1, a.off64);
-    });
-    return;
-  }
-  const Lanes lanes(a.queries.rotary);
-  if (warp == 0) lanes.write_weight(s_weight, a.queries.t[1].weight, a.queries.t[1].weight_is_bf16);
-  for (int i = threadIdx.x; i < a.queries.rotary.pairs; i += W * 32) {
-    const int at = Lanes::slot_of_pair(a.queries.rotary, i);
-    s_frequency[at] = frequency_of_pair(a.queries.rotary, i), s_axis[at] = axis_of_pair(a.queries.rotary, i);
-  }
-  __syncthreads();
-  const CacheAppendArgs& ca = a.cache;
-  const int S = 1 << ca.block_shift;
-  const int part = blockIdx.x / a.kv_windows;
-  const long long base = static_cast<long long>(blockIdx.x - part * a.kv_windows) * 32;
-  const long long slots = ca.num_blocks << ca.block_shift;
-  auto slot_of = [&](long long t) -> long long {
+  __device__ __forceinline__ long long slot_of(long long t) const {
+    const CacheAppendArgs& ca = a.cache;
     if (t < 0 || t >= ca.tokens) return -1;
     const long long s = ca.slot_mapping[t];
-    return s >= 0 && s < slots ? s : -1;
-  };
-  const long long slot = slot_of(base + lane);
-  long long before = __shfl_up_sync(kAllLanes, slot, 1);
-  if (lane == 0) before = slot_of(base - 1);
-  const bool leads = slot >= 0 && ((slot & (S - 1)) == 0 || before != slot - 1);
-  const unsigned leaders = __ballot_sync(kAllLanes, leads);
-  const int runs = __popc(leaders);
-  if (runs == 0) return;
-  // position of the first token of the run that this lane leads, less its index
-  auto origin_of_run = [&]() -> long long {
-    if (given) return 0;
+    return s >= 0 && s < (ca.num_blocks << ca.block_shift) ? s : -1;
+  }
+  __device__ __forceinline__ Window(const RotatedAppendArgs& args, long long first) : a(args), base(first) {
+    const int lane = threadIdx.x & 31;
+    slot = slot_of(base + lane);
+    long long before = __shfl_up_sync(kAllLanes, slot, 1);
+    if (lane == 0) before = slot_of(base - 1);
+    leaders = __ballot_sync(kAllLanes, slot >= 0 && ((slot & ((1 << a.cache.block_shift) - 1)) == 0 || before != slot - 1));
+  }
+  // position of the first token of the run that the lane leads, less its index
+  __device__ __forceinline__ long long origin() const {
+    if (a.queries.t[0].positions != nullptr) return 0;
     // the requests of the 32 tokens: the first one's, and whose beginnings follow
-    const int b0 = owner_of(a, base);
+    const int lane = threadIdx.x & 31, b0 = owner_of(a, base);
     int owner = b0;
     for (int b = b0 + 1; b < a.batch; b += 32) {
       const long long begin = b + lane < a.batch ? load_offset(a.q_off, b + lane, a.off64) : 0x7fffffffffffffffll;
@@ -232,10 +211,10 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gdpa_rotated_append_kernel(con
       if (__shfl_sync(kAllLanes, begin, 31) > base + 31) break;
     }
     return origin_of(a, owner);
-  };
-  // tokens of the run that begins with token base + at: as far as the slots go on, at most to the end of the block
-  auto length_of = [&](int at, long long s0) -> int {
-    const int o = static_cast<int>(s0 & (S - 1));
+  }
+  // tokens of the run that begins with token base + at, in slot s0: as far as the slots go on, at most to the end of the block
+  __device__ __forceinline__ int length_of(int at, long long s0) const {
+    const int lane = threadIdx.x & 31, S = 1 << a.cache.block_shift, o = static_cast<int>(s0 & (S - 1));
     int len = 0;
     for (bool more = true; more;) {
       const int i = len + lane;
@@ -246,196 +225,337 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gdpa_rotated_append_kernel(con
       more = stops == 0;
     }
     return len;
-  };
-  auto none = [](int, uint64_t (&)[C], uint64_t (&)[C]) {};
-  if (runs <= 2) {
-    // all warps on one run of one head after the other; the next ones are on their way
-    constexpr int AHEAD = RING / HOLD;
-    unsigned turn = 0;
-    auto top_of = [&](uint32_t top) {
-      top = __reduce_max_sync(kAllLanes, top);
-      uint32_t* const s = s_top[turn++ & 1u];  // two in turn: the next maximum is written while this one may still be read
-      if (lane == 0) s[warp] = top;
-      __syncthreads();
-      top = s[0];
+  }
+};
+
+// What the lanes make angles from by themselves, for a whole CTA: frequency and axis of the pairs, in a lane's order.
+template <int D>
+struct PairTable {
+  double frequency[D / 2];
+  int axis[D / 2];
+};
+template <class T, int D>
+__device__ __forceinline__ void write_pairs(const RotarySpec& r, PairTable<D>& table) {
+  for (int i = threadIdx.x; i < r.pairs; i += blockDim.x) {
+    const int at = HeadLanes<T, D>::slot_of_pair(r, i);
+    table.frequency[at] = frequency_of_pair(r, i), table.axis[at] = axis_of_pair(r, i);
+  }
+}
+
+// A window's runs over the warps: a warp to each run and head, its heads' lanes to a row each; or (SINGLE) a head's lanes to each run and head.
+// This is warp `me` of `warps`.
+template <class T, int D, bool SINGLE>
+__device__ __forceinline__ void deal(const Window& window, const HeadLanes<T, D>& lanes, const float* s_weight, const PairTable<D>& pairs, int me, int warps) {
+  using Lanes = HeadLanes<T, D>;
+  constexpr int C = Lanes::C, a_warp = SINGLE ? Lanes::H : 1, step = SINGLE ? 1 : Lanes::H;
+  const RotatedAppendArgs& a = window.a;
+  const CacheAppendArgs& ca = a.cache;
+  const bool given = a.queries.t[0].positions != nullptr;
+  const long long origin = window.origin();
+  const int tasks = __popc(window.leaders) * ca.heads, rounds = (tasks + a_warp - 1) / a_warp;
+  for (int i = me; i < 2 * rounds; i += warps) {
+    const bool is_key = i < rounds;
+    const int task = (is_key ? i : i - rounds) * a_warp + (SINGLE ? lanes.sub : 0);
+    const bool there = task < tasks;
+    const int at = there ? __fns(window.leaders, 0, task / ca.heads + 1) : 0, h = there ? task % ca.heads : 0;
+    const long long s0 = __shfl_sync(kAllLanes, window.slot, at), run_origin = __shfl_sync(kAllLanes, origin, at), t0 = window.base + at;
+    int len = 0;
+    if constexpr (SINGLE) {
 #pragma unroll
-      for (int i = 1; i < W; ++i) top = max(top, s[i]);
+      for (int k = 0; k < Lanes::H; ++k) {  // each by the whole warp
+        const int l = window.length_of(__shfl_sync(kAllLanes, at, k * Lanes::L), __shfl_sync(kAllLanes, s0, k * Lanes::L));
+        if (lanes.sub == k) len = l;
+      }
+    } else {
+      len = window.length_of(at, s0);
+    }
+    if (!there) len = 0;
+    const long long blk = there ? s0 >> ca.block_shift : 0;
+    const int o = there ? static_cast<int>(s0 & ((1 << ca.block_shift) - 1)) : 0, r0 = SINGLE ? 0 : lanes.sub;
+    auto top_of = [&](float top) {
+      if (!SINGLE) return __uint_as_float(__reduce_max_sync(kAllLanes, __float_as_uint(top)));
+#pragma unroll
+      for (int s = 1; s < Lanes::L; s <<= 1) top = fmaxf(top, __shfl_xor_sync(kAllLanes, top, s));
       return top;
     };
-    long long origin = 0;
-    bool found = false;
-    for (unsigned left = leaders; left != 0; left &= left - 1) {
-      const int at = __ffs(left) - 1;
-      const long long s0 = __shfl_sync(kAllLanes, slot, at), t0 = base + at, blk = s0 >> ca.block_shift;
-      const int len = length_of(at, s0), o = static_cast<int>(s0 & (S - 1)), r0 = warp * Lanes::H + lanes.sub;
-      constexpr int step = W * Lanes::H;
-      int ahead = part, ahead_slot = 0;
-      auto fetch = [&]() {
-        if (ahead < 2 * ca.heads) {
-          const bool key = ahead < ca.heads;
-          const int h = key ? ahead : ahead - ca.heads;
-          const long long* const xs = key ? ca.key_strides : ca.value_strides;
-          HeadWalk<T, D> walk;
-          walk.at = static_cast<T*>(const_cast<void*>(key ? ca.key : ca.value)) + (t0 + r0) * xs[0] + h * xs[1];
-          walk.unit = step * xs[0];
+    const bool first = lanes.l == 0 && (SINGLE || lanes.sub == 0);
+    if (is_key) {
+      store_run<T, D, true>(a, lanes, s_weight, r0, step, h, t0, blk, o, len, first, [&](int r, uint64_t (&c)[C], uint64_t (&s)[C]) {
 #pragma unroll
-          for (int i = 0; i < HOLD; ++i) {
-            walk.fetch(lanes, ring + (ahead_slot * HOLD + i) * kUnitPieces, r0 + i * step < len);
-            walk.next(false);
+        for (int e = 0; e < C; ++e) {
+          float sn[2], cs[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int pair = Lanes::slot(lanes.l, 2 * e + j);
+            sin_cos<T>(pairs.frequency[pair], given ? given_position(a, pairs.axis[pair], t0 + r) : run_origin + t0 + r, sn[j], cs[j]);
           }
-          ahead += a.kv_parts;
+          c[e] = pack_f32x2(cs[0], cs[1]), s[e] = pack_f32x2(sn[0], sn[1]);
         }
-        fetch_commit();
-        ahead_slot = ahead_slot + 1 == AHEAD ? 0 : ahead_slot + 1;
-      };
-#pragma unroll
-      for (int i = 0; i + 1 < AHEAD; ++i) fetch();
-      if (!found) origin = origin_of_run(), found = true;
-      if (part < ca.heads) {  // this CTA has keys of the run: its angles
-        const long long run_origin = __shfl_sync(kAllLanes, origin, at);
-        __syncthreads();      // the last run's have been read
-        const WarpAngles<T, D> angles(a.queries.rotary);
-        for (int r = warp; r < len; r += W)
-          angles.write(tables + r * D, [&](int axis) { return given ? given_position(a, axis, t0 + r) : run_origin + t0 + r; });
-        __syncthreads();
-      }
-      int at_slot = 0;
-      for (int head2 = part; head2 < 2 * ca.heads; head2 += a.kv_parts) {
-        fetch();
-        fetch_wait<AHEAD - 1>();
-        uint4 u[HOLD][2];
-#pragma unroll
-        for (int i = 0; i < HOLD; ++i) fetched(ring + (at_slot * HOLD + i) * kUnitPieces, u[i]);
-        at_slot = at_slot + 1 == AHEAD ? 0 : at_slot + 1;
-        if (head2 < ca.heads) {
-          store_run<T, D, HOLD, true, true>(a, lanes, s_weight, u, r0, step, head2, t0, blk, o, len, threadIdx.x == 0, [&](int r, uint64_t (&c)[C], uint64_t (&s)[C]) {
-            lanes.take(tables + r * D, c);
-            lanes.take(tables + r * D + D / 2, s);
-          }, top_of);
-        } else {
-          store_run<T, D, HOLD, true, false>(a, lanes, s_weight, u, r0, step, head2 - ca.heads, t0, blk, o, len, threadIdx.x == 0, none, top_of);
-        }
-      }
+      }, top_of);
+    } else {
+      store_run<T, D, false>(a, lanes, s_weight, r0, step, h, t0, blk, o, len, first, [](int, uint64_t (&)[C], uint64_t (&)[C]) {}, top_of);
     }
+  }
+}
+
+// The lane's position of an item's of the queries.
+struct QueryPositions {
+  const RotatedAppendArgs& a;
+  long long origin = 0, begin = 0, end = -1;  // of the request at hand: its first token and the one behind its last
+  __device__ __forceinline__ long long operator()(const Item& it) {
+    const int lane = threadIdx.x & 31, axis = lane / kMostItemTokens, j = lane % kMostItemTokens;
+    if (a.queries.t[0].positions != nullptr) return axis < a.queries.rotary.axes && j < it.tokens ? given_position(a, axis, it.token + j) : 0;
+    long long p = 0;
+    for (int i = 0; i < it.tokens; ++i) {
+      const long long t = it.token + i;
+      if (!(t >= begin && t < end)) {
+        const int owner = owner_of(a, t);
+        origin = origin_of(a, owner);
+        begin = a.batch == 0 ? 0 : load_offset(a.q_off, owner, a.off64);
+        end = a.batch == 0 ? 0x7fffffffffffffffll : load_offset(a.q_off, owner + 1, a.off64);
+      }
+      if (j == i) p = origin + t;  // on every axis
+    }
+    return p;
+  }
+};
+
+// ------------------------------------------------------------------------------------------ a few tokens of each request: one launch
+
+constexpr int kWarps = 4, kQueryRing = 3;  // groups of units of a warp on their way
+constexpr int kQueryBytes = kWarps * kQueryRing * kTogether * kUnitPieces * 16;
+
+template <class T, int D>
+__global__ void __launch_bounds__(kWarps * 32, 4) gdpa_rotated_step_kernel(const __grid_constant__ RotatedAppendArgs a) {
+  extern __shared__ uint4 s_ring[];
+  __shared__ float4 s_tables[kWarps][kTokens][D / 4];
+  __shared__ float4 s_weight4[D / 4];
+  __shared__ PairTable<D> s_pairs;
+  float* const s_weight = reinterpret_cast<float*>(s_weight4);
+  const int warp = threadIdx.x >> 5, kv_ctas = a.kv_windows * a.kv_parts;
+  if (static_cast<int>(blockIdx.x) >= kv_ctas) {
+    QueryPositions positions{a};
+    rotate_items<T, D, kQueryRing>(a.queries, s_ring + warp * kQueryRing * kTogether * kUnitPieces, reinterpret_cast<float*>(s_tables[warp]), s_weight, 1,
+                                   Cursor((blockIdx.x - kv_ctas) * kWarps + warp, (gridDim.x - kv_ctas) * kWarps), positions);
     return;
   }
-  const long long origin = origin_of_run();
-  // a lane's angles, made by itself
-  auto own_angles = [&](long long t, long long run_origin, uint64_t (&c)[C], uint64_t (&s)[C]) {
+  const HeadLanes<T, D> lanes(a.queries.rotary);
+  const int part = blockIdx.x / a.kv_windows;
+  const Window window(a, static_cast<long long>(blockIdx.x - part * a.kv_windows) * 32);
+  if (window.leaders == 0) return;
+  if (warp == 0) lanes.write_weight(s_weight, a.queries.t[1].weight, a.queries.t[1].weight_is_bf16);
+  write_pairs<T, D>(a.queries.rotary, s_pairs);
+  __syncthreads();
+  // with two tokens a run at most, on average: a head's lanes to a run
+  if (__popc(window.leaders) > 16) deal<T, D, true>(window, lanes, s_weight, s_pairs, part * kWarps + warp, a.kv_parts * kWarps);
+  else deal<T, D, false>(window, lanes, s_weight, s_pairs, part * kWarps + warp, a.kv_parts * kWarps);
+}
+
+// ------------------------------------------------------------------------------------------ prompts: queries, then keys and values
+
+template <class T, int D>
+__global__ void __launch_bounds__(kWarps * 32, 4) gdpa_rotated_queries_kernel(const __grid_constant__ RotatedAppendArgs a) {
+  extern __shared__ uint4 s_ring[];
+  __shared__ float4 s_tables[kWarps][kTokens][D / 4];
+  __shared__ float4 s_weight[D / 4];
+  const int warp = threadIdx.x >> 5;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // keys and values may begin when there is room: neither reads what the other writes
+  QueryPositions positions{a};
+  rotate_items<T, D, kQueryRing>(a.queries, s_ring + warp * kQueryRing * kTogether * kUnitPieces, reinterpret_cast<float*>(s_tables[warp]),
+                                 reinterpret_cast<float*>(s_weight), 1, Cursor(blockIdx.x * kWarps + warp, gridDim.x * kWarps), positions);
+}
+
+// W warps on one run of one head after the other, keys, then values; the next head is on its way while one is worked on.  HOLD rows of a lane, so that a
+// whole block is held.
+template <class T, int D, int W, int HOLD>
+__global__ void __launch_bounds__(W * 32, 12 / W) gdpa_rotated_runs_kernel(const __grid_constant__ RotatedAppendArgs a) {
+  using Lanes = HeadLanes<T, D>;
+  constexpr int C = Lanes::C, step = W * Lanes::H;
+  extern __shared__ uint4 s_dynamic[];  // [warp][HOLD] units; angles of a block's rows, [row][D]
+  __shared__ float4 s_weight4[D / 4];
+  __shared__ PairTable<D> s_pairs;
+  __shared__ float s_top[2][W];
+  float* const s_weight = reinterpret_cast<float*>(s_weight4);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint4* const ring = s_dynamic + warp * HOLD * kUnitPieces;
+  float* const tables = reinterpret_cast<float*>(s_dynamic + W * HOLD * kUnitPieces);
+  const Lanes lanes(a.queries.rotary);
+  const CacheAppendArgs& ca = a.cache;
+  const int part = blockIdx.x / a.kv_windows;
+  const Window window(a, static_cast<long long>(blockIdx.x - part * a.kv_windows) * 32);
+  if (window.leaders != 0) {
+    if (warp == 0) lanes.write_weight(s_weight, a.queries.t[1].weight, a.queries.t[1].weight_is_bf16);
+    if (__popc(window.leaders) > 2) {  // short ones
+      write_pairs<T, D>(a.queries.rotary, s_pairs);
+      __syncthreads();
+      deal<T, D, false>(window, lanes, s_weight, s_pairs, part * W + warp, a.kv_parts * W);
+    } else {
+      const bool given = a.queries.t[0].positions != nullptr;
+      unsigned turn = 0;
+      auto top_of = [&](float top) {
+        top = __uint_as_float(__reduce_max_sync(kAllLanes, __float_as_uint(top)));
+        float* const s = s_top[turn++ & 1u];  // two in turn: the next maximum is written while this one may still be read
+        if (lane == 0) s[warp] = top;
+        __syncthreads();
+        top = s[0];
 #pragma unroll
-    for (int e = 0; e < C; ++e) {
-      float sn[2], cs[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = Lanes::slot(lanes.l, 2 * e + i);
-        sin_cos<T>(s_frequency[at], given ? given_position(a, s_axis[at], t) : run_origin + t, sn[i], cs[i]);
-      }
-      c[e] = pack_f32x2(cs[0], cs[1]), s[e] = pack_f32x2(sn[0], sn[1]);
-    }
-  };
-  // a warp to each run and head, its heads' lanes to a row each; or, with two tokens a run at most on average, a head's lanes to each run and head
-  auto deal = [&](auto lanes_of_a_head) {
-    constexpr bool single = decltype(lanes_of_a_head)::value;
-    constexpr int a_warp = single ? Lanes::H : 1, HELD = 1, step = single ? 1 : Lanes::H;
-    const int tasks = runs * ca.heads, rounds = (tasks + a_warp - 1) / a_warp;
-    for (int i = part * W + warp; i < 2 * rounds; i += a.kv_parts * W) {
-      const bool is_key = i < rounds;
-      const int task = (is_key ? i : i - rounds) * a_warp + (single ? lanes.sub : 0);
-      const bool there = task < tasks;
-      const int at = there ? __fns(leaders, 0, task / ca.heads + 1) : 0, h = there ? task % ca.heads : 0;
-      const long long s0 = __shfl_sync(kAllLanes, slot, at), run_origin = __shfl_sync(kAllLanes, origin, at), t0 = base + at;
-      int len = 0;
-      if constexpr (single) {
-#pragma unroll
-        for (int k = 0; k < Lanes::H; ++k) {  // each by the whole warp
-          const int l = length_of(__shfl_sync(kAllLanes, at, k * Lanes::L), __shfl_sync(kAllLanes, s0, k * Lanes::L));
-          if (lanes.sub == k) len = l;
-        }
-      } else {
-        len = length_of(at, s0);
-      }
-      if (!there) len = 0;
-      const long long blk = there ? s0 >> ca.block_shift : 0;
-      const int o = there ? static_cast<int>(s0 & (S - 1)) : 0, r0 = single ? 0 : lanes.sub;
-      auto top_of = [&](uint32_t top) {
-        if (!single) return __reduce_max_sync(kAllLanes, top);
-#pragma unroll
-        for (int s = 1; s < Lanes::L; s <<= 1) top = max(top, __shfl_xor_sync(kAllLanes, top, s));
+        for (int i = 1; i < W; ++i) top = fmaxf(top, s[i]);
         return top;
       };
-      const bool first = lanes.l == 0 && (single || lanes.sub == 0);
-      const long long* const xs = is_key ? ca.key_strides : ca.value_strides;
-      const T* const x = static_cast<const T*>(is_key ? ca.key : ca.value) + t0 * xs[0] + h * xs[1];
-      uint4 u[HELD][2];
+      const int r0 = warp * Lanes::H + lanes.sub, S = 1 << ca.block_shift;
+      long long origin = 0;
+      for (unsigned left = window.leaders; left != 0; left &= left - 1) {
+        const int at = __ffs(left) - 1;
+        const long long s0 = __shfl_sync(kAllLanes, window.slot, at), t0 = window.base + at, blk = s0 >> ca.block_shift;
+        const int len = window.length_of(at, s0), o = static_cast<int>(s0 & (S - 1));
+        auto fetch = [&](int head2) {
+          const bool key = head2 < ca.heads;
+          const long long* const xs = key ? ca.key_strides : ca.value_strides;
+          HeadWalk<T, D> walk;
+          walk.at = static_cast<T*>(const_cast<void*>(key ? ca.key : ca.value)) + (t0 + r0) * xs[0] + (key ? head2 : head2 - ca.heads) * xs[1];
+          walk.unit = step * xs[0];
 #pragma unroll
-      for (int k = 0; k < HELD; ++k) {
-        u[k][0] = u[k][1] = make_uint4(0, 0, 0, 0);
-        if (r0 + k * step < len) {
-          const uint4* const p = reinterpret_cast<const uint4*>(x + (r0 + k * step) * xs[0]);
-          u[k][0] = __ldg(p + lanes.g0), u[k][1] = __ldg(p + lanes.g1);
+          for (int i = 0; i < HOLD; ++i) walk.fetch(lanes, i, ring + i * kUnitPieces, r0 + i * step < len);
+          fetch_commit();
+        };
+        if (part < 2 * ca.heads) fetch(part);
+        if (left == window.leaders) origin = window.origin();
+        if (part < ca.heads) {  // this CTA has keys of the run: its angles
+          const long long run_origin = __shfl_sync(kAllLanes, origin, at);
+          __syncthreads();      // the last run's have been read
+          const WarpAngles<T, D> angles(a.queries.rotary);
+          for (int r = warp; r < len; r += W)
+            angles.write(tables + r * D, [&](int axis) { return given ? given_position(a, axis, t0 + r) : run_origin + t0 + r; });
+          __syncthreads();
+        }
+        for (int head2 = part; head2 < 2 * ca.heads; head2 += a.kv_parts) {
+          const bool key = head2 < ca.heads;
+          const int h = key ? head2 : head2 - ca.heads;
+          float* const scale_at = (key ? ca.k_scales : ca.v_scales) + blk * ca.heads + h;
+          const float old = o > 0 ? *scale_at : 0.f;
+          fetch_wait<0>();
+          uint64_t v[HOLD][2 * C];
+#pragma unroll
+          for (int i = 0; i < HOLD; ++i) {
+            uint4 p[2];
+            fetched(ring + i * kUnitPieces, p);
+            Lanes::unpack(p, v[i]);
+          }
+          if (head2 + a.kv_parts < 2 * ca.heads) fetch(head2 + a.kv_parts);
+          if (key) {
+            lanes.template norm<HOLD>(a.queries.rotary, s_weight, v);
+            if (lanes.rotated) {
+#pragma unroll
+              for (int i = 0; i < HOLD; ++i) {
+                uint64_t c[C], s[C];
+                const float* const table = tables + min(r0 + i * step, S - 1) * D;
+                lanes.take(table, c), lanes.take(table + D / 2, s);
+                Lanes::template turn<false>(a.queries.rotary.interleaved, c, s, v[i]);
+              }
+            }
+          }
+          float top = 0;
+#pragma unroll
+          for (int i = 0; i < HOLD; ++i)
+            if (r0 + i * step < len) top = largest(top, v[i], false);
+          top = top_of(top);
+          if (top == INFINITY) {  // rare; the same for all warps
+            top = 0;
+#pragma unroll
+            for (int i = 0; i < HOLD; ++i)
+              if (r0 + i * step < len) top = largest(top, v[i], true);
+            top = top_of(top);
+          }
+          const long long* const cs = key ? ca.k_cache_strides : ca.v_cache_strides;
+          uint8_t* const block = (key ? ca.k_cache : ca.v_cache) + blk * cs[0] + h * cs[2];
+          const float scale = scale_of_run<T, D>(lanes, top, old, block, cs[1], o, r0, step), inv = 1.f / scale;
+          uint8_t* const row = block + (o + r0) * cs[1];
+#pragma unroll
+          for (int i = 0; i < HOLD; ++i)
+            if (r0 + i * step < len) store_row<T, D>(lanes, row + i * step * cs[1], v[i], inv);
+          if (threadIdx.x == 0 && scale != old) *scale_at = scale;
         }
       }
-      if (is_key) {
-        store_run<T, D, HELD, false, true>(a, lanes, s_weight, u, r0, step, h, t0, blk, o, len, first,
-                                    [&](int r, uint64_t (&c)[C], uint64_t (&s)[C]) { own_angles(t0 + r, run_origin, c, s); }, top_of);
-      } else {
-        store_run<T, D, HELD, false, false>(a, lanes, s_weight, u, r0, step, h, t0, blk, o, len, first, none, top_of);
-      }
     }
-  };
-  if (runs > 16) deal(std::true_type{});
-  else deal(std::false_type{});
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // this kernel ends after the queries': what follows on the stream waits for both
 }
 
 }  // namespace
 
 int launch_rotated_append(RotatedAppendArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream) {
   if (a.cache.tokens == 0) return 0;
+  const long long windows = (a.cache.tokens + 31) / 32, resident = 4ll * sm_count;
+  const int heads_a_warp = (is_fp32 ? 256 : 512) / head_dim;
+  // CTAs for a window, of `warps` warps: until `wanted` of them are there, at most one warp for each run and head of single tokens
+  auto parts = [&](long long wanted, int warps) -> long long {
+    if (a.cache.num_blocks == 0) return 0;
+    const long long most = (32ll * 2 * a.cache.heads / heads_a_warp + warps - 1) / warps, n = (wanted + windows - 1) / windows;
+    return n > most ? most : n;
+  };
+  auto query_ctas = [&]() {
+    const long long n = (static_cast<long long>(a.queries.items[0]) + kWarps - 1) / kWarps;
+    return n < resident ? n : resident;
+  };
+  auto by_type = [&](auto body) -> int {
+    using D64 = std::integral_constant<int, 64>;
+    using D128 = std::integral_constant<int, 128>;
+    if (is_fp32) return head_dim == 128 ? body(float{}, D128{}) : body(float{}, D64{});
+    return head_dim == 128 ? body(__nv_bfloat16{}, D128{}) : body(__nv_bfloat16{}, D64{});
+  };
+  a.kv_windows = static_cast<int>(windows);
+  // Few tokens of each request (or few at all): one launch, in which keys and values have a third of the CTAs that are resident.
+  if (a.cache.tokens < 16ll * a.batch || a.cache.tokens < 2048) {
+    a.kv_parts = static_cast<int>(parts(resident / 3, kWarps));
+    plan_items(a.queries, head_dim, is_fp32, (resident - (resident / 3)) * kWarps, kTokens);
+    const long long grid = windows * a.kv_parts + query_ctas();
+    if (grid > 0x7fffffffll) return GDPA_ERR_LAUNCH_;
+    return by_type([&](auto type, auto dim) -> int {
+      gdpa_rotated_step_kernel<decltype(type), decltype(dim)::value><<<static_cast<unsigned>(grid), kWarps * 32, kQueryBytes, stream>>>(a);
+      return cudaGetLastError() == cudaSuccess ? 0 : GDPA_ERR_LAUNCH_;
+    });
+  }
+  plan_items(a.queries, head_dim, is_fp32, resident * kWarps, kTokens);
+  const int rc = by_type([&](auto type, auto dim) -> int {
+    gdpa_rotated_queries_kernel<decltype(type), decltype(dim)::value><<<static_cast<unsigned>(query_ctas()), kWarps * 32, kQueryBytes, stream>>>(a);
+    return cudaGetLastError() == cudaSuccess ? 0 : GDPA_ERR_LAUNCH_;
+  });
+  if (rc != 0 || a.cache.num_blocks == 0) return rc;
   auto launch = [&](auto type, auto dim, auto warps, auto hold) -> int {
     using T = decltype(type);
     constexpr int D = decltype(dim)::value, W = decltype(warps)::value, HOLD = decltype(hold)::value;
-    using Lanes = HeadLanes<T, D>;
-    const int S = 1 << a.cache.block_shift;
-    // keys and values: as many CTAs for a window as make two waves, at most one warp for each run and head of single tokens
-    const long long windows = (a.cache.tokens + 31) / 32, wanted = (32ll / W) * sm_count;
-    const long long most = (32ll * 2 * a.cache.heads / Lanes::H + W - 1) / W;
-    long long parts = a.cache.num_blocks > 0 ? (wanted + windows - 1) / windows : 0;
-    parts = parts > most ? most : parts;
-    a.kv_windows = static_cast<int>(windows);
-    a.kv_parts = static_cast<int>(parts);
-    plan_items(a.queries, head_dim, is_fp32, 10ll * sm_count);
-    long long query_ctas = (static_cast<long long>(a.queries.items[0]) + W - 1) / W;
-    if (query_ctas > (16ll / W) * sm_count) query_ctas = (16ll / W) * sm_count;
-    const long long grid = windows * parts + query_ctas;
+    a.kv_parts = static_cast<int>(parts((24ll / W) * sm_count, W));
+    const long long grid = windows * a.kv_parts;
     if (grid > 0x7fffffffll) return GDPA_ERR_LAUNCH_;
-    auto kernel = gdpa_rotated_append_kernel<T, D, W, HOLD>;
-    const int rows = S > W * kItemTokens ? S : W * kItemTokens;
-    const int smem = W * kRing<HOLD> * kUnitPieces * 16 + rows * D * static_cast<int>(sizeof(float));
+    auto kernel = gdpa_rotated_runs_kernel<T, D, W, HOLD>;
+    const int smem = W * HOLD * kUnitPieces * 16 + (D << a.cache.block_shift) * static_cast<int>(sizeof(float));
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return GDPA_ERR_LAUNCH_;
-    kernel<<<static_cast<unsigned>(grid), W * 32, smem, stream>>>(a);
-    return cudaGetLastError() == cudaSuccess ? 0 : GDPA_ERR_LAUNCH_;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(static_cast<unsigned>(grid));
+    c.blockDim = dim3(W * 32);
+    c.dynamicSmemBytes = smem;
+    c.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, static_cast<const RotatedAppendArgs&>(a)) == cudaSuccess ? 0 : GDPA_ERR_LAUNCH_;
   };
-  // Warps so that a lane holds 32 values of a block at most: those of one head of 64 tokens and 128 values take eight.
-  auto by_block = [&](auto type, auto dim) -> int {
+  // Warps so that a lane holds 64 values of a block at most: a head of 64 tokens and 128 values takes four, one of 128 tokens eight.
+  return by_type([&](auto type, auto dim) -> int {
     using T = decltype(type);
-    constexpr int D = decltype(dim)::value, H = HeadLanes<T, D>::H;
+    constexpr int D = decltype(dim)::value, V = 2 * HeadLanes<T, D>::E;
     using W4 = std::integral_constant<int, 4>;
     using W8 = std::integral_constant<int, 8>;
-    using W16 = std::integral_constant<int, 16>;
-    using Most = std::integral_constant<int, 128 * 128 / (16 * HeadLanes<T, 128>::H * 128)>;  // 2 (bf16), 4 (fp32)
-    using Half = std::integral_constant<int, Most::value / 2>;
     const int values = D << a.cache.block_shift;
     if constexpr (D == 128) {
-      if (values == 128 * 128) return launch(type, dim, W16{}, Most{});
+      if (values == 16384) return launch(type, dim, W8{}, std::integral_constant<int, 64 / V>{});
     }
-    if (values == 128 * 64) return launch(type, dim, W8{}, std::integral_constant<int, 128 * 64 / (8 * H * D)>{});
-    if (values == 128 * 32) return launch(type, dim, W4{}, std::integral_constant<int, 128 * 32 / (4 * H * D)>{});
-    return launch(type, dim, W4{}, Half{});
-  };
-  using D64 = std::integral_constant<int, 64>;
-  using D128 = std::integral_constant<int, 128>;
-  if (is_fp32) return head_dim == 128 ? by_block(float{}, D128{}) : by_block(float{}, D64{});
-  return head_dim == 128 ? by_block(__nv_bfloat16{}, D128{}) : by_block(__nv_bfloat16{}, D64{});
+    if (values == 8192) return launch(type, dim, W4{}, std::integral_constant<int, 64 / V>{});
+    if (values == 4096) return launch(type, dim, W4{}, std::integral_constant<int, 32 / V>{});
+    return launch(type, dim, W4{}, std::integral_constant<int, 16 / V>{});
+  });
 }
 
 }  // namespace gdpa

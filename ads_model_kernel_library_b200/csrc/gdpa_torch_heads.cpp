@@ -18,6 +18,7 @@ struct EntryPoints {
   int (*append)(const GdpaRotatedAppendParams*, gdpa_stream_t);
   int (*read)(const GdpaCacheReadParams*, gdpa_stream_t);
   int (*verify)(const GdpaVerifyParams*, gdpa_stream_t);
+  size_t (*drop_workspace)(int32_t);
   int (*drop)(const GdpaDropParams*, gdpa_stream_t);
 } g_call{};
 
@@ -434,6 +435,13 @@ std::tuple<at::Tensor, at::Tensor> drop_tokens(const at::Tensor& block_tables, c
   p.num_free = num_free.const_data_ptr<int32_t>();
   p.seq_lens_after = lens.mutable_data_ptr<int32_t>();
   p.num_free_after = left.mutable_data_ptr<int32_t>();
+  const size_t bytes = g_call.drop_workspace(p.batch);
+  at::Tensor workspace;
+  if (bytes > 0) {
+    workspace = empty({static_cast<int64_t>(bytes)}, at::kByte, seq_lens);
+    p.workspace = workspace.mutable_data_ptr();
+    p.workspace_bytes = static_cast<int64_t>(bytes);
+  }
   check(g_call.drop(&p, stream()), "gdpa_drop_cached_tokens");
   return {lens, left};
 }
@@ -448,7 +456,8 @@ extern "C" __attribute__((visibility("default"))) void gdpa_torch_init_heads(voi
   g_call.append = reinterpret_cast<decltype(g_call.append)>(f[3]);
   g_call.read = reinterpret_cast<decltype(g_call.read)>(f[4]);
   g_call.verify = reinterpret_cast<decltype(g_call.verify)>(f[5]);
-  g_call.drop = reinterpret_cast<decltype(g_call.drop)>(f[6]);
+  g_call.drop_workspace = reinterpret_cast<decltype(g_call.drop_workspace)>(f[6]);
+  g_call.drop = reinterpret_cast<decltype(g_call.drop)>(f[7]);
 }
 
 TORCH_LIBRARY_FRAGMENT(gdpa, m) {

@@ -45,6 +45,7 @@ EXPORTS = (
     "gdpa_append_rotated_kv_cache_fp8",
     "gdpa_read_kv_cache_fp8",
     "gdpa_verify_draft_tokens",
+    "gdpa_drop_workspace_bytes",
     "gdpa_drop_cached_tokens",
     "gdpa_bwd_workspace_bytes",
     "gdpa_bwd",
@@ -461,6 +462,8 @@ class GdpaDropParams(C.Structure):
         ("num_free", C.c_void_p),
         ("seq_lens_after", C.c_void_p),
         ("num_free_after", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
     ]
 
 
@@ -504,6 +507,8 @@ def _load() -> C.CDLL:
         fn.argtypes = [C.POINTER(params), C.c_void_p]
     lib.gdpa_paged_workspace_bytes.restype = C.c_size_t
     lib.gdpa_paged_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32]
+    lib.gdpa_drop_workspace_bytes.restype = C.c_size_t
+    lib.gdpa_drop_workspace_bytes.argtypes = [C.c_int32]
     lib.gdpa_rotary_workspace_bytes.restype = C.c_size_t
     lib.gdpa_rotary_workspace_bytes.argtypes = [C.c_int32]
     lib.gdpa_strerror.restype = C.c_char_p

@@ -634,7 +634,12 @@ typedef struct GdpaDropParams {
   const int32_t* num_free;     /* device; negative counts as 0 */
   int32_t* seq_lens_after;     /* out [batch] */
   int32_t* num_free_after;     /* out [1], not the word num_free points to */
+  void* workspace;             /* gdpa_drop_workspace_bytes() bytes, 16-byte aligned; one per call in flight */
+  int64_t workspace_bytes;
 } GdpaDropParams;
+
+/* Bytes of the workspace of a call; 0 for small batches, which need none. */
+size_t gdpa_drop_workspace_bytes(int32_t batch);
 
 int gdpa_drop_cached_tokens(const GdpaDropParams* params, gdpa_stream_t stream);
 

@@ -839,6 +839,10 @@ int gdpa_read_kv_cache_fp8(const GdpaCacheReadParams* p, gdpa_stream_t stream) {
   return rc;
 }
 
+size_t gdpa_verify_workspace_bytes(int32_t batch, int32_t vocab, int32_t is_bf16) {
+  return batch > 0 && vocab > 0 ? static_cast<size_t>(verify_workspace(batch, vocab, is_bf16).bytes) : 0;
+}
+
 int gdpa_verify_draft_tokens(const GdpaVerifyParams* p, gdpa_stream_t stream) {
   if (p == nullptr || p->struct_size != sizeof(GdpaVerifyParams)) return GDPA_ERR_BAD_ARG;
   if (p->rows < 0 || p->drafts < 0 || p->vocab < 1 || p->vocab > verify_most_vocab() || p->batch < 0 || p->batch > (1 << 27)) return GDPA_ERR_BAD_ARG;
@@ -849,6 +853,10 @@ int gdpa_verify_draft_tokens(const GdpaVerifyParams* p, gdpa_stream_t stream) {
     return GDPA_ERR_BAD_ARG;
   if (p->rows > 0 && p->target == nullptr) return GDPA_ERR_BAD_ARG;
   if (p->drafts > 0 && (p->tokens == nullptr || p->accept == nullptr)) return GDPA_ERR_BAD_ARG;
+  const VerifyWorkspace w = verify_workspace(p->batch, p->vocab, p->is_bf16 != 0);
+  if (w.bytes > 0 && p->workspace == nullptr) return GDPA_ERR_BAD_ARG;
+  if (p->workspace_bytes < w.bytes) return GDPA_ERR_CAPACITY;
+  if (!aligned16(p->workspace, nullptr)) return GDPA_ERR_MISALIGNED;
   DeviceInfo di;
   int rc = device_info(&di);
   if (rc != GDPA_OK) return rc;
@@ -873,8 +881,10 @@ int gdpa_verify_draft_tokens(const GdpaVerifyParams* p, gdpa_stream_t stream) {
   a.out_tokens = p->out_tokens;
   a.accepted = p->accepted;
   a.refused = p->refused;
+  a.draws = p->workspace;
+  a.sums = reinterpret_cast<double*>(static_cast<uint8_t*>(p->workspace) + w.sums);
   rc = launch_verify(a, p->is_bf16 != 0, di.sm_count, static_cast<cudaStream_t>(stream));
-  if (rc == 0) g_launches.fetch_add(1);
+  if (rc == 0) g_launches.fetch_add(w.bytes > 0 ? 3 : 1);
   return rc;
 }
 

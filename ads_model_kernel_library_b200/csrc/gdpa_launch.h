@@ -349,6 +349,13 @@ struct VerifyArgs {
   void* out_tokens;        // [batch, max_drafts + 1], as tokens
   int* accepted;
   int* refused;
+  // many requests: what each draws from, and its stretches' sums, most_stretches for each
+  void* draws;
+  double* sums;
+  int most_stretches;
+};
+struct VerifyWorkspace {
+  long long sums, bytes;  // where the sums are; all of it, 0 for calls that need none
 };
 
 struct DropArgs {
@@ -395,7 +402,8 @@ int launch_rotary_bwd(RotaryArgs& a, int head_dim, int is_fp32, int sm_count, cu
 int rotary_bwd_ctas(int sm_count);  // CTAs that have a row of RotaryArgs::partial each
 int launch_rotated_append(RotatedAppendArgs& a, int head_dim, int is_fp32, int sm_count, cudaStream_t stream);
 int launch_cache_read(CacheReadArgs& a, int head_dim, int out_is_fp32, int sm_count, cudaStream_t stream);
-int launch_verify(const VerifyArgs& a, int is_bf16, int sm_count, cudaStream_t stream);
+VerifyWorkspace verify_workspace(long long batch, long long vocab, int is_bf16);
+int launch_verify(VerifyArgs& a, int is_bf16, int sm_count, cudaStream_t stream);
 int verify_most_vocab();
 long long drop_workspace_ints(long long batch);
 int launch_drop(const DropArgs& a, cudaStream_t stream);

@@ -17,6 +17,7 @@ struct EntryPoints {
   size_t (*rotary_workspace)(int32_t);
   int (*append)(const GdpaRotatedAppendParams*, gdpa_stream_t);
   int (*read)(const GdpaCacheReadParams*, gdpa_stream_t);
+  size_t (*verify_workspace)(int32_t, int32_t, int32_t);
   int (*verify)(const GdpaVerifyParams*, gdpa_stream_t);
   size_t (*drop_workspace)(int32_t);
   int (*drop)(const GdpaDropParams*, gdpa_stream_t);
@@ -400,6 +401,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_drafts(const at::Tensor& t
   p.out_tokens = tokens.mutable_data_ptr();
   p.accepted = accepted.mutable_data_ptr<int32_t>();
   p.refused = refused.mutable_data_ptr<int32_t>();
+  const size_t bytes = g_call.verify_workspace(p.batch, p.vocab, p.is_bf16);
+  at::Tensor workspace;
+  if (bytes > 0) {
+    workspace = empty({static_cast<int64_t>(bytes)}, at::kByte, target_probs);
+    p.workspace = workspace.mutable_data_ptr();
+    p.workspace_bytes = static_cast<int64_t>(bytes);
+  }
   check(g_call.verify(&p, stream()), "gdpa_verify_draft_tokens");
   return {tokens, accepted, refused};
 }
@@ -455,9 +463,10 @@ extern "C" __attribute__((visibility("default"))) void gdpa_torch_init_heads(voi
   g_call.rotary_workspace = reinterpret_cast<decltype(g_call.rotary_workspace)>(f[2]);
   g_call.append = reinterpret_cast<decltype(g_call.append)>(f[3]);
   g_call.read = reinterpret_cast<decltype(g_call.read)>(f[4]);
-  g_call.verify = reinterpret_cast<decltype(g_call.verify)>(f[5]);
-  g_call.drop_workspace = reinterpret_cast<decltype(g_call.drop_workspace)>(f[6]);
-  g_call.drop = reinterpret_cast<decltype(g_call.drop)>(f[7]);
+  g_call.verify_workspace = reinterpret_cast<decltype(g_call.verify_workspace)>(f[5]);
+  g_call.verify = reinterpret_cast<decltype(g_call.verify)>(f[6]);
+  g_call.drop_workspace = reinterpret_cast<decltype(g_call.drop_workspace)>(f[7]);
+  g_call.drop = reinterpret_cast<decltype(g_call.drop)>(f[8]);
 }
 
 TORCH_LIBRARY_FRAGMENT(gdpa, m) {

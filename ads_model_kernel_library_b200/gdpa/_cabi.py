@@ -44,6 +44,7 @@ EXPORTS = (
     "gdpa_rotary_workspace_bytes",
     "gdpa_append_rotated_kv_cache_fp8",
     "gdpa_read_kv_cache_fp8",
+    "gdpa_verify_workspace_bytes",
     "gdpa_verify_draft_tokens",
     "gdpa_drop_workspace_bytes",
     "gdpa_drop_cached_tokens",
@@ -442,6 +443,8 @@ class GdpaVerifyParams(C.Structure):
         ("out_tokens", C.c_void_p),
         ("accepted", C.c_void_p),
         ("refused", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
     ]
 
 
@@ -507,6 +510,8 @@ def _load() -> C.CDLL:
         fn.argtypes = [C.POINTER(params), C.c_void_p]
     lib.gdpa_paged_workspace_bytes.restype = C.c_size_t
     lib.gdpa_paged_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32]
+    lib.gdpa_verify_workspace_bytes.restype = C.c_size_t
+    lib.gdpa_verify_workspace_bytes.argtypes = [C.c_int32, C.c_int32, C.c_int32]
     lib.gdpa_drop_workspace_bytes.restype = C.c_size_t
     lib.gdpa_drop_workspace_bytes.argtypes = [C.c_int32]
     lib.gdpa_rotary_workspace_bytes.restype = C.c_size_t

@@ -60,7 +60,7 @@ class _Operators:
         entries = (lib.gdpa_build_block_tables, lib.gdpa_append_kv_cache_fp8, lib.gdpa_paged_workspace_bytes, lib.gdpa_fwd_paged_fp8, lib.gdpa_strerror)
         self.native.gdpa_torch_init(*(C.cast(f, C.c_void_p) for f in entries))
         entries = (lib.gdpa_qk_norm_rotary, lib.gdpa_qk_norm_rotary_bwd, lib.gdpa_rotary_workspace_bytes, lib.gdpa_append_rotated_kv_cache_fp8,
-                   lib.gdpa_read_kv_cache_fp8, lib.gdpa_verify_draft_tokens, lib.gdpa_drop_workspace_bytes, lib.gdpa_drop_cached_tokens)
+                   lib.gdpa_read_kv_cache_fp8, lib.gdpa_verify_workspace_bytes, lib.gdpa_verify_draft_tokens, lib.gdpa_drop_workspace_bytes, lib.gdpa_drop_cached_tokens)
         self.native.gdpa_torch_init_heads((C.c_void_p * len(entries))(*(C.cast(f, C.c_void_p) for f in entries)))
         self.native.gdpa_torch_set_timing.argtypes = [C.c_void_p, C.c_void_p]
         self.native.gdpa_torch_set_status_look(_look_at_status)

@@ -611,7 +611,12 @@ typedef struct GdpaVerifyParams {
   void* out_tokens;            /* out [batch, max_drafts + 1]: the accepted drafts, the next token, then -1; a request without rows: -1 */
   int32_t* accepted;           /* out [batch] */
   int32_t* refused;            /* out [batch]: n - a */
+  void* workspace;             /* gdpa_verify_workspace_bytes() bytes, 16-byte aligned; one per call in flight */
+  int64_t workspace_bytes;
 } GdpaVerifyParams;
+
+/* Bytes of the workspace of a call; 0 for few requests, which need none. */
+size_t gdpa_verify_workspace_bytes(int32_t batch, int32_t vocab, int32_t is_bf16);
 
 int gdpa_verify_draft_tokens(const GdpaVerifyParams* params, gdpa_stream_t stream);
 

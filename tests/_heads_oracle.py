@@ -163,7 +163,7 @@ def verify(target, draft, tokens, offsets, draft_offsets, accept, sample, most):
             if draft is None:
                 left = [0.0 if i == tokens[d0 + a] else v for i, v in enumerate(p)]
             else:
-                left = [_share(t - (q if q > 0 else 0.0)) for t, q in zip(target[offsets[b] + a], draft[d0 + a])]
+                left = [_share(_share(t) - _share(q)) for t, q in zip(target[offsets[b] + a], draft[d0 + a])]
             if not sum(left) > 0:
                 left = p
         mark, below, token = sample[b] * math.fsum(left), 0.0, -1

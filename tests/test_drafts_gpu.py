@@ -74,14 +74,29 @@ def test_verify_many():
     check_verify([1], 300000, torch.bfloat16)
 
 
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 65537), (torch.bfloat16, 131079)])
+def test_verify_many_long_rows(dtype, vocab):
+    """Rows that are enough for the three kernels."""
+    def edit(target, draft, tokens, accept, sample):
+        target[3, 700], target[4, 65000], draft[2] = math.nan, math.inf, 9.0
+        target[9:14] = 0.0
+        sample[1], sample[2] = 0.0, 1.0
+
+    drafts = [i % 3 for i in range(32)]
+    check_verify(drafts, vocab, dtype, edit=edit)
+    check_verify(drafts, vocab, dtype, lookup=True, edit=lambda t, d, x, a, s: a.mul_(1e-4), seed=1)
+    check_verify(drafts, vocab, dtype, padded=3, rows=[0, 2, 1] * 10 + [3, 0], ints=torch.int32, agree=0.95, seed=2)
+
+
 def test_verify_marks_on_borders():
     for seed in range(6):
         check_verify([1, 2, 0, 1] * 8, (50, 1024, 2050, 5000, 9000, 16384)[seed], exact_sums=True, seed=seed)
+    check_verify([1, 2, 0, 1] * 8, 65600, exact_sums=True, seed=6)
 
 
 def test_verify_numbers_that_are_none():
     def edit(target, draft, tokens, accept, sample):
-        target[0, 5], target[1, 3], draft[0, 2], target[2] = math.nan, math.inf, math.nan, -1.0
+        target[0, 5], target[1, 3], draft[0, 2], draft[0, 7], draft[0, 8], target[2] = math.nan, math.inf, math.nan, math.inf, -0.5, -1.0
         target[3] = 0.0
         draft[1] = 9.0  # nothing is left of the difference
         target[6, :], target[6, 77] = 0.0, 1e-38
@@ -90,6 +105,7 @@ def test_verify_numbers_that_are_none():
 
     for lookup in (False, True):
         check_verify([1, 1, 1, 1, 0], 100, edit=edit, lookup=lookup)
+        check_verify([1, 1, 1, 1, 0], 9001, torch.bfloat16, edit=edit, lookup=lookup)
         check_verify([1, 1, 1, 1, 0], 5000, edit=edit, lookup=lookup, ints=torch.int32)
 
 

@@ -793,8 +793,9 @@ int gdpa_append_rotated_kv_cache_fp8(const GdpaRotatedAppendParams* p, gdpa_stre
   a.lens64 = p->lens_are_int64 != 0 ? kOffsets64 : 0;
   a.batch = p->batch;
   rc = launch_rotated_append(a, p->cache.head_dim, p->cache.x_is_fp32 != 0, di.sm_count, static_cast<cudaStream_t>(stream));
-  if (rc == 0) g_launches.fetch_add(1);
-  return rc;
+  if (rc < 0) return -rc;
+  g_launches.fetch_add(rc);
+  return GDPA_OK;
 }
 
 int gdpa_read_kv_cache_fp8(const GdpaCacheReadParams* p, gdpa_stream_t stream) {

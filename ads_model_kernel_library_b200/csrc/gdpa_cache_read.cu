@@ -52,8 +52,8 @@ __global__ void __launch_bounds__(kReadWarps * 32) gdpa_cache_read_kernel(const 
   int block = -1, row = 0;
   if (a.batch > 0 && lane < tokens) {
     const long long begin = load_offset(a.offsets, owner, a.off64), end = load_offset(a.offsets, owner + 1, a.off64);
-    const long long p = (a.first != nullptr ? load_offset(a.first, owner, a.first64) : 0) + (base + lane - begin);
-    if (base + lane >= begin && base + lane < end && p >= 0 && (p >> a.block_shift) < a.table_width) {
+    const long long first = a.first != nullptr ? load_offset(a.first, owner, a.first64) : 0, p = first + (base + lane - begin);
+    if (base + lane >= begin && base + lane < end && first < (1ll << 31) && p >= 0 && (p >> a.block_shift) < a.table_width) {
       block = a.block_tables[owner * a.table_stride + (p >> a.block_shift)];
       row = static_cast<int>(p & ((1 << a.block_shift) - 1));
       if (block < 0 || block >= a.num_blocks) block = -1;

@@ -13,8 +13,8 @@
 // passes its mark is looked at again (it is in the L2 cache).
 //
 // Few requests: one launch, a cluster of CTAs to each, and latency is all of it.  Many: three kernels, whose beginnings overlap the ends of those before
-// them: who is accepted; the stretches' sums, dealt out over the whole GPU (a CTA to a request leaves SMs with one row to add up and SMs with four: 256
-// requests of 131071 bf16 tokens, 116 MB, 46 us so); the token.
+// them: who is accepted; the stretches' sums, dealt out over the whole GPU (a CTA to a request leaves SMs with one row to add up and SMs with four);
+// the token.  256 requests of 131071 bf16 tokens, 116 MB: 49 us in one kernel, 43 in three, 34 of them for the sums.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -253,8 +253,8 @@ __device__ __forceinline__ int accept(const VerifyArgs& a, const Request& r) {
       const double u = a.accept[r.d0 + j];
       refused = true;
       if (x >= 0 && x < a.vocab) {
-        const double p = as_float(target[(r.row0 + j) * a.target_stride + x]);
-        const double q = draft != nullptr ? static_cast<double>(as_float(draft[(r.d0 + j) * a.draft_stride + x])) : 1.0;
+        const double p = share(as_float(target[(r.row0 + j) * a.target_stride + x]));
+        const double q = draft != nullptr ? static_cast<double>(share(as_float(draft[(r.d0 + j) * a.draft_stride + x]))) : 1.0;
         refused = !(u * q < p);
       }
     }
@@ -524,7 +524,8 @@ __global__ void __launch_bounds__(kVerifyThreads) gdpa_verify_draw_kernel(const 
 //
 // Latency is all of it.  A warp has four requests, up to 128 entries of each, all asked for at once and kept in registers until it is known how many go
 // before them.  Up to 256 requests, a cluster of CTAs adds that up in shared memory.  More of them: one kernel counts, another, whose loads the end
-// of the first overlaps, adds up the counts of the CTAs before its own; 4096 requests with 64 entries each 48 us in one cluster, 9 so.
+// of the first overlaps, adds up the counts of the CTAs before its own (4096 requests with 64 entries each: 11 us; up to
+// 256 requests a cluster is 2 us faster).
 constexpr int kDropWarps = 8, kDropRequests = 4;
 
 enum DropWay { kDropCluster, kDropCount, kDropStore };
@@ -659,7 +660,8 @@ int launch_cluster(K kernel, const A& args, unsigned grid, unsigned threads, uns
 int verify_most_vocab() { return kMostVocab; }
 
 namespace {
-// Whether a call takes the three kernels: where its rows are enough to keep the whole GPU busy with either of them.
+// Whether a call takes the three kernels: where its rows keep the whole GPU busy.  One kernel against three, us, rows of bf16: 64 requests of 32000 tokens (4 MB) 14
+// and 16, 32 of 131071 (8 MB) 20 and 18, 256 of 32000 22 and 22, 256 of 131071 49 and 43.
 bool many_requests(long long batch, long long vocab, int size) { return batch >= 32 && batch * vocab * size >= (8ll << 20); }
 long long most_stretches(long long vocab, int size) { return (vocab * size + 15) / (32 * kManyBlocks * 16) + 1; }
 }  // namespace

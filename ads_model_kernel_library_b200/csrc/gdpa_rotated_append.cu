@@ -1,13 +1,16 @@
 // A serving step's queries, keys and values between the projection and the attention: queries and keys are normed and rotated
 // (gdpa_rotary.cuh), keys and values quantised into their slots of the paged cache as gdpa_cache.cu does it (the same runs, scales and
-// rules), queries written for the attention.  One launch: the first CTAs have keys and values, the others queries.
+// rules), queries written for the attention.
 //
 // What bounds it: HBM for prompts (a query value is 2 bytes in and 2 out, a key or value 2 and 1), latency for single tokens.  Rotated keys stay in
 // fp32 registers between the maximum of a run and its conversion: they are rounded once, to e4m3.
 //
-// Keys and values: a CTA looks at a window of 32 tokens for the runs that begin there.  Three ways to share the work, by the window's
-// number of runs: all warps on one (run, head), the run's angles in shared memory for all its heads (prompts); a warp to each (run, head), a
-// head's lanes to a row (drafts); a head's lanes to each (run, head) (single tokens).
+// A few tokens of each request are one launch: the first CTAs have keys and values, the others queries.  Prompts are two: queries as in
+// gdpa_rotary.cu, then keys and values, a CTA to a block's run, whose loads overlap the end of the first.  In one kernel, each kind of work has the registers of all.
+//
+// Keys and values: a CTA looks at a window of 32 tokens for the runs that begin there, and each run is taken according to its length: by
+// a head's lanes (one or two tokens), by a warp with a head's lanes to a row, or by a CTA, so that a prompt among single tokens does not keep a few lanes busy for
+// long (255 single tokens and a prompt of 512: 118 us with one way for all of a window's runs, 21 so).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -181,6 +184,7 @@ struct Window {
   const RotatedAppendArgs& a;
   long long base, slot;  // its first token; the lane's slot, or -1
   unsigned leaders;      // lanes whose token begins a run
+  int len;               // the lane's run, as far as the slots go on, at most to the end of the block; 0: it leads none
 
   __device__ __forceinline__ long long slot_of(long long t) const {
     const CacheAppendArgs& ca = a.cache;
@@ -189,11 +193,27 @@ struct Window {
     return s >= 0 && s < (ca.num_blocks << ca.block_shift) ? s : -1;
   }
   __device__ __forceinline__ Window(const RotatedAppendArgs& args, long long first) : a(args), base(first) {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, S = 1 << a.cache.block_shift;
     slot = slot_of(base + lane);
     long long before = __shfl_up_sync(kAllLanes, slot, 1);
     if (lane == 0) before = slot_of(base - 1);
-    leaders = __ballot_sync(kAllLanes, slot >= 0 && ((slot & ((1 << a.cache.block_shift) - 1)) == 0 || before != slot - 1));
+    leaders = __ballot_sync(kAllLanes, slot >= 0 && ((slot & (S - 1)) == 0 || before != slot - 1));
+    const unsigned ends = (leaders | __ballot_sync(kAllLanes, slot < 0)) & ~((2u << lane) - 1);  // behind the lane
+    len = (leaders >> lane & 1u) == 0 ? 0 : ends != 0 ? __ffs(ends) - 1 - lane : 32 - lane;
+    // the last run may go on behind the window
+    if (leaders == 0) return;
+    const int last = 31 - __clz(leaders);
+    int its = __shfl_sync(kAllLanes, len, last);
+    if (last + its < 32) return;
+    const long long s0 = __shfl_sync(kAllLanes, slot, last);
+    const int o = static_cast<int>(s0 & (S - 1));
+    for (bool more = true; more;) {
+      const int i = its + lane;
+      const unsigned stops = __ballot_sync(kAllLanes, !(o + i < S && slot_of(base + last + i) == s0 + i));
+      its += stops ? __ffs(stops) - 1 : 32;
+      more = stops == 0;
+    }
+    if (lane == last) len = its;
   }
   // position of the first token of the run that the lane leads, less its index
   __device__ __forceinline__ long long origin() const {
@@ -212,20 +232,6 @@ struct Window {
     }
     return origin_of(a, owner);
   }
-  // tokens of the run that begins with token base + at, in slot s0: as far as the slots go on, at most to the end of the block
-  __device__ __forceinline__ int length_of(int at, long long s0) const {
-    const int lane = threadIdx.x & 31, S = 1 << a.cache.block_shift, o = static_cast<int>(s0 & (S - 1));
-    int len = 0;
-    for (bool more = true; more;) {
-      const int i = len + lane;
-      const long long near = __shfl_sync(kAllLanes, slot, (at + i) & 31);
-      const bool goes_on = o + i < S && (at + i < 32 ? near : slot_of(base + at + i)) == s0 + i;
-      const unsigned stops = __ballot_sync(kAllLanes, !goes_on);
-      len += stops ? __ffs(stops) - 1 : 32;
-      more = stops == 0;
-    }
-    return len;
-  }
 };
 
 // What the lanes make angles from by themselves, for a whole CTA: frequency and axis of the pairs, in a lane's order.
@@ -242,43 +248,54 @@ __device__ __forceinline__ void write_pairs(const RotarySpec& r, PairTable<D>& t
   }
 }
 
-// A window's runs over the warps: a warp to each run and head, its heads' lanes to a row each; or (SINGLE) a head's lanes to each run and head.
-// This is warp `me` of `warps`.
-template <class T, int D, bool SINGLE>
-__device__ __forceinline__ void deal(const Window& window, const HeadLanes<T, D>& lanes, const float* s_weight, const PairTable<D>& pairs, int me, int warps) {
+// The maximum of W warps' numbers.  Two places for each, in turn: the next maximum is written while this one may still be read.
+template <int W>
+__device__ __forceinline__ float top_of_cta(float top, float* tops, unsigned& turn) {
+  float* const s = tops + (turn++ & 1u) * W;
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = top;
+  __syncthreads();
+  top = s[0];
+#pragma unroll
+  for (int i = 1; i < W; ++i) top = fmaxf(top, s[i]);
+  return top;
+}
+
+// Some of a window's runs, dealt out: a head's lanes to each run and head; a warp to each, its heads' lanes to a row each; or a CTA to each, by its warps' lanes.
+// This is taker `me` of `takers` (warps, or CTAs); `tops`: two words for each warp, of a CTA's maximum.
+enum Taker { kHeadLanes, kWarp, kCta };
+template <class T, int D, Taker TAKER, int W>
+__device__ __forceinline__ void deal(const Window& window, unsigned leaders, long long origin, const HeadLanes<T, D>& lanes, const float* s_weight, const PairTable<D>& pairs,
+                                     int me, int takers, float* tops) {
   using Lanes = HeadLanes<T, D>;
-  constexpr int C = Lanes::C, a_warp = SINGLE ? Lanes::H : 1, step = SINGLE ? 1 : Lanes::H;
+  constexpr bool SINGLE = TAKER == kHeadLanes;
+  constexpr int C = Lanes::C, a_warp = SINGLE ? Lanes::H : 1, step = SINGLE ? 1 : TAKER == kWarp ? Lanes::H : W * Lanes::H;
+  const int warp = threadIdx.x >> 5;
+  unsigned turn = 0;
+  if (leaders == 0) return;
   const RotatedAppendArgs& a = window.a;
   const CacheAppendArgs& ca = a.cache;
   const bool given = a.queries.t[0].positions != nullptr;
-  const long long origin = window.origin();
-  const int tasks = __popc(window.leaders) * ca.heads, rounds = (tasks + a_warp - 1) / a_warp;
-  for (int i = me; i < 2 * rounds; i += warps) {
+  const int tasks = __popc(leaders) * ca.heads, rounds = (tasks + a_warp - 1) / a_warp;
+  for (int i = me; i < 2 * rounds; i += takers) {
     const bool is_key = i < rounds;
     const int task = (is_key ? i : i - rounds) * a_warp + (SINGLE ? lanes.sub : 0);
     const bool there = task < tasks;
-    const int at = there ? __fns(window.leaders, 0, task / ca.heads + 1) : 0, h = there ? task % ca.heads : 0;
+    const int at = there ? __fns(leaders, 0, task / ca.heads + 1) : 0, h = there ? task % ca.heads : 0;
     const long long s0 = __shfl_sync(kAllLanes, window.slot, at), run_origin = __shfl_sync(kAllLanes, origin, at), t0 = window.base + at;
-    int len = 0;
-    if constexpr (SINGLE) {
-#pragma unroll
-      for (int k = 0; k < Lanes::H; ++k) {  // each by the whole warp
-        const int l = window.length_of(__shfl_sync(kAllLanes, at, k * Lanes::L), __shfl_sync(kAllLanes, s0, k * Lanes::L));
-        if (lanes.sub == k) len = l;
-      }
-    } else {
-      len = window.length_of(at, s0);
-    }
-    if (!there) len = 0;
+    const int run_len = __shfl_sync(kAllLanes, window.len, at), len = there ? run_len : 0;
     const long long blk = there ? s0 >> ca.block_shift : 0;
-    const int o = there ? static_cast<int>(s0 & ((1 << ca.block_shift) - 1)) : 0, r0 = SINGLE ? 0 : lanes.sub;
+    const int o = there ? static_cast<int>(s0 & ((1 << ca.block_shift) - 1)) : 0, r0 = SINGLE ? 0 : TAKER == kWarp ? lanes.sub : warp * Lanes::H + lanes.sub;
     auto top_of = [&](float top) {
-      if (!SINGLE) return __uint_as_float(__reduce_max_sync(kAllLanes, __float_as_uint(top)));
+      if constexpr (SINGLE) {
 #pragma unroll
-      for (int s = 1; s < Lanes::L; s <<= 1) top = fmaxf(top, __shfl_xor_sync(kAllLanes, top, s));
+        for (int s = 1; s < Lanes::L; s <<= 1) top = fmaxf(top, __shfl_xor_sync(kAllLanes, top, s));
+      } else {
+        top = __uint_as_float(__reduce_max_sync(kAllLanes, __float_as_uint(top)));
+        if constexpr (TAKER == kCta) top = top_of_cta<W>(top, tops, turn);
+      }
       return top;
     };
-    const bool first = lanes.l == 0 && (SINGLE || lanes.sub == 0);
+    const bool first = lanes.l == 0 && (SINGLE || r0 == 0);
     if (is_key) {
       store_run<T, D, true>(a, lanes, s_weight, r0, step, h, t0, blk, o, len, first, [&](int r, uint64_t (&c)[C], uint64_t (&s)[C]) {
 #pragma unroll
@@ -331,6 +348,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) gdpa_rotated_step_kernel(const
   __shared__ float4 s_tables[kWarps][kTokens][D / 4];
   __shared__ float4 s_weight4[D / 4];
   __shared__ PairTable<D> s_pairs;
+  __shared__ float s_top[2 * kWarps];
   float* const s_weight = reinterpret_cast<float*>(s_weight4);
   const int warp = threadIdx.x >> 5, kv_ctas = a.kv_windows * a.kv_parts;
   if (static_cast<int>(blockIdx.x) >= kv_ctas) {
@@ -346,9 +364,11 @@ __global__ void __launch_bounds__(kWarps * 32, 4) gdpa_rotated_step_kernel(const
   if (warp == 0) lanes.write_weight(s_weight, a.queries.t[1].weight, a.queries.t[1].weight_is_bf16);
   write_pairs<T, D>(a.queries.rotary, s_pairs);
   __syncthreads();
-  // with two tokens a run at most, on average: a head's lanes to a run
-  if (__popc(window.leaders) > 16) deal<T, D, true>(window, lanes, s_weight, s_pairs, part * kWarps + warp, a.kv_parts * kWarps);
-  else deal<T, D, false>(window, lanes, s_weight, s_pairs, part * kWarps + warp, a.kv_parts * kWarps);
+  const long long origin = window.origin();
+  const unsigned longer = __ballot_sync(kAllLanes, window.len > 2), longest = __ballot_sync(kAllLanes, window.len > kWarps * HeadLanes<T, D>::H);
+  deal<T, D, kCta, kWarps>(window, longest, origin, lanes, s_weight, s_pairs, part, a.kv_parts, s_top);
+  deal<T, D, kWarp, kWarps>(window, longer & ~longest, origin, lanes, s_weight, s_pairs, part * kWarps + warp, a.kv_parts * kWarps, s_top);
+  deal<T, D, kHeadLanes, kWarps>(window, window.leaders & ~longer, origin, lanes, s_weight, s_pairs, part * kWarps + warp, a.kv_parts * kWarps, s_top);
 }
 
 // ------------------------------------------------------------------------------------------ prompts: queries, then keys and values
@@ -374,7 +394,7 @@ __global__ void __launch_bounds__(W * 32, 12 / W) gdpa_rotated_runs_kernel(const
   extern __shared__ uint4 s_dynamic[];  // [warp][HOLD] units; angles of a block's rows, [row][D]
   __shared__ float4 s_weight4[D / 4];
   __shared__ PairTable<D> s_pairs;
-  __shared__ float s_top[2][W];
+  __shared__ float s_top[2 * W];
   float* const s_weight = reinterpret_cast<float*>(s_weight4);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint4* const ring = s_dynamic + warp * HOLD * kUnitPieces;
@@ -385,96 +405,89 @@ __global__ void __launch_bounds__(W * 32, 12 / W) gdpa_rotated_runs_kernel(const
   const Window window(a, static_cast<long long>(blockIdx.x - part * a.kv_windows) * 32);
   if (window.leaders != 0) {
     if (warp == 0) lanes.write_weight(s_weight, a.queries.t[1].weight, a.queries.t[1].weight_is_bf16);
-    if (__popc(window.leaders) > 2) {  // short ones
+    const long long origin = window.origin();
+    unsigned mine = window.leaders;  // runs that are taken by the whole CTA, one after the other: long ones, and a few short ones
+    if (__popc(mine) > 2) {
+      mine = __ballot_sync(kAllLanes, window.len > step);
       write_pairs<T, D>(a.queries.rotary, s_pairs);
       __syncthreads();
-      deal<T, D, false>(window, lanes, s_weight, s_pairs, part * W + warp, a.kv_parts * W);
-    } else {
-      const bool given = a.queries.t[0].positions != nullptr;
-      unsigned turn = 0;
-      auto top_of = [&](float top) {
-        top = __uint_as_float(__reduce_max_sync(kAllLanes, __float_as_uint(top)));
-        float* const s = s_top[turn++ & 1u];  // two in turn: the next maximum is written while this one may still be read
-        if (lane == 0) s[warp] = top;
-        __syncthreads();
-        top = s[0];
+      deal<T, D, kWarp, W>(window, window.leaders & ~mine, origin, lanes, s_weight, s_pairs, part * W + warp, a.kv_parts * W, s_top);
+    }
+    const bool given = a.queries.t[0].positions != nullptr;
+    unsigned turn = 0;
+    auto top_of = [&](float top) {
+      return top_of_cta<W>(__uint_as_float(__reduce_max_sync(kAllLanes, __float_as_uint(top))), s_top, turn);
+    };
+    const int r0 = warp * Lanes::H + lanes.sub, S = 1 << ca.block_shift;
+    for (unsigned left = mine; left != 0; left &= left - 1) {
+      const int at = __ffs(left) - 1;
+      const long long s0 = __shfl_sync(kAllLanes, window.slot, at), t0 = window.base + at, blk = s0 >> ca.block_shift;
+      const int len = __shfl_sync(kAllLanes, window.len, at), o = static_cast<int>(s0 & (S - 1));
+      auto fetch = [&](int head2) {
+        const bool key = head2 < ca.heads;
+        const long long* const xs = key ? ca.key_strides : ca.value_strides;
+        HeadWalk<T, D> walk;
+        walk.at = static_cast<T*>(const_cast<void*>(key ? ca.key : ca.value)) + (t0 + r0) * xs[0] + (key ? head2 : head2 - ca.heads) * xs[1];
+        walk.unit = step * xs[0];
 #pragma unroll
-        for (int i = 1; i < W; ++i) top = fmaxf(top, s[i]);
-        return top;
+        for (int i = 0; i < HOLD; ++i) walk.fetch(lanes, i, ring + i * kUnitPieces, r0 + i * step < len);
+        fetch_commit();
       };
-      const int r0 = warp * Lanes::H + lanes.sub, S = 1 << ca.block_shift;
-      long long origin = 0;
-      for (unsigned left = window.leaders; left != 0; left &= left - 1) {
-        const int at = __ffs(left) - 1;
-        const long long s0 = __shfl_sync(kAllLanes, window.slot, at), t0 = window.base + at, blk = s0 >> ca.block_shift;
-        const int len = window.length_of(at, s0), o = static_cast<int>(s0 & (S - 1));
-        auto fetch = [&](int head2) {
-          const bool key = head2 < ca.heads;
-          const long long* const xs = key ? ca.key_strides : ca.value_strides;
-          HeadWalk<T, D> walk;
-          walk.at = static_cast<T*>(const_cast<void*>(key ? ca.key : ca.value)) + (t0 + r0) * xs[0] + (key ? head2 : head2 - ca.heads) * xs[1];
-          walk.unit = step * xs[0];
+      if (part < 2 * ca.heads) fetch(part);
+      if (part < ca.heads) {  // this CTA has keys of the run: its angles
+        const long long run_origin = __shfl_sync(kAllLanes, origin, at);
+        __syncthreads();      // the last run's have been read
+        const WarpAngles<T, D> angles(a.queries.rotary);
+        for (int r = warp; r < len; r += W)
+          angles.write(tables + r * D, [&](int axis) { return given ? given_position(a, axis, t0 + r) : run_origin + t0 + r; });
+        __syncthreads();
+      }
+      for (int head2 = part; head2 < 2 * ca.heads; head2 += a.kv_parts) {
+        const bool key = head2 < ca.heads;
+        const int h = key ? head2 : head2 - ca.heads;
+        float* const scale_at = (key ? ca.k_scales : ca.v_scales) + blk * ca.heads + h;
+        const float old = o > 0 ? *scale_at : 0.f;
+        fetch_wait<0>();
+        uint64_t v[HOLD][2 * C];
 #pragma unroll
-          for (int i = 0; i < HOLD; ++i) walk.fetch(lanes, i, ring + i * kUnitPieces, r0 + i * step < len);
-          fetch_commit();
-        };
-        if (part < 2 * ca.heads) fetch(part);
-        if (left == window.leaders) origin = window.origin();
-        if (part < ca.heads) {  // this CTA has keys of the run: its angles
-          const long long run_origin = __shfl_sync(kAllLanes, origin, at);
-          __syncthreads();      // the last run's have been read
-          const WarpAngles<T, D> angles(a.queries.rotary);
-          for (int r = warp; r < len; r += W)
-            angles.write(tables + r * D, [&](int axis) { return given ? given_position(a, axis, t0 + r) : run_origin + t0 + r; });
-          __syncthreads();
+        for (int i = 0; i < HOLD; ++i) {
+          uint4 p[2];
+          fetched(ring + i * kUnitPieces, p);
+          Lanes::unpack(p, v[i]);
         }
-        for (int head2 = part; head2 < 2 * ca.heads; head2 += a.kv_parts) {
-          const bool key = head2 < ca.heads;
-          const int h = key ? head2 : head2 - ca.heads;
-          float* const scale_at = (key ? ca.k_scales : ca.v_scales) + blk * ca.heads + h;
-          const float old = o > 0 ? *scale_at : 0.f;
-          fetch_wait<0>();
-          uint64_t v[HOLD][2 * C];
+        if (head2 + a.kv_parts < 2 * ca.heads) fetch(head2 + a.kv_parts);
+        if (key) {
+          lanes.template norm<HOLD>(a.queries.rotary, s_weight, v);
+          if (lanes.rotated) {
 #pragma unroll
-          for (int i = 0; i < HOLD; ++i) {
-            uint4 p[2];
-            fetched(ring + i * kUnitPieces, p);
-            Lanes::unpack(p, v[i]);
-          }
-          if (head2 + a.kv_parts < 2 * ca.heads) fetch(head2 + a.kv_parts);
-          if (key) {
-            lanes.template norm<HOLD>(a.queries.rotary, s_weight, v);
-            if (lanes.rotated) {
-#pragma unroll
-              for (int i = 0; i < HOLD; ++i) {
-                uint64_t c[C], s[C];
-                const float* const table = tables + min(r0 + i * step, S - 1) * D;
-                lanes.take(table, c), lanes.take(table + D / 2, s);
-                Lanes::template turn<false>(a.queries.rotary.interleaved, c, s, v[i]);
-              }
+            for (int i = 0; i < HOLD; ++i) {
+              uint64_t c[C], s[C];
+              const float* const table = tables + min(r0 + i * step, S - 1) * D;
+              lanes.take(table, c), lanes.take(table + D / 2, s);
+              Lanes::template turn<false>(a.queries.rotary.interleaved, c, s, v[i]);
             }
           }
-          float top = 0;
-#pragma unroll
-          for (int i = 0; i < HOLD; ++i)
-            if (r0 + i * step < len) top = largest(top, v[i], false);
-          top = top_of(top);
-          if (top == INFINITY) {  // rare; the same for all warps
-            top = 0;
-#pragma unroll
-            for (int i = 0; i < HOLD; ++i)
-              if (r0 + i * step < len) top = largest(top, v[i], true);
-            top = top_of(top);
-          }
-          const long long* const cs = key ? ca.k_cache_strides : ca.v_cache_strides;
-          uint8_t* const block = (key ? ca.k_cache : ca.v_cache) + blk * cs[0] + h * cs[2];
-          const float scale = scale_of_run<T, D>(lanes, top, old, block, cs[1], o, r0, step), inv = 1.f / scale;
-          uint8_t* const row = block + (o + r0) * cs[1];
-#pragma unroll
-          for (int i = 0; i < HOLD; ++i)
-            if (r0 + i * step < len) store_row<T, D>(lanes, row + i * step * cs[1], v[i], inv);
-          if (threadIdx.x == 0 && scale != old) *scale_at = scale;
         }
+        float top = 0;
+#pragma unroll
+        for (int i = 0; i < HOLD; ++i)
+          if (r0 + i * step < len) top = largest(top, v[i], false);
+        top = top_of(top);
+        if (top == INFINITY) {  // rare; the same for all warps
+          top = 0;
+#pragma unroll
+          for (int i = 0; i < HOLD; ++i)
+            if (r0 + i * step < len) top = largest(top, v[i], true);
+          top = top_of(top);
+        }
+        const long long* const cs = key ? ca.k_cache_strides : ca.v_cache_strides;
+        uint8_t* const block = (key ? ca.k_cache : ca.v_cache) + blk * cs[0] + h * cs[2];
+        const float scale = scale_of_run<T, D>(lanes, top, old, block, cs[1], o, r0, step), inv = 1.f / scale;
+        uint8_t* const row = block + (o + r0) * cs[1];
+#pragma unroll
+        for (int i = 0; i < HOLD; ++i)
+          if (r0 + i * step < len) store_row<T, D>(lanes, row + i * step * cs[1], v[i], inv);
+        if (threadIdx.x == 0 && scale != old) *scale_at = scale;
       }
     }
   }
@@ -504,32 +517,34 @@ int launch_rotated_append(RotatedAppendArgs& a, int head_dim, int is_fp32, int s
     return head_dim == 128 ? body(__nv_bfloat16{}, D128{}) : body(__nv_bfloat16{}, D64{});
   };
   a.kv_windows = static_cast<int>(windows);
-  // Few tokens of each request (or few at all): one launch, in which keys and values have a third of the CTAs that are resident.
-  if (a.cache.tokens < 16ll * a.batch || a.cache.tokens < 2048) {
+  // One launch for a few tokens of each request; keys and values then have a third of the CTAs that are resident.  bf16, 16 and 4 heads of 128 values, one
+  // launch against two, us: 256 requests with 16 tokens 26 and 36, with 32 tokens 42 and 44; 1024 with 32 126 and 103; 64 with 64 39 and 26; one with
+  // 8 tokens 11 and 11, with 4096 38 and 26.  How the tokens are spread over the requests is not known here.
+  if (a.cache.tokens < 24ll * a.batch) {
     a.kv_parts = static_cast<int>(parts(resident / 3, kWarps));
     plan_items(a.queries, head_dim, is_fp32, (resident - (resident / 3)) * kWarps, kTokens);
     const long long grid = windows * a.kv_parts + query_ctas();
-    if (grid > 0x7fffffffll) return GDPA_ERR_LAUNCH_;
+    if (grid > 0x7fffffffll) return -GDPA_ERR_LAUNCH_;
     return by_type([&](auto type, auto dim) -> int {
       gdpa_rotated_step_kernel<decltype(type), decltype(dim)::value><<<static_cast<unsigned>(grid), kWarps * 32, kQueryBytes, stream>>>(a);
-      return cudaGetLastError() == cudaSuccess ? 0 : GDPA_ERR_LAUNCH_;
+      return cudaGetLastError() == cudaSuccess ? 1 : -GDPA_ERR_LAUNCH_;
     });
   }
   plan_items(a.queries, head_dim, is_fp32, resident * kWarps, kTokens);
   const int rc = by_type([&](auto type, auto dim) -> int {
     gdpa_rotated_queries_kernel<decltype(type), decltype(dim)::value><<<static_cast<unsigned>(query_ctas()), kWarps * 32, kQueryBytes, stream>>>(a);
-    return cudaGetLastError() == cudaSuccess ? 0 : GDPA_ERR_LAUNCH_;
+    return cudaGetLastError() == cudaSuccess ? 1 : -GDPA_ERR_LAUNCH_;
   });
-  if (rc != 0 || a.cache.num_blocks == 0) return rc;
+  if (rc < 0 || a.cache.num_blocks == 0) return rc;
   auto launch = [&](auto type, auto dim, auto warps, auto hold) -> int {
     using T = decltype(type);
     constexpr int D = decltype(dim)::value, W = decltype(warps)::value, HOLD = decltype(hold)::value;
     a.kv_parts = static_cast<int>(parts((24ll / W) * sm_count, W));
     const long long grid = windows * a.kv_parts;
-    if (grid > 0x7fffffffll) return GDPA_ERR_LAUNCH_;
+    if (grid > 0x7fffffffll) return -GDPA_ERR_LAUNCH_;
     auto kernel = gdpa_rotated_runs_kernel<T, D, W, HOLD>;
     const int smem = W * HOLD * kUnitPieces * 16 + (D << a.cache.block_shift) * static_cast<int>(sizeof(float));
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return GDPA_ERR_LAUNCH_;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -GDPA_ERR_LAUNCH_;
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(static_cast<unsigned>(grid));
     c.blockDim = dim3(W * 32);
@@ -540,7 +555,7 @@ int launch_rotated_append(RotatedAppendArgs& a, int head_dim, int is_fp32, int s
     at[0].val.programmaticStreamSerializationAllowed = 1;
     c.attrs = at;
     c.numAttrs = 1;
-    return cudaLaunchKernelEx(&c, kernel, static_cast<const RotatedAppendArgs&>(a)) == cudaSuccess ? 0 : GDPA_ERR_LAUNCH_;
+    return cudaLaunchKernelEx(&c, kernel, static_cast<const RotatedAppendArgs&>(a)) == cudaSuccess ? 2 : -GDPA_ERR_LAUNCH_;
   };
   // Warps so that a lane holds 64 values of a block at most: a head of 64 tokens and 128 values takes four, one of 128 tokens eight.
   return by_type([&](auto type, auto dim) -> int {

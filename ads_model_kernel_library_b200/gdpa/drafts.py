@@ -21,7 +21,7 @@ def verify_draft_tokens(
     sample_uniform: torch.Tensor,
     max_drafts: int,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Accept drafts and draw the next token so that what comes out is distributed as the target's own tokens, in one kernel.
+    """Accept drafts and draw the next token so that what comes out is distributed as the target's own tokens.
 
     Request ``b`` has the drafts ``draft_tokens[draft_offset[b]:draft_offset[b + 1]]``, ``n`` of them (at most ``max_drafts``), and the rows
     ``query_offset[b]:query_offset[b + 1]`` of ``target_probs`` ``[rows, vocabulary]`` (fp32 or bf16): row ``j`` is the target's distribution of

@@ -153,7 +153,7 @@ def verify(target, draft, tokens, offsets, draft_offsets, accept, sample, most):
         a = 0
         while a < n:
             x = tokens[d0 + a]
-            if not (0 <= x < len(target[0]) and accept[d0 + a] * (1.0 if draft is None else draft[d0 + a][x]) < target[offsets[b] + a][x]):
+            if not (0 <= x < len(target[0]) and accept[d0 + a] * (1.0 if draft is None else _share(draft[d0 + a][x])) < _share(target[offsets[b] + a][x])):
                 break
             line[a] = x
             a += 1

@@ -109,6 +109,20 @@ def test_verify_numbers_that_are_none():
         check_verify([1, 1, 1, 1, 0], 5000, edit=edit, lookup=lookup, ints=torch.int32)
 
 
+def test_verify_numbers_that_are_none_for_a_draft():
+    def edit(target, draft, tokens, accept, sample):
+        tokens[:] = 7
+        accept[:] = 0.25
+        target[::2, 7] = 0.5
+        draft[0, 7], draft[1, 7], draft[2, 7], draft[3, 7] = math.nan, math.inf, -1.0, 0.0  # count as 0: accepted
+        for i, bad in enumerate((math.inf, math.nan, -1.0, 0.0)):  # ... and refused
+            draft[4 + i, 7], target[2 * (4 + i), 7] = 0.5, bad
+
+    for lookup in (False, True):
+        check_verify([1] * 8, 100, edit=edit, lookup=lookup)
+        check_verify([1] * 8, 1001, torch.bfloat16, edit=edit, lookup=lookup)
+
+
 def test_verify_nothing():
     check_verify([], 10)
     check_verify([0, 0], 10)
@@ -312,7 +326,7 @@ def test_training_through_norm_rotation_and_attention():
     want += torch.autograd.grad(want[0], plain, do.double())
     for name, x, y in zip(("o", "dq", "dk", "dv", "dwq", "dwk"), got, want):
         # the attention's operands and P are bf16: 2^-8 each, a handful of them in a row
-        assert float((x.double().cpu() - y).norm() / y.norm()) < 8 * 2.0 ** -8, name
+        assert float((x.detach().double().cpu() - y).norm() / y.norm()) < 8 * 2.0 ** -8, name
 
 
 def test_a_step_replays_from_a_graph():

@@ -323,6 +323,17 @@ def test_append_ragged(size, dim, dtype):
     check_append([size // 2] * 2, [2 * size, 11], 6, 2, dim, dtype, size, seed=4, weight=BF)
 
 
+@pytest.mark.parametrize("size,dim,dtype", [(16, 64, BF), (64, 128, BF), (128, 128, BF), (128, 64, F32), (64, 128, F32)])
+@pytest.mark.parametrize("given", [False, True])
+def test_append_prompts_among_single_tokens(size, dim, dtype, given):
+    """Runs of every length in the same windows, where single tokens are most of the requests and where they are not."""
+    before = [size - 3, 0, 5, 2 * size, 11, size - 1, 40, 0, 7]
+    new = [1, 2, 9, 70, 3, 40, 200, 1, 17]
+    check_append(before * 3, [1] * 18 + new, 3, 2, dim, dtype, size, given=given)
+    check_append(before, new, 3, 2, dim, dtype, size, seed=1, given=given, loud=1e3 if size == 64 else 1.0)
+    check_append(before, list(reversed(new)), 1, 1, dim, dtype, size, seed=2, given=given)
+
+
 @pytest.mark.parametrize("options", [
     dict(given=True), dict(given=True, sections=(16, 24, 24)), dict(sections=(32, 32)), dict(norm=False), dict(norm=False, given=True, interleaved=True),
     dict(pairs=8), dict(pairs=0), dict(pairs=24, interleaved=True), dict(weight=None), dict(lens=torch.int64), dict(head_major=True), dict(loud=1e4, norm=False),

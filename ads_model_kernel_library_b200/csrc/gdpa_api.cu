@@ -889,7 +889,9 @@ int gdpa_verify_draft_tokens(const GdpaVerifyParams* p, gdpa_stream_t stream) {
   return rc;
 }
 
-size_t gdpa_drop_workspace_bytes(int32_t batch) { return batch > 0 ? static_cast<size_t>(drop_workspace_ints(batch)) * sizeof(int) : 0; }
+size_t gdpa_drop_workspace_bytes(int32_t batch, int32_t table_width) {
+  return batch > 0 && table_width >= 0 ? static_cast<size_t>(drop_workspace_ints(batch, table_width)) * sizeof(int) : 0;
+}
 
 int gdpa_drop_cached_tokens(const GdpaDropParams* p, gdpa_stream_t stream) {
   if (p == nullptr || p->struct_size != sizeof(GdpaDropParams)) return GDPA_ERR_BAD_ARG;
@@ -900,7 +902,7 @@ int gdpa_drop_cached_tokens(const GdpaDropParams* p, gdpa_stream_t stream) {
   if (p->batch > 0 && (p->seq_lens == nullptr || p->dropped == nullptr || p->seq_lens_after == nullptr)) return GDPA_ERR_BAD_ARG;
   if (p->batch > 0 && p->table_width > 0 && p->block_tables == nullptr) return GDPA_ERR_BAD_ARG;
   if (p->free_capacity > 0 && p->free_blocks == nullptr) return GDPA_ERR_BAD_ARG;
-  const size_t bytes = gdpa_drop_workspace_bytes(p->batch);
+  const size_t bytes = gdpa_drop_workspace_bytes(p->batch, p->table_width);
   if (bytes > 0 && p->workspace == nullptr) return GDPA_ERR_BAD_ARG;
   if (p->workspace_bytes < static_cast<int64_t>(bytes)) return GDPA_ERR_CAPACITY;
   if (!aligned16(p->workspace, nullptr)) return GDPA_ERR_MISALIGNED;

@@ -14,7 +14,8 @@
 //
 // Few requests: one launch, a cluster of CTAs to each, and latency is all of it.  Many: three kernels, whose beginnings overlap the ends of those before
 // them: who is accepted; the stretches' sums, dealt out over the whole GPU (a CTA to a request leaves SMs with one row to add up and SMs with four);
-// the token.  256 requests of 131071 bf16 tokens, 116 MB: 49 us in one kernel, 43 in three, 34 of them for the sums.
+// the token.  256 requests of 131071 bf16 tokens, 116 MB: 49 us in one kernel, 42 in three, 28 of them for the sums
+// (4.1 TB/s; half of their time waits for memory, half goes to instructions: rows staged through shared memory, with more on its way, took 33).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -34,7 +35,7 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kVerifyThreads = 256, kVerifyWarps = kVerifyThreads / 32;
-constexpr int kVerifyCtas = 4;          // resident on an SM
+constexpr int kVerifyCtas = 3, kSumCtas = 4;  // resident on an SM
 constexpr int kMostVocab = 1 << 20;
 constexpr int kMaxCluster = 8;
 
@@ -98,13 +99,11 @@ struct Sum<float, SHIFT, WITH_Q> {
     const uint32_t a[4] = {p.x, p.y, p.z, p.w}, b[8] = {q[0].x, q[0].y, q[0].z, q[0].w, q[1].x, q[1].y, q[1].z, q[1].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      largest = max(largest, a[j]);
-      if constexpr (WITH_Q) {
-        largest = max(largest, b[j + SHIFT]);
-        sums[j & 1] += value(max(a[j], b[j + SHIFT])) - value(b[j + SHIFT]);
-      } else {
-        sums[j & 1] += value(a[j]);
-      }
+      uint32_t m = a[j];
+      if constexpr (WITH_Q) m = max(m, b[j + SHIFT]);
+      largest = max(largest, m);
+      if constexpr (WITH_Q) sums[j & 1] += value(m) - value(b[j + SHIFT]);
+      else sums[j & 1] += value(m);
     }
   }
 };
@@ -117,16 +116,18 @@ struct Sum<__nv_bfloat16, SHIFT, WITH_Q> {  // two in a word
     const uint32_t a[4] = {p.x, p.y, p.z, p.w}, w[8] = {q[0].x, q[0].y, q[0].z, q[0].w, q[1].x, q[1].y, q[1].z, q[1].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      largest = max_u16x2(largest, a[j]);
+      uint32_t m = a[j], b = 0;
       if constexpr (WITH_Q) {
-        const uint32_t b = SHIFT % 2 == 0 ? w[j + SHIFT / 2] : __funnelshift_r(w[j + SHIFT / 2], w[j + SHIFT / 2 + 1], 16);
-        largest = max_u16x2(largest, b);
-        const uint32_t m = max_u16x2(a[j], b);
+        b = SHIFT % 2 == 0 ? w[j + SHIFT / 2] : __funnelshift_r(w[j + SHIFT / 2], w[j + SHIFT / 2 + 1], 16);
+        m = max_u16x2(m, b);
+      }
+      largest = max_u16x2(largest, m);
+      if constexpr (WITH_Q) {
         sums[0] += low(m) - low(b);
         sums[1] += high(m) - high(b);
       } else {
-        sums[0] += low(a[j]);
-        sums[1] += high(a[j]);
+        sums[0] += low(m);
+        sums[1] += high(m);
       }
     }
   }
@@ -453,7 +454,7 @@ __global__ void __launch_bounds__(kVerifyThreads) gdpa_verify_accept_kernel(cons
 
 // A warp takes stretch after stretch, the w-th of every n of all requests' together: rows with and without a second one to read mix on every SM.
 template <class T>
-__global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas) gdpa_verify_sum_kernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(kVerifyThreads, kSumCtas) gdpa_verify_sum_kernel(const __grid_constant__ VerifyArgs a) {
   const int lane = threadIdx.x & 31;
   const unsigned most = static_cast<unsigned>(a.most_stretches), all = static_cast<unsigned>(a.batch) * most, step = gridDim.x * kVerifyWarps;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -475,44 +476,92 @@ __global__ void __launch_bounds__(kVerifyThreads, kVerifyCtas) gdpa_verify_sum_k
   }
 }
 
+// Of n sums: their total, and the first one whose end lies above sample times that, or, if none does, the last with a share; and what lies before
+// it.  By a CTA.
+struct Found {
+  double total, before, mark;
+  int k;
+};
+__device__ __forceinline__ Found find_stretch(const double* sums, int n, double sample) {
+  __shared__ double s_of_warp[kVerifyWarps], s_before[2][kVerifyWarps];
+  __shared__ int s_k[2][kVerifyWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int each = (n + kVerifyThreads - 1) / kVerifyThreads, k0 = threadIdx.x * each, k1 = min(k0 + each, n);
+  double own = 0;
+  for (int k = k0; k < k1; ++k) own += sums[k];
+  double up_to = own;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const double o = __shfl_up_sync(kFull, up_to, s);
+    if (lane >= s) up_to += o;
+  }
+  if (lane == 31) s_of_warp[warp] = up_to;
+  __syncthreads();
+  Found f{0, 0, 0, 0};
+  double run = __shfl_up_sync(kFull, up_to, 1);
+  if (lane == 0) run = 0;
+#pragma unroll
+  for (int w = 0; w < kVerifyWarps; ++w) {
+    if (w == warp) run += f.total;
+    f.total += s_of_warp[w];
+  }
+  f.mark = sample * f.total;
+  int at[2] = {-1, -1};  // the lane's first one above the mark, its last one with a share
+  double before[2] = {0, 0};
+  for (int k = k0; k < k1; ++k) {
+    const double x = sums[k];
+    if (x > 0) {
+      at[1] = k, before[1] = run;
+      if (at[0] < 0 && run + x > f.mark) at[0] = k, before[0] = run;
+    }
+    run += x;
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const unsigned those = __ballot_sync(kFull, at[c] >= 0);
+    const int of = c == 0 ? __ffs(those) - 1 : 31 - __clz(those);
+    const int k = __shfl_sync(kFull, at[c], of & 31);
+    const double x = __shfl_sync(kFull, before[c], of & 31);
+    if (lane == 0) s_k[c][warp] = those != 0 ? k : -1, s_before[c][warp] = x;
+  }
+  __syncthreads();
+  f.k = -1;
+#pragma unroll
+  for (int w = 0; w < kVerifyWarps; ++w)
+    if (f.k < 0 && s_k[0][w] >= 0) f.k = s_k[0][w], f.before = s_before[0][w];
+  if (f.k < 0) {
+#pragma unroll
+    for (int w = 0; w < kVerifyWarps; ++w)
+      if (s_k[1][w] >= 0) f.k = s_k[1][w], f.before = s_before[1][w];
+  }
+  return f;
+}
+
 template <class T>
 __global__ void __launch_bounds__(kVerifyThreads) gdpa_verify_draw_kernel(const __grid_constant__ VerifyArgs a) {
   using C = Cut<T, kManyBlocks>;
   __shared__ double s_sum[kMostVocab / C::kStretch + 1];
   __shared__ double s_share[32 * (C::U + 1)];
-  __shared__ double s_total;
-  __shared__ int s_stretch;
   const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const float sample = a.sample[b];
+  const double sample = a.sample[b];
   asm volatile("griddepcontrol.wait;" ::: "memory");  // for the sums, and with them for the draws and what is accepted
   const Draw d = static_cast<const Draw*>(a.draws)[b];
   if (d.stretches == 0) return;
   const int accepted = a.accepted[b];
   Left<T> left = left_of<T>(d);
   for (int k = threadIdx.x; k < d.stretches; k += kVerifyThreads) s_sum[k] = a.sums[static_cast<long long>(b) * a.most_stretches + k];
-  double mark;
-  for (;;) {
-    __syncthreads();
-    if (warp == 0) {
-      const double total = add_up(s_sum, d.stretches);
-      const int k = find(s_sum, d.stretches, 0, static_cast<double>(sample) * total);
-      if (lane == 0) s_total = total, s_stretch = k;
-    }
-    __syncthreads();
-    mark = static_cast<double>(sample) * s_total;
-    if (s_total > 0) break;
-    if (left.q == nullptr && left.without < 0) {  // nothing to draw from
-      if (threadIdx.x == 0) put(a, b, accepted, -1);
-      return;
-    }
-    left.q = nullptr, left.without = -1;  // nothing is left of the difference
-    __syncthreads();
+  __syncthreads();
+  Found f = find_stretch(s_sum, d.stretches, sample);
+  if (f.k < 0 && (left.q != nullptr || left.without >= 0)) {  // nothing is left of the difference
+    left.q = nullptr, left.without = -1;
     for (int k = warp; k < d.stretches; k += kVerifyWarps) {
       const double sum = sum_stretch<T, kManyBlocks>(left, k, a.vocab);
       if (lane == 0) s_sum[k] = sum;
     }
+    __syncthreads();
+    f = find_stretch(s_sum, d.stretches, sample);
   }
-  const int k = s_stretch, token = find_token<T, kManyBlocks>(a, left, k, k > 0 ? s_sum[k - 1] : 0, mark, s_share);
+  const int token = f.k < 0 ? -1 : find_token<T, kManyBlocks>(a, left, f.k, f.before, f.mark, s_share);  // -1: nothing to draw from
   if (threadIdx.x == 0) put(a, b, accepted, token);
 }
 
@@ -523,10 +572,10 @@ __global__ void __launch_bounds__(kVerifyThreads) gdpa_verify_draw_kernel(const 
 // request's length is not looked at.
 //
 // Latency is all of it.  A warp has four requests, up to 128 entries of each, all asked for at once and kept in registers until it is known how many go
-// before them.  Up to 256 requests, a cluster of CTAs adds that up in shared memory.  More of them: one kernel counts, another, whose loads the end
-// of the first overlaps, adds up the counts of the CTAs before its own (4096 requests with 64 entries each: 11 us; up to
-// 256 requests a cluster is 2 us faster).
-constexpr int kDropWarps = 8, kDropRequests = 4;
+// before them; where tables are wide, four chunks of requests: one request of 2^20 tokens in blocks of 16, all of which leave, 377 us by a warp, 19
+// by many.  Up to 256 of those, a cluster of CTAs adds that up in shared memory.  More of them: one kernel counts, another, whose loads the end of the first
+// overlaps, adds up the counts of the CTAs before its own (4096 requests with 64 entries each: 11 us; up to 256 a cluster is 2 us faster).
+constexpr int kDropWarps = 8, kDropChunks = 4;
 
 enum DropWay { kDropCluster, kDropCount, kDropStore };
 
@@ -537,21 +586,24 @@ __global__ void __launch_bounds__(kDropWarps * 32) gdpa_drop_kernel(const __grid
   __shared__ long long s_before[kDropWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int S = 1 << a.block_shift;
-  const int b0 = (blockIdx.x * kDropWarps + warp) * kDropRequests;
-  // the warp's requests, and those of their entries that may go
-  int keep = 0, held = 0;
-  if (lane < kDropRequests && b0 + lane < a.batch) {
-    const long long len = clamp_ll(load_offset(a.seq_lens, b0 + lane, a.lens64), 0, 0x7fffff00);
-    const long long after = len - clamp_ll(load_offset(a.dropped, b0 + lane, a.dropped64), 0, len);
-    if (WAY != kDropCount) a.seq_lens_after[b0 + lane] = static_cast<int>(after);
-    keep = static_cast<int>(min((after + S - 1) >> a.block_shift, static_cast<long long>(a.table_width)));
-    held = static_cast<int>(min((len + S - 1) >> a.block_shift, static_cast<long long>(a.table_width)));
+  // the warp's chunks, and those of their entries that may go
+  const unsigned v = (blockIdx.x * kDropWarps + warp) * kDropChunks + lane, b = v / static_cast<unsigned>(a.chunks);
+  const int c = static_cast<int>(v - b * a.chunks);
+  int from_here = 0, to_here = 0;
+  if (lane < kDropChunks && b < static_cast<unsigned>(a.batch)) {
+    const long long len = clamp_ll(load_offset(a.seq_lens, b, a.lens64), 0, 0x7fffff00);
+    const long long after = len - clamp_ll(load_offset(a.dropped, b, a.dropped64), 0, len);
+    if (WAY != kDropCount && c == 0) a.seq_lens_after[b] = static_cast<int>(after);
+    const int keep = static_cast<int>(min((after + S - 1) >> a.block_shift, static_cast<long long>(a.table_width)));
+    const int held = static_cast<int>(min((len + S - 1) >> a.block_shift, static_cast<long long>(a.table_width)));
+    from_here = min(keep + c * a.chunk_entries, held);
+    to_here = c + 1 == a.chunks ? held : min(from_here + a.chunk_entries, held);
   }
-  int entry[kDropRequests][4];
+  int entry[kDropChunks][4];
 #pragma unroll
-  for (int i = 0; i < kDropRequests; ++i) {
-    const int from = __shfl_sync(kFull, keep, i), to = __shfl_sync(kFull, held, i);
-    const int* const row = a.block_tables + static_cast<long long>(b0 + i) * a.table_stride;
+  for (int i = 0; i < kDropChunks; ++i) {
+    const int from = __shfl_sync(kFull, from_here, i), to = __shfl_sync(kFull, to_here, i);
+    const int* const row = a.block_tables + static_cast<long long>(__shfl_sync(kFull, b, i)) * a.table_stride;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int j = from + 32 * u + lane;
@@ -561,15 +613,18 @@ __global__ void __launch_bounds__(kDropWarps * 32) gdpa_drop_kernel(const __grid
   // all of them in order: body(the lane's entry or -1, votes of the lanes that have one)
   auto walk = [&](auto body) {
 #pragma unroll
-    for (int i = 0; i < kDropRequests; ++i) {
-      const int from = __shfl_sync(kFull, keep, i), to = __shfl_sync(kFull, held, i);
+    for (int i = 0; i < kDropChunks; ++i) {
+      const int from = __shfl_sync(kFull, from_here, i), to = __shfl_sync(kFull, to_here, i);
 #pragma unroll
       for (int u = 0; u < 4; ++u) body(entry[i][u], __ballot_sync(kFull, entry[i][u] >= 0));
-      // a request with more
-      const int* const row = a.block_tables + static_cast<long long>(b0 + i) * a.table_stride;
-      for (int j = from + 128 + lane; j - lane < to; j += 32) {
-        const int e = j < to ? row[j] : -1;
-        body(e, __ballot_sync(kFull, e >= 0));
+      // a chunk with more
+      const int* const row = a.block_tables + static_cast<long long>(__shfl_sync(kFull, b, i)) * a.table_stride;
+      for (int j0 = from + 128; j0 < to; j0 += 512) {
+        int e[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) e[u] = j0 + 32 * u + lane < to ? row[j0 + 32 * u + lane] : -1;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) body(e[u], __ballot_sync(kFull, e[u] >= 0));
       }
     }
   };
@@ -684,7 +739,7 @@ int launch_verify(VerifyArgs& a, int is_bf16, int sm_count, cudaStream_t stream)
       using T = decltype(type);
       gdpa_verify_accept_kernel<T><<<(a.batch + kVerifyWarps - 1) / kVerifyWarps, kVerifyThreads, 0, stream>>>(a);
       if (cudaGetLastError() != cudaSuccess) return GDPA_ERR_LAUNCH_;
-      int rc = launch_cluster(gdpa_verify_sum_kernel<T>, a, static_cast<unsigned>(kVerifyCtas * sm_count), kVerifyThreads, 0, stream);
+      int rc = launch_cluster(gdpa_verify_sum_kernel<T>, a, static_cast<unsigned>(kSumCtas * sm_count), kVerifyThreads, 0, stream);
       if (rc == 0) rc = launch_cluster(gdpa_verify_draw_kernel<T>, a, static_cast<unsigned>(a.batch), kVerifyThreads, 0, stream);
       return rc;
     };
@@ -708,16 +763,23 @@ int launch_verify(VerifyArgs& a, int is_bf16, int sm_count, cudaStream_t stream)
 }
 
 namespace {
-unsigned drop_ctas(long long batch) { return static_cast<unsigned>((batch + kDropWarps * kDropRequests - 1) / (kDropWarps * kDropRequests)); }
+// Chunks of a request: as many as give each 512 entries at least, and no more than 2^17 of them all together (a CTA reads the counts of all).
+int drop_chunks(long long batch, int table_width) {
+  const long long most = batch > 0 ? (1ll << 17) / batch : 1, wanted = table_width > 640 ? (table_width + 511) / 512 : 1;
+  return static_cast<int>(most < 1 ? 1 : wanted < most ? wanted : most);
+}
+unsigned drop_ctas(long long chunks) { return static_cast<unsigned>((chunks + kDropWarps * kDropChunks - 1) / (kDropWarps * kDropChunks)); }
 }  // namespace
 
-long long drop_workspace_ints(long long batch) {
-  const unsigned ctas = drop_ctas(batch);
+long long drop_workspace_ints(long long batch, int table_width) {
+  const unsigned ctas = drop_ctas(batch * drop_chunks(batch, table_width));
   return ctas <= kMaxCluster ? 0 : static_cast<long long>(ctas) * (kDropWarps + 1);
 }
 
-int launch_drop(const DropArgs& a, cudaStream_t stream) {
-  const unsigned ctas = a.batch > 0 ? drop_ctas(a.batch) : 1;
+int launch_drop(DropArgs& a, cudaStream_t stream) {
+  a.chunks = drop_chunks(a.batch, a.table_width);
+  a.chunk_entries = (a.table_width + a.chunks - 1) / a.chunks;
+  const unsigned ctas = a.batch > 0 ? drop_ctas(static_cast<long long>(a.batch) * a.chunks) : 1;
   if (ctas <= kMaxCluster) return launch_cluster(gdpa_drop_kernel<kDropCluster>, a, ctas, kDropWarps * 32, ctas, stream);
   gdpa_drop_kernel<kDropCount><<<ctas, kDropWarps * 32, 0, stream>>>(a);
   if (cudaGetLastError() != cudaSuccess) return GDPA_ERR_LAUNCH_;

@@ -372,6 +372,8 @@ struct DropArgs {
   const int* num_free;
   int* seq_lens_after;
   int* num_free_after;
+  int chunks;   // that a request's entries are taken in, chunk_entries each: drop_chunks, set by launch_drop
+  int chunk_entries;
   int* counts;  // drop_workspace_ints
 };
 
@@ -405,8 +407,8 @@ int launch_cache_read(CacheReadArgs& a, int head_dim, int out_is_fp32, int sm_co
 VerifyWorkspace verify_workspace(long long batch, long long vocab, int is_bf16);
 int launch_verify(VerifyArgs& a, int is_bf16, int sm_count, cudaStream_t stream);
 int verify_most_vocab();
-long long drop_workspace_ints(long long batch);
-int launch_drop(const DropArgs& a, cudaStream_t stream);
+long long drop_workspace_ints(long long batch, int table_width);
+int launch_drop(DropArgs& a, cudaStream_t stream);
 int launch_paged(const PagedLaunch& l, int head_dim);
 int launch_paged_rows(const PagedLaunch& l, int head_dim);  // of launch_paged, for row tiles of 256
 int paged_ctas_per_sm(int rows, int head_dim);  // resident CTAs of the kernel for row tiles of `rows`: a launch has that many

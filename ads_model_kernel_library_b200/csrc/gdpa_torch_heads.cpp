@@ -19,7 +19,7 @@ struct EntryPoints {
   int (*read)(const GdpaCacheReadParams*, gdpa_stream_t);
   size_t (*verify_workspace)(int32_t, int32_t, int32_t);
   int (*verify)(const GdpaVerifyParams*, gdpa_stream_t);
-  size_t (*drop_workspace)(int32_t);
+  size_t (*drop_workspace)(int32_t, int32_t);
   int (*drop)(const GdpaDropParams*, gdpa_stream_t);
 } g_call{};
 
@@ -443,7 +443,7 @@ std::tuple<at::Tensor, at::Tensor> drop_tokens(const at::Tensor& block_tables, c
   p.num_free = num_free.const_data_ptr<int32_t>();
   p.seq_lens_after = lens.mutable_data_ptr<int32_t>();
   p.num_free_after = left.mutable_data_ptr<int32_t>();
-  const size_t bytes = g_call.drop_workspace(p.batch);
+  const size_t bytes = g_call.drop_workspace(p.batch, p.table_width);
   at::Tensor workspace;
   if (bytes > 0) {
     workspace = empty({static_cast<int64_t>(bytes)}, at::kByte, seq_lens);

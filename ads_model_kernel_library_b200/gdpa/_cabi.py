@@ -513,7 +513,7 @@ def _load() -> C.CDLL:
     lib.gdpa_verify_workspace_bytes.restype = C.c_size_t
     lib.gdpa_verify_workspace_bytes.argtypes = [C.c_int32, C.c_int32, C.c_int32]
     lib.gdpa_drop_workspace_bytes.restype = C.c_size_t
-    lib.gdpa_drop_workspace_bytes.argtypes = [C.c_int32]
+    lib.gdpa_drop_workspace_bytes.argtypes = [C.c_int32, C.c_int32]
     lib.gdpa_rotary_workspace_bytes.restype = C.c_size_t
     lib.gdpa_rotary_workspace_bytes.argtypes = [C.c_int32]
     lib.gdpa_strerror.restype = C.c_char_p

@@ -643,8 +643,8 @@ typedef struct GdpaDropParams {
   int64_t workspace_bytes;
 } GdpaDropParams;
 
-/* Bytes of the workspace of a call; 0 for small batches, which need none. */
-size_t gdpa_drop_workspace_bytes(int32_t batch);
+/* Bytes of the workspace of a call; 0 for small ones, which need none. */
+size_t gdpa_drop_workspace_bytes(int32_t batch, int32_t table_width);
 
 int gdpa_drop_cached_tokens(const GdpaDropParams* params, gdpa_stream_t stream);
 

@@ -204,6 +204,12 @@ def test_drop_nothing_and_full_stacks():
     check_drop([-5, 60], [3, 7], 16, 4)
 
 
+def test_drop_long_requests():
+    """More entries of a request than a warp has in registers."""
+    check_drop([16 * 1500 - 3, 5, 16 * 640, 16 * 129], [16 * 1500 - 3, 1, 16 * 513, 16 * 128 + 4], 16, 1500)
+    check_drop([16 * 700] * 300, [16 * 700 - 5] * 300, 16, 700, holes=0.3)
+
+
 @pytest.mark.parametrize("batch", [31, 256, 257, 2049, 9000])
 def test_drop_many(batch):
     g = torch.Generator().manual_seed(batch)

@@ -315,22 +315,42 @@ __device__ __forceinline__ void deal(const Window& window, unsigned leaders, lon
   }
 }
 
-// The lane's position of an item's of the queries.
+// The lane's position of an item's of the queries.  Items come in the order of their tokens, so the next request is this one or, mostly, one of the next 32: what
+// is needed of those comes in one trip to memory.
 struct QueryPositions {
   const RotatedAppendArgs& a;
-  long long origin = 0, begin = 0, end = -1;  // of the request at hand: its first token and the one behind its last
+  int owner = -1;                       // request at hand
+  long long origin = 0, begin = 0, end = -1;  // position of token 0 by it, its first token and the one behind its last
+  __device__ __forceinline__ void find(long long t) {
+    if (a.batch == 0) {
+      end = 0x7fffffffffffffffll;
+      return;
+    }
+    const int lane = threadIdx.x & 31;
+    if (owner < 0) owner = owner_of(a, t);
+    for (;;) {
+      const int next = min(owner + 1 + lane, a.batch);
+      const long long ends = load_offset(a.q_off, next, a.off64), len = load_offset(a.seq_lens, min(owner + lane, a.batch - 1), a.lens64);
+      const unsigned behind = __ballot_sync(kAllLanes, owner + 1 + lane < a.batch && ends <= t);
+      const int count = behind == kAllLanes ? 32 : __ffs(~behind) - 1;
+      if (count == 32) {
+        owner = owner_of(a, t);
+        continue;
+      }
+      end = __shfl_sync(kAllLanes, ends, count);
+      origin = __shfl_sync(kAllLanes, len, count) - end;
+      owner += count;
+      begin = count > 0 ? __shfl_sync(kAllLanes, ends, count - 1) : load_offset(a.q_off, owner, a.off64);
+      return;
+    }
+  }
   __device__ __forceinline__ long long operator()(const Item& it) {
     const int lane = threadIdx.x & 31, axis = lane / kMostItemTokens, j = lane % kMostItemTokens;
     if (a.queries.t[0].positions != nullptr) return axis < a.queries.rotary.axes && j < it.tokens ? given_position(a, axis, it.token + j) : 0;
     long long p = 0;
     for (int i = 0; i < it.tokens; ++i) {
       const long long t = it.token + i;
-      if (!(t >= begin && t < end)) {
-        const int owner = owner_of(a, t);
-        origin = origin_of(a, owner);
-        begin = a.batch == 0 ? 0 : load_offset(a.q_off, owner, a.off64);
-        end = a.batch == 0 ? 0x7fffffffffffffffll : load_offset(a.q_off, owner + 1, a.off64);
-      }
+      if (!(t >= begin && t < end)) find(t);
       if (j == i) p = origin + t;  // on every axis
     }
     return p;
@@ -385,10 +405,14 @@ __global__ void __launch_bounds__(kWarps * 32, 4) gdpa_rotated_queries_kernel(co
                                  reinterpret_cast<float*>(s_weight), 1, Cursor(blockIdx.x * kWarps + warp, gridDim.x * kWarps), positions);
 }
 
+// Warps of an SM: a lane that holds 64 values needs 168 registers, one that holds 32 or 16 has enough in 128 (prompts of 512 to 4096 tokens in blocks of 16: 283
+// us with 12 warps, 262 with 16; blocks of 64 with 32 values a lane and 16 warps: 240, with 64 and 12: 225).
+__host__ __device__ constexpr int runs_ctas(int W, int values) { return (values >= 64 ? 12 : 16) / W; }
+
 // W warps on one run of one head after the other, keys, then values; the next head is on its way while one is worked on.  HOLD rows of a lane, so that a
 // whole block is held.
 template <class T, int D, int W, int HOLD>
-__global__ void __launch_bounds__(W * 32, 12 / W) gdpa_rotated_runs_kernel(const __grid_constant__ RotatedAppendArgs a) {
+__global__ void __launch_bounds__(W * 32, runs_ctas(W, HOLD * 2 * HeadLanes<T, D>::E)) gdpa_rotated_runs_kernel(const __grid_constant__ RotatedAppendArgs a) {
   using Lanes = HeadLanes<T, D>;
   constexpr int C = Lanes::C, step = W * Lanes::H;
   extern __shared__ uint4 s_dynamic[];  // [warp][HOLD] units; angles of a block's rows, [row][D]
@@ -539,7 +563,7 @@ int launch_rotated_append(RotatedAppendArgs& a, int head_dim, int is_fp32, int s
   auto launch = [&](auto type, auto dim, auto warps, auto hold) -> int {
     using T = decltype(type);
     constexpr int D = decltype(dim)::value, W = decltype(warps)::value, HOLD = decltype(hold)::value;
-    a.kv_parts = static_cast<int>(parts((24ll / W) * sm_count, W));
+    a.kv_parts = static_cast<int>(parts(2ll * runs_ctas(W, HOLD * 2 * HeadLanes<T, D>::E) * sm_count, W));
     const long long grid = windows * a.kv_parts;
     if (grid > 0x7fffffffll) return -GDPA_ERR_LAUNCH_;
     auto kernel = gdpa_rotated_runs_kernel<T, D, W, HOLD>;

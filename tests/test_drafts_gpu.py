@@ -332,7 +332,7 @@ def test_training_through_norm_rotation_and_attention():
     want += torch.autograd.grad(want[0], plain, do.double())
     for name, x, y in zip(("o", "dq", "dk", "dv", "dwq", "dwk"), got, want):
         # the attention's operands and P are bf16: 2^-8 each, a handful of them in a row
-        assert float((x.detach().double().cpu() - y).norm() / y.norm()) < 8 * 2.0 ** -8, name
+        assert float(((x.double().cpu() - y).norm() / y.norm()).detach()) < 8 * 2.0 ** -8, name
 
 
 def test_a_step_replays_from_a_graph():

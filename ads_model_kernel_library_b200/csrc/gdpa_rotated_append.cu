@@ -304,7 +304,7 @@ __device__ __forceinline__ void deal(const Window& window, unsigned leaders, lon
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int pair = Lanes::slot(lanes.l, 2 * e + j);
-            sin_cos<T>(pairs.frequency[pair], given ? given_position(a, pairs.axis[pair], t0 + r) : run_origin + t0 + r, sn[j], cs[j]);
+            sin_cos(pairs.frequency[pair], given ? given_position(a, pairs.axis[pair], t0 + r) : run_origin + t0 + r, sn[j], cs[j]);
           }
           c[e] = pack_f32x2(cs[0], cs[1]), s[e] = pack_f32x2(sn[0], sn[1]);
         }

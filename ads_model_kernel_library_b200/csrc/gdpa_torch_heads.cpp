@@ -170,6 +170,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rotary_backwa
 }
 
 bool wants(const OptionalTensor& t) { return t.has_value() && t->defined() && t->requires_grad(); }
+bool has_tangent(const OptionalTensor& t) { return t.has_value() && t->defined() && t->_fw_grad(/*level=*/0).defined(); }
 
 class QkNormRotary : public torch::autograd::Function<QkNormRotary> {
  public:
@@ -216,6 +217,9 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rotary_autograd(const at::Tensor& que
                                                            const at::Tensor& query_positions, const at::Tensor& key_positions,
                                                            const OptionalTensor& query_weight, const OptionalTensor& key_weight, double eps, bool norm,
                                                            bool interleaved, at::IntArrayRef sections) {
+  // Below autograd a tangent would be lost without a word.
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(query) && !has_tangent(key) && !has_tangent(query_weight) && !has_tangent(key_weight) && !has_tangent(inv_freq),
+                              "gdpa::qk_norm_rotary has no forward-mode derivative: its inputs cannot have tangents");
   if (at::GradMode::is_enabled()) {
     TORCH_CHECK(!inv_freq.requires_grad(), "inv_freq cannot be differentiated: detach it");
     if (wants(query) || wants(key) || wants(query_weight) || wants(key_weight)) {

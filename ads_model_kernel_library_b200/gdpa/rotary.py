@@ -39,7 +39,8 @@ def qk_norm_rotary(
     ``key_positions`` are ``query_positions`` if left out (both tensors then have the same tokens).
 
     bf16 or fp32, head_dim 64 or 128, tokens and heads strided as in the attention (slices of a packed projection).  Gradients flow to query, key
-    and the weights (``norm=False``: the weights take no part); their sums have an order that does not vary.  Not to ``inv_freq``.
+    and the weights (``norm=False``: the weights take no part); their sums have an order that does not vary.  Not to ``inv_freq``.  Inputs with a
+    tangent (forward-mode derivatives) are refused.
     """
     return (paged._operators or paged._load()).rotary(
         query, key, inv_freq, query_positions, query_positions if key_positions is None else key_positions, query_weight, key_weight, eps, norm, interleaved,

@@ -1,0 +1,37 @@
+"""Calls of the operators on either side of the attention that are easily got wrong and need no GPU."""
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import ads_model_kernel_library_b200.gdpa as G
+
+
+def empty(*shape, dtype=torch.bfloat16):
+    return torch.empty(shape, dtype=dtype, device="cuda")
+
+
+def rotary_arguments():
+    """query, key, query_weight, key_weight, inv_freq, positions"""
+    return [empty(7, 4, 128), empty(7, 2, 128), empty(128, dtype=torch.float32), empty(128, dtype=torch.float32), empty(64, dtype=torch.float64),
+            empty(7, dtype=torch.int32)]
+
+
+@pytest.mark.parametrize("which", range(5))
+@pytest.mark.parametrize("grad", ["wanted", "not wanted", "off"])
+def test_tangents_are_refused(which, grad):
+    """No forward-mode derivative: a call with a tangent raises, as the other operators' do; it does not return results without one."""
+    with FakeTensorMode(), forward_ad.dual_level(), torch.set_grad_enabled(grad != "off"):
+        args = rotary_arguments()
+        if grad == "wanted":
+            args[:4] = [t.requires_grad_() for t in args[:4]]
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError):
+            G.qk_norm_rotary(args[0], args[1], args[4], args[5], query_weight=args[2], key_weight=args[3])
+
+
+def test_tangents_of_a_functional_call_are_refused():
+    with FakeTensorMode():
+        q, k, _, _, f, p = rotary_arguments()
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(lambda x: G.qk_norm_rotary(x, k, f, p)[0], (q,), (q,))

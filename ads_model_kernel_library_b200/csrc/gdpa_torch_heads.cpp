@@ -130,25 +130,33 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rotary(const at::Tensor& query, const
   return {q, k};
 }
 
-// Without the norm x is not needed: the gradients of the results stand in for it.
+// A gradient of a result as the kernel can read it: expanded ones and those of other strides or addresses are copied.
+at::Tensor readable_grad(const char* name, const at::Tensor& g, const at::Tensor& x) {
+  check_device(name, g, x);
+  check_type(name, g, x.scalar_type());
+  TORCH_CHECK_VALUE(g.dim() == 3 && g.sizes() == x.sizes(), name, " must have the shape of the result, got ", g.sizes());
+  bool own = !misaligned(g, 2);
+  for (int i = 0; i < 2; ++i) own &= g.numel() == 0 || g.size(i) <= 1 || g.stride(i) >= g.size(2);
+  return own ? g : g.contiguous();
+}
+
+// Without the norm x is not read: the gradients of the results, once they are readable, stand in for it.
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rotary_backward(
     const at::Tensor& query_grad, const at::Tensor& key_grad, const at::Tensor& query, const at::Tensor& key, const at::Tensor& inv_freq,
     const at::Tensor& query_positions, const at::Tensor& key_positions, const OptionalTensor& query_weight, const OptionalTensor& key_weight, double eps, bool norm,
     bool interleaved, at::IntArrayRef sections, bool weight_grads) {
-  GdpaRotaryParams p = rotary_params(query, key, inv_freq, query_positions, key_positions, query_weight, key_weight, eps, norm, interleaved, sections);
+  check_cuda("query", query);
+  check_device("key", key, query);
   const c10::cuda::CUDAGuard guard(query.device());
-  auto grad_of = [&](const char* name, const at::Tensor& g, const at::Tensor& x, GdpaRotaryTensor& t) {
-    check_device(name, g, query);
-    check_type(name, g, query.scalar_type());
-    TORCH_CHECK_VALUE(g.sizes() == x.sizes(), name, " must have the shape of the result, got ", g.sizes());
-    bool own = !misaligned(g, 2);
-    for (int i = 0; i < 2; ++i) own &= g.numel() == 0 || g.size(i) <= 1 || g.stride(i) >= g.size(2);
-    const at::Tensor c = own ? g : g.contiguous();
-    t.dy = c.const_data_ptr();
-    strides(t.dy_strides, c);
-    return c;
+  const at::Tensor gq = readable_grad("query_grad", query_grad, query), gk = readable_grad("key_grad", key_grad, key);
+  GdpaRotaryParams p = rotary_params(norm ? query : gq, norm ? key : gk, inv_freq, query_positions, key_positions, query_weight, key_weight, eps, norm,
+                                     interleaved, sections);
+  auto take = [](const at::Tensor& g, GdpaRotaryTensor& t) {
+    t.dy = g.const_data_ptr();
+    strides(t.dy_strides, g);
   };
-  const at::Tensor gq = grad_of("query_grad", query_grad, query, p.query), gk = grad_of("key_grad", key_grad, key, p.key);
+  take(gq, p.query);
+  take(gk, p.key);
   at::Tensor dq = empty(query.sizes(), query.scalar_type(), query), dk = empty(key.sizes(), key.scalar_type(), key), workspace;
   p.query.y = dq.mutable_data_ptr();
   p.key.y = dk.mutable_data_ptr();

@@ -206,12 +206,14 @@ int launch_rotary_bwd(RotaryArgs& a, int head_dim, int is_fp32, int sm_count, cu
   plan_items(a, head_dim, is_fp32, static_cast<long long>(kBwdCtas) * kWarps * sm_count, kBwdTokens);
   const unsigned grid = ctas(a, rotary_bwd_ctas(sm_count));
   if (grid > 0) {
-    // the ring, and a lane's sums of both tensors
-    const int smem = kWarps * kBwdRing * 2 * kUnitPieces * 16 + (a.partial != nullptr ? kWarps * 2 * (is_fp32 ? 8 : 16) * 32 * static_cast<int>(sizeof(float)) : 0);
+    // The ring and, for the weights' gradients, a lane's sums of both tensors.  What a kernel may have at most is its own state, which other host threads'
+    // calls set too: always the most that it ever takes.
     const int rc = by_type(head_dim, is_fp32, [&](auto type, auto dim) {
-      auto kernel = gdpa_rotary_bwd_kernel<decltype(type), decltype(dim)::value>;
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return;  // the launch then fails, and says so
-      kernel<<<grid, kWarps * 32, smem, stream>>>(a);
+      using T = decltype(type);
+      constexpr int D = decltype(dim)::value, kRing = kWarps * kBwdRing * 2 * kUnitPieces * 16, kSums = kWarps * 2 * 2 * HeadLanes<T, D>::C * 32 * sizeof(uint64_t);
+      auto kernel = gdpa_rotary_bwd_kernel<T, D>;
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing + kSums) != cudaSuccess) return;  // the launch then fails, and says so
+      kernel<<<grid, kWarps * 32, kRing + (a.partial != nullptr ? kSums : 0), stream>>>(a);
     });
     if (rc != 0) return -rc;
   }

@@ -567,12 +567,13 @@ int launch_rotated_append(RotatedAppendArgs& a, int head_dim, int is_fp32, int s
     const long long grid = windows * a.kv_parts;
     if (grid > 0x7fffffffll) return -GDPA_ERR_LAUNCH_;
     auto kernel = gdpa_rotated_runs_kernel<T, D, W, HOLD>;
-    const int smem = W * HOLD * kUnitPieces * 16 + (D << a.cache.block_shift) * static_cast<int>(sizeof(float));
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -GDPA_ERR_LAUNCH_;
+    // A block of fewer rows than the lanes hold takes less; what the kernel may have at most, which other host threads' calls set too, stays the same.
+    constexpr int kRing = W * HOLD * kUnitPieces * 16, kTables = W * HOLD * HeadLanes<T, D>::H * D * static_cast<int>(sizeof(float));
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing + kTables) != cudaSuccess) return -GDPA_ERR_LAUNCH_;
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(static_cast<unsigned>(grid));
     c.blockDim = dim3(W * 32);
-    c.dynamicSmemBytes = smem;
+    c.dynamicSmemBytes = kRing + (D << a.cache.block_shift) * static_cast<int>(sizeof(float));
     c.stream = stream;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -1,9 +1,14 @@
 """Calls of the operators on either side of the attention that are easily got wrong, on the GPU."""
+import ctypes as C
+import threading
+
 import pytest
 import torch
 
 import ads_model_kernel_library_b200.gdpa as G
+from ads_model_kernel_library_b200.gdpa import _cabi
 from tests import _heads_oracle as ref
+from tests.test_heads_cpu import nested
 from tests.test_heads_gpu import BF, DEV, F32, frequencies, weights
 
 pytestmark = pytest.mark.gpu
@@ -64,3 +69,71 @@ def test_gradient_refusals(norm):
                         ((x[..., :32], x), ValueError), ((x[0], x), ValueError), ((x, x, x.half(), x), TypeError), ((x, x, x[0], x), ValueError)):
         with pytest.raises(error):
             call(*args)
+
+
+# ------------------------------------------------------------------------------------------ two threads
+
+
+def calls_of_two_threads(fn, params, repeats=20000):
+    """The return codes other than 0 of two host threads that call the same entry point, each with parameters and a stream of its own."""
+    codes, begin = [[], []], threading.Barrier(2)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+
+    def work(i):
+        torch.cuda.set_device(0)
+        ref_to, stream = C.byref(params[i]), C.c_void_p(streams[i].cuda_stream)
+        begin.wait()
+        for n in range(repeats):  # the call gives up Python's lock
+            code = fn(ref_to, stream)
+            if code != 0:
+                codes[i].append(code)
+            if n % 200 == 0:
+                streams[i].synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    return codes
+
+
+@pytest.mark.parametrize("dim,is_fp32", [(64, 0), (128, 0), (64, 1), (128, 1)])
+def test_two_threads_gradients_with_and_without_the_weights(dim, is_fp32):
+    dtype = F32 if is_fp32 else BF
+    f, p = frequencies(dim // 2).to(DEV), torch.arange(4, device=DEV)
+    hold, params = [], []
+    for with_weights in (True, False):
+        x = {n: [torch.randn(4, 1, dim, device=DEV).to(dtype) for _ in range(3)] for n in ("query", "key")}
+        w = torch.ones(dim, device=DEV)
+        dw, workspace = torch.zeros(2, dim, device=DEV), torch.empty(_cabi.lib.gdpa_rotary_workspace_bytes(dim), dtype=torch.uint8, device=DEV)
+        values = {"head_dim": dim, "is_fp32": is_fp32, "rotary.inv_freq": f.data_ptr(), "rotary.inv_freq_is_fp64": 1, "rotary.pairs": dim // 2, "rotary.axes": 1,
+                  "rotary.norm": 1, "rotary.eps": 1e-6, "workspace": workspace.data_ptr(), "workspace_bytes": workspace.numel()}
+        for i, (name, (a, y, dy)) in enumerate(x.items()):
+            values.update({f"{name}.x": a.data_ptr(), f"{name}.y": y.data_ptr(), f"{name}.dy": dy.data_ptr(), f"{name}.weight": w.data_ptr(), f"{name}.heads": 1,
+                           f"{name}.tokens": 4, f"{name}.positions": p.data_ptr(), f"{name}.positions_are_int64": 1})
+            if with_weights:
+                values[f"{name}.dweight"] = dw[i].data_ptr()
+        hold.append((x, w, dw, workspace))
+        params.append(nested(_cabi.GdpaRotaryParams, values))
+    assert calls_of_two_threads(_cabi.lib.gdpa_qk_norm_rotary_bwd, params) == [[], []]
+
+
+@pytest.mark.parametrize("is_fp32", [0, 1])
+def test_two_threads_appends_to_blocks_of_two_sizes(is_fp32):
+    dtype, dim, tokens = F32 if is_fp32 else BF, 64, 32
+    f, p, slots = frequencies(dim // 2).to(DEV), torch.arange(tokens, device=DEV), torch.arange(tokens, device=DEV)
+    hold, params = [], []
+    for size in (16, 32):
+        q, k, v, out = (torch.randn(tokens, 1, dim, device=DEV).to(dtype) for _ in range(4))
+        caches, scales = torch.zeros(2, 64, 1, dim, dtype=torch.uint8, device=DEV), torch.ones(2, 64, device=DEV)
+        hold.append((q, k, v, out, caches, scales))
+        params.append(nested(_cabi.GdpaRotatedAppendParams, {
+            "heads": 1, "cache.struct_size": C.sizeof(_cabi.GdpaCacheAppendParams), "cache.x_is_fp32": is_fp32, "cache.key": k.data_ptr(), "cache.value": v.data_ptr(),
+            "cache.k_cache": caches[0].data_ptr(), "cache.v_cache": caches[1].data_ptr(), "cache.k_scales": scales[0].data_ptr(), "cache.v_scales": scales[1].data_ptr(),
+            "cache.slot_mapping": slots.data_ptr(), "cache.tokens": tokens, "cache.num_blocks": 64 // size, "cache.block_size": size, "cache.kv_heads": 1,
+            "cache.head_dim": dim, "rotary.inv_freq": f.data_ptr(), "rotary.inv_freq_is_fp64": 1, "rotary.pairs": dim // 2, "rotary.axes": 1, "rotary.norm": 1,
+            "rotary.eps": 1e-6, "query": q.data_ptr(), "query_out": out.data_ptr(), "positions": p.data_ptr(), "positions_are_int64": 1}))
+    assert calls_of_two_threads(_cabi.lib.gdpa_append_rotated_kv_cache_fp8, params) == [[], []]

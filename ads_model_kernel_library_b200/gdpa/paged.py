@@ -347,11 +347,20 @@ class PagedKVCache:
         self.free_blocks = torch.arange(num_blocks - 1, -1, -1, dtype=torch.int32, device=device)
         self.num_free = torch.full((1,), num_blocks, dtype=torch.int32, device=device)
 
-    def append(self, key: torch.Tensor, value: torch.Tensor, new_lens: torch.Tensor) -> torch.Tensor:
-        """Store the keys and values of ``new_lens[b]`` (int32) new tokens of each request; returns their offsets ``[B + 1]``."""
+    def _append(self, query, key, value, new_lens, rotary):
+        """Store new tokens without counting them: the queries (rotated, if they are to be), their offsets, and the lengths and free blocks from then on."""
         slots, query_offset, seq_lens, num_free = build_block_tables(
             self.block_tables, self.seq_lens, new_lens, self.free_blocks, self.num_free, self.block_size, key.shape[0])
-        append_kv_cache_fp8(key, value, self.k_cache, self.v_cache, self.k_scales, self.v_scales, slots)
+        if rotary is None:
+            append_kv_cache_fp8(key, value, self.k_cache, self.v_cache, self.k_scales, self.v_scales, slots)
+        else:
+            query = append_rotated_kv_cache_fp8(query, key, value, self.k_cache, self.v_cache, self.k_scales, self.v_scales, slots, query_offset, seq_lens,
+                                                **rotary)
+        return query, query_offset, seq_lens, num_free
+
+    def append(self, key: torch.Tensor, value: torch.Tensor, new_lens: torch.Tensor) -> torch.Tensor:
+        """Store the keys and values of ``new_lens[b]`` (int32) new tokens of each request; returns their offsets ``[B + 1]``."""
+        _, query_offset, seq_lens, num_free = self._append(None, key, value, new_lens, None)
         # not before: keys or values that were refused are not in the cache (the blocks that the tables have for them count as free)
         self.seq_lens, self.num_free = seq_lens, num_free
         return query_offset
@@ -359,9 +368,7 @@ class PagedKVCache:
     def append_rotated(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, new_lens: torch.Tensor, rotary: dict):
         """As :meth:`append`, with queries and keys normed and rotated on the way (``rotary``: :func:`append_rotated_kv_cache_fp8`'s arguments from
         ``inv_freq`` on); returns ``(queries, offsets)``."""
-        slots, query_offset, seq_lens, num_free = build_block_tables(
-            self.block_tables, self.seq_lens, new_lens, self.free_blocks, self.num_free, self.block_size, key.shape[0])
-        query = append_rotated_kv_cache_fp8(query, key, value, self.k_cache, self.v_cache, self.k_scales, self.v_scales, slots, query_offset, seq_lens, **rotary)
+        query, query_offset, seq_lens, num_free = self._append(query, key, value, new_lens, rotary)
         self.seq_lens, self.num_free = seq_lens, num_free  # not before, as in append
         return query, query_offset
 
@@ -382,12 +389,15 @@ class PagedKVCache:
     def step(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, new_lens: torch.Tensor, max_seq_len_q: int,
              rotary: Optional[dict] = None, **options) -> torch.Tensor:
         """Append, then attend with the new tokens' queries (causal unless ``is_causal=False`` is given); with ``rotary``, queries and keys are
-        normed and rotated first (:meth:`append_rotated`)."""
-        if rotary is None:
-            query_offset = self.append(key, value, new_lens)
-        else:
-            query, query_offset = self.append_rotated(query, key, value, new_lens, rotary)
-        return self.attend(query, query_offset, max_seq_len_q, **{"is_causal": True, **options})
+        normed and rotated first (:meth:`append_rotated`).  A step that is refused, by its append or by its attention, counts no tokens: it can be made again."""
+        if query.dtype != torch.bfloat16:  # of all that the attention refuses what an append of fp32 lets through: before anything is stored
+            raise TypeError(f"query must be bf16 for a step (the attention's type), got {query.dtype}")
+        query, query_offset, seq_lens, num_free = self._append(query, key, value, new_lens, rotary)
+        out = generalized_dot_product_attention_paged_fp8(
+            query, self.k_cache, self.v_cache, self.k_scales, self.v_scales, self.block_tables, query_offset, seq_lens, max_seq_len_q,
+            **{"is_causal": True, **options})
+        self.seq_lens, self.num_free = seq_lens, num_free  # not before
+        return out
 
     def release(self, requests: Sequence[int]) -> None:
         """Give back the blocks of these requests (rows of the tables, negative ones from the end), which are empty afterwards."""

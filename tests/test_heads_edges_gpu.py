@@ -137,3 +137,30 @@ def test_two_threads_appends_to_blocks_of_two_sizes(is_fp32):
             "cache.head_dim": dim, "rotary.inv_freq": f.data_ptr(), "rotary.inv_freq_is_fp64": 1, "rotary.pairs": dim // 2, "rotary.axes": 1, "rotary.norm": 1,
             "rotary.eps": 1e-6, "query": q.data_ptr(), "query_out": out.data_ptr(), "positions": p.data_ptr(), "positions_are_int64": 1}))
     assert calls_of_two_threads(_cabi.lib.gdpa_append_rotated_kv_cache_fp8, params) == [[], []]
+
+
+# ------------------------------------------------------------------------------------------ a step that is refused
+
+
+@pytest.mark.parametrize("rotated", [False, True])
+def test_a_refused_step_can_be_made_again(rotated):
+    g = torch.Generator().manual_seed(6)
+    q, k, v = (torch.randn(2, 40, h, 64, generator=g).bfloat16().to(DEV) for h in (4, 2, 2))
+    new = torch.tensor([[30, 10], [10, 30]], dtype=torch.int32, device=DEV)
+    rotary = dict(inv_freq=frequencies(32).to(DEV)) if rotated else None
+
+    def serve(refused):
+        cache, outs = G.PagedKVCache(12, 16, 2, 64, 2, 64), []
+        for x, y, z, n in zip(q, k, v, new):
+            if refused:
+                lens, left = cache.seq_lens.tolist(), int(cache.num_free)
+                for args, options, error in (((x.float(), y.float(), z.float()), {}, TypeError), ((x[:, :3].contiguous(), y, z), {}, ValueError),
+                                             ((x, y, z), dict(activation="none of them"), (KeyError, ValueError))):
+                    with pytest.raises(error):
+                        cache.step(*args, n, 30, rotary=rotary, **options)
+                    assert cache.seq_lens.tolist() == lens and int(cache.num_free) == left
+            outs.append(cache.step(x, y, z, n, 30, rotary=rotary, qk_scale=0.125))
+        return (*outs, cache.seq_lens, cache.num_free, cache.block_tables, cache.k_cache.view(torch.uint8), cache.v_cache.view(torch.uint8), cache.k_scales,
+                cache.v_scales)
+
+    assert all(torch.equal(a, b) for a, b in zip(serve(False), serve(True)))

@@ -478,6 +478,15 @@ int make_q8_tmap(CUtensorMap* m, const void* base, int planes, long long rows, i
 }
 
 bool aligned16(const void* a, const void* b) { return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u) == 0; }
+// memory of a call: `bytes` from `at` on
+struct Span {
+  const void* at;
+  long long bytes;
+};
+bool overlap(const Span& a, const Span& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return a.bytes > 0 && b.bytes > 0 && (x < y ? y - x < static_cast<uintptr_t>(a.bytes) : x - y < static_cast<uintptr_t>(b.bytes));
+}
 
 // Rows of an item: the smallest of the kernels' that holds a request's (query, head of the group) rows, 256 at most.  The narrower kernel
 // against the wider, one B200, 64 requests of 4096 tokens, 8 heads on 2 of 128 values: 16 rows 46 us against 60, 64 rows 77 against 101; at
@@ -902,6 +911,17 @@ int gdpa_drop_cached_tokens(const GdpaDropParams* p, gdpa_stream_t stream) {
   if (p->batch > 0 && (p->seq_lens == nullptr || p->dropped == nullptr || p->seq_lens_after == nullptr)) return GDPA_ERR_BAD_ARG;
   if (p->batch > 0 && p->table_width > 0 && p->block_tables == nullptr) return GDPA_ERR_BAD_ARG;
   if (p->free_capacity > 0 && p->free_blocks == nullptr) return GDPA_ERR_BAD_ARG;
+  // Several warps may look at a request, each at its length: what is written lies apart from all that is read.
+  const long long entries = p->batch > 0 && p->table_width > 0 ? (p->batch - 1ll) * p->table_stride + p->table_width : 0;
+  const Span written[] = {{p->seq_lens_after, p->batch * 4ll}, {p->num_free_after, 4}, {p->free_blocks, p->free_capacity * 4}};
+  const Span read[] = {{p->seq_lens, p->batch * (p->lens_are_int64 != 0 ? 8ll : 4ll)}, {p->dropped, p->batch * (p->dropped_is_int64 != 0 ? 8ll : 4ll)},
+                       {p->num_free, 4}, {p->block_tables, entries * 4}};
+  for (int i = 0; i < 3; ++i) {
+    for (const Span& r : read)
+      if (overlap(written[i], r)) return GDPA_ERR_BAD_ARG;
+    for (int j = 0; j < i; ++j)
+      if (overlap(written[i], written[j])) return GDPA_ERR_BAD_ARG;
+  }
   const size_t bytes = gdpa_drop_workspace_bytes(p->batch, p->table_width);
   if (bytes > 0 && p->workspace == nullptr) return GDPA_ERR_BAD_ARG;
   if (p->workspace_bytes < static_cast<int64_t>(bytes)) return GDPA_ERR_CAPACITY;

@@ -622,7 +622,8 @@ int gdpa_verify_draft_tokens(const GdpaVerifyParams* params, gdpa_stream_t strea
 
 /* The last dropped[b] tokens (clamped to [0, seq_lens[b]]) of each request leave the cache: blocks that none of its tokens needs go onto the stack
  * free_blocks[0 .. *num_free), in the order of the requests and their tables; entries that are no block do not, nor those that the stack has
- * no place for.  Tables are only read. */
+ * no place for.  Tables are only read.  Nothing is updated in place: seq_lens_after, num_free_after and free_blocks overlap neither one another nor
+ * seq_lens, dropped, num_free and the tables (GDPA_ERR_BAD_ARG). */
 typedef struct GdpaDropParams {
   uint32_t struct_size;        /* sizeof(GdpaDropParams) */
   int32_t block_size;
@@ -638,7 +639,7 @@ typedef struct GdpaDropParams {
   int64_t free_capacity;
   const int32_t* num_free;     /* device; negative counts as 0 */
   int32_t* seq_lens_after;     /* out [batch] */
-  int32_t* num_free_after;     /* out [1], not the word num_free points to */
+  int32_t* num_free_after;     /* out [1] */
   void* workspace;             /* gdpa_drop_workspace_bytes() bytes, 16-byte aligned; one per call in flight */
   int64_t workspace_bytes;
 } GdpaDropParams;

@@ -1,10 +1,14 @@
 """Calls of the operators on either side of the attention that are easily got wrong and need no GPU."""
+import ctypes as C
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 import ads_model_kernel_library_b200.gdpa as G
+from ads_model_kernel_library_b200.gdpa import _cabi
+from tests.test_paged_cache_cpu import BAD_ARG, OK, fields
 
 
 def empty(*shape, dtype=torch.bfloat16):
@@ -65,3 +69,36 @@ def test_a_step_whose_attention_is_refused_counts_no_tokens(monkeypatch, rotary)
     assert calls == ["append"] and cache.seq_lens.tolist() == [0, 0] and int(cache.num_free) == 8
     assert torch.equal(cache.step(x, x, x, new, 3, rotary=rotary), x)
     assert attended == [[3, 1]] * 2 and cache.seq_lens.tolist() == [3, 1] and int(cache.num_free) == 6
+
+
+# ------------------------------------------------------------------------------------------ lengths that are updated in place
+
+
+def drop_call(**change):
+    """Refused calls only: the addresses are made up."""
+    good = dict(block_size=16, block_tables=0x10000, table_stride=4, table_width=4, batch=2, seq_lens=0x20000, dropped=0x30000, free_blocks=0x40000, free_capacity=4,
+                num_free=0x50000, seq_lens_after=0x60000, num_free_after=0x70000)
+    return _cabi.lib.gdpa_drop_cached_tokens(C.byref(fields(_cabi.GdpaDropParams, **{**good, **change})), None)
+
+
+@pytest.mark.parametrize("change", [
+    dict(seq_lens_after=0x20000), dict(seq_lens_after=0x30000), dict(seq_lens_after=0x20004), dict(seq_lens_after=0x20008, lens_are_int64=1),
+    dict(seq_lens_after=0x2fffc), dict(seq_lens_after=0x3000c, dropped_is_int64=1), dict(seq_lens_after=0x10010), dict(seq_lens_after=0x40000),
+    dict(seq_lens_after=0x50000), dict(seq_lens_after=0x6fffc, num_free_after=0x70000), dict(num_free_after=0x20004), dict(num_free_after=0x3000c, dropped_is_int64=1),
+    dict(num_free_after=0x50000), dict(num_free_after=0x4000c), dict(num_free_after=0x1001c), dict(free_blocks=0x10010), dict(free_blocks=0x4fff4)])
+def test_drop_refuses_outputs_over_its_inputs(change):
+    assert drop_call(**change) == BAD_ARG
+
+
+@pytest.mark.parametrize("change", [dict(block_size=8), dict(batch=-1), dict(table_width=-1), dict(table_stride=-1), dict(free_capacity=-1), dict(table_width=1 << 27),
+                                    dict(num_free=0), dict(num_free_after=0), dict(seq_lens=0), dict(dropped=0), dict(seq_lens_after=0), dict(block_tables=0),
+                                    dict(free_blocks=0)])
+def test_drop_refusals_with_memory_of_their_own(change):
+    assert drop_call(**change) == BAD_ARG
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: only where no kernel can be launched")
+@pytest.mark.parametrize("change", [{}, dict(seq_lens_after=0x20008), dict(seq_lens_after=0x1fff8), dict(seq_lens_after=0x20010, lens_are_int64=1),
+                                    dict(seq_lens_after=0x10020), dict(num_free_after=0x60008), dict(free_blocks=0x4fff0), dict(seq_lens_after=0x30008)])
+def test_drop_takes_neighbours(change):
+    assert drop_call(**change) not in (BAD_ARG, OK)  # the arguments are good, there is no device

@@ -691,9 +691,8 @@ __global__ void __launch_bounds__(kDropWarps * 32) gdpa_drop_kernel(const __grid
 
 // `ranks`: CTAs of a cluster; 0: none, and the kernel before it on the stream may still run.
 template <class K, class A>
-int launch_cluster(K kernel, const A& args, unsigned grid, unsigned threads, unsigned ranks, cudaStream_t stream, int smem = 0) {
+int launch_cluster(K kernel, const A& args, unsigned grid, unsigned threads, unsigned ranks, cudaStream_t stream) {
   cudaLaunchConfig_t c = {};
-  c.dynamicSmemBytes = smem;
   c.gridDim = dim3(grid);
   c.blockDim = dim3(threads);
   c.stream = stream;

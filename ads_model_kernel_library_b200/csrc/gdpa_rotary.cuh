@@ -54,12 +54,6 @@ struct HeadLanes {
     g0 = rotated ? l : np + l;  // behind the 2 np rotated pieces, in two halves: 2 np + (l - np)
     g1 = rotated ? l + np : L + l;
   }
-  // the sum over a head's lanes
-  static __device__ __forceinline__ float sum(float x) {
-#pragma unroll
-    for (int s = 1; s < L; s <<= 1) x += __shfl_xor_sync(kAllLanes, x, s);
-    return x;
-  }
   // Which lane of a head has piece g, and whether as its second one.
   static __device__ __forceinline__ int lane_of_piece(const RotarySpec& r, int g, bool& second) {
     const int np = r.pairs / E;

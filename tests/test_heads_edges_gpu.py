@@ -164,3 +164,57 @@ def test_a_refused_step_can_be_made_again(rotated):
                 cache.v_scales)
 
     assert all(torch.equal(a, b) for a, b in zip(serve(False), serve(True)))
+
+
+# ------------------------------------------------------------------------------------------ fp32 as near as its roundings
+#
+# With u = 2^-24, each fp32 rounding's share.  A sum of D squares: 4 in a lane's chain, the two halves, 4 over lanes: 9 u; with eps 10, so 5 of its root's inverse, and 4
+# of rsqrt itself (2 units in the last place): r 9 u, x r w 11 u.  Sine and cosine 2 u each, of which 1.3 are the reduced angle's and the result's own
+# rounding.  Two products and their sum: 2 u.  A value of a pair: (11 + 2 + 2) u (|n_a| + |n_b|), so
+FORWARD = 16 * 2.0 ** -24
+# Backwards dn = R^T dy is 4 u off (of both values' magnitudes), g = dn w 5 u; mean(g x) 5 + 9 u, times r^2 18 + 2 more: 34 u; g r 14 u; x r times that mean 10 + 34 + 1 u;
+# their sum 1 u: 46 u of r (|g| + |u| mean |g u|) at most, so
+BACKWARD = 48 * 2.0 ** -24
+# A weight's gradient sums products that are 4 + 10 u off, one after the other: 18 of an item's heads and tokens, the item's into the warp's 1, 16 warps' heads, 14 rows of
+# CTAs, 32 of these: 95 u, so
+WEIGHTS = 128 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("tokens,far,pairs", [(200, 5000, None), (200, 4 * 10 ** 6, 16), (3000, 5000, None), (1, 9, 24)])
+def test_fp32_is_as_near_as_its_roundings(dim, interleaved, norm, tokens, far, pairs):
+    g = torch.Generator().manual_seed(8)
+    pairs = dim // 2 if pairs is None else pairs
+    x, dy = ([torch.randn(tokens, h, dim, generator=g) for h in (5, 3)] for _ in range(2))
+    w = [weights(dim, g) for _ in range(2)]
+    f, p = frequencies(pairs), torch.randint(0, far, (tokens,), generator=g)
+    angle = ref.angles(f, p)
+    leaves = [t.to(DEV).requires_grad_() for t in (*x, *w)]
+    out = G.qk_norm_rotary(*leaves[:2], f.to(DEV), p.to(DEV), query_weight=leaves[2], key_weight=leaves[3], norm=norm, interleaved=interleaved)
+    got = torch.autograd.grad(out, leaves[:4 if norm else 2], [t.to(DEV) for t in dy])
+    for i, name in enumerate("qk"):
+        want, tol = ref.norm_rotary(x[i], w[i], 1e-6, norm, angle, interleaved)
+        ref.check_close(out[i], want, tol * (2.0 ** 16 * FORWARD), name)
+        (dx, tol), of_weight = ref.norm_rotary_grad(x[i], dy[i], w[i], 1e-6, norm, angle, interleaved)
+        ref.check_close(got[i], dx, tol * (2.0 ** 15 * BACKWARD if norm else 2.0 ** 16 * FORWARD), "d" + name)
+        if norm:
+            ref.check_close(got[2 + i], of_weight[0], of_weight[1] * (2.0 ** 15 * WEIGHTS), "dw of " + name)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens", [[1] * 9, [70, 1, 200]])
+def test_fp32_queries_of_an_append_are_as_near_as_their_roundings(dim, lens):
+    g = torch.Generator().manual_seed(9)
+    n, before = sum(lens), 3000
+    q, k, v = (torch.randn(n, h, dim, generator=g) for h in (5, 3, 3))
+    w, f = weights(dim, g), frequencies(dim // 2)
+    p = torch.cat([before + torch.arange(m) for m in lens])
+    offsets = torch.tensor([sum(lens[:b]) for b in range(len(lens) + 1)], dtype=torch.int32, device=DEV)
+    cache, scales = torch.zeros(2, 1, 16, 3, dim, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn), torch.ones(2, 1, 3, device=DEV)
+    out = G.append_rotated_kv_cache_fp8(q.to(DEV), k.to(DEV), v.to(DEV), cache[0], cache[1], scales[0], scales[1], torch.full((n,), -1, device=DEV), offsets,
+                                        torch.tensor([before + m for m in lens], dtype=torch.int32, device=DEV), f.to(DEV), query_weight=w.to(DEV))
+    want, tol = ref.norm_rotary(q, w, 1e-6, True, ref.angles(f, p), False)
+    ref.check_close(out, want, tol * (2.0 ** 16 * FORWARD))
+    assert not cache.view(torch.uint8).any()

@@ -33,23 +33,7 @@ __global__ void __launch_bounds__(kReadWarps * 32) gdpa_cache_read_kernel(const 
   if (base >= a.total) return;
   const int tokens = static_cast<int>(min(static_cast<long long>(a.warp_tokens), a.total - base));
   // where the lane's token is: its block (-1: nowhere) and row
-  int lo = 0, hi = a.batch;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-    const unsigned below = __ballot_sync(kFull, at < hi && load_offset(a.offsets, at, a.off64) <= base);
-    lo += (below == 0 ? 0 : __popc(below) - 1) * step;
-    hi = min(hi, lo + step);
-  }
-  int owner = lo;
-  for (int b = lo + 1; b < a.batch; b += 32) {
-    const long long begin = b + lane < a.batch ? load_offset(a.offsets, b + lane, a.off64) : 0x7fffffffffffffffll;
-    int count = 0;
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) count += __shfl_sync(kFull, begin, count + s - 1) <= base + lane ? s : 0;
-    count += __shfl_sync(kFull, begin, count) <= base + lane;
-    owner += count;
-    if (__shfl_sync(kFull, begin, 31) > base + tokens - 1) break;
-  }
+  const int owner = request_of_lane(a.offsets, a.off64, a.batch, base, base + tokens - 1);
   int block = -1, row = 0;
   if (a.batch > 0 && lane < tokens) {
     const long long begin = load_offset(a.offsets, owner, a.off64), end = load_offset(a.offsets, owner + 1, a.off64);

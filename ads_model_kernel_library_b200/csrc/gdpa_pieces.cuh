@@ -1,5 +1,5 @@
-// Rows of bf16 or fp32 values taken 16 bytes at a time, and the scale of a run of them in 8 bits: what the kernels share that fill
-// and read the paged cache.
+// Rows of bf16 or fp32 values taken 16 bytes at a time, the scale of a run of them in 8 bits, and the request that a token belongs to: what the kernels share
+// that fill and read the paged cache.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -7,6 +7,7 @@
 
 #include <cstdint>
 
+#include "gdpa_common.cuh"
 #include "sm100_ptx.cuh"
 
 namespace gdpa {
@@ -65,5 +66,33 @@ __device__ __forceinline__ int scale_exponent(uint32_t bits) {
 }
 
 constexpr uint32_t kInfBits = 0x7f800000u;
+
+// The request that has token t: the last of `batch` whose offset is at or before it.  By the whole warp; it ends whatever the offsets say.
+__device__ __forceinline__ int request_of(const void* offsets, int off64, int batch, long long t) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = batch;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const unsigned below = __ballot_sync(0xffffffffu, at < hi && load_offset(offsets, at, off64) <= t);
+    lo += (below == 0 ? 0 : __popc(below) - 1) * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+// The same for the lane's one of neighbouring tokens, base + lane; those behind `last` need not come out right.
+__device__ __forceinline__ int request_of_lane(const void* offsets, int off64, int batch, long long base, long long last) {
+  const int lane = threadIdx.x & 31, b0 = request_of(offsets, off64, batch, base);
+  int owner = b0;
+  for (int b = b0 + 1; b < batch; b += 32) {
+    const long long begin = b + lane < batch ? load_offset(offsets, b + lane, off64) : 0x7fffffffffffffffll;
+    int count = 0;  // of these 32 that begin at or before the lane's token
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) count += __shfl_sync(0xffffffffu, begin, count + s - 1) <= base + lane ? s : 0;
+    count += __shfl_sync(0xffffffffu, begin, count) <= base + lane;
+    owner += count;
+    if (__shfl_sync(0xffffffffu, begin, 31) > last) break;
+  }
+  return owner;
+}
 
 }  // namespace gdpa

@@ -23,18 +23,6 @@ namespace gdpa {
 
 namespace {
 
-// The request that has token t, by the whole warp: the last one that begins at or before it.
-__device__ __forceinline__ int owner_of(const RotatedAppendArgs& a, long long t) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, hi = a.batch;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-    const unsigned below = __ballot_sync(kAllLanes, at < hi && load_offset(a.q_off, at, a.off64) <= t);
-    lo += (below == 0 ? 0 : __popc(below) - 1) * step;
-    hi = min(hi, lo + step);
-  }
-  return lo;
-}
 // position of the request's token with index 0 of the call
 __device__ __forceinline__ long long origin_of(const RotatedAppendArgs& a, int owner) {
   return a.batch == 0 ? 0 : load_offset(a.seq_lens, owner, a.lens64) - load_offset(a.q_off, owner + 1, a.off64);
@@ -218,19 +206,7 @@ struct Window {
   // position of the first token of the run that the lane leads, less its index
   __device__ __forceinline__ long long origin() const {
     if (a.queries.t[0].positions != nullptr) return 0;
-    // the requests of the 32 tokens: the first one's, and whose beginnings follow
-    const int lane = threadIdx.x & 31, b0 = owner_of(a, base);
-    int owner = b0;
-    for (int b = b0 + 1; b < a.batch; b += 32) {
-      const long long begin = b + lane < a.batch ? load_offset(a.q_off, b + lane, a.off64) : 0x7fffffffffffffffll;
-      int count = 0;  // of these 32 that begin at or before the lane's token
-#pragma unroll
-      for (int s = 16; s > 0; s >>= 1) count += __shfl_sync(kAllLanes, begin, count + s - 1) <= base + lane ? s : 0;
-      count += __shfl_sync(kAllLanes, begin, count) <= base + lane;
-      owner += count;
-      if (__shfl_sync(kAllLanes, begin, 31) > base + 31) break;
-    }
-    return origin_of(a, owner);
+    return origin_of(a, request_of_lane(a.q_off, a.off64, a.batch, base, base + 31));
   }
 };
 
@@ -327,13 +303,13 @@ struct QueryPositions {
       return;
     }
     const int lane = threadIdx.x & 31;
-    if (owner < 0) owner = owner_of(a, t);
+    if (owner < 0) owner = request_of(a.q_off, a.off64, a.batch, t);
     for (bool searched = false;; searched = true) {
       const int next = min(owner + 1 + lane, a.batch);
       const long long ends = load_offset(a.q_off, next, a.off64), len = load_offset(a.seq_lens, min(owner + lane, a.batch - 1), a.lens64);
       const unsigned behind = __ballot_sync(kAllLanes, owner + 1 + lane < a.batch && ends <= t);
       if (behind == kAllLanes && !searched) {
-        owner = owner_of(a, t);
+        owner = request_of(a.q_off, a.off64, a.batch, t);
         continue;
       }
       const int count = behind == kAllLanes ? 0 : __ffs(~behind) - 1;  // all of them after a search: offsets that are none

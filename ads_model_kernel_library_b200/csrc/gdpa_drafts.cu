@@ -14,8 +14,9 @@
 //
 // Few requests: one launch, a cluster of CTAs to each, and latency is all of it.  Many: three kernels, whose beginnings overlap the ends of those before
 // them: who is accepted; the stretches' sums, dealt out over the whole GPU (a CTA to a request leaves SMs with one row to add up and SMs with four);
-// the token.  256 requests of 131071 bf16 tokens, 116 MB: 49 us in one kernel, 42 in three, 28 of them for the sums
-// (4.1 TB/s; half of their time waits for memory, half goes to instructions: rows staged through shared memory, with more on its way, took 33).
+// the token.  256 requests of 131071 bf16 tokens, 116 MB, cold: 55 us in one kernel, 43 in three, 28 of them for the sums
+// (4.1 TB/s; half of their time waits for memory, half goes to instructions: rows staged through shared memory, with more on its way, took 33).  Calls in a row: 47
+// and 39.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -714,8 +715,8 @@ int launch_cluster(K kernel, const A& args, unsigned grid, unsigned threads, uns
 int verify_most_vocab() { return kMostVocab; }
 
 namespace {
-// Whether a call takes the three kernels: where its rows keep the whole GPU busy.  One kernel against three, us, rows of bf16: 64 requests of 32000 tokens (4 MB) 14
-// and 16, 32 of 131071 (8 MB) 20 and 18, 256 of 32000 22 and 22, 256 of 131071 49 and 43.
+// Whether a call takes the three kernels: where its rows keep the whole GPU busy.  One kernel against three, us, rows of bf16, cold (calls in a row): 64 requests of 32000
+// tokens (4 MB) 14 and 16 (12 and 15), 32 of 131071 (8 MB) 18 and 20 (16 and 17), 256 of 32000 (16 MB) 22 and 22 (18 and 20), 256 of 131071 (67 MB) 55 and 43 (47 and 39).
 bool many_requests(long long batch, long long vocab, int size) { return batch >= 32 && batch * vocab * size >= (8ll << 20); }
 long long most_stretches(long long vocab, int size) { return (vocab * size + 15) / (32 * kManyBlocks * 16) + 1; }
 }  // namespace

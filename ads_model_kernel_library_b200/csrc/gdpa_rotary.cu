@@ -9,7 +9,8 @@
 // warp takes the heads of a token, four heads of 128 bf16 values at a time, so that a token's angles are made once.  Units come through shared memory, fetched ahead by the
 // lanes that use them, so that no barrier stands between; a few tokens to a warp, then the next ones far behind, keep what all warps have in hand close together in memory.
 // bf16, 128 values, cold: 16 and 4 heads of 67 000 tokens 115 us, 690 MB, 6.0 TB/s (a plain copy 6.5); 8 and 8 heads of 300 000 tokens 398 us forward (6.2), 600
-// to 633 backward (5.8 to 6.1), of it 5 to 6 the joining of the weights' gradients; 64 tokens of 32 and 4 heads 5.4 us.
+// to 633 backward (5.8 to 6.1), of it 5 to 6 the joining of the weights' gradients; 64 tokens of 32 and 4 heads 5.4 us.  The rotation alone, 8 and 8 heads of 300 000 tokens: 436
+// us forward (5.6), 387 backward (6.3; x is not read).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

@@ -324,6 +324,9 @@ def drop_cached_tokens(
     requests and of their tables; entries that are no block (-1) do not.  ``dropped`` is clamped to what a request has, a negative ``num_free``
     counts as 0.  Returns ``(seq_lens_after, num_free_after)``, int32 ``[B]`` and ``[1]``.  The tables are left as they are: what lies behind
     a request's length is not looked at, and :func:`build_block_tables` writes over it.
+
+    Tokens that stay in a block with dropped ones keep the block's scale.  Where the append of a draft made it grow, they were rescaled then, and the bits of
+    theirs that fell below e4m3's smallest normal value do not come back (:func:`append_kv_cache_fp8`).
     """
     return (_operators or _load()).drop(block_tables, seq_lens, dropped, free_blocks, num_free, block_size)
 

@@ -388,7 +388,7 @@ typedef struct GdpaBlockTableParams {
   int64_t total_new;           /* entries of slots; entries past the batch's new tokens become -1 */
   int64_t* slots;              /* out [total_new] */
   int32_t* query_offset;       /* out [batch + 1]: exclusive prefix sum of new_lens */
-  int32_t* seq_lens;           /* out [batch]: cached_lens + new_lens */
+  int32_t* seq_lens;           /* out [batch]: cached_lens + new_lens.  Not in place: every CTA reads all of cached_lens */
   int32_t* num_free_after;     /* out [1], not the word num_free points to */
 } GdpaBlockTableParams;
 
@@ -623,7 +623,8 @@ int gdpa_verify_draft_tokens(const GdpaVerifyParams* params, gdpa_stream_t strea
 /* The last dropped[b] tokens (clamped to [0, seq_lens[b]]) of each request leave the cache: blocks that none of its tokens needs go onto the stack
  * free_blocks[0 .. *num_free), in the order of the requests and their tables; entries that are no block do not, nor those that the stack has
  * no place for.  Tables are only read.  Nothing is updated in place: seq_lens_after, num_free_after and free_blocks overlap neither one another nor
- * seq_lens, dropped, num_free and the tables (GDPA_ERR_BAD_ARG). */
+ * seq_lens, dropped, num_free and the tables (GDPA_ERR_BAD_ARG).  The rows that stay keep their block's scale, and what an append that made it grow took from them:
+ * bits below e4m3's smallest normal value. */
 typedef struct GdpaDropParams {
   uint32_t struct_size;        /* sizeof(GdpaDropParams) */
   int32_t block_size;

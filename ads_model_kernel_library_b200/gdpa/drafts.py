@@ -26,7 +26,8 @@ def verify_draft_tokens(
     Request ``b`` has the drafts ``draft_tokens[draft_offset[b]:draft_offset[b + 1]]``, ``n`` of them (at most ``max_drafts``), and the rows
     ``query_offset[b]:query_offset[b + 1]`` of ``target_probs`` ``[rows, vocabulary]`` (fp32 or bf16): row ``j`` is the target's distribution of
     draft ``j``, row ``n`` that of the token after them, so a step has one row more than drafts (its first query is the last token that was known).
-    Without a row more, that many drafts are not looked at; a request without rows takes no part.  ``draft_probs`` ``[drafts, vocabulary]`` are the
+    Without a row more, that many drafts are not looked at, nor are those past ``max_drafts``: they count as neither accepted nor refused, so a caller that
+    has stored more than ``max_drafts`` takes the others out of the cache itself.  A request without rows takes no part.  ``draft_probs`` ``[drafts, vocabulary]`` are the
     distributions that the drafts were drawn from, ``None`` for drafts that were not drawn at all.
 
     Draft ``j`` is accepted if ``accept_uniform[j] * draft_probs[j, token] < target_probs[j, token]`` and all before it are (``None``: the factor is

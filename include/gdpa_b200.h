@@ -584,7 +584,7 @@ typedef struct GdpaCacheReadParams {
 int gdpa_read_kv_cache_fp8(const GdpaCacheReadParams* params, gdpa_stream_t stream);
 
 /* Drafted tokens against the target's probabilities.  Request b has rows row_offsets[b] .. of target and drafts draft_offsets[b] .. (n of them: at
- * most max_drafts and one less than its rows).  Draft j is accepted if accept[j] * draft[j, x_j] < target[row j, x_j] (draft null: the
+ * most max_drafts and one less than its rows; others are not looked at and count as neither accepted nor refused).  Draft j is accepted if accept[j] * draft[j, x_j] < target[row j, x_j] (draft null: the
  * factor is one) and all before it are; with a of them accepted, the next token is the first at which the partial sum of
  * max(target - draft, 0) (a = n: of target; draft null: of target without the refused token) exceeds sample[b] times its total, where there is
  * no total, that of target; -1 if that has none either.  Shares that are not positive finite numbers count as zero; sums are in 64 bits. */
